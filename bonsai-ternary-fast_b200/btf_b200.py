@@ -14,6 +14,7 @@ library is missing, loading raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from dataclasses import dataclass
@@ -41,6 +42,7 @@ EXPORTS = (
     "btf_plan_memory", "btf_plan_memory_synthetic", "btf_decoder_stats", "btf_decoder_reset_stats",
     "btf_gemm_f32_noalloc", "btf_chain_program_bytes", "btf_chain_encode", "btf_chain_run", "btf_stamp_next",
     "btf_gemm_idot", "btf_decoder_prefill", "btf_gemm_wm", "btf_gemm_wm_idot", "btf_gemv_mma", "btf_gemv_mma_idot",
+    "btf_rope_table", "btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample",
 )
 
 
@@ -140,6 +142,35 @@ class MemoryPlanC(ctypes.Structure):
     _fields_ = [(f, ctypes.c_uint64) for f in PLAN_FIELDS] + [("n_matrices", ctypes.c_int), ("dims", DecoderDimsC)]
 
 
+class RopeCfgC(ctypes.Structure):
+    """btf_rope_cfg: rotary frequencies and their scaling for long contexts."""
+
+    _fields_ = [("n_rot", ctypes.c_int), ("scaling", ctypes.c_int), ("base", ctypes.c_double),
+                ("factor", ctypes.c_double), ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double),
+                ("orig_ctx", ctypes.c_int)]
+
+
+class RopeSegC(ctypes.Structure):
+    """btf_rope_seg: one tensor of a btf_rope call."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("x_type", ctypes.c_int), ("y_type", ctypes.c_int),
+                ("heads", ctypes.c_int), ("rotate", ctypes.c_int), ("x_token", ctypes.c_int64),
+                ("x_head", ctypes.c_int64), ("y_token", ctypes.c_int64), ("y_head", ctypes.c_int64),
+                ("normw", ctypes.c_void_p), ("rows", ctypes.c_void_p), ("n_rows", ctypes.c_int64)]
+
+
+class TreeAttnC(ctypes.Structure):
+    """btf_tree_attn: attention for a tree of drafted tokens over a cache."""
+
+    _fields_ = [("q", ctypes.c_void_p)] + [(f, ctypes.c_int64) for f in ("q_batch", "q_node", "q_head")] + [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [
+        (f, ctypes.c_int64) for f in ("kv_batch", "kv_row", "kv_head")] + [("o", ctypes.c_void_p)] + [
+        (f, ctypes.c_int64) for f in ("o_batch", "o_node", "o_head")] + [
+        (f, ctypes.c_int) for f in ("type", "B", "n", "H", "HK", "D", "n_ctx")] + [
+        (f, ctypes.c_void_p) for f in ("lens", "parents", "counts")] + [
+        ("scale", ctypes.c_float), ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_int64)]
+
+
 def lib() -> ctypes.CDLL:
     """Loads libbtf_b200.so (raises if it was not built)."""
     global _lib
@@ -214,6 +245,12 @@ def lib() -> ctypes.CDLL:
         "btf_decoder_stats": (i32, [vp, ctypes.POINTER(StepStatsC)]),
         "btf_decoder_reset_stats": (i32, [vp]),
         "btf_plan_memory": (i32, [ctypes.c_char_p, ctypes.POINTER(DecoderOptsC), i32, i32, ctypes.POINTER(MemoryPlanC)]),
+        "btf_rope_table": (i32, [ctypes.POINTER(RopeCfgC), vp, ctypes.POINTER(ctypes.c_float)]),
+        "btf_rope": (i32, [ctypes.POINTER(RopeSegC), i32, i32, i32, i32, vp, ctypes.c_float, i32, i32, ctypes.c_float,
+                           vp, vp]),
+        "btf_tree_attention_work": (i64, [i32] * 6),
+        "btf_tree_attention": (i32, [ctypes.POINTER(TreeAttnC), vp]),
+        "btf_sample": (i32, [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
         "btf_plan_memory_synthetic": (i32, [ctypes.POINTER(DecoderDimsC), ctypes.POINTER(DecoderOptsC), i32, i32,
                                             ctypes.POINTER(MemoryPlanC)]),
     }
@@ -574,6 +611,196 @@ def prep(x, normw=None, eps: float = 1e-6, block: int = 0, perm=(0, 0, 0), signs
     check(lib().btf_prep(_ptr(x), x.stride(0), M, n, _ptr(normw), eps, hx, _ptr(xn_out), ldxn, act.c(),
                          _stream(stream)), "btf_prep")
     return act
+
+
+# ---------------------------------------------------------------- operators of new tokens: rotary positions,
+# attention for a tree of drafted tokens, sampling
+F32, F16, BF16 = 0, 1, 2  # BTF_F32 / BTF_F16 / BTF_BF16
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+TREE_MAX_NODES = 64  # BTF_TREE_MAX_NODES
+SAMPLE_MAX_V = 524288  # BTF_SAMPLE_MAX_V
+
+
+def _elem(t, what: str) -> int:
+    torch = _torch()
+    types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    if t.dtype not in types:
+        raise RuntimeError(f"{what}: float32, float16 or bfloat16 expected, got {t.dtype}")
+    return types[t.dtype]
+
+
+def _same_device(what: str, dev, tensors: dict) -> None:
+    if dev.type != "cuda":
+        raise RuntimeError(f"{what}: CUDA tensors expected, got one on {dev}")
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, not on {dev}")
+
+
+def _vector(what: str, name: str, t, dtype, shape) -> None:
+    """A parameter tensor of the call: contiguous, of this type and shape."""
+    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+        raise RuntimeError(f"{what}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} "
+                           f"{tuple(t.shape)}")
+
+
+@contextlib.contextmanager
+def _launching(dev, stream):
+    """The stream handle to launch on with `dev` current: dev's current stream, or `stream`, which is then current too
+    (so that what is allocated for the call belongs to it)."""
+    torch = _torch()
+    ensure_init(dev.index)
+    if stream is None:
+        if torch.cuda.current_device() == dev.index:
+            yield torch.cuda.current_stream(dev).cuda_stream
+            return
+        with torch.cuda.device(dev):
+            yield torch.cuda.current_stream(dev).cuda_stream
+        return
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
+    if stream.device != dev:
+        raise RuntimeError(f"a stream of {stream.device} for tensors on {dev}")
+    with torch.cuda.stream(stream):
+        yield stream.cuda_stream
+
+
+def _strides(t) -> list:
+    """Strides in elements; of a dim with one entry none matters."""
+    return [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+
+
+class RopeTable:
+    """Rotary frequencies (btf_rope_table) kept on the device: n_rot rotated dims of a head, base, the scaling for
+    long contexts ("none", "linear", "ntk", "yarn" with its factor, trained context and betas) and the layout of the
+    pairs (interleaved: (2i, 2i + 1), else (i, i + n_rot / 2)). device=None: host only."""
+
+    def __init__(self, n_rot: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, orig_ctx: int = 0,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, interleaved: bool = False, device="cuda"):
+        import numpy as np
+
+        if scaling not in ROPE_SCALINGS:
+            raise RuntimeError(f"RopeTable: scaling must be one of {sorted(ROPE_SCALINGS)}, got {scaling!r}")
+        cfg = RopeCfgC(n_rot, ROPE_SCALINGS[scaling], base, factor, beta_fast, beta_slow, orig_ctx)
+        self.host = np.zeros(max(1, n_rot // 2), dtype=np.float64)
+        m = ctypes.c_float()
+        check(lib().btf_rope_table(ctypes.byref(cfg), self.host.ctypes.data, ctypes.byref(m)), "btf_rope_table")
+        self.n_rot, self.mscale, self.interleaved = n_rot, m.value, interleaved
+        self.turns = None if device is None else _torch().from_numpy(self.host).to(device)
+
+
+@dataclass
+class RopeSeg:
+    """One tensor of a rope() call: x [T][heads][D] to y (None: in place), optionally normed per head with normw [D]
+    first, rotated unless rotate=False, token t to row rows[t] of y (a cache's slots; rows outside y are not written)."""
+
+    x: object
+    y: object = None
+    normw: object = None
+    rotate: bool = True
+    rows: object = None
+
+
+def rope(segs: Sequence[RopeSeg], table: RopeTable, pos, inverse: bool = False, eps: float = 1e-6, stream=None) -> None:
+    """Rotates up to 3 tensors of the same tokens by their positions pos [T] (int32) in one launch (btf_rope).
+    inverse: the transposed map, the gradient of the rotation."""
+    torch = _torch()
+    if not 1 <= len(segs) <= 3:
+        raise RuntimeError(f"rope: 1..3 tensors expected, got {len(segs)}")
+    T, D, dev = segs[0].x.shape[0], segs[0].x.shape[-1], segs[0].x.device
+    arr = (RopeSegC * len(segs))()
+    for i, s in enumerate(segs):
+        y = s.x if s.y is None else s.y
+        if s.x.dim() != 3 or y.dim() != 3 or s.x.shape[0] != T or s.x.shape[2] != D or y.shape[1:] != s.x.shape[1:]:
+            raise RuntimeError(f"rope: x [T][heads][D] and y [rows][heads][D] expected, got {tuple(s.x.shape)} and "
+                               f"{tuple(y.shape)}")
+        if s.rows is None and y.shape[0] != T:
+            raise RuntimeError(f"rope: y has {y.shape[0]} rows for {T} tokens")
+        if D > 1 and (s.x.stride(2) != 1 or y.stride(2) != 1):
+            raise RuntimeError("rope: the dims of a head must be contiguous")
+        _same_device("rope", dev, {"x": s.x, "y": y, "normw": s.normw, "rows": s.rows})
+        _vector("rope", "normw", s.normw, torch.float32, (D,))
+        _vector("rope", "rows", s.rows, torch.int32, (T,))
+        xs, ys = _strides(s.x), _strides(y)
+        arr[i] = RopeSegC(_ptr(s.x), _ptr(y), _elem(s.x, "rope"), _elem(y, "rope"), s.x.shape[1], int(s.rotate), xs[0],
+                          xs[1], ys[0], ys[1], _ptr(s.normw), _ptr(s.rows), y.shape[0])
+    _same_device("rope", dev, {"pos": pos, "table": table.turns})
+    _vector("rope", "pos", pos, torch.int32, (T,))
+    with _launching(dev, stream) as st:
+        check(lib().btf_rope(arr, len(segs), T, D, table.n_rot, _ptr(table.turns), table.mscale, int(table.interleaved),
+                             int(inverse), eps, _ptr(pos), st), "btf_rope")
+
+
+def tree_attention_work(q, k):
+    """A workspace for tree_attention calls of these shapes (q [B][n][H][D], k [B][n_ctx][HK][D]). Calls that may
+    run at the same time need one each."""
+    B, n, H, D = q.shape
+    ensure_init(q.device.index)
+    with _torch().cuda.device(q.device):
+        size = lib().btf_tree_attention_work(B, n, H, k.shape[2], D, k.shape[1])
+    if size < 0:
+        check(1, "btf_tree_attention_work")
+    return _torch().empty(size, dtype=_torch().uint8, device=q.device)
+
+
+def tree_attention(q, k, v, lens, parents, counts=None, scale: Optional[float] = None, out=None, work=None,
+                   stream=None):
+    """Attention of a tree of drafted tokens over a cache (btf_tree_attention): q [B][n][H][D]; k and v
+    [B][n_ctx][HK][D] hold lens[b] cached tokens and the nodes behind them; node i sees the cache, itself and its
+    ancestors by parents [B][n] (int32, -1: hangs on the cache). counts [B]: nodes of each sequence (None: n)."""
+    torch = _torch()
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise RuntimeError(f"tree_attention: q [B][n][H][D] and k, v [B][n_ctx][HK][D] expected, got {tuple(q.shape)}, "
+                           f"{tuple(k.shape)}, {tuple(v.shape)}")
+    B, n, H, D = q.shape
+    dev = q.device
+    _same_device("tree_attention", dev, {"k": k, "v": v, "lens": lens, "parents": parents, "counts": counts, "out": out,
+                                         "work": work})
+    _vector("tree_attention", "lens", lens, torch.int32, (B,))
+    _vector("tree_attention", "parents", parents, torch.int32, (B, n))
+    _vector("tree_attention", "counts", counts, torch.int32, (B,))
+    with _launching(dev, stream) as st:
+        if out is None:
+            out = (torch.empty if counts is None else torch.zeros)((B, n, H, D), dtype=q.dtype, device=dev)
+        if out.shape != q.shape or k.dtype != q.dtype or v.dtype != q.dtype or out.dtype != q.dtype:
+            raise RuntimeError("tree_attention: q, k, v and out must have one type, and out the shape of q")
+        qs, ks, vs, os_ = _strides(q), _strides(k), _strides(v), _strides(out)
+        if any(t.stride(3) != 1 for t in (q, k, v, out)) or ks != vs:
+            raise RuntimeError("tree_attention: the dims of a head must be contiguous, and k and v strided alike")
+        if B == 0:
+            return out
+        if work is None:
+            work = tree_attention_work(q, k)
+        a = TreeAttnC(_ptr(q), *qs[:3], _ptr(k), _ptr(v), *ks[:3], _ptr(out), *os_[:3], _elem(q, "tree_attention"), B, n,
+                      H, k.shape[2], D, k.shape[1], _ptr(lens), _ptr(parents), _ptr(counts),
+                      D ** -0.5 if scale is None else scale, _ptr(work), work.numel() * work.element_size())
+        check(lib().btf_tree_attention(ctypes.byref(a), st), "btf_tree_attention")
+    return out
+
+
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprobs=None, stream=None):
+    """Draws a token of each row of logits [B][V] from the random numbers u [B] in [0, 1) (btf_sample); temperature,
+    top_p, min_p (float32) and top_k (int32) are [B] or None. Returns (tokens int32 [B], logprobs float32 [B])."""
+    torch = _torch()
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise RuntimeError("sample: logits [B][V] with contiguous rows expected")
+    B, V = logits.shape
+    dev = logits.device
+    params = {"u": (u, torch.float32), "temperature": (temperature, torch.float32), "top_k": (top_k, torch.int32),
+              "top_p": (top_p, torch.float32), "min_p": (min_p, torch.float32), "tokens": (tokens, torch.int32),
+              "logprobs": (logprobs, torch.float32)}
+    _same_device("sample", dev, {n: t for n, (t, _) in params.items()})
+    for name, (t, dtype) in params.items():
+        _vector("sample", name, t, dtype, (B,))
+    with _launching(dev, stream) as st:
+        if tokens is None:
+            tokens = torch.empty(B, dtype=torch.int32, device=dev)
+        if logprobs is None:
+            logprobs = torch.empty(B, dtype=torch.float32, device=dev)
+        ld = logits.stride(0) if B > 1 else V
+        check(lib().btf_sample(_ptr(logits), _elem(logits, "sample"), ld, B, V, _ptr(u), _ptr(temperature), _ptr(top_k),
+                               _ptr(top_p), _ptr(min_p), _ptr(tokens), _ptr(logprobs), st), "btf_sample")
+    return tokens, logprobs
 
 
 PTQ1_0 = 143

@@ -508,6 +508,107 @@ int btf_plan_memory(const char* gguf_path, const btf_decoder_opts* opts, int wor
 int btf_plan_memory_synthetic(const btf_decoder_dims* dims, const btf_decoder_opts* opts, int world, int rank,
                               btf_memory_plan* out);
 
+/* ---- operators around the attention of new tokens: rotary positions, attention
+ * for a tree of drafted tokens over a cache, sampling. The reference does the first
+ * and the last inside its decode step for one token (src/emu_decoder.cpp:307-375,
+ * :214-217) and has no counterpart of the second. Element types: */
+#define BTF_F32 0
+#define BTF_F16 1
+#define BTF_BF16 2
+
+/* Rotary frequencies. Pair i < n_rot / 2 turns by f_i per position, f_i = base^(-2 i / n_rot), scaled for
+ * contexts longer than the model was trained on:
+ *   BTF_ROPE_LINEAR  f_i / factor
+ *   BTF_ROPE_NTK     base * factor^(n_rot / (n_rot - 2)) in place of base (n_rot >= 4)
+ *   BTF_ROPE_YARN    f_i (1 - r_i) + f_i / factor * r_i with r_i = clamp((i - lo) / max(hi - lo, 0.001), 0, 1),
+ *                    lo = max(floor(d(beta_fast)), 0), hi = min(ceil(d(beta_slow)), n_rot - 1),
+ *                    d(b) = n_rot ln(orig_ctx / (2 pi b)) / (2 ln base); cos and sin times 0.1 ln(factor) + 1 */
+#define BTF_ROPE_NONE 0
+#define BTF_ROPE_LINEAR 1
+#define BTF_ROPE_NTK 2
+#define BTF_ROPE_YARN 3
+typedef struct btf_rope_cfg {
+  int n_rot;    /* rotated dims of a head, even, 2..BTF_ROPE_MAX_D */
+  int scaling;  /* BTF_ROPE_* */
+  double base;  /* > 1 */
+  double factor;               /* context stretch, >= 1 (ignored by BTF_ROPE_NONE) */
+  double beta_fast, beta_slow; /* BTF_ROPE_YARN: beta_fast >= beta_slow > 0 */
+  int orig_ctx;                /* BTF_ROPE_YARN: the trained context */
+} btf_rope_cfg;
+#define BTF_ROPE_MAX_D 1024
+/* Host only: fills turns_host[n_rot / 2] with f_i / (2 pi) and *mscale with the factor on cos and sin.
+ * The caller keeps the table on the device for btf_rope. */
+int btf_rope_table(const btf_rope_cfg* cfg, double* turns_host, float* mscale);
+
+/* One tensor [T][heads][D] of a btf_rope call; strides in elements, the D dims of a head contiguous.
+ * x and y may be the same tensor (same pointer, type and strides, rows NULL), else they must not overlap. */
+typedef struct btf_rope_seg {
+  const void* x;
+  void* y;
+  int x_type, y_type; /* BTF_F32 / BTF_F16 / BTF_BF16 */
+  int heads;          /* 0: nothing */
+  int rotate;         /* 0: norm and type conversion only (values on their way to a cache) */
+  int64_t x_token, x_head, y_token, y_head;
+  const float* normw;   /* [D]: x / sqrt(mean(x^2) + eps) * normw first (the decoder's q/k norm), or NULL */
+  const int32_t* rows;  /* [T]: token t goes to row rows[t] of y (a cache's slot), or NULL: to row t. Rows < 0
+                           or >= n_rows are not written. Rows must differ. */
+  int64_t n_rows;       /* rows of y, with rows */
+} btf_rope_seg;
+/* Rotates up to 3 tensors by their tokens' positions pos[T] in one launch: pairs (i, i + n_rot / 2) of the
+ * first n_rot dims, or (2 i, 2 i + 1) when interleaved, by pos * f_i; the other dims are copied. Angles are
+ * reduced in 64 bits, so any int32 position keeps fp32 accuracy. inverse: the transposed map, which is the
+ * gradient (normw must be NULL). 1 <= D <= BTF_ROPE_MAX_D, n_rot even, 0..D (0: turns may be NULL).
+ * Replaces the RoPE of src/emu_decoder.cpp:307-338 for many tokens and other layouts. */
+int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const double* turns, float mscale,
+             int interleaved, int inverse, float eps, const int32_t* pos, void* stream);
+
+/* Attention for a tree of drafted tokens over a cache. Sequence b has lens[b] cached tokens in rows
+ * [0, lens[b]) of k and v, and its counts[b] <= n drafted nodes' k and v in the rows behind them (node j in row
+ * lens[b] + j). Node i attends to every cached row, to itself and to its ancestors: parents[b][j] < j is the
+ * node that j hangs on, any other value hangs it on the cache (a chain 0, 1, 2, ... is causal attention).
+ *   o = sum_j softmax_j(scale * q . k_j) v_j for each of the H q-heads; q-head h reads kv-head h / (H / HK).
+ * Rows behind lens[b] + counts[b] are never part of a result whatever they hold; output rows of nodes
+ * >= counts[b] are left as they were. lens is taken as at most n_ctx - counts[b], and as at least 0. */
+typedef struct btf_tree_attn {
+  const void* q;               /* [B][n][H][D] */
+  int64_t q_batch, q_node, q_head; /* strides in elements; the D dims are contiguous */
+  const void* k;               /* [B][n_ctx][HK][D], as the decoder's caches */
+  const void* v;
+  int64_t kv_batch, kv_row, kv_head;
+  void* o;                     /* [B][n][H][D] */
+  int64_t o_batch, o_node, o_head;
+  int type;                    /* BTF_F16 or BTF_BF16: q, k, v and o */
+  int B, n, H, HK, D;          /* 1 <= n <= BTF_TREE_MAX_NODES; H % HK == 0; D % 8 == 0, 8..256 */
+  int n_ctx;                   /* rows of k and v per sequence, >= n */
+  const int32_t* lens;         /* [B] */
+  const int32_t* parents;      /* [B][n] */
+  const int32_t* counts;       /* [B], or NULL: n nodes each */
+  float scale;                 /* usually 1 / sqrt(D) */
+  void* work;                  /* btf_tree_attention_work(...) bytes, 256-byte aligned; calls that may run at the
+                                  same time need a workspace each */
+  int64_t work_bytes;
+} btf_tree_attn;
+#define BTF_TREE_MAX_NODES 64
+/* Workspace bytes of a call with these sizes on the current device (host only; -1 on bad sizes). */
+int64_t btf_tree_attention_work(int B, int n, int H, int HK, int D, int n_ctx);
+/* q, k, v and o 16-byte aligned, their strides multiples of 8 elements. */
+int btf_tree_attention(const btf_tree_attn* args, void* stream);
+
+/* Draws one token of each of B rows of logits [B][ld] (V values each) from given random numbers. Per row:
+ *   w_i = exp((l_i - max l) / temperature)  (temperature <= 0: the first largest logit, as the argmax);
+ *   order by (l descending, i ascending); keep the first top_k; of these the shortest prefix whose mass is
+ *   >= top_p times theirs; of these w_i >= min_p;
+ *   token = the first kept i, in index order, whose running mass exceeds u times the kept mass.
+ * tokens[b] gets it, logprobs[b] the log of its share of the kept mass. A NaN logit counts as -inf; a row with
+ * nothing above -inf gives token 0 and a NaN logprob. Each parameter is [B] on the device or NULL (1, off, off,
+ * off); top_k <= 0, top_p >= 1 and min_p <= 0 are off for their row. u in [0, 1). Masses are 2^-44 fixed point
+ * (coarser for V > 2^18), so results do not depend on an order of summation; V <= BTF_SAMPLE_MAX_V.
+ * Beside the greedy token of src/emu_decoder.cpp:214-217. */
+#define BTF_SAMPLE_MAX_V 524288
+int btf_sample(const void* logits, int type, int64_t ld, int B, int V, const float* u, const float* temperature,
+               const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, float* logprobs,
+               void* stream);
+
 #ifdef __cplusplus
 }
 #endif
