@@ -56,6 +56,7 @@ int gemm_wm_setup(DeviceInfo& d);
 int gemv_mma_setup(DeviceInfo& d);
 int chain_setup(DeviceInfo& d);
 int sample_setup(DeviceInfo& d);
+int tree_attn_setup(DeviceInfo& d);
 
 }  // namespace btf
 
@@ -111,7 +112,8 @@ int btf_init(int device) {
     st = BTF_OK;  // already initialised
   } else if ((st = gemv_setup(d)) == BTF_OK && (st = gemm_setup(d)) == BTF_OK && (st = gemm_wm_setup(d)) == BTF_OK &&
              (st = gemv_mma_setup(d)) == BTF_OK && (st = chain_setup(d)) == BTF_OK &&
-             (st = sample_setup(d)) == BTF_OK) {
+             (st = sample_setup(d)) == BTF_OK &&
+             (st = tree_attn_setup(d)) == BTF_OK) {
     d.ready = true;
     g_dev[device] = d;
   }
