@@ -14,7 +14,6 @@ library is missing, loading raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from dataclasses import dataclass
@@ -621,48 +620,60 @@ TREE_MAX_NODES = 64  # BTF_TREE_MAX_NODES
 SAMPLE_MAX_V = 524288  # BTF_SAMPLE_MAX_V
 
 
+_ELEM: dict = {}  # torch dtype -> element type id
+
+
 def _elem(t, what: str) -> int:
-    torch = _torch()
-    types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if t.dtype not in types:
+    if not _ELEM:
+        torch = _torch()
+        _ELEM.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    e = _ELEM.get(t.dtype)
+    if e is None:
         raise RuntimeError(f"{what}: float32, float16 or bfloat16 expected, got {t.dtype}")
-    return types[t.dtype]
+    return e
 
 
-def _same_device(what: str, dev, tensors: dict) -> None:
+def _cuda_device(what: str, t):
+    dev = t.device
     if dev.type != "cuda":
         raise RuntimeError(f"{what}: CUDA tensors expected, got one on {dev}")
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, not on {dev}")
+    return dev
 
 
-def _vector(what: str, name: str, t, dtype, shape) -> None:
-    """A parameter tensor of the call: contiguous, of this type and shape."""
-    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+def _on(what: str, dev, name: str, t) -> None:
+    if t.device != dev:
+        raise RuntimeError(f"{what}: {name} is on {t.device}, not on {dev}")
+
+
+def _vector(what: str, dev, name: str, t, dtype, shape) -> Optional[int]:
+    """Address of a parameter tensor of the call (None: null): on dev, contiguous, of this type and shape."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise RuntimeError(f"{what}: {name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} "
                            f"{tuple(t.shape)}")
+    if t.device != dev:
+        raise RuntimeError(f"{what}: {name} is on {t.device}, not on {dev}")
+    return t.data_ptr()
 
 
-@contextlib.contextmanager
-def _launching(dev, stream):
-    """The stream handle to launch on with `dev` current: dev's current stream, or `stream`, which is then current too
-    (so that what is allocated for the call belongs to it)."""
+def _launch(dev, stream, fn):
+    """fn(stream handle) with `dev` current: on dev's current stream, or on `stream`, which is then current too (so
+    that what fn allocates belongs to it)."""
     torch = _torch()
-    ensure_init(dev.index)
+    if dev.index not in _initialised:
+        ensure_init(dev.index)
     if stream is None:
         if torch.cuda.current_device() == dev.index:
-            yield torch.cuda.current_stream(dev).cuda_stream
-            return
+            return fn(torch._C._cuda_getCurrentRawStream(dev.index))
         with torch.cuda.device(dev):
-            yield torch.cuda.current_stream(dev).cuda_stream
-        return
+            return fn(torch.cuda.current_stream(dev).cuda_stream)
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
     if stream.device != dev:
         raise RuntimeError(f"a stream of {stream.device} for tensors on {dev}")
     with torch.cuda.stream(stream):
-        yield stream.cuda_stream
+        return fn(stream.cuda_stream)
 
 
 def _strides(t) -> list:
@@ -705,42 +716,56 @@ def rope(segs: Sequence[RopeSeg], table: RopeTable, pos, inverse: bool = False, 
     """Rotates up to 3 tensors of the same tokens by their positions pos [T] (int32) in one launch (btf_rope).
     inverse: the transposed map, the gradient of the rotation."""
     torch = _torch()
-    if not 1 <= len(segs) <= 3:
-        raise RuntimeError(f"rope: 1..3 tensors expected, got {len(segs)}")
-    T, D, dev = segs[0].x.shape[0], segs[0].x.shape[-1], segs[0].x.device
-    arr = (RopeSegC * len(segs))()
-    for i, s in enumerate(segs):
-        y = s.x if s.y is None else s.y
-        if s.x.dim() != 3 or y.dim() != 3 or s.x.shape[0] != T or s.x.shape[2] != D or y.shape[1:] != s.x.shape[1:]:
-            raise RuntimeError(f"rope: x [T][heads][D] and y [rows][heads][D] expected, got {tuple(s.x.shape)} and "
-                               f"{tuple(y.shape)}")
-        if s.rows is None and y.shape[0] != T:
-            raise RuntimeError(f"rope: y has {y.shape[0]} rows for {T} tokens")
-        if D > 1 and (s.x.stride(2) != 1 or y.stride(2) != 1):
+    n = len(segs)
+    if not 1 <= n <= 3:
+        raise RuntimeError(f"rope: 1..3 tensors expected, got {n}")
+    x0 = segs[0].x
+    T, D, dev = x0.shape[0], x0.shape[-1], _cuda_device("rope", x0)
+    i32 = torch.int32
+    arr = (RopeSegC * n)()
+    for s, a in zip(segs, arr):
+        x, y = s.x, s.x if s.y is None else s.y
+        xs, ys = x.shape, y.shape
+        if len(xs) != 3 or len(ys) != 3 or xs[0] != T or xs[2] != D or ys[1:] != xs[1:]:
+            raise RuntimeError(f"rope: x [T][heads][D] and y [rows][heads][D] expected, got {tuple(xs)} and {tuple(ys)}")
+        if s.rows is None and ys[0] != T:
+            raise RuntimeError(f"rope: y has {ys[0]} rows for {T} tokens")
+        _on("rope", dev, "x", x)
+        _on("rope", dev, "y", y)
+        a.x_token, a.x_head, xd = x.stride()
+        a.y_token, a.y_head, yd = y.stride()
+        if D > 1 and (xd != 1 or yd != 1):
             raise RuntimeError("rope: the dims of a head must be contiguous")
-        _same_device("rope", dev, {"x": s.x, "y": y, "normw": s.normw, "rows": s.rows})
-        _vector("rope", "normw", s.normw, torch.float32, (D,))
-        _vector("rope", "rows", s.rows, torch.int32, (T,))
-        xs, ys = _strides(s.x), _strides(y)
-        arr[i] = RopeSegC(_ptr(s.x), _ptr(y), _elem(s.x, "rope"), _elem(y, "rope"), s.x.shape[1], int(s.rotate), xs[0],
-                          xs[1], ys[0], ys[1], _ptr(s.normw), _ptr(s.rows), y.shape[0])
-    _same_device("rope", dev, {"pos": pos, "table": table.turns})
-    _vector("rope", "pos", pos, torch.int32, (T,))
-    with _launching(dev, stream) as st:
-        check(lib().btf_rope(arr, len(segs), T, D, table.n_rot, _ptr(table.turns), table.mscale, int(table.interleaved),
-                             int(inverse), eps, _ptr(pos), st), "btf_rope")
+        if xs[1] == 1:  # strides of dims with one entry do not matter
+            a.x_head = a.y_head = 0
+        if T == 1:
+            a.x_token = 0
+        if ys[0] == 1:
+            a.y_token = 0
+        a.x, a.y, a.x_type, a.y_type = x.data_ptr(), y.data_ptr(), _elem(x, "rope"), _elem(y, "rope")
+        a.heads, a.rotate, a.n_rows = xs[1], s.rotate, ys[0]
+        if s.normw is not None:
+            a.normw = _vector("rope", dev, "normw", s.normw, torch.float32, (D,))
+        if s.rows is not None:
+            a.rows = _vector("rope", dev, "rows", s.rows, i32, (T,))
+    pos_ptr = _vector("rope", dev, "pos", pos, i32, (T,))
+    _on("rope", dev, "table", table.turns)
+    _launch(dev, stream, lambda st: check(
+        lib().btf_rope(arr, n, T, D, table.n_rot, table.turns.data_ptr(), table.mscale, table.interleaved, inverse, eps,
+                       pos_ptr, st), "btf_rope"))
 
 
 def tree_attention_work(q, k):
     """A workspace for tree_attention calls of these shapes (q [B][n][H][D], k [B][n_ctx][HK][D]). Calls that may
     run at the same time need one each."""
+    torch = _torch()
     B, n, H, D = q.shape
-    ensure_init(q.device.index)
-    with _torch().cuda.device(q.device):
+    ensure_init(_cuda_device("tree_attention_work", q).index)
+    with torch.cuda.device(q.device):
         size = lib().btf_tree_attention_work(B, n, H, k.shape[2], D, k.shape[1])
     if size < 0:
         check(1, "btf_tree_attention_work")
-    return _torch().empty(size, dtype=_torch().uint8, device=q.device)
+    return torch.empty(size, dtype=torch.uint8, device=q.device)
 
 
 def tree_attention(q, k, v, lens, parents, counts=None, scale: Optional[float] = None, out=None, work=None,
@@ -749,33 +774,44 @@ def tree_attention(q, k, v, lens, parents, counts=None, scale: Optional[float] =
     [B][n_ctx][HK][D] hold lens[b] cached tokens and the nodes behind them; node i sees the cache, itself and its
     ancestors by parents [B][n] (int32, -1: hangs on the cache). counts [B]: nodes of each sequence (None: n)."""
     torch = _torch()
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise RuntimeError(f"tree_attention: q [B][n][H][D] and k, v [B][n_ctx][HK][D] expected, got {tuple(q.shape)}, "
-                           f"{tuple(k.shape)}, {tuple(v.shape)}")
-    B, n, H, D = q.shape
-    dev = q.device
-    _same_device("tree_attention", dev, {"k": k, "v": v, "lens": lens, "parents": parents, "counts": counts, "out": out,
-                                         "work": work})
-    _vector("tree_attention", "lens", lens, torch.int32, (B,))
-    _vector("tree_attention", "parents", parents, torch.int32, (B, n))
-    _vector("tree_attention", "counts", counts, torch.int32, (B,))
-    with _launching(dev, stream) as st:
-        if out is None:
-            out = (torch.empty if counts is None else torch.zeros)((B, n, H, D), dtype=q.dtype, device=dev)
-        if out.shape != q.shape or k.dtype != q.dtype or v.dtype != q.dtype or out.dtype != q.dtype:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[0] != qs[0] or ks[3] != qs[3]:
+        raise RuntimeError(f"tree_attention: q [B][n][H][D] and k, v [B][n_ctx][HK][D] expected, got {tuple(qs)}, "
+                           f"{tuple(ks)}, {tuple(v.shape)}")
+    B, n, H, D = qs
+    dev, dtype, i32 = _cuda_device("tree_attention", q), q.dtype, torch.int32
+    _on("tree_attention", dev, "k", k)
+    _on("tree_attention", dev, "v", v)
+    a = TreeAttnC()
+    a.lens = _vector("tree_attention", dev, "lens", lens, i32, (B,))
+    a.parents = _vector("tree_attention", dev, "parents", parents, i32, (B, n))
+    if counts is not None:
+        a.counts = _vector("tree_attention", dev, "counts", counts, i32, (B,))
+
+    def call(st):
+        o = out
+        if o is None:
+            o = (torch.empty if counts is None else torch.zeros)(qs, dtype=dtype, device=dev)
+        if o.shape != qs or k.dtype != dtype or v.dtype != dtype or o.dtype != dtype:
             raise RuntimeError("tree_attention: q, k, v and out must have one type, and out the shape of q")
-        qs, ks, vs, os_ = _strides(q), _strides(k), _strides(v), _strides(out)
-        if any(t.stride(3) != 1 for t in (q, k, v, out)) or ks != vs:
+        _on("tree_attention", dev, "out", o)
+        a.q_batch, a.q_node, a.q_head, qd = _strides(q)
+        a.kv_batch, a.kv_row, a.kv_head, kd = kv = _strides(k)
+        a.o_batch, a.o_node, a.o_head, od = _strides(o)
+        if kv != _strides(v) or (D > 1 and not qd == kd == od == 1):
             raise RuntimeError("tree_attention: the dims of a head must be contiguous, and k and v strided alike")
         if B == 0:
-            return out
-        if work is None:
-            work = tree_attention_work(q, k)
-        a = TreeAttnC(_ptr(q), *qs[:3], _ptr(k), _ptr(v), *ks[:3], _ptr(out), *os_[:3], _elem(q, "tree_attention"), B, n,
-                      H, k.shape[2], D, k.shape[1], _ptr(lens), _ptr(parents), _ptr(counts),
-                      D ** -0.5 if scale is None else scale, _ptr(work), work.numel() * work.element_size())
+            return o
+        w = tree_attention_work(q, k) if work is None else work
+        _on("tree_attention", dev, "work", w)
+        a.q, a.k, a.v, a.o, a.work = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), w.data_ptr()
+        a.type, a.B, a.n, a.H, a.HK, a.D, a.n_ctx = _elem(q, "tree_attention"), B, n, H, ks[2], D, ks[1]
+        a.scale = D ** -0.5 if scale is None else scale
+        a.work_bytes = w.numel() * w.element_size()
         check(lib().btf_tree_attention(ctypes.byref(a), st), "btf_tree_attention")
-    return out
+        return o
+
+    return _launch(dev, stream, call)
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprobs=None, stream=None):
@@ -785,22 +821,23 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise RuntimeError("sample: logits [B][V] with contiguous rows expected")
     B, V = logits.shape
-    dev = logits.device
-    params = {"u": (u, torch.float32), "temperature": (temperature, torch.float32), "top_k": (top_k, torch.int32),
-              "top_p": (top_p, torch.float32), "min_p": (min_p, torch.float32), "tokens": (tokens, torch.int32),
-              "logprobs": (logprobs, torch.float32)}
-    _same_device("sample", dev, {n: t for n, (t, _) in params.items()})
-    for name, (t, dtype) in params.items():
-        _vector("sample", name, t, dtype, (B,))
-    with _launching(dev, stream) as st:
-        if tokens is None:
-            tokens = torch.empty(B, dtype=torch.int32, device=dev)
-        if logprobs is None:
-            logprobs = torch.empty(B, dtype=torch.float32, device=dev)
-        ld = logits.stride(0) if B > 1 else V
-        check(lib().btf_sample(_ptr(logits), _elem(logits, "sample"), ld, B, V, _ptr(u), _ptr(temperature), _ptr(top_k),
-                               _ptr(top_p), _ptr(min_p), _ptr(tokens), _ptr(logprobs), st), "btf_sample")
-    return tokens, logprobs
+    dev, f32, i32, rows = _cuda_device("sample", logits), torch.float32, torch.int32, (B,)
+    pu = _vector("sample", dev, "u", u, f32, rows)
+    pt = _vector("sample", dev, "temperature", temperature, f32, rows)
+    pk = _vector("sample", dev, "top_k", top_k, i32, rows)
+    pp = _vector("sample", dev, "top_p", top_p, f32, rows)
+    pm = _vector("sample", dev, "min_p", min_p, f32, rows)
+    ld = logits.stride(0) if B > 1 else V
+
+    def call(st):
+        tok = torch.empty(B, dtype=i32, device=dev) if tokens is None else tokens
+        lp = torch.empty(B, dtype=f32, device=dev) if logprobs is None else logprobs
+        check(lib().btf_sample(logits.data_ptr(), _elem(logits, "sample"), ld, B, V, pu, pt, pk, pp, pm,
+                               _vector("sample", dev, "tokens", tok, i32, rows),
+                               _vector("sample", dev, "logprobs", lp, f32, rows), st), "btf_sample")
+        return tok, lp
+
+    return _launch(dev, stream, call)
 
 
 PTQ1_0 = 143
