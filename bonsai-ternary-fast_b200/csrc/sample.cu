@@ -1,13 +1,15 @@
 // Sampling from given random numbers (btf_sample): temperature, top-k, top-p and
-// min-p on one row of logits per thread-block cluster.
+// min-p on one row of logits per thread-block cluster, whose shared memory holds the
+// row: the logits are read once.
 //
 // All three filters keep a prefix of the order (logit descending, index
-// ascending), so the kept set is one cut (key, index) in that order plus a bound
-// on the exponent, and nothing is sorted. A cut is found by a histogram over
-// 2048 bins of (max - l) / T, then, inside the one bin that it falls in, by the
-// exact order of the bin's few elements (or by further histograms over the bits
-// of their keys, when there are many). The token comes from a walk over running
-// masses in index order.
+// ascending), so nothing is sorted: a cut (key, index) in that order plus a bound on
+// the exponent is the kept set. A cut is found by a histogram over 2048 bins of
+// (max - l) / T. When the bins down to the cut's hold few elements (a top-k of 50, a
+// peaked nucleus), those go to the cluster's first CTA, which ranks them exactly and
+// finishes the row. Else the elements of the cut's own bin are ranked (or, when there
+// are many, split further by the bits of their keys), and the token comes from a
+// walk over running masses in index order, each CTA over its own part of the row.
 //
 // Masses are 64-bit integers, w = rint(exp((l - max) / T) 2^S): sums are exact in
 // any order, so the CTAs of a cluster, the histogram and the final walk agree on
@@ -27,14 +29,14 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kCand = 256;     // elements of a bin resolved by their exact order
+constexpr int kCand = 512;     // elements that one CTA ranks exactly, one per thread
 constexpr int kMaxCluster = 16;
 constexpr float kSpan = 32.0f;  // exponents below -kSpan have mass 0: e^-32 < 2^-46
 
 struct SampleParams {
   const void* x;
   int64_t ld;
-  int type, V, chunk, S;
+  int type, V, chunk, S;  // chunk: logits per CTA, a multiple of 4 x kThreads
   const float *u, *temp, *top_p, *min_p;
   const int32_t* top_k;
   int32_t *tok, *tok2;
@@ -42,6 +44,7 @@ struct SampleParams {
 };
 
 // Order-preserving key of a logit: larger key, larger logit; -0 as +0, NaN as -inf.
+// Key 0 is no logit (what pads a chunk).
 constexpr uint32_t kNegInf = 0x007fffffu;
 __device__ __forceinline__ uint32_t key_of(float v) {
   if (v != v) return kNegInf;
@@ -73,15 +76,19 @@ __device__ __forceinline__ void cluster_barrier() {
 }
 
 struct Shared {
-  uint32_t cnt[kBins];
-  uint32_t mass[3][kBins];  // 16-bit limbs of the bins' masses (a CTA holds at most 2^16 elements)
   uint64_t slot[2][kMaxCluster][2];  // values that the CTAs send one another, in turn
+  uint64_t total[kMaxCluster];       // each CTA's part of a histogram's total
   uint64_t warp[kWarps][2];
-  uint64_t found[2];      // what this CTA found for the others to read
-  uint64_t result[4];
-  uint32_t ckey[kCand], cidx[kCand];
+  uint64_t found[2];
+  double exp2_64[64];  // 2^(i / 64)
   uint64_t cmass[kCand];
+  uint32_t ckey[kCand], cidx[kCand];
   uint32_t ncand;
+};
+// The histograms: counts, and the bins' masses in 16-bit limbs (a CTA holds at most 2^16 elements).
+struct Hist {
+  uint32_t cnt[kBins];
+  uint32_t mass[3][kBins];
 };
 
 // One row's state, the same in every thread of the cluster.
@@ -91,21 +98,38 @@ struct Row {
   double m, inv_t;  // the largest logit and 1 / T
   float bin_scale;
   double min_e;     // min-p: exponents below are dropped
+  float min_bin;    // a bound on their place among the bins, with room for rounding
   int S;
   uint32_t cut_key, cut_idx;  // kept: key > cut_key, or == and idx <= cut_idx
+  const double* table;
+
   __device__ __forceinline__ double exponent(uint32_t key) const {
-    return key == top ? 0.0 : ((double)key_value(key) - m) * inv_t;  // NaN for -inf at an infinite T
+    return key == top ? 0.0 : ((double)key_value(key) - m) * inv_t;
   }
-  __device__ __forceinline__ bool alive(uint32_t key) const { return exponent(key) > -(double)kSpan; }
-  __device__ __forceinline__ uint64_t weight_of(double e) const { return (uint64_t)rint(exp(e) * (double)(1ull << S)); }
+  // (max - l) / T in bins: fp32 subtraction and product are monotone, so it follows the order. At least kBins, or
+  // NaN, has no mass.
+  __device__ __forceinline__ float place(uint32_t key) const {
+    return key == top ? 0.0f : (top_value - key_value(key)) * bin_scale;
+  }
+  // rint(2^S e^x) for -33 < x <= 0 by a table of 2^(i / 64) and the Taylor polynomial of the rest (Tang's method):
+  // x = n ln2 / 64 + r, |r| <= ln2 / 128, e^r to r^5 / 120 (the rest below 2^-54), in all within 2^-48 relative.
+  __device__ __forceinline__ uint64_t weight_of(double x) const {
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+    const double big = fma(x, 92.332482616893656877, kRound);  // 64 / ln 2
+    const int n = __double2loint(big);
+    const double r = fma(big - kRound, -0.010830424696249145, x);  // ln 2 / 64
+    double p = fma(r, 1.0 / 120, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    const double t = table[n & 63];
+    const double scaled = __hiloint2double(__double2hiint(t) + (((n >> 6) + S) << 20), __double2loint(t));
+    // w <= 2^44: the low bits of w + 1.5 * 2^52 are w rounded
+    return (uint64_t)__double_as_longlong(fma(scaled, p, kRound)) & ((1ull << 51) - 1);
+  }
   __device__ __forceinline__ uint64_t weight(uint32_t key) const {
-    const double e = exponent(key);
-    return e > -(double)kSpan ? weight_of(e) : 0ull;
-  }
-  // Bin of an element that is alive: fp32 subtraction and product are monotone, so bins follow the order.
-  __device__ __forceinline__ int bin(uint32_t key) const {
-    if (key == top) return 0;
-    return min(kBins - 1, (int)((top_value - key_value(key)) * bin_scale));
+    return place(key) < (float)kBins ? weight_of(exponent(key)) : 0ull;
   }
   __device__ __forceinline__ bool inside(uint32_t key, uint32_t idx) const {
     return key > cut_key || (key == cut_key && idx <= cut_idx);
@@ -114,9 +138,10 @@ struct Row {
 
 struct Cluster {
   Shared& sh;
+  Hist& hist;
   int rank, size, turn;
   __device__ __forceinline__ uint32_t at(const void* p, int r) const { return mapa_shared(smem_u32(p), r); }
-  // Every CTA sends (a, b) (its thread 0's) to all; on return slots() holds all of them. All threads call.
+  // Every CTA sends (a, b) to all; on return slots() holds all of them. All threads call.
   __device__ __forceinline__ const uint64_t (*exchange(uint64_t a, uint64_t b))[2] {
     const int t = turn;
     turn ^= 1;
@@ -131,20 +156,17 @@ struct Cluster {
   }
 };
 
-// Block sum of two values; every thread gets the totals.
-__device__ __forceinline__ void block_sum2(Shared& sh, uint64_t& a, uint64_t& b) {
+// Block sum; every thread gets it.
+__device__ __forceinline__ uint64_t block_sum(Shared& sh, uint64_t a) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
+  for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5][0] = a, sh.warp[threadIdx.x >> 5][1] = b;
+  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5][0] = a;
   __syncthreads();
-  a = b = 0;
-  for (int i = 0; i < kWarps; ++i) a += sh.warp[i][0], b += sh.warp[i][1];
+  a = 0;
+  for (int i = 0; i < kWarps; ++i) a += sh.warp[i][0];
+  return a;
 }
-
 // Exclusive block scan of a value in thread order; the total in *total.
 __device__ __forceinline__ uint64_t block_scan(Shared& sh, uint64_t v, uint64_t* total) {
   uint64_t inc = v;
@@ -166,153 +188,232 @@ __device__ __forceinline__ uint64_t block_scan(Shared& sh, uint64_t v, uint64_t*
   return before + inc - v;
 }
 
-// The bins' values: counts, or masses from their limbs, summed over the cluster.
+// fn(key, position in the chunk) for this thread's keys, four neighbours at a time
+template <typename Fn>
+__device__ __forceinline__ void each_key(const uint32_t* keys, int n4, Fn fn) {
+#pragma unroll 2
+  for (int i = threadIdx.x; i < n4; i += kThreads) {
+    const uint4 k = reinterpret_cast<const uint4*>(keys)[i];
+    fn(k.x, 4 * i);
+    fn(k.y, 4 * i + 1);
+    fn(k.z, 4 * i + 2);
+    fn(k.w, 4 * i + 3);
+  }
+}
+
+__device__ __forceinline__ void clear_hist(Hist& h, bool mass) {
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    h.cnt[b] = 0;
+    if (mass) h.mass[0][b] = h.mass[1][b] = h.mass[2][b] = 0;
+  }
+}
+
+// A bin's value over the whole cluster: its count, or its mass.
 template <bool MASS>
 __device__ __forceinline__ uint64_t bin_value(const Cluster& c, int b) {
   uint64_t v = 0;
+#pragma unroll 4
   for (int r = 0; r < c.size; ++r) {
+    const uint32_t base = c.at(&c.hist, r) + b * 4;
     if (MASS)
-      v += (uint64_t)ld_cluster_u32(c.at(&c.sh.mass[0][b], r)) + ((uint64_t)ld_cluster_u32(c.at(&c.sh.mass[1][b], r)) << 16) +
-           ((uint64_t)ld_cluster_u32(c.at(&c.sh.mass[2][b], r)) << 32);
+      v += (uint64_t)ld_cluster_u32(base + 4 * kBins) + ((uint64_t)ld_cluster_u32(base + 8 * kBins) << 16) +
+           ((uint64_t)ld_cluster_u32(base + 12 * kBins) << 32);
     else
-      v += ld_cluster_u32(c.at(&c.sh.cnt[b], r));
+      v += ld_cluster_u32(base);
   }
   return v;
 }
 
-// The cut of the shortest prefix whose value (count, or mass) reaches a goal.
-// GOAL(total) gives the goal from the value of everything inside the present cut
-// and returns 0 to leave the cut alone. All threads of the cluster call it, and
-// every branch below is the same for all of them.
-template <bool MASS, typename Goal>
-__device__ void select(Cluster& c, Row& row, const uint32_t* keys, int n, uint32_t idx0, Goal goal_of) {
+__device__ __forceinline__ uint64_t goal_of_u(float uf, uint64_t z) {
+  const double u = (double)uf, g = u > 0.0 ? u * (double)z : 0.0;
+  return g < (double)z ? min((uint64_t)g, z - 1) : z - 1;
+}
+__device__ __forceinline__ void put_token(const SampleParams& p, int b, const Row& row, uint32_t key, uint32_t idx,
+                                          uint64_t z) {
+  p.tok[b] = (int32_t)idx;
+  if (p.tok2) p.tok2[b] = (int32_t)idx;
+  if (p.logprob) p.logprob[b] = (float)(row.exponent(key) - log((double)z / (double)(1ull << row.S)));
+}
+
+// The share of `total` that top-p keeps, rounded up: the prefix ends with the element that reaches it.
+__device__ __forceinline__ uint64_t goal_of_p(float p, uint64_t total) {
+  const double g = ceil((double)p * (double)total);
+  return g < 1.0 ? 1ull : (uint64_t)g < total ? (uint64_t)g : total;
+}
+
+// The cluster's first CTA finishes a row from its list of candidates, which holds
+// every element down to the cut: one per thread, against all others. k: elements to
+// keep; goal: mass to reach, or with RANKED top_p of the first k's.
+template <bool RANKED>
+__device__ void finish(Shared& sh, const SampleParams& p, int b, const Row& row, uint64_t k, uint64_t goal, float top_p) {
+  const int tid = threadIdx.x, n = (int)sh.ncand;
+  const bool mine = tid < n;
+  const uint32_t key = mine ? sh.ckey[tid] : 0, idx = mine ? sh.cidx[tid] : 0;
+  const uint64_t w = mine ? row.weight(key) : 0;
+  if (mine) sh.cmass[tid] = w;
+  __syncthreads();
+  uint64_t before = 0;
+  uint32_t rank = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const uint32_t kj = sh.ckey[j];
+    if (kj > key || (kj == key && sh.cidx[j] < idx)) {
+      before += sh.cmass[j];
+      ++rank;
+    }
+  }
+  bool keep = mine && w > 0;
+  if (RANKED) {
+    keep = keep && rank < k;
+    const uint64_t zk = block_sum(sh, keep ? w : 0);
+    goal = top_p < 1.0f ? goal_of_p(top_p, zk) : zk;
+  }
+  keep = keep && before < goal && row.exponent(key) >= row.min_e;
+  __syncthreads();
+  if (mine) sh.cmass[tid] = keep ? w : 0;
+  const uint64_t z = block_sum(sh, keep ? w : 0);  // (its barriers publish cmass)
+  const uint64_t g = goal_of_u(p.u[b], z);
+  uint64_t run = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j)
+    if (sh.cidx[j] < idx) run += sh.cmass[j];
+  if (keep && run <= g && g < run + w) put_token(p, b, row, key, idx, z);
+}
+
+// The cut of the shortest prefix whose value (its count: top-k; its mass: top-p)
+// reaches a goal: k, or top_p of the mass inside the present cut. True when the row
+// is finished. All threads of the cluster call it, and every branch on the way to a
+// barrier is the same for all of them.
+template <bool MASS>
+__device__ bool select(Cluster& c, const SampleParams& p, int row_b, Row& row, const uint32_t* keys, int n4,
+                       uint32_t idx0, uint64_t k, float top_p) {
   Shared& sh = c.sh;
-  const int tid = threadIdx.x, per = kBins / c.size, each = (per + kThreads - 1) / kThreads;
-  uint64_t before = 0, goal = 0;  // the value of what lies above the range; the goal
+  Hist& h = c.hist;
+  const int tid = threadIdx.x;
+  uint64_t before = 0, goal = 0;      // the value of what lies above the range; the goal
   uint32_t lo = 0, hi = 0xffffffffu;  // keys of the range, inclusive
   int shift = 0;
-  bool first = true;                  // the first histogram is over the bins of Row::bin
+  bool first = true;  // the first histogram is over Row::place (it was cleared by the caller)
   // bin of an element of the range, or -1
   auto bin_of = [&](uint32_t key, uint32_t idx) -> int {
-    if (!row.inside(key, idx) || !row.alive(key)) return -1;
-    if (first) return row.bin(key);
-    if (key < lo || key > hi) return -1;
-    return (int)((hi - key) >> shift);
+    const float at = row.place(key);
+    if (!(at < (float)kBins) || !row.inside(key, idx)) return -1;
+    if (first) return (int)at;
+    return key < lo || key > hi ? -1 : (int)((hi - key) >> shift);
   };
   for (int pass = 0; pass < 6; ++pass) {  // at most 4 are needed: 2048 bins, then 11 bits of the key each
-    __syncthreads();
-    for (int b = tid; b < kBins; b += kThreads) {
-      sh.cnt[b] = 0;
-      if (MASS) sh.mass[0][b] = sh.mass[1][b] = sh.mass[2][b] = 0;
-    }
-    if (tid == 0) sh.ncand = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kThreads) {
-      const int b = bin_of(keys[i], idx0 + i);
-      if (b < 0) continue;
-      atomicAdd(&sh.cnt[b], 1u);
+    uint64_t sum = 0;
+    each_key(keys, n4, [&](uint32_t key, int i) {
+      const int b = bin_of(key, idx0 + i);
+      if (b < 0) return;
+      atomicAdd(&h.cnt[b], 1u);
       if (MASS) {
-        const uint64_t w = row.weight(keys[i]);
-        atomicAdd(&sh.mass[0][b], (uint32_t)(w & 0xffffu));
-        atomicAdd(&sh.mass[1][b], (uint32_t)((w >> 16) & 0xffffu));
-        atomicAdd(&sh.mass[2][b], (uint32_t)(w >> 32));
+        const uint64_t w = row.weight_of(row.exponent(key));
+        atomicAdd(&h.mass[0][b], (uint32_t)(w & 0xffffu));
+        atomicAdd(&h.mass[1][b], (uint32_t)((w >> 16) & 0xffffu));
+        atomicAdd(&h.mass[2][b], (uint32_t)(w >> 32));
+        sum += w;
+      } else {
+        ++sum;
       }
+    });
+    if (first) {
+      sum = block_sum(sh, sum);
+      if (tid < c.size) st_cluster_u64(c.at(&sh.total[c.rank], tid), sum);
+      if (tid == 0) sh.ncand = 0;
     }
     __syncthreads();
     cluster_barrier();
-    // this CTA's slice of the bins, each thread `each` bins in order
-    uint64_t mine = 0;
-    const int s0 = c.rank * per;
-    for (int e = 0; e < each; ++e) {
-      const int b = tid * each + e;
-      if (b < per) mine += bin_value<MASS>(c, s0 + b);
-    }
-    uint64_t slice;
-    const uint64_t pre = block_scan(sh, mine, &slice);
-    const auto slots = c.exchange(slice, 0);
-    uint64_t total = 0, above = before;
-    for (int r = 0; r < c.size; ++r) {
-      if (r < c.rank) above += slots[r][0];
-      total += slots[r][0];
-    }
     if (first) {
-      goal = goal_of(total);
-      if (goal == 0) return;  // (the same in every thread of the cluster)
-    }
-    // the thread whose bins the goal falls in finds the bin
-    if (tid == 0) sh.found[0] = ~0ull;
-    __syncthreads();
-    uint64_t run = above + pre;
-    if (run < goal && goal <= run + mine) {
-      for (int e = 0; e < each; ++e) {
-        const int b = s0 + tid * each + e;
-        const uint64_t v = bin_value<MASS>(c, b);
-        if (run < goal && goal <= run + v) {
-          sh.found[0] = ((uint64_t)b << 32) | (uint32_t)bin_value<false>(c, b);
-          sh.found[1] = run;
-        }
-        run += v;
+      uint64_t total = 0;
+      for (int r = 0; r < c.size; ++r) total += sh.total[r];
+      goal = MASS ? goal_of_p(top_p, total) : k;
+      if (goal > total || (!MASS && goal == total)) {  // nothing to cut off
+        cluster_barrier();  // (sh.total is read before it is written again)
+        return false;
       }
     }
-    __syncthreads();
-    const auto got = c.exchange(sh.found[0], sh.found[1]);
+    // every CTA finds the bin for itself, a thread per bin from the largest on
     int bin = 0;
     uint32_t count = 0;
-    for (int r = 0; r < c.size; ++r)
-      if (got[r][0] != ~0ull) {
-        bin = (int)(got[r][0] >> 32);
-        count = (uint32_t)got[r][0];
-        before = got[r][1];
+    for (int b0 = 0;; b0 += kThreads) {
+      const uint64_t v = bin_value<MASS>(c, b0 + tid);
+      uint64_t all;
+      const uint64_t pre = before + block_scan(sh, v, &all);
+      if (pre < goal && goal <= pre + v) {
+        sh.found[0] = ((uint64_t)(b0 + tid) << 32) | (uint32_t)bin_value<false>(c, b0 + tid);
+        sh.found[1] = pre;
       }
-    const bool single = !first && shift == 0;  // every element of the bin has the same key
-    if (count <= (uint32_t)kCand) {
-      // the bin's elements to CTA 0, which puts them in their exact order
-      for (int i = tid; i < n; i += kThreads) {
-        if (bin_of(keys[i], idx0 + i) != bin) continue;
-        const uint32_t at = atom_cluster_inc(c.at(&sh.ncand, 0));
-        if (at >= (uint32_t)kCand) continue;
-        st_cluster_b32(c.at(&sh.ckey[at], 0), keys[i]);
-        st_cluster_b32(c.at(&sh.cidx[at], 0), idx0 + i);
+      __syncthreads();
+      if (goal <= before + all || b0 + kThreads >= kBins) break;
+      before += all;
+    }
+    bin = (int)(sh.found[0] >> 32);
+    count = (uint32_t)sh.found[0];
+    before = sh.found[1];
+    // few elements down to this bin: the first CTA ranks them and finishes the row
+    uint64_t down = ~0ull;
+    if (first) {
+      if (!MASS) {
+        down = before + count;
+      } else {
+        uint64_t part = 0;
+        for (int b = tid; b < bin; b += kThreads) part += bin_value<false>(c, b);
+        down = block_sum(sh, part) + count;
       }
+    }
+    if (down <= (uint64_t)kCand || count <= (uint32_t)kCand) {
+      const bool all = down <= (uint64_t)kCand;
+      const uint32_t n_at = c.at(&sh.ncand, 0), key_at = c.at(sh.ckey, 0), idx_at = c.at(sh.cidx, 0);
+      each_key(keys, n4, [&](uint32_t key, int i) {
+        const int b = bin_of(key, idx0 + i);
+        if (b < 0 || (all ? b > bin : b != bin)) return;
+        const uint32_t at = atom_cluster_inc(n_at);
+        if (at >= (uint32_t)kCand) return;
+        st_cluster_b32(key_at + at * 4, key);
+        st_cluster_b32(idx_at + at * 4, idx0 + i);
+      });
       cluster_barrier();
+      if (all) {
+        if (c.rank == 0) finish<!MASS>(sh, p, row_b, row, k, goal, top_p);
+        return true;
+      }
       if (c.rank == 0) {
-        const int m = (int)min(count, (uint32_t)kCand);
-        for (int i = tid; i < m; i += kThreads) sh.cmass[i] = MASS ? row.weight(sh.ckey[i]) : 1ull;
+        const int m = (int)min(sh.ncand, (uint32_t)kCand);
+        if (tid < m) sh.cmass[tid] = MASS ? row.weight(sh.ckey[tid]) : 1ull;
         if (tid == 0) sh.found[0] = sh.found[1] = 0;
         __syncthreads();
-        // two threads per element: the value of what precedes it in the bin
-        const int i = tid >> 1;
-        uint64_t v = 0;
-        if (i < m) {
-          const uint32_t ki = sh.ckey[i], xi = sh.cidx[i];
-          for (int j = tid & 1; j < m; j += 2) {
+        if (tid < m) {
+          const uint32_t ki = sh.ckey[tid], xi = sh.cidx[tid];
+          uint64_t v = before;
+#pragma unroll 4
+          for (int j = 0; j < m; ++j) {
             const uint32_t kj = sh.ckey[j];
             if (kj > ki || (kj == ki && sh.cidx[j] < xi)) v += sh.cmass[j];
           }
-        }
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        if (i < m && (tid & 1) == 0 && before + v < goal && goal <= before + v + sh.cmass[i]) {
-          sh.found[0] = sh.ckey[i];
-          sh.found[1] = sh.cidx[i];
+          if (v < goal && goal <= v + sh.cmass[tid]) {
+            sh.found[0] = ki;
+            sh.found[1] = xi;
+          }
         }
         __syncthreads();
       }
       const auto cut = c.exchange(sh.found[0], sh.found[1]);
       row.cut_key = (uint32_t)cut[0][0];
       row.cut_idx = (uint32_t)cut[0][1];
-      return;
+      return false;
     }
-    if (single) {
+    if (!first && shift == 0) {
       // many equal keys: the goal's place among them, in index order
       const uint32_t key = hi - bin;
       const uint64_t g = MASS ? row.weight(key) : 1ull;
       const uint64_t need = (goal - before + g - 1) / g;  // ties to keep, >= 1
-      uint64_t ties = 0, unused = 0;
-      const int blk = (n + kThreads - 1) / kThreads, i0 = min(n, tid * blk), i1 = min(n, i0 + blk);
+      uint64_t ties = 0;
+      const int blk = (n4 + kThreads - 1) / kThreads * 4, i0 = min(4 * n4, tid * blk), i1 = min(4 * n4, i0 + blk);
       for (int i = i0; i < i1; ++i) ties += keys[i] == key && row.inside(key, idx0 + i);
       uint64_t all;
       const uint64_t tpre = block_scan(sh, ties, &all);
-      const auto tslots = c.exchange(all, unused);
+      const auto tslots = c.exchange(all, 0);
       uint64_t tb = tpre;
       for (int r = 0; r < c.rank; ++r) tb += tslots[r][0];
       if (tid == 0) sh.found[0] = ~0ull;
@@ -328,19 +429,21 @@ __device__ void select(Cluster& c, Row& row, const uint32_t* keys, int n, uint32
           row.cut_key = key;
           row.cut_idx = (uint32_t)cut[r][0];
         }
-      return;
+      return false;
     }
+    // many elements of unlike keys: another histogram over the range of the bin's keys
     if (first) {
-      // the bin's keys: their least and greatest bound the next histogram
       uint32_t kmin = 0xffffffffu, kmax = 0;
-      for (int i = tid; i < n; i += kThreads)
-        if (bin_of(keys[i], idx0 + i) == bin) kmin = min(kmin, keys[i]), kmax = max(kmax, keys[i]);
+      each_key(keys, n4, [&](uint32_t key, int i) {
+        if (bin_of(key, idx0 + i) == bin) kmin = min(kmin, key), kmax = max(kmax, key);
+      });
       kmin = __reduce_min_sync(0xffffffffu, kmin);
       kmax = __reduce_max_sync(0xffffffffu, kmax);
       __syncthreads();
       if ((tid & 31) == 0) sh.warp[tid >> 5][0] = kmin, sh.warp[tid >> 5][1] = kmax;
       __syncthreads();
-      for (int i = 0; i < kWarps; ++i) kmin = min(kmin, (uint32_t)sh.warp[i][0]), kmax = max(kmax, (uint32_t)sh.warp[i][1]);
+      for (int i = 0; i < kWarps; ++i)
+        kmin = min(kmin, (uint32_t)sh.warp[i][0]), kmax = max(kmax, (uint32_t)sh.warp[i][1]);
       const auto ks = c.exchange(kmin, kmax);
       for (int r = 0; r < c.size; ++r) kmin = min(kmin, (uint32_t)ks[r][0]), kmax = max(kmax, (uint32_t)ks[r][1]);
       lo = kmin;
@@ -350,44 +453,68 @@ __device__ void select(Cluster& c, Row& row, const uint32_t* keys, int n, uint32
       const uint32_t top = hi - ((uint32_t)bin << shift), width = (1u << shift) - 1;
       hi = top;
       lo = top - lo > width ? top - width : lo;
+      cluster_barrier();  // every CTA has read the histograms
     }
     const int bits = hi > lo ? 32 - __clz(hi - lo) : 0;  // hi - lo < 2^bits
     shift = max(0, bits - 11);
+    clear_hist(h, MASS);
+    __syncthreads();
   }
+  return false;
 }
 
 __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleParams p) {
-  extern __shared__ uint32_t keys[];
+  extern __shared__ __align__(16) uint32_t keys[];  // [chunk], then the histograms when there are top_k or top_p
   __shared__ Shared sh;
-  uint32_t size, rank;
+  uint32_t size;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
-  rank = cluster_ctarank();
-  Cluster c{sh, (int)rank, (int)size, 0};
+  Cluster c{sh, *reinterpret_cast<Hist*>(keys + p.chunk), (int)cluster_ctarank(), (int)size, 0};
+  const int b = blockIdx.x / size, tid = threadIdx.x, n4 = p.chunk / 4;
+  const uint32_t idx0 = c.rank * p.chunk;
+  if (tid < 64) sh.exp2_64[tid] = exp2(tid / 64.0);
+  if (p.top_k || p.top_p) clear_hist(c.hist, p.top_p != nullptr);
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.x / size, tid = threadIdx.x;
-  const int idx0 = min(p.V, (int)rank * p.chunk), n = min(p.V - idx0, p.chunk);
   // the chunk's keys, and its largest with the lowest index
+  const float T = p.temp ? p.temp[b] : 1.0f;
+  const int k = p.top_k ? p.top_k[b] : 0;
+  const float tp = p.top_p ? p.top_p[b] : 1.0f;
   uint64_t best = 0;
-  {
-    const int64_t o = (int64_t)b * p.ld + idx0;
-    auto put = [&](int i, float v) {
-      const uint32_t k = key_of(v);
-      keys[i] = k;
-      const uint64_t cand = ((uint64_t)k << 32) | (uint32_t)~(idx0 + i);
-      best = cand > best ? cand : best;
-    };
-    if (p.type == BTF_F32) {
-      const float* x = static_cast<const float*>(p.x) + o;
-      for (int i = tid; i < n; i += kThreads) put(i, x[i]);
-    } else if (p.type == BTF_F16) {
-      const __half* x = static_cast<const __half*>(p.x) + o;
-      for (int i = tid; i < n; i += kThreads) put(i, __half2float(x[i]));
-    } else {
-      const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.x) + o;
-      for (int i = tid; i < n; i += kThreads) put(i, __bfloat162float(x[i]));
+  auto put = [&](int i, const float (&v)[4], int n) {  // four neighbours, n of them logits
+    uint32_t q[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      q[e] = e < n ? key_of(v[e]) : 0;
+      const uint64_t cand = ((uint64_t)q[e] << 32) | (uint32_t)~(idx0 + 4 * i + e);
+      if (e < n && cand > best) best = cand;
     }
-  }
+    reinterpret_cast<uint4*>(keys)[i] = make_uint4(q[0], q[1], q[2], q[3]);
+  };
+  auto load = [&](auto type) {
+    using T_ = decltype(type);
+    const T_* x = static_cast<const T_*>(p.x) + (int64_t)b * p.ld + idx0;
+    const int n = min((int)max((int64_t)0, (int64_t)p.V - idx0), p.chunk);
+    // rows that begin off a 4-logit boundary are read one by one
+    const bool whole = (reinterpret_cast<uintptr_t>(static_cast<const T_*>(p.x) + (int64_t)b * p.ld) % (4 * sizeof(T_))) == 0;
+    const int full = whole ? n / 4 : 0;
+    int i = tid;
+#pragma unroll 4
+    for (; i < full; i += kThreads) {
+      Pack<T_, 4> w;
+      w.load(x + 4 * i);
+      const float v[4] = {w.get(0), w.get(1), w.get(2), w.get(3)};
+      put(i, v, 4);
+    }
+    for (; i < n4; i += kThreads) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = 4 * i + e < n ? to_f32(x[4 * i + e]) : 0.0f;
+      put(i, v, n - 4 * i);
+    }
+  };
+  if (p.type == BTF_F32) load(0.0f);
+  else if (p.type == BTF_F16) load(__half());
+  else load(__nv_bfloat16());
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const uint64_t q = __shfl_xor_sync(0xffffffffu, best, o);
@@ -403,11 +530,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   Row row;
   row.top = (uint32_t)(best >> 32);
   const uint32_t top_idx = ~(uint32_t)best;
-  const float T = p.temp ? p.temp[b] : 1.0f;
   const bool none = row.top <= kNegInf;
   if (none || !(T > 0.0f)) {  // nothing to draw from, or greedy
-    cluster_barrier();        // no CTA leaves while another may still write its slots
-    if (rank == 0 && tid == 0) {
+    if (c.rank == 0 && tid == 0) {
       const int32_t t = none ? 0 : (int32_t)top_idx;
       p.tok[b] = t;
       if (p.tok2) p.tok2[b] = t;
@@ -422,30 +547,39 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   row.S = p.S;
   row.cut_key = 0;
   row.cut_idx = 0xffffffffu;
+  row.table = sh.exp2_64;
+  row.min_e = -INFINITY;
+  row.min_bin = (float)kBins;
   {
     const float mp = p.min_p ? p.min_p[b] : 0.0f;
-    row.min_e = mp > 0.0f ? fmin(log((double)mp), 0.0) : -INFINITY;
+    if (mp > 0.0f) {
+      row.min_e = fmin(log((double)mp), 0.0);
+      // place() is within 2^-22 of the exact one, relative
+      row.min_bin = fminf(row.min_bin, (float)(-row.min_e * (kBins / kSpan)) * (1.0f + 0x1p-20f) + 0x1p-20f);
+    }
   }
-  const int k = p.top_k ? p.top_k[b] : 0;
-  if (k > 0 && k < p.V)
-    select<false>(c, row, keys, n, idx0, [k](uint64_t total) { return (uint64_t)k < total ? (uint64_t)k : 0ull; });
-  const float tp = p.top_p ? p.top_p[b] : 1.0f;
-  if (tp < 1.0f)
-    select<true>(c, row, keys, n, idx0, [tp](uint64_t total) {
-      const double g = ceil((double)tp * (double)total);
-      return g < 1.0 ? 1ull : (uint64_t)g < total ? (uint64_t)g : total;
-    });
+  if (k > 0 && k < p.V && select<false>(c, p, b, row, keys, n4, idx0, (uint64_t)k, tp)) return;
+  if (tp < 1.0f) {
+    if (k > 0 && k < p.V) {
+      __syncthreads();
+      clear_hist(c.hist, true);
+      __syncthreads();
+    }
+    if (select<true>(c, p, b, row, keys, n4, idx0, 0, tp)) return;
+  }
   // running masses in index order: a warp owns a contiguous block
-  const int lane = tid & 31, w = tid >> 5, blk = (n + kWarps - 1) / kWarps;
-  const int w0 = min(n, w * blk), w1 = min(n, w0 + blk);
-  auto kept = [&](int i) -> uint64_t {
-    const uint32_t key = keys[i];
-    if (!row.inside(key, idx0 + i)) return 0ull;
+  const int lane = tid & 31, w = tid >> 5, blk = n4 / kWarps, w0 = w * blk;  // in fours of keys
+  auto kept = [&](uint32_t key, int i) -> uint64_t {
+    if (!(row.place(key) < row.min_bin) || !row.inside(key, idx0 + i)) return 0ull;
     const double e = row.exponent(key);
-    return e > -(double)kSpan && e >= row.min_e ? row.weight_of(e) : 0ull;
+    return e >= row.min_e ? row.weight_of(e) : 0ull;
   };
   uint64_t mine = 0;
-  for (int i = w0 + lane; i < w1; i += 32) mine += kept(i);
+#pragma unroll 2
+  for (int i = w0 + lane; i < w0 + blk; i += 32) {
+    const uint4 q = reinterpret_cast<const uint4*>(keys)[i];
+    mine += kept(q.x, 4 * i) + kept(q.y, 4 * i + 1) + kept(q.z, 4 * i + 2) + kept(q.w, 4 * i + 3);
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   __syncthreads();
@@ -462,32 +596,39 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     if (r < c.rank) pre += s[r][0];
     z += s[r][0];
   }
-  const double u = (double)p.u[b];
-  const double goal_d = u > 0.0 ? u * (double)z : 0.0;
-  const uint64_t goal = goal_d < (double)z ? min((uint64_t)goal_d, z - 1) : z - 1;
+  const uint64_t goal = goal_of_u(p.u[b], z);
   if (pre <= goal && goal < pre + mine) {
     // the warp that holds the token walks its block
-    uint64_t run = pre;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-      const uint64_t v = i0 + lane < w1 ? kept(i0 + lane) : 0ull;
-      uint64_t inc = v;
+    for (int i0 = w0; i0 < w0 + blk; i0 += 32) {
+      const int i = i0 + lane;
+      const uint4 q = i < w0 + blk ? reinterpret_cast<const uint4*>(keys)[i] : make_uint4(0, 0, 0, 0);
+      const uint32_t key[4] = {q.x, q.y, q.z, q.w};
+      uint64_t v[4], inc = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = kept(key[e], 4 * i + e), inc += v[e];
+      const uint64_t four = inc;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t q = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += q;
+        const uint64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, run + inc > goal);
+      const unsigned hit = __ballot_sync(0xffffffffu, pre + inc > goal);
       if (hit) {
         if (lane == __ffs(hit) - 1) {
-          const int32_t t = idx0 + i0 + lane;
-          p.tok[b] = t;
-          if (p.tok2) p.tok2[b] = t;
-          if (p.logprob)
-            p.logprob[b] = (float)(row.exponent(keys[i0 + lane]) - log((double)z / (double)(1ull << row.S)));
+          uint64_t run = pre + inc - four;
+          bool done = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            run += v[e];
+            if (!done && run > goal) {
+              put_token(p, b, row, key[e], idx0 + 4 * i + e, z);
+              done = true;
+            }
+          }
         }
         break;
       }
-      run += __shfl_sync(0xffffffffu, inc, 31);
+      pre += __shfl_sync(0xffffffffu, inc, 31);
     }
   }
 }
@@ -495,7 +636,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
 }  // namespace
 
 int sample_setup(DeviceInfo& d) {
-  constexpr int kMost = BTF_SAMPLE_MAX_V / kMaxCluster * 4;  // the largest chunk's keys
+  constexpr int kMost = BTF_SAMPLE_MAX_V / kMaxCluster * 4 + (int)sizeof(Hist);  // the largest chunk's keys
   if (kMost + (int)sizeof(Shared) + 1024 > d.optin_smem)
     return fail(BTF_ERR_UNSUPPORTED, "sample_kernel needs %d bytes of shared memory", kMost + (int)sizeof(Shared));
   cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
@@ -512,9 +653,10 @@ cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
   // a CTA per about 16384 logits: its keys stay in shared memory
   int size = 1;
   while (size < kMaxCluster && (a.V + size - 1) / size > 16384) size *= 2;
-  p.chunk = (a.V + size - 1) / size;
-  return launch_pdl_cluster(sample_kernel, dim3((unsigned)(a.B * size)), dim3(kThreads), (size_t)p.chunk * 4, st, size,
-                            p);
+  constexpr int kStep = 4 * kThreads;
+  p.chunk = ((a.V + size - 1) / size + kStep - 1) / kStep * kStep;
+  const size_t smem = (size_t)p.chunk * 4 + (a.top_k || a.top_p ? sizeof(Hist) : 0);
+  return launch_pdl_cluster(sample_kernel, dim3((unsigned)(a.B * size)), dim3(kThreads), smem, st, size, p);
 }
 
 }  // namespace btf
