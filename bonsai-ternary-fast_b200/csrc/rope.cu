@@ -28,7 +28,7 @@ struct RopeSeg {
 struct RopeParams {
   RopeSeg seg[3];
   int nseg, T, D, R, inter, inverse;
-  int lanes;  // threads per token: a power of two >= items per head, <= 32
+  int lanes;  // threads per token: its items (with a norm a power of two, at most 32)
   int hl;     // heads per thread
   const double* turns;
   const int32_t* pos;
@@ -37,19 +37,24 @@ struct RopeParams {
 
 // One token's heads [h0, h1) of one tensor. A thread owns the C pairs of its
 // item (and item + lanes, ... when a head has more items than lanes) and keeps
-// their cos and sin over the heads.
-template <typename TX, typename TY, int C>
-__device__ void rope_heads(const RopeParams& p, const RopeSeg& s, int t, int64_t row, int h0, int h1, int lane) {
+// their cos and sin over the heads. The loads of kBatch heads are issued before
+// the first store: x and y may be one tensor, so the compiler would keep each
+// head's loads behind the stores of the one before.
+template <typename TX, typename TY, int C, bool NORM>
+__device__ __forceinline__ void rope_heads(const RopeParams& p, const RopeSeg& s, int t, int64_t row, int h0, int h1,
+                                           int lane) {
+  constexpr int kBatch = NORM ? 1 : C * (int)sizeof(TX) >= 32 ? 2 : 4;
   const int R = s.rotate ? p.R : 0, half = R / 2, D = p.D;
-  const int nrot = half / C;                             // rotated items: C pairs each
+  const int nrot = half / C;                               // rotated items: C pairs each
   const int items = nrot + (D - R + 2 * C - 1) / (2 * C);  // copied items: 2 C elements each
   const TX* x = static_cast<const TX*>(s.x) + (int64_t)t * s.x_token;
   TY* y = static_cast<TY*>(s.y) + row * s.y_token;
-  // the lanes of this token: they take the same branches
+  // with a norm: the lanes of this token, which take the same branches
   const unsigned mask = p.lanes == 32 ? 0xffffffffu : ((1u << p.lanes) - 1) << (threadIdx.x & 31 & ~(p.lanes - 1));
   for (int it0 = 0; it0 < items; it0 += p.lanes) {
     const int it = it0 + lane;
     const bool active = it < items, rot = it < nrot;
+    if (!NORM && !active) return;
     // the item's two chunks of C elements
     const int i = it * C, ca = rot ? (p.inter ? 2 * i : i) : R + (it - nrot) * 2 * C;
     const int cb = rot && !p.inter ? half + i : ca + C;
@@ -68,94 +73,103 @@ __device__ void rope_heads(const RopeParams& p, const RopeSeg& s, int t, int64_t
       }
     }
     float wa[C], wb[C];
-    if (s.normw) {
+    if (NORM && s.normw) {
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         wa[j] = active ? s.normw[ca + j] : 0.f;
         wb[j] = hasb ? s.normw[cb + j] : 0.f;
       }
     }
-#pragma unroll 2
-    for (int h = h0; h < h1; ++h) {
-      const TX* xh = x + (int64_t)h * s.x_head;
-      Pack<TX, C> a{}, b{};
-      if (active) a.load(xh + ca);
-      if (hasb) b.load(xh + cb);
-      float fa[C], fb[C];
+#pragma unroll 1
+    for (int hb = h0; hb < h1; hb += kBatch) {
+      Pack<TX, C> a[kBatch] = {}, b[kBatch] = {};
 #pragma unroll
-      for (int j = 0; j < C; ++j) fa[j] = a.get(j), fb[j] = b.get(j);
-      if (s.normw) {
-        float ss = 0.f;
-        if (items <= p.lanes) {  // the token's lanes hold the whole head
+      for (int k = 0; k < kBatch; ++k) {
+        const TX* xh = x + (int64_t)(hb + k) * s.x_head;
+        if (active && hb + k < h1) a[k].load(xh + ca);
+        if (hasb && hb + k < h1) b[k].load(xh + cb);
+      }
 #pragma unroll
-          for (int j = 0; j < C; ++j) ss = fmaf(fa[j], fa[j], fmaf(fb[j], fb[j], ss));
-        } else {
-          for (int e = lane; e < D; e += p.lanes) {
-            const float v = to_f32(xh[e]);
-            ss = fmaf(v, v, ss);
+      for (int k = 0; k < kBatch; ++k) {
+        if (kBatch > 1 && hb + k >= h1) break;
+        float fa[C], fb[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) fa[j] = a[k].get(j), fb[j] = b[k].get(j);
+        if (NORM && s.normw) {
+          float ss = 0.f;
+          if (items <= p.lanes) {  // the token's lanes hold the whole head
+#pragma unroll
+            for (int j = 0; j < C; ++j) ss = fmaf(fa[j], fa[j], fmaf(fb[j], fb[j], ss));
+          } else {
+            const TX* xh = x + (int64_t)hb * s.x_head;
+            for (int e = lane; e < D; e += p.lanes) {
+              const float v = to_f32(xh[e]);
+              ss = fmaf(v, v, ss);
+            }
           }
-        }
-        for (int o = p.lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float scale = 1.0f / sqrtf(ss / (float)D + p.eps);
+          for (int o = p.lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+          const float scale = 1.0f / sqrtf(ss / (float)D + p.eps);
 #pragma unroll
-        for (int j = 0; j < C; ++j) fa[j] *= scale * wa[j], fb[j] *= scale * wb[j];
+          for (int j = 0; j < C; ++j) fa[j] *= scale * wa[j], fb[j] *= scale * wb[j];
+        }
+        Pack<TY, C> oa, ob;
+        if (!rot) {
+#pragma unroll
+          for (int j = 0; j < C; ++j) oa.set(j, fa[j]), ob.set(j, fb[j]);
+        } else if (!p.inter) {
+#pragma unroll
+          for (int j = 0; j < C; ++j) {
+            oa.set(j, fmaf(fa[j], cs[j], -fb[j] * sn[j]));
+            ob.set(j, fmaf(fa[j], sn[j], fb[j] * cs[j]));
+          }
+        } else {
+          float v[2 * C];
+#pragma unroll
+          for (int j = 0; j < C; ++j) v[j] = fa[j], v[C + j] = fb[j];
+#pragma unroll
+          for (int j = 0; j < C; ++j) {
+            const float e = v[2 * j], o = v[2 * j + 1];
+            v[2 * j] = fmaf(e, cs[j], -o * sn[j]);
+            v[2 * j + 1] = fmaf(e, sn[j], o * cs[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < C; ++j) oa.set(j, v[j]), ob.set(j, v[C + j]);
+        }
+        TY* yh = y + (int64_t)(hb + k) * s.y_head;
+        if (active) oa.store(yh + ca);
+        if (hasb) ob.store(yh + cb);
       }
-      Pack<TY, C> oa, ob;
-      if (!rot) {
-#pragma unroll
-        for (int j = 0; j < C; ++j) oa.set(j, fa[j]), ob.set(j, fb[j]);
-      } else if (!p.inter) {
-#pragma unroll
-        for (int j = 0; j < C; ++j) {
-          oa.set(j, fmaf(fa[j], cs[j], -fb[j] * sn[j]));
-          ob.set(j, fmaf(fa[j], sn[j], fb[j] * cs[j]));
-        }
-      } else {
-        float v[2 * C];
-#pragma unroll
-        for (int j = 0; j < C; ++j) v[j] = fa[j], v[C + j] = fb[j];
-#pragma unroll
-        for (int j = 0; j < C; ++j) {
-          const float e = v[2 * j], o = v[2 * j + 1];
-          v[2 * j] = fmaf(e, cs[j], -o * sn[j]);
-          v[2 * j + 1] = fmaf(e, sn[j], o * cs[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < C; ++j) oa.set(j, v[j]), ob.set(j, v[C + j]);
-      }
-      TY* yh = y + (int64_t)h * s.y_head;
-      if (active) oa.store(yh + ca);
-      if (hasb) ob.store(yh + cb);
     }
   }
 }
 
-template <typename TX, int C>
+template <typename TX, int C, bool NORM>
 __device__ __forceinline__ void rope_to(const RopeParams& p, const RopeSeg& s, int t, int64_t row, int h0, int h1,
                                         int lane) {
-  if (s.y_type == BTF_F32) rope_heads<TX, float, C>(p, s, t, row, h0, h1, lane);
-  else if (s.y_type == BTF_F16) rope_heads<TX, __half, C>(p, s, t, row, h0, h1, lane);
-  else rope_heads<TX, __nv_bfloat16, C>(p, s, t, row, h0, h1, lane);
+  if (s.y_type == BTF_F32) rope_heads<TX, float, C, NORM>(p, s, t, row, h0, h1, lane);
+  else if (s.y_type == BTF_F16) rope_heads<TX, __half, C, NORM>(p, s, t, row, h0, h1, lane);
+  else rope_heads<TX, __nv_bfloat16, C, NORM>(p, s, t, row, h0, h1, lane);
 }
 
-template <int C>
+template <int C, bool NORM>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int t = blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes, lane = threadIdx.x % p.lanes;
+  const int per = kThreads / p.lanes, in = threadIdx.x / p.lanes;
+  const int t = blockIdx.x * per + in, lane = threadIdx.x - in * p.lanes;
   int si = 0;
   while (si + 1 < p.nseg && (int)blockIdx.y >= p.seg[si + 1].block0) ++si;
   const RopeSeg& s = p.seg[si];
   const int h0 = ((int)blockIdx.y - s.block0) * p.hl, h1 = min(h0 + p.hl, s.heads);
-  if (t >= p.T) return;
+  if (in >= per || t >= p.T) return;
   int64_t row = t;
   if (s.rows) {
     row = s.rows[t];
     if (row < 0 || row >= s.n_rows) return;
   }
-  if (s.x_type == BTF_F32) rope_to<float, C>(p, s, t, row, h0, h1, lane);
-  else if (s.x_type == BTF_F16) rope_to<__half, C>(p, s, t, row, h0, h1, lane);
-  else rope_to<__nv_bfloat16, C>(p, s, t, row, h0, h1, lane);
+  if (s.x_type == BTF_F32) rope_to<float, C, NORM>(p, s, t, row, h0, h1, lane);
+  else if (s.x_type == BTF_F16) rope_to<__half, C, NORM>(p, s, t, row, h0, h1, lane);
+  else rope_to<__nv_bfloat16, C, NORM>(p, s, t, row, h0, h1, lane);
 }
 
 bool aligned_for(const btf_rope_seg& s, int C) {
@@ -250,8 +264,11 @@ int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const 
   p.T = T, p.D = D, p.R = n_rot, p.inter = interleaved != 0, p.inverse = inverse != 0;
   p.turns = turns, p.pos = pos, p.mscale = mscale, p.eps = eps;
   const int items = std::max(n_rot / 2 / C + (D - n_rot + 2 * C - 1) / (2 * C), (D + 2 * C - 1) / (2 * C));
-  p.lanes = 1;
-  while (p.lanes < items && p.lanes < 32) p.lanes *= 2;
+  bool norm = false;
+  for (int i = 0; i < nseg; ++i) norm |= segs[i].heads && segs[i].normw;
+  // with a norm a token's lanes sum over a head by shuffles: a power of two of them
+  p.lanes = norm ? 1 : std::min(items, kThreads);
+  while (norm && p.lanes < items && p.lanes < 32) p.lanes *= 2;
   // heads per thread: more of them share one cos and sin, as long as the card
   // stays full
   const int64_t full = (int64_t)dev->sm_count * 2048;
@@ -268,9 +285,9 @@ int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const 
   const int per = kThreads / p.lanes;
   const dim3 grid((T + per - 1) / per, blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = C == 8   ? launch_pdl(rope_kernel<8>, grid, dim3(kThreads), 0, st, p)
-                        : C == 4 ? launch_pdl(rope_kernel<4>, grid, dim3(kThreads), 0, st, p)
-                                 : launch_pdl(rope_kernel<1>, grid, dim3(kThreads), 0, st, p);
+  const auto kernel = norm ? (C == 8 ? rope_kernel<8, true> : C == 4 ? rope_kernel<4, true> : rope_kernel<1, true>)
+                           : (C == 8 ? rope_kernel<8, false> : C == 4 ? rope_kernel<4, false> : rope_kernel<1, false>);
+  const cudaError_t e = launch_pdl(kernel, grid, dim3(kThreads), 0, st, p);
   return e == cudaSuccess ? BTF_OK : cuda_fail(e, "btf_rope");
 }
 

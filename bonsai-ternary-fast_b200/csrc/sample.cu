@@ -4,12 +4,19 @@
 //
 // All three filters keep a prefix of the order (logit descending, index
 // ascending), so nothing is sorted: a cut (key, index) in that order plus a bound on
-// the exponent is the kept set. A cut is found by a histogram over 2048 bins of
-// (max - l) / T. When the bins down to the cut's hold few elements (a top-k of 50, a
-// peaked nucleus), those go to the cluster's first CTA, which ranks them exactly and
-// finishes the row. Else the elements of the cut's own bin are ranked (or, when there
-// are many, split further by the bits of their keys), and the token comes from a
-// walk over running masses in index order, each CTA over its own part of the row.
+// the exponent is the kept set. What bounds the kernel is the number of passes over
+// the row and of cluster barriers (about 0.7 us each), so the common cases take few:
+//   top-k: a histogram of each thread's largest logit (of its 32 or so) gives a bound
+//     that at least k logits reach and few more than k exceed; those go to the
+//     cluster's first CTA, which ranks them exactly and finishes the row: 3 barriers;
+//   top-p: a histogram of masses over 2048 bins of (max - l) / T gives the cut's bin.
+//     Few elements down to it: the same finish. Else the bin's own elements are ranked
+//     (or, when there are many, split further by the bits of their keys), and the
+//     token comes from a walk over running masses in index order, each CTA over its
+//     own part of the row;
+//   no such filter: the walk alone: 2 barriers.
+// Bounds on (max - l) / T are turned into bounds on keys once, so that a pass over the
+// row compares integers and only what it keeps is worked out.
 //
 // Masses are 64-bit integers, w = rint(exp((l - max) / T) 2^S): sums are exact in
 // any order, so the CTAs of a cluster, the histogram and the final walk agree on
@@ -61,6 +68,11 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t a) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
+__device__ __forceinline__ uint64_t ld_cluster_u64(uint32_t a) {
+  uint64_t v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ void st_cluster_u64(uint32_t a, uint64_t v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
@@ -77,18 +89,18 @@ __device__ __forceinline__ void cluster_barrier() {
 
 struct Shared {
   uint64_t slot[2][kMaxCluster][2];  // values that the CTAs send one another, in turn
-  uint64_t total[kMaxCluster];       // each CTA's part of a histogram's total
+  uint64_t group[kMaxCluster][kBins / 32];  // every CTA's sums of 32 bins
   uint64_t warp[kWarps][2];
   uint64_t found[2];
+  int found_bin;
   double exp2_64[64];  // 2^(i / 64)
   uint64_t cmass[kCand];
   uint32_t ckey[kCand], cidx[kCand];
   uint32_t ncand;
 };
-// The histograms: counts, and the bins' masses in 16-bit limbs (a CTA holds at most 2^16 elements).
+// A histogram of counts or of masses. Its groups of 32 bins are summed for the whole cluster's use.
 struct Hist {
-  uint32_t cnt[kBins];
-  uint32_t mass[3][kBins];
+  unsigned long long bin[kBins];
 };
 
 // One row's state, the same in every thread of the cluster.
@@ -98,7 +110,7 @@ struct Row {
   double m, inv_t;  // the largest logit and 1 / T
   float bin_scale;
   double min_e;     // min-p: exponents below are dropped
-  float min_bin;    // a bound on their place among the bins, with room for rounding
+  uint32_t alive;   // keys below have no mass
   int S;
   uint32_t cut_key, cut_idx;  // kept: key > cut_key, or == and idx <= cut_idx
   const double* table;
@@ -129,7 +141,26 @@ struct Row {
     return (uint64_t)__double_as_longlong(fma(scaled, p, kRound)) & ((1ull << 51) - 1);
   }
   __device__ __forceinline__ uint64_t weight(uint32_t key) const {
-    return place(key) < (float)kBins ? weight_of(exponent(key)) : 0ull;
+    return key >= alive ? weight_of(exponent(key)) : 0ull;
+  }
+  // The least key above -inf with a place below `bound` > 0, for a converged warp: around where the bound's logit
+  // should be, then by a 32-way search.
+  __device__ __forceinline__ uint32_t least_key(float bound) const {
+    uint32_t lo = kNegInf, hi = top;  // lo fails, hi holds
+    const int lane = threadIdx.x & 31;
+    auto narrow = [&](uint32_t k) {
+      const bool holds = place(k) < bound;
+      hi = min(hi, __reduce_min_sync(0xffffffffu, holds ? k : top));
+      lo = max(lo, __reduce_max_sync(0xffffffffu, holds ? kNegInf : k));
+    };
+    const float at = top_value - bound / bin_scale;
+    if (hi - lo > 32 && fabsf(at) < INFINITY) {
+      const uint32_t g = key_of(at), d = 1u << (2 * (lane & 15));
+      const uint32_t k = lane < 16 ? (g > kNegInf + d ? g - d : kNegInf + 1) : (top - kNegInf > d && g < top - d ? g + d : top);
+      narrow(min(max(k, kNegInf + 1), top));
+    }
+    while (hi - lo > 1) narrow(lo + 1 + (uint32_t)(((uint64_t)(hi - lo - 1) * lane) >> 5));
+    return hi;
   }
   __device__ __forceinline__ bool inside(uint32_t key, uint32_t idx) const {
     return key > cut_key || (key == cut_key && idx <= cut_idx);
@@ -201,27 +232,73 @@ __device__ __forceinline__ void each_key(const uint32_t* keys, int n4, Fn fn) {
   }
 }
 
-__device__ __forceinline__ void clear_hist(Hist& h, bool mass) {
-  for (int b = threadIdx.x; b < kBins; b += kThreads) {
-    h.cnt[b] = 0;
-    if (mass) h.mass[0][b] = h.mass[1][b] = h.mass[2][b] = 0;
-  }
+__device__ __forceinline__ void clear_hist(Hist& h) {
+  uint4* w = reinterpret_cast<uint4*>(&h);
+  for (int b = threadIdx.x; b < (int)(sizeof(Hist) / 16); b += kThreads) w[b] = make_uint4(0, 0, 0, 0);
 }
 
-// A bin's value over the whole cluster: its count, or its mass.
-template <bool MASS>
-__device__ __forceinline__ uint64_t bin_value(const Cluster& c, int b) {
-  uint64_t v = 0;
-#pragma unroll 4
-  for (int r = 0; r < c.size; ++r) {
-    const uint32_t base = c.at(&c.hist, r) + b * 4;
-    if (MASS)
-      v += (uint64_t)ld_cluster_u32(base + 4 * kBins) + ((uint64_t)ld_cluster_u32(base + 8 * kBins) << 16) +
-           ((uint64_t)ld_cluster_u32(base + 12 * kBins) << 32);
-    else
-      v += ld_cluster_u32(base);
+// Publishes this CTA's histogram: the sums of its groups of 32 bins go to every CTA (reading whole histograms
+// through the cluster costs 16 CTAs 7 us). All threads call it; ends with a barrier of the cluster.
+__device__ __forceinline__ void publish(const Cluster& c) {
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int g = threadIdx.x >> 5; g < kBins / 32; g += kWarps) {
+    uint64_t v = c.hist.bin[g * 32 + lane];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane < c.size) st_cluster_u64(c.at(&c.sh.group[c.rank][g], lane), v);
   }
-  return v;
+  cluster_barrier();
+}
+// The sum of all published bins.
+__device__ __forceinline__ uint64_t published(const Cluster& c) {
+  uint64_t v = 0;
+  if (threadIdx.x < kBins / 32)
+    for (int r = 0; r < c.size; ++r) v += c.sh.group[r][threadIdx.x];
+  return block_sum(c.sh, v);
+}
+
+// The bin in which the running value (from the largest logits on, `before` ahead of the first) reaches the goal,
+// over the whole cluster's histograms: every CTA finds it for itself. The goal is within reach.
+struct Found {
+  int bin;
+  uint64_t before, value;
+};
+__device__ __forceinline__ Found find_bin(const Cluster& c, uint64_t before, uint64_t goal) {
+  static_assert(kBins / 32 <= kThreads);
+  Shared& sh = c.sh;
+  uint64_t v = 0, all;
+  if (threadIdx.x < kBins / 32)
+    for (int r = 0; r < c.size; ++r) v += sh.group[r][threadIdx.x];
+  const uint64_t run = before + block_scan(sh, v, &all);
+  if (run < goal && goal <= run + v) {
+    sh.found[0] = run;
+    sh.found_bin = threadIdx.x;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {  // the group's bins, a lane each
+    const int b = sh.found_bin * 32 + threadIdx.x;
+    uint64_t w = 0, inc;
+#pragma unroll 4
+    for (int r = 0; r < c.size; ++r) w += ld_cluster_u64(c.at(&c.hist.bin[b], r));
+    inc = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+      if ((int)threadIdx.x >= o) inc += up;
+    }
+    const uint64_t from = sh.found[0] + inc - w;
+    __syncwarp();
+    if (from < goal && goal <= from + w) {
+      sh.found[0] = from;
+      sh.found[1] = w;
+      sh.found_bin = b;
+    }
+  }
+  __syncthreads();
+  const Found f{sh.found_bin, sh.found[0], sh.found[1]};
+  __syncthreads();
+  return f;
 }
 
 __device__ __forceinline__ uint64_t goal_of_u(float uf, uint64_t z) {
@@ -247,170 +324,190 @@ __device__ __forceinline__ uint64_t goal_of_p(float p, uint64_t total) {
 template <bool RANKED>
 __device__ void finish(Shared& sh, const SampleParams& p, int b, const Row& row, uint64_t k, uint64_t goal, float top_p) {
   const int tid = threadIdx.x, n = (int)sh.ncand;
-  const bool mine = tid < n;
-  const uint32_t key = mine ? sh.ckey[tid] : 0, idx = mine ? sh.cidx[tid] : 0;
+  // 2^lg threads per candidate share the comparisons
+  int lg = 0;
+  while (lg < 5 && (n << (lg + 1)) <= kThreads) ++lg;
+  const int i = tid >> lg, part = tid & ((1 << lg) - 1), step = 1 << lg;
+  const bool mine = i < n, lead = mine && part == 0;
+  const uint32_t key = mine ? sh.ckey[i] : 0, idx = mine ? sh.cidx[i] : 0;
   const uint64_t w = mine ? row.weight(key) : 0;
-  if (mine) sh.cmass[tid] = w;
+  if (lead) sh.cmass[i] = w;
   __syncthreads();
   uint64_t before = 0;
   uint32_t rank = 0;
+  if (((tid & ~31) >> lg) < n) {
 #pragma unroll 4
-  for (int j = 0; j < n; ++j) {
-    const uint32_t kj = sh.ckey[j];
-    if (kj > key || (kj == key && sh.cidx[j] < idx)) {
-      before += sh.cmass[j];
-      ++rank;
+    for (int j = part; j < n; j += step) {
+      const uint32_t kj = sh.ckey[j], xj = sh.cidx[j];
+      const uint64_t wj = sh.cmass[j];
+      const bool ahead = kj > key || (kj == key && xj < idx);
+      before += ahead ? wj : 0;
+      rank += ahead;
+    }
+    for (int o = step >> 1; o; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      rank += __shfl_xor_sync(0xffffffffu, rank, o);
     }
   }
   bool keep = mine && w > 0;
   if (RANKED) {
     keep = keep && rank < k;
-    const uint64_t zk = block_sum(sh, keep ? w : 0);
+    const uint64_t zk = block_sum(sh, keep && lead ? w : 0);
     goal = top_p < 1.0f ? goal_of_p(top_p, zk) : zk;
   }
   keep = keep && before < goal && row.exponent(key) >= row.min_e;
   __syncthreads();
-  if (mine) sh.cmass[tid] = keep ? w : 0;
-  const uint64_t z = block_sum(sh, keep ? w : 0);  // (its barriers publish cmass)
+  if (lead) sh.cmass[i] = keep ? w : 0;
+  const uint64_t z = block_sum(sh, keep && lead ? w : 0);  // (its barriers publish cmass)
   const uint64_t g = goal_of_u(p.u[b], z);
   uint64_t run = 0;
+  if (((tid & ~31) >> lg) < n) {
 #pragma unroll 4
-  for (int j = 0; j < n; ++j)
-    if (sh.cidx[j] < idx) run += sh.cmass[j];
-  if (keep && run <= g && g < run + w) put_token(p, b, row, key, idx, z);
+    for (int j = part; j < n; j += step) {
+      const uint32_t xj = sh.cidx[j];
+      const uint64_t wj = sh.cmass[j];
+      run += xj < idx ? wj : 0;
+    }
+    for (int o = step >> 1; o; o >>= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
+  }
+  if (keep && lead && run <= g && g < run + w) put_token(p, b, row, key, idx, z);
+}
+
+// Sends this CTA's elements with keys in [lo, hi] (inside the cut) to the first CTA's list. Ends with a barrier of
+// the cluster; returns how many there were in all: at most kCand of them are in the list.
+__device__ __forceinline__ uint32_t gather(const Cluster& c, const Row& row, const uint32_t* keys, int n4, uint32_t idx0,
+                                           uint32_t lo, uint32_t hi, bool skip) {
+  const uint32_t n_at = c.at(&c.sh.ncand, 0), key_at = c.at(c.sh.ckey, 0), idx_at = c.at(c.sh.cidx, 0);
+  if (!skip)
+    each_key(keys, n4, [&](uint32_t key, int i) {
+      if (key < lo || key > hi || !row.inside(key, idx0 + i)) return;
+      const uint32_t at = atom_cluster_inc(n_at);
+      if (at >= (uint32_t)kCand) return;
+      st_cluster_b32(key_at + at * 4, key);
+      st_cluster_b32(idx_at + at * 4, idx0 + i);
+    });
+  cluster_barrier();
+  return ld_cluster_u32(n_at);
+}
+
+// The first CTA works, and leaves only after every CTA of the cluster has read its shared memory for the last time.
+template <typename Fn>
+__device__ __forceinline__ void last_read(const Cluster& c, Fn work) {
+  __syncwarp();
+  cluster_arrive_release();
+  if (c.rank == 0) work();
+  __syncwarp();
+  cluster_wait_acquire();
+}
+
+// Top-k from the threads' largest logits (see the top): true when the row is
+// finished, false when there are too few or too many for it. All threads of the
+// cluster call it.
+__device__ bool top_of_threads(Cluster& c, const SampleParams& p, int b, Row& row, const uint32_t* keys, int n4,
+                               uint32_t idx0, uint32_t largest, uint64_t k, float top_p) {
+  if (largest >= row.alive) atomicAdd(&c.hist.bin[(int)row.place(largest)], 1ull);
+  if (threadIdx.x == 0) c.sh.ncand = 0;
+  publish(c);
+  bool done = false;
+  if (published(c) >= k) {
+    const Found f = find_bin(c, 0, k);
+    if (f.before + f.value <= (uint64_t)kCand) {
+      const uint32_t lo = row.least_key((float)(f.bin + 1));
+      done = gather(c, row, keys, n4, idx0, lo, 0xffffffffu, largest < lo) <= (uint32_t)kCand;
+    }
+  }
+  if (done) {
+    last_read(c, [&] { finish<true>(c.sh, p, b, row, k, 0, top_p); });
+    return true;
+  }
+  cluster_barrier();  // the histograms and the list have been read
+  clear_hist(c.hist);
+  __syncthreads();
+  return false;
 }
 
 // The cut of the shortest prefix whose value (its count: top-k; its mass: top-p)
 // reaches a goal: k, or top_p of the mass inside the present cut. True when the row
-// is finished. All threads of the cluster call it, and every branch on the way to a
-// barrier is the same for all of them.
+// is finished. The histogram is clear on entry. All threads of the cluster call it,
+// and every branch on the way to a barrier is the same for all of them.
 template <bool MASS>
 __device__ bool select(Cluster& c, const SampleParams& p, int row_b, Row& row, const uint32_t* keys, int n4,
                        uint32_t idx0, uint64_t k, float top_p) {
   Shared& sh = c.sh;
-  Hist& h = c.hist;
   const int tid = threadIdx.x;
-  uint64_t before = 0, goal = 0;      // the value of what lies above the range; the goal
-  uint32_t lo = 0, hi = 0xffffffffu;  // keys of the range, inclusive
+  uint64_t before = 0, goal = 0;              // the value of what lies above the range; the goal
+  uint32_t lo = row.alive, hi = 0xffffffffu;  // keys of the range, inclusive
   int shift = 0;
-  bool first = true;  // the first histogram is over Row::place (it was cleared by the caller)
-  // bin of an element of the range, or -1
-  auto bin_of = [&](uint32_t key, uint32_t idx) -> int {
-    const float at = row.place(key);
-    if (!(at < (float)kBins) || !row.inside(key, idx)) return -1;
-    if (first) return (int)at;
-    return key < lo || key > hi ? -1 : (int)((hi - key) >> shift);
-  };
+  bool first = true;  // the first histogram is over Row::place, the others over the bits of the keys
   for (int pass = 0; pass < 6; ++pass) {  // at most 4 are needed: 2048 bins, then 11 bits of the key each
-    uint64_t sum = 0;
     each_key(keys, n4, [&](uint32_t key, int i) {
-      const int b = bin_of(key, idx0 + i);
-      if (b < 0) return;
-      atomicAdd(&h.cnt[b], 1u);
-      if (MASS) {
-        const uint64_t w = row.weight_of(row.exponent(key));
-        atomicAdd(&h.mass[0][b], (uint32_t)(w & 0xffffu));
-        atomicAdd(&h.mass[1][b], (uint32_t)((w >> 16) & 0xffffu));
-        atomicAdd(&h.mass[2][b], (uint32_t)(w >> 32));
-        sum += w;
-      } else {
-        ++sum;
-      }
+      if (key < lo || key > hi || !row.inside(key, idx0 + i)) return;
+      const int b = first ? (int)row.place(key) : (int)((hi - key) >> shift);
+      const uint64_t v = MASS ? row.weight_of(row.exponent(key)) : 1ull;
+      if (v) atomicAdd(&c.hist.bin[b], (unsigned long long)v);
     });
+    if (tid == 0) sh.ncand = 0;
+    publish(c);
     if (first) {
-      sum = block_sum(sh, sum);
-      if (tid < c.size) st_cluster_u64(c.at(&sh.total[c.rank], tid), sum);
-      if (tid == 0) sh.ncand = 0;
-    }
-    __syncthreads();
-    cluster_barrier();
-    if (first) {
-      uint64_t total = 0;
-      for (int r = 0; r < c.size; ++r) total += sh.total[r];
+      const uint64_t total = published(c);
       goal = MASS ? goal_of_p(top_p, total) : k;
       if (goal > total || (!MASS && goal == total)) {  // nothing to cut off
-        cluster_barrier();  // (sh.total is read before it is written again)
+        cluster_barrier();                             // (the sums are read before they are written again)
         return false;
       }
     }
-    // every CTA finds the bin for itself, a thread per bin from the largest on
-    int bin = 0;
-    uint32_t count = 0;
-    for (int b0 = 0;; b0 += kThreads) {
-      const uint64_t v = bin_value<MASS>(c, b0 + tid);
-      uint64_t all;
-      const uint64_t pre = before + block_scan(sh, v, &all);
-      if (pre < goal && goal <= pre + v) {
-        sh.found[0] = ((uint64_t)(b0 + tid) << 32) | (uint32_t)bin_value<false>(c, b0 + tid);
-        sh.found[1] = pre;
-      }
-      __syncthreads();
-      if (goal <= before + all || b0 + kThreads >= kBins) break;
-      before += all;
-    }
-    bin = (int)(sh.found[0] >> 32);
-    count = (uint32_t)sh.found[0];
-    before = sh.found[1];
-    // few elements down to this bin: the first CTA ranks them and finishes the row
-    uint64_t down = ~0ull;
+    const Found f = find_bin(c, before, goal);
+    before = f.before;
+    uint32_t klo, khi;  // the keys of its bin
     if (first) {
-      if (!MASS) {
-        down = before + count;
-      } else {
-        uint64_t part = 0;
-        for (int b = tid; b < bin; b += kThreads) part += bin_value<false>(c, b);
-        down = block_sum(sh, part) + count;
-      }
+      klo = row.least_key((float)(f.bin + 1));
+      khi = f.bin ? row.least_key((float)f.bin) - 1 : 0xffffffffu;
+    } else {
+      khi = hi - ((uint32_t)f.bin << shift);
+      klo = khi - lo > (1u << shift) - 1 ? khi - ((1u << shift) - 1) : lo;
     }
-    if (down <= (uint64_t)kCand || count <= (uint32_t)kCand) {
-      const bool all = down <= (uint64_t)kCand;
-      const uint32_t n_at = c.at(&sh.ncand, 0), key_at = c.at(sh.ckey, 0), idx_at = c.at(sh.cidx, 0);
-      each_key(keys, n4, [&](uint32_t key, int i) {
-        const int b = bin_of(key, idx0 + i);
-        if (b < 0 || (all ? b > bin : b != bin)) return;
-        const uint32_t at = atom_cluster_inc(n_at);
-        if (at >= (uint32_t)kCand) return;
-        st_cluster_b32(key_at + at * 4, key);
-        st_cluster_b32(idx_at + at * 4, idx0 + i);
-      });
-      cluster_barrier();
-      if (all) {
-        if (c.rank == 0) finish<!MASS>(sh, p, row_b, row, k, goal, top_p);
-        return true;
-      }
-      if (c.rank == 0) {
-        const int m = (int)min(sh.ncand, (uint32_t)kCand);
-        if (tid < m) sh.cmass[tid] = MASS ? row.weight(sh.ckey[tid]) : 1ull;
-        if (tid == 0) sh.found[0] = sh.found[1] = 0;
-        __syncthreads();
-        if (tid < m) {
-          const uint32_t ki = sh.ckey[tid], xi = sh.cidx[tid];
-          uint64_t v = before;
-#pragma unroll 4
-          for (int j = 0; j < m; ++j) {
-            const uint32_t kj = sh.ckey[j];
-            if (kj > ki || (kj == ki && sh.cidx[j] < xi)) v += sh.cmass[j];
-          }
-          if (v < goal && goal <= v + sh.cmass[tid]) {
-            sh.found[0] = ki;
-            sh.found[1] = xi;
-          }
+    // how many elements there are: counted, or bounded by the least and the greatest mass that they may have
+    const uint64_t w_lo = MASS ? row.weight(klo) : 1, w_hi = MASS ? row.weight(min(khi, row.top)) : 1;
+    const bool down = first && before + f.value <= kCand * w_lo;
+    if (down || f.value <= kCand * w_hi) {
+      const uint32_t m = gather(c, row, keys, n4, idx0, klo, down ? 0xffffffffu : khi, false);
+      if (m <= (uint32_t)kCand) {
+        if (down) {
+          last_read(c, [&] { finish<!MASS>(sh, p, row_b, row, k, goal, top_p); });
+          return true;
         }
-        __syncthreads();
+        if (c.rank == 0) {
+          if (tid < (int)m) sh.cmass[tid] = MASS ? row.weight(sh.ckey[tid]) : 1ull;
+          if (tid == 0) sh.found[0] = sh.found[1] = 0;
+          __syncthreads();
+          if (tid < (int)m) {
+            const uint32_t ki = sh.ckey[tid], xi = sh.cidx[tid];
+            uint64_t v = before;
+#pragma unroll 4
+            for (int j = 0; j < (int)m; ++j) {
+              const uint32_t kj = sh.ckey[j], xj = sh.cidx[j];
+              const uint64_t wj = sh.cmass[j];
+              v += kj > ki || (kj == ki && xj < xi) ? wj : 0;
+            }
+            if (v < goal && goal <= v + sh.cmass[tid]) {
+              sh.found[0] = ki;
+              sh.found[1] = xi;
+            }
+          }
+          __syncthreads();
+        }
+        const auto cut = c.exchange(sh.found[0], sh.found[1]);
+        row.cut_key = (uint32_t)cut[0][0];
+        row.cut_idx = (uint32_t)cut[0][1];
+        return false;
       }
-      const auto cut = c.exchange(sh.found[0], sh.found[1]);
-      row.cut_key = (uint32_t)cut[0][0];
-      row.cut_idx = (uint32_t)cut[0][1];
-      return false;
     }
-    if (!first && shift == 0) {
+    if (klo == min(khi, row.top)) {
       // many equal keys: the goal's place among them, in index order
-      const uint32_t key = hi - bin;
-      const uint64_t g = MASS ? row.weight(key) : 1ull;
-      const uint64_t need = (goal - before + g - 1) / g;  // ties to keep, >= 1
+      const uint64_t g = w_lo, need = (goal - before + g - 1) / g;  // ties to keep, >= 1
       uint64_t ties = 0;
       const int blk = (n4 + kThreads - 1) / kThreads * 4, i0 = min(4 * n4, tid * blk), i1 = min(4 * n4, i0 + blk);
-      for (int i = i0; i < i1; ++i) ties += keys[i] == key && row.inside(key, idx0 + i);
+      for (int i = i0; i < i1; ++i) ties += keys[i] == klo && row.inside(klo, idx0 + i);
       uint64_t all;
       const uint64_t tpre = block_scan(sh, ties, &all);
       const auto tslots = c.exchange(all, 0);
@@ -420,44 +517,24 @@ __device__ bool select(Cluster& c, const SampleParams& p, int row_b, Row& row, c
       __syncthreads();
       if (tb < need && need <= tb + ties) {
         for (int i = i0; i < i1; ++i)
-          if (keys[i] == key && row.inside(key, idx0 + i) && ++tb == need) sh.found[0] = idx0 + i;
+          if (keys[i] == klo && row.inside(klo, idx0 + i) && ++tb == need) sh.found[0] = idx0 + i;
       }
       __syncthreads();
       const auto cut = c.exchange(sh.found[0], 0);
       for (int r = 0; r < c.size; ++r)
         if (cut[r][0] != ~0ull) {
-          row.cut_key = key;
+          row.cut_key = klo;
           row.cut_idx = (uint32_t)cut[r][0];
         }
       return false;
     }
-    // many elements of unlike keys: another histogram over the range of the bin's keys
-    if (first) {
-      uint32_t kmin = 0xffffffffu, kmax = 0;
-      each_key(keys, n4, [&](uint32_t key, int i) {
-        if (bin_of(key, idx0 + i) == bin) kmin = min(kmin, key), kmax = max(kmax, key);
-      });
-      kmin = __reduce_min_sync(0xffffffffu, kmin);
-      kmax = __reduce_max_sync(0xffffffffu, kmax);
-      __syncthreads();
-      if ((tid & 31) == 0) sh.warp[tid >> 5][0] = kmin, sh.warp[tid >> 5][1] = kmax;
-      __syncthreads();
-      for (int i = 0; i < kWarps; ++i)
-        kmin = min(kmin, (uint32_t)sh.warp[i][0]), kmax = max(kmax, (uint32_t)sh.warp[i][1]);
-      const auto ks = c.exchange(kmin, kmax);
-      for (int r = 0; r < c.size; ++r) kmin = min(kmin, (uint32_t)ks[r][0]), kmax = max(kmax, (uint32_t)ks[r][1]);
-      lo = kmin;
-      hi = kmax;
-      first = false;
-    } else {
-      const uint32_t top = hi - ((uint32_t)bin << shift), width = (1u << shift) - 1;
-      hi = top;
-      lo = top - lo > width ? top - width : lo;
-      cluster_barrier();  // every CTA has read the histograms
-    }
-    const int bits = hi > lo ? 32 - __clz(hi - lo) : 0;  // hi - lo < 2^bits
-    shift = max(0, bits - 11);
-    clear_hist(h, MASS);
+    // many elements of unlike keys: another histogram over the bin's keys
+    cluster_barrier();  // every CTA has read the histograms
+    lo = klo;
+    hi = min(khi, row.top);
+    first = false;
+    shift = max(0, 32 - __clz(hi - lo) - 11);  // hi - lo < 2^(32 - clz)
+    clear_hist(c.hist);
     __syncthreads();
   }
   return false;
@@ -472,7 +549,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   const int b = blockIdx.x / size, tid = threadIdx.x, n4 = p.chunk / 4;
   const uint32_t idx0 = c.rank * p.chunk;
   if (tid < 64) sh.exp2_64[tid] = exp2(tid / 64.0);
-  if (p.top_k || p.top_p) clear_hist(c.hist, p.top_p != nullptr);
+  if (p.top_k || p.top_p) clear_hist(c.hist);
   pdl_launch_dependents();
   pdl_wait();
   // the chunk's keys, and its largest with the lowest index
@@ -515,6 +592,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   if (p.type == BTF_F32) load(0.0f);
   else if (p.type == BTF_F16) load(__half());
   else load(__nv_bfloat16());
+  const uint32_t largest = (uint32_t)(best >> 32);  // this thread's
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const uint64_t q = __shfl_xor_sync(0xffffffffu, best, o);
@@ -548,29 +626,37 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   row.cut_key = 0;
   row.cut_idx = 0xffffffffu;
   row.table = sh.exp2_64;
+  row.alive = row.least_key((float)kBins);
   row.min_e = -INFINITY;
-  row.min_bin = (float)kBins;
+  uint32_t least = row.alive;  // keys below are not kept
   {
     const float mp = p.min_p ? p.min_p[b] : 0.0f;
     if (mp > 0.0f) {
       row.min_e = fmin(log((double)mp), 0.0);
       // place() is within 2^-22 of the exact one, relative
-      row.min_bin = fminf(row.min_bin, (float)(-row.min_e * (kBins / kSpan)) * (1.0f + 0x1p-20f) + 0x1p-20f);
+      const float bound = (float)(-row.min_e * (kBins / kSpan)) * (1.0f + 0x1p-20f) + 0x1p-20f;
+      if (bound < (float)kBins) least = row.least_key(bound);
     }
   }
-  if (k > 0 && k < p.V && select<false>(c, p, b, row, keys, n4, idx0, (uint64_t)k, tp)) return;
+  const bool ks = k > 0 && k < p.V;
+  if (ks) {
+    // (more than the ranking can hold needs no try)
+    if (k <= kCand && top_of_threads(c, p, b, row, keys, n4, idx0, largest, (uint64_t)k, tp)) return;
+    if (select<false>(c, p, b, row, keys, n4, idx0, (uint64_t)k, tp)) return;
+  }
   if (tp < 1.0f) {
-    if (k > 0 && k < p.V) {
+    if (ks) {
       __syncthreads();
-      clear_hist(c.hist, true);
+      clear_hist(c.hist);
       __syncthreads();
     }
     if (select<true>(c, p, b, row, keys, n4, idx0, 0, tp)) return;
   }
+  least = max(least, row.cut_key);
   // running masses in index order: a warp owns a contiguous block
   const int lane = tid & 31, w = tid >> 5, blk = n4 / kWarps, w0 = w * blk;  // in fours of keys
   auto kept = [&](uint32_t key, int i) -> uint64_t {
-    if (!(row.place(key) < row.min_bin) || !row.inside(key, idx0 + i)) return 0ull;
+    if (key < least || !row.inside(key, idx0 + i)) return 0ull;
     const double e = row.exponent(key);
     return e >= row.min_e ? row.weight_of(e) : 0ull;
   };
