@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -158,6 +159,9 @@ class RopeSegC(ctypes.Structure):
                 ("normw", ctypes.c_void_p), ("rows", ctypes.c_void_p), ("n_rows", ctypes.c_int64)]
 
 
+_ROPE_SEG = struct.Struct("@PPiiiiqqqqPPq")  # a btf_rope_seg; filling one this way takes a call's time less than fields do
+
+
 class TreeAttnC(ctypes.Structure):
     """btf_tree_attn: attention for a tree of drafted tokens over a cache."""
 
@@ -168,6 +172,9 @@ class TreeAttnC(ctypes.Structure):
         (f, ctypes.c_int) for f in ("type", "B", "n", "H", "HK", "D", "n_ctx")] + [
         (f, ctypes.c_void_p) for f in ("lens", "parents", "counts")] + [
         ("scale", ctypes.c_float), ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_int64)]
+
+
+_TREE_ATTN = struct.Struct("@PqqqPPqqqPqqqiiiiiiiPPPfPq")  # a btf_tree_attn
 
 
 def lib() -> ctypes.CDLL:
@@ -245,10 +252,10 @@ def lib() -> ctypes.CDLL:
         "btf_decoder_reset_stats": (i32, [vp]),
         "btf_plan_memory": (i32, [ctypes.c_char_p, ctypes.POINTER(DecoderOptsC), i32, i32, ctypes.POINTER(MemoryPlanC)]),
         "btf_rope_table": (i32, [ctypes.POINTER(RopeCfgC), vp, ctypes.POINTER(ctypes.c_float)]),
-        "btf_rope": (i32, [ctypes.POINTER(RopeSegC), i32, i32, i32, i32, vp, ctypes.c_float, i32, i32, ctypes.c_float,
+        "btf_rope": (i32, [vp, i32, i32, i32, i32, vp, ctypes.c_float, i32, i32, ctypes.c_float,
                            vp, vp]),
         "btf_tree_attention_work": (i64, [i32] * 6),
-        "btf_tree_attention": (i32, [ctypes.POINTER(TreeAttnC), vp]),
+        "btf_tree_attention": (i32, [vp, vp]),
         "btf_sample": (i32, [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
         "btf_plan_memory_synthetic": (i32, [ctypes.POINTER(DecoderDimsC), ctypes.POINTER(DecoderOptsC), i32, i32,
                                             ctypes.POINTER(MemoryPlanC)]),
@@ -657,28 +664,29 @@ def _vector(what: str, dev, name: str, t, dtype, shape) -> Optional[int]:
     return t.data_ptr()
 
 
-def _launch(dev, stream, fn):
-    """fn(stream handle) with `dev` current: on dev's current stream, or on `stream`, which is then current too (so
-    that what fn allocates belongs to it)."""
+def _launch(dev, stream, fn, args):
+    """fn(stream handle, args) with `dev` current: on dev's current stream, or on `stream`, which is then current too
+    (so that what fn allocates belongs to it)."""
     torch = _torch()
     if dev.index not in _initialised:
         ensure_init(dev.index)
     if stream is None:
         if torch.cuda.current_device() == dev.index:
-            return fn(torch._C._cuda_getCurrentRawStream(dev.index))
+            return fn(torch._C._cuda_getCurrentRawStream(dev.index), args)
         with torch.cuda.device(dev):
-            return fn(torch.cuda.current_stream(dev).cuda_stream)
+            return fn(torch.cuda.current_stream(dev).cuda_stream, args)
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
     if stream.device != dev:
         raise RuntimeError(f"a stream of {stream.device} for tensors on {dev}")
     with torch.cuda.stream(stream):
-        return fn(stream.cuda_stream)
+        return fn(stream.cuda_stream, args)
 
 
-def _strides(t) -> list:
+def _strides(t) -> tuple:
     """Strides in elements; of a dim with one entry none matters."""
-    return [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+    st = t.stride()
+    return st if 1 not in t.shape else tuple([0 if n == 1 else s for n, s in zip(t.shape, st)])
 
 
 class RopeTable:
@@ -721,38 +729,46 @@ def rope(segs: Sequence[RopeSeg], table: RopeTable, pos, inverse: bool = False, 
         raise RuntimeError(f"rope: 1..3 tensors expected, got {n}")
     x0 = segs[0].x
     T, D, dev = x0.shape[0], x0.shape[-1], _cuda_device("rope", x0)
-    i32 = torch.int32
-    arr = (RopeSegC * n)()
-    for s, a in zip(segs, arr):
+    i32, f32, packed = torch.int32, torch.float32, b""
+    for s in segs:
         x, y = s.x, s.x if s.y is None else s.y
         xs, ys = x.shape, y.shape
-        if len(xs) != 3 or len(ys) != 3 or xs[0] != T or xs[2] != D or ys[1:] != xs[1:]:
+        if len(xs) != 3 or len(ys) != 3 or xs[0] != T or xs[2] != D or ys[1] != xs[1] or ys[2] != D:
             raise RuntimeError(f"rope: x [T][heads][D] and y [rows][heads][D] expected, got {tuple(xs)} and {tuple(ys)}")
-        if s.rows is None and ys[0] != T:
-            raise RuntimeError(f"rope: y has {ys[0]} rows for {T} tokens")
-        _on("rope", dev, "x", x)
-        _on("rope", dev, "y", y)
-        a.x_token, a.x_head, xd = x.stride()
-        a.y_token, a.y_head, yd = y.stride()
+        if x.device != dev or y.device != dev:
+            raise RuntimeError(f"rope: x and y must be on {dev}, got {x.device} and {y.device}")
+        xt, xh, xd = x.stride()
+        yt, yh, yd = y.stride()
         if D > 1 and (xd != 1 or yd != 1):
             raise RuntimeError("rope: the dims of a head must be contiguous")
-        if xs[1] == 1:  # strides of dims with one entry do not matter
-            a.x_head = a.y_head = 0
+        heads, n_rows = xs[1], ys[0]
+        if heads == 1:  # strides of dims with one entry do not matter
+            xh = yh = 0
         if T == 1:
-            a.x_token = 0
-        if ys[0] == 1:
-            a.y_token = 0
-        a.x, a.y, a.x_type, a.y_type = x.data_ptr(), y.data_ptr(), _elem(x, "rope"), _elem(y, "rope")
-        a.heads, a.rotate, a.n_rows = xs[1], s.rotate, ys[0]
+            xt = 0
+        if n_rows == 1:
+            yt = 0
+        normw = rows = 0
         if s.normw is not None:
-            a.normw = _vector("rope", dev, "normw", s.normw, torch.float32, (D,))
+            normw = _vector("rope", dev, "normw", s.normw, f32, (D,))
         if s.rows is not None:
-            a.rows = _vector("rope", dev, "rows", s.rows, i32, (T,))
+            rows = _vector("rope", dev, "rows", s.rows, i32, (T,))
+        elif n_rows != T:
+            raise RuntimeError(f"rope: y has {n_rows} rows for {T} tokens")
+        packed += _ROPE_SEG.pack(x.data_ptr(), y.data_ptr(), _elem(x, "rope"), _elem(y, "rope"), heads, s.rotate, xt, xh,
+                                 yt, yh, normw, rows, n_rows)
     pos_ptr = _vector("rope", dev, "pos", pos, i32, (T,))
-    _on("rope", dev, "table", table.turns)
-    _launch(dev, stream, lambda st: check(
-        lib().btf_rope(arr, n, T, D, table.n_rot, table.turns.data_ptr(), table.mscale, table.interleaved, inverse, eps,
-                       pos_ptr, st), "btf_rope"))
+    turns = table.turns
+    if turns is None or turns.device != dev:
+        raise RuntimeError(f"rope: the table must be on {dev}")
+    _launch(dev, stream, _rope_call, (packed, n, T, D, table.n_rot, turns.data_ptr(), table.mscale, table.interleaved,
+                                      inverse, eps, pos_ptr))
+
+
+def _rope_call(st, args) -> None:
+    status = _lib.btf_rope(*args, st)
+    if status:
+        check(status, "btf_rope")
 
 
 def tree_attention_work(q, k):
@@ -780,38 +796,42 @@ def tree_attention(q, k, v, lens, parents, counts=None, scale: Optional[float] =
                            f"{tuple(ks)}, {tuple(v.shape)}")
     B, n, H, D = qs
     dev, dtype, i32 = _cuda_device("tree_attention", q), q.dtype, torch.int32
-    _on("tree_attention", dev, "k", k)
-    _on("tree_attention", dev, "v", v)
-    a = TreeAttnC()
-    a.lens = _vector("tree_attention", dev, "lens", lens, i32, (B,))
-    a.parents = _vector("tree_attention", dev, "parents", parents, i32, (B, n))
-    if counts is not None:
-        a.counts = _vector("tree_attention", dev, "counts", counts, i32, (B,))
+    if k.device != dev or v.device != dev:
+        raise RuntimeError(f"tree_attention: k and v must be on {dev}, got {k.device} and {v.device}")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise RuntimeError("tree_attention: q, k and v must have one type")
+    vectors = (_vector("tree_attention", dev, "lens", lens, i32, (B,)),
+               _vector("tree_attention", dev, "parents", parents, i32, (B, n)),
+               0 if counts is None else _vector("tree_attention", dev, "counts", counts, i32, (B,)))
+    return _launch(dev, stream, _tree_call, (q, k, v, vectors, D ** -0.5 if scale is None else scale, out, work))
 
-    def call(st):
-        o = out
-        if o is None:
-            o = (torch.empty if counts is None else torch.zeros)(qs, dtype=dtype, device=dev)
-        if o.shape != qs or k.dtype != dtype or v.dtype != dtype or o.dtype != dtype:
-            raise RuntimeError("tree_attention: q, k, v and out must have one type, and out the shape of q")
-        _on("tree_attention", dev, "out", o)
-        a.q_batch, a.q_node, a.q_head, qd = _strides(q)
-        a.kv_batch, a.kv_row, a.kv_head, kd = kv = _strides(k)
-        a.o_batch, a.o_node, a.o_head, od = _strides(o)
-        if kv != _strides(v) or (D > 1 and not qd == kd == od == 1):
-            raise RuntimeError("tree_attention: the dims of a head must be contiguous, and k and v strided alike")
-        if B == 0:
-            return o
-        w = tree_attention_work(q, k) if work is None else work
-        _on("tree_attention", dev, "work", w)
-        a.q, a.k, a.v, a.o, a.work = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), w.data_ptr()
-        a.type, a.B, a.n, a.H, a.HK, a.D, a.n_ctx = _elem(q, "tree_attention"), B, n, H, ks[2], D, ks[1]
-        a.scale = D ** -0.5 if scale is None else scale
-        a.work_bytes = w.numel() * w.element_size()
-        check(lib().btf_tree_attention(ctypes.byref(a), st), "btf_tree_attention")
-        return o
 
-    return _launch(dev, stream, call)
+def _tree_call(st, args):
+    q, k, v, vectors, scale, out, work = args
+    torch = _torch()
+    (B, n, H, D), ks, dev = q.shape, k.shape, q.device
+    if out is None:
+        out = (torch.zeros if vectors[2] else torch.empty)(q.shape, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+        raise RuntimeError("tree_attention: out must be as q")
+    if B == 0:
+        return out
+    if work is None:
+        work = tree_attention_work(q, k)
+    elif work.device != dev:
+        raise RuntimeError(f"tree_attention: work is on {work.device}, not on {dev}")
+    q0, q1, q2, qd = _strides(q)
+    k0, k1, k2, kd = kv = _strides(k)
+    o0, o1, o2, od = _strides(out)
+    if kv != _strides(v) or (D > 1 and not qd == kd == od == 1):
+        raise RuntimeError("tree_attention: the dims of a head must be contiguous, and k and v strided alike")
+    packed = _TREE_ATTN.pack(q.data_ptr(), q0, q1, q2, k.data_ptr(), v.data_ptr(), k0, k1, k2, out.data_ptr(), o0, o1, o2,
+                             _elem(q, "tree_attention"), B, n, H, ks[2], D, ks[1], *vectors, scale, work.data_ptr(),
+                             work.nbytes)
+    status = _lib.btf_tree_attention(packed, st)
+    if status:
+        check(status, "btf_tree_attention")
+    return out
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprobs=None, stream=None):
@@ -827,17 +847,22 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     pk = _vector("sample", dev, "top_k", top_k, i32, rows)
     pp = _vector("sample", dev, "top_p", top_p, f32, rows)
     pm = _vector("sample", dev, "min_p", min_p, f32, rows)
-    ld = logits.stride(0) if B > 1 else V
+    return _launch(dev, stream, _sample_call, (logits, (pu, pt, pk, pp, pm), tokens, logprobs))
 
-    def call(st):
-        tok = torch.empty(B, dtype=i32, device=dev) if tokens is None else tokens
-        lp = torch.empty(B, dtype=f32, device=dev) if logprobs is None else logprobs
-        check(lib().btf_sample(logits.data_ptr(), _elem(logits, "sample"), ld, B, V, pu, pt, pk, pp, pm,
-                               _vector("sample", dev, "tokens", tok, i32, rows),
-                               _vector("sample", dev, "logprobs", lp, f32, rows), st), "btf_sample")
-        return tok, lp
 
-    return _launch(dev, stream, call)
+def _sample_call(st, args):
+    logits, params, tokens, logprobs = args
+    (B, V), dev, torch = logits.shape, logits.device, _torch()
+    if tokens is None:
+        tokens = torch.empty(B, dtype=torch.int32, device=dev)
+    if logprobs is None:
+        logprobs = torch.empty(B, dtype=torch.float32, device=dev)
+    status = _lib.btf_sample(logits.data_ptr(), _elem(logits, "sample"), logits.stride(0) if B > 1 else V, B, V, *params,
+                             _vector("sample", dev, "tokens", tokens, torch.int32, (B,)),
+                             _vector("sample", dev, "logprobs", logprobs, torch.float32, (B,)), st)
+    if status:
+        check(status, "btf_sample")
+    return tokens, logprobs
 
 
 PTQ1_0 = 143

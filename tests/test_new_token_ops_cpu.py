@@ -140,3 +140,16 @@ def test_python_wrappers_refuse_host_tensors(btf):
         btf.sample(torch.zeros(2, 10), torch.zeros(2))
     with pytest.raises(RuntimeError, match="contiguous"):
         btf.sample(torch.zeros(10, 2).t(), torch.zeros(2))
+
+
+def test_packed_arguments_are_the_structs(btf):
+    """The wrappers fill the argument structs by struct.pack: the same bytes as the ctypes fields."""
+    v = list(range(1, 14))
+    v[5] = 1
+    assert btf._ROPE_SEG.pack(*v) == bytes(btf.RopeSegC(*v))
+    v = list(range(1, 27))
+    assert len(v) == len(btf.TreeAttnC._fields_)
+    a, b = btf._TREE_ATTN.pack(*v), btf.TreeAttnC(*v)
+    assert btf.TreeAttnC.from_buffer_copy(a).work_bytes == 26 and len(a) == ctypes.sizeof(b)
+    for name, _ in btf.TreeAttnC._fields_:
+        assert getattr(btf.TreeAttnC.from_buffer_copy(a), name) == getattr(b, name), name
