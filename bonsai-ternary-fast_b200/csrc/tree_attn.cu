@@ -14,10 +14,10 @@
 // So up to 128 rows a kv-head the kernel is bound by the cache's bytes, and beyond
 // that (more M tiles over the same cache, which then comes from L2) by the MMAs.
 //
-// Work: the 64-row tiles of all (sequence, kv-head) pairs in one line, by their
-// present lengths, cut into equal ranges, one per resident CTA (per M tile: the
-// CTAs of one range's M tiles read the same rows at the same time). A pair that
-// crosses a border is finished by a second kernel from its parts; a short cache, a
+// Work: the 64-row tiles of all (sequence, kv-head) pairs, by their present
+// lengths, in as many equal ranges as there are resident CTAs (per M tile: the
+// CTAs of one range's M tiles read the same rows at the same time). A pair of
+// several ranges is finished by a second kernel from its parts; a short cache, a
 // long one and a ragged batch all fill the card. Warp 4 loads K and V tiles by TMA
 // into a ring, warp 5 issues the MMAs, warps 0..3 hold one q row per thread:
 //   S = Q K^T (64 columns of tensor memory, two of them in turn) -> registers,
@@ -48,7 +48,6 @@ using namespace tc;
 constexpr int kTile = 64;  // rows of K and V per tile
 constexpr int kRowsM = 128;
 constexpr int kThreads = 192;
-constexpr int kMinTiles = 2;  // fewest tiles of a range
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr float kLag = 8.0f;  // log2 of how far a row's maximum may run ahead of m
 
@@ -83,7 +82,8 @@ struct TreeParams {
   const int32_t *lens, *parents, *counts;
   float scale2;     // |scale| log2(e), at least 2^-100 (0 times the -inf of a masked score would be NaN)
   uint32_t q_flip;  // sign bits of two q when scale < 0
-  int32_t* first;   // workspace: first tile of each sequence in the line of all tiles; behind the last: tiles per range
+  int32_t* first;   // workspace: each sequence's first range, or first tile in the line of all tiles; then tiles per
+                    // range, and which of the two it is
   float* part;      // parts: [mtiles][2 ranges][128][D]
   float* ml;        // their (m, l): [mtiles][2 ranges][128][2]
   int* err;
@@ -101,6 +101,12 @@ struct Seq {
 };
 
 // The segments of a CTA's range: runs of tiles of one (sequence, kv-head).
+//
+// Up to 32 sequences with fewer pairs than ranges: every pair is cut into its own
+// number of equal ranges, n_b = ceil(tiles / per) with the least `per` that fits, and a
+// CTA has one segment (a second one costs its q and its way out again, about 5 tiles
+// of time: 1 x 1 node over 513 rows took 15.5 us with ranges across pairs, 11.1
+// without). Otherwise the line of all tiles is cut into equal ranges.
 struct Segments {
   const TreeParams& p;
   int b, kvh, tile, nt, index;  // the present one; index: in the CTA
@@ -110,15 +116,12 @@ struct Segments {
   __device__ __forceinline__ Segments(const TreeParams& p_, int range, bool table)
       : p(p_), b(0), kvh(0), tile(0), nt(0), index(0), left(0) {
     const int lane = threadIdx.x & 31;
-    // the lane's sequence of the 32 from b0: its tiles, and those of all up to it
-    Seq mine;
-    auto line = [&](int b0, int* own) {
-      int t = 0;
-      if (b0 + lane < p.B) {
-        mine = Seq(p, b0 + lane);
-        t = mine.tiles * p.HK;
-      }
-      *own = t;
+    Seq mine;  // the lane's sequence of the 32 from b0
+    auto load = [&](int b0) {
+      mine.count = mine.len = mine.tiles = 0;
+      if (b0 + lane < p.B) mine = Seq(p, b0 + lane);
+    };
+    auto up_to = [&](int t) {  // the sum of the lanes up to this one
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int q = __shfl_up_sync(0xffffffffu, t, o);
@@ -126,29 +129,57 @@ struct Segments {
       }
       return t;
     };
-    int total = 0, own, t = 0;
+    // the sequence of the 32 from b0 in whose share of a line (up to `t` for each lane) `at` lies
+    auto pick = [&](int b0, int t, int* at) -> bool {
+      const unsigned in = __ballot_sync(0xffffffffu, t > *at);
+      if (!in) return false;
+      const int l = __ffs(in) - 1, before = __shfl_sync(0xffffffffu, t, max(l - 1, 0));
+      b = b0 + l;
+      *at -= l ? before : 0;
+      seq.count = __shfl_sync(0xffffffffu, mine.count, l);
+      seq.len = __shfl_sync(0xffffffffu, mine.len, l);
+      seq.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
+      return true;
+    };
+    load(0);
+    const int pairs = p.HK * __popc(__ballot_sync(0xffffffffu, mine.tiles > 0));
+    if (p.B <= 32 && pairs <= p.ranges) {
+      const int total = p.HK * __reduce_add_sync(0xffffffffu, mine.tiles);
+      int per = max(1, (total + p.ranges - 1) / p.ranges);
+      // sum ceil(tiles / per) <= total / per + pairs
+      int most = pairs < p.ranges ? max(per, (total + p.ranges - pairs - 1) / (p.ranges - pairs)) : max(1, total);
+      while (per < most) {
+        const int mid = (per + most) / 2;
+        if (p.HK * __reduce_add_sync(0xffffffffu, (mine.tiles + mid - 1) / mid) <= p.ranges) most = mid;
+        else per = mid + 1;
+      }
+      const int n = (mine.tiles + per - 1) / per, t = up_to(n * p.HK);
+      if (table && lane < p.B) p.first[lane] = t - n * p.HK;
+      if (table && lane == 0) p.first[p.B] = per, p.first[p.B + 1] = 1;
+      int at = range;
+      if (!pick(0, t, &at)) return;
+      const int ns = (seq.tiles + per - 1) / per, part = at % ns;
+      kvh = at / ns;
+      tile = (int)((int64_t)part * seq.tiles / ns);
+      nt = (int)((int64_t)(part + 1) * seq.tiles / ns) - tile;
+      return;
+    }
+    int total = 0, t = 0;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
-      t = line(b0, &own);
-      if (table && b0 + lane < p.B) p.first[b0 + lane] = total + t - own;
+      load(b0);
+      t = up_to(mine.tiles * p.HK);
+      if (table && b0 + lane < p.B) p.first[b0 + lane] = total + t - mine.tiles * p.HK;
       total += __shfl_sync(0xffffffffu, t, 31);
     }
-    const int per = max(kMinTiles, (total + p.ranges - 1) / p.ranges);
-    if (table && lane == 0) p.first[p.B] = per;
+    const int per = max(1, (total + p.ranges - 1) / p.ranges);
+    if (table && lane == 0) p.first[p.B] = per, p.first[p.B + 1] = 0;
     if ((int64_t)range * per >= total) return;
     int start = range * per;
     left = min(per, total - start);
     for (int b0 = 0;; b0 += 32) {  // the sequence that the range starts in
-      if (p.B > 32) t = line(b0, &own);
-      const unsigned in = __ballot_sync(0xffffffffu, t > start);
-      if (in) {
-        const int l = __ffs(in) - 1, before = __shfl_sync(0xffffffffu, t, max(l - 1, 0));
-        b = b0 + l;
-        start -= l ? before : 0;
-        seq.count = __shfl_sync(0xffffffffu, mine.count, l);
-        seq.len = __shfl_sync(0xffffffffu, mine.len, l);
-        seq.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
-        break;
-      }
+      load(b0);
+      t = up_to(mine.tiles * p.HK);
+      if (pick(b0, t, &start)) break;
       start -= __shfl_sync(0xffffffffu, t, 31);
     }
     kvh = start / seq.tiles;
@@ -778,12 +809,18 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   const int per = p.first[p.B], first = p.first[b];
   const Seq seq(p, b);
   if (node >= seq.count) return;
-  const int t0 = first + head / G * seq.tiles, t1 = t0 + seq.tiles - 1;
-  const int r0 = t0 / per, parts = t1 / per - r0 + 1;
+  int r0, parts;
+  bool second = false;  // whether r0 begins with another pair's tiles
+  if (p.first[p.B + 1]) {
+    parts = (seq.tiles + per - 1) / per;
+    r0 = first + head / G * parts;
+  } else {
+    const int t0 = first + head / G * seq.tiles, t1 = t0 + seq.tiles - 1;
+    r0 = t0 / per, parts = t1 / per - r0 + 1;
+    second = r0 * per < t0;
+  }
   if (parts == 1) return;  // written whole
   const int rr = node * G + head % G;
-  // part s is range r0 + s's first segment when the range starts at the pair's first tile or behind it
-  const bool second = r0 * per < t0;
   const int64_t base = ((int64_t)(rr / kRowsM) * 2 * p.ranges + 2 * r0) * kRowsM + rr % kRowsM;
   auto at = [&](int s) { return base + (2 * s + (s == 0 && second)) * kRowsM; };
   const float2* ml = reinterpret_cast<const float2*>(p.ml);
@@ -861,8 +898,8 @@ Plan tree_plan(const DeviceInfo& d, int B, int n, int H, int HK, int D, int n_ct
   r.mtiles = (n * (H / HK) + kRowsM - 1) / kRowsM;
   const int64_t tiles = (int64_t)B * HK * ((n_ctx + kTile - 1) / kTile);
   const int64_t slots = std::max(1, d.sm_count * (D <= 128 ? 2 : 1) / r.mtiles);
-  r.ranges = (int)std::max<int64_t>(1, std::min(slots, (tiles + kMinTiles - 1) / kMinTiles));
-  r.off_part = ((int64_t)(B + 1) * 4 + 255) / 256 * 256;
+  r.ranges = (int)std::max<int64_t>(1, std::min(slots, tiles));
+  r.off_part = ((int64_t)(B + 2) * 4 + 255) / 256 * 256;
   const int64_t rows = (int64_t)r.mtiles * 2 * r.ranges * kRowsM;
   r.off_ml = r.off_part + rows * D * 4;
   r.bytes = r.off_ml + rows * 8;
@@ -899,8 +936,8 @@ cudaError_t launch_tree_d(const CUtensorMap& mk, const CUtensorMap& mv, const Tr
                                      : launch_tree<T, 256>(mk, mv, p, st);
   if (e != cudaSuccess || p.ranges == 1) return e;
   const int rows = p.B * p.n * p.H;
-  // up to two CTAs per SM of one row each are one wave of latency
-  if (rows <= 2 * sms) return launch_pdl(tree_join_kernel<T, 8>, dim3(rows), dim3(kJoinThreads), 0, st, p);
+  // a CTA per row while all of them are resident at once
+  if (rows <= 8 * sms) return launch_pdl(tree_join_kernel<T, 8>, dim3(rows), dim3(kJoinThreads), 0, st, p);
   return launch_pdl(tree_join_kernel<T, 1>, dim3((rows + 7) / 8), dim3(kJoinThreads), 0, st, p);
 }
 
