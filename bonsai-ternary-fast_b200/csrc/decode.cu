@@ -86,7 +86,9 @@ __device__ __forceinline__ float rms_scale(double sumsq, int n, float eps) {
 // One CTA per transform block of `blk` columns (blk threads; blk = 0: no
 // transform, 256 columns per CTA). Row r of the panel matrix: group r/8, quad
 // (r%8)/4, bit pair 2*(r%4) of byte (c%4) of word (c%16)/4 of the 16-column half.
-__global__ void embed_kernel(const uint8_t* __restrict__ pan, int V, int E, int S, const int32_t* __restrict__ tok,
+// What an earlier kernel writes has no __restrict__ here and below: the compiler
+// takes such a load for one of constant memory and may move it above pdl_wait().
+__global__ void embed_kernel(const uint8_t* __restrict__ pan, int V, int E, int S, const int32_t* tok,
                              int blk, const float* __restrict__ signs, float* __restrict__ x) {
   extern __shared__ float sh[];
   pdl_launch_dependents();
@@ -507,7 +509,7 @@ __device__ __forceinline__ void better(float& v, int& i, float v2, int i2) {
     i = i2;
   }
 }
-__global__ void argmax1_kernel(const float* __restrict__ x, int n, float* __restrict__ pv, int* __restrict__ pi) {
+__global__ void argmax1_kernel(const float* x, int n, float* pv, int* pi) {
   __shared__ float sv[32];
   __shared__ int si[32];
   pdl_launch_dependents();
@@ -531,8 +533,8 @@ __global__ void argmax1_kernel(const float* __restrict__ x, int n, float* __rest
 }
 // Stage 2: one warp; writes the token, and the next step's input token and
 // position (pos += 1) when those pointers are given.
-__global__ void argmax2_kernel(const float* __restrict__ pv, const int* __restrict__ pi, int parts,
-                               int32_t* __restrict__ out, int32_t* __restrict__ tok_next, int32_t* __restrict__ pos) {
+__global__ void argmax2_kernel(const float* pv, const int* pi, int parts, int32_t* out, int32_t* tok_next,
+                               int32_t* pos) {
   pdl_launch_dependents();
   pdl_wait();
   float v = -INFINITY;

@@ -15,7 +15,7 @@ constexpr int kQThreads = 256;
 
 // One thread per 4 consecutive values, 8 lanes per 32-block (q8_quad).
 __global__ void __launch_bounds__(kQThreads)
-    quant_q8_kernel(const float* __restrict__ x, int ldx, int K, int8_t* __restrict__ q, float* __restrict__ d,
+    quant_q8_kernel(const float* x, int ldx, int K, int8_t* __restrict__ q, float* __restrict__ d,
                     int32_t* __restrict__ s, unsigned long long* stamp) {
   const int nquad = K / 4;
   const int qi = blockIdx.x * kQThreads + threadIdx.x;
