@@ -43,6 +43,7 @@ EXPORTS = (
     "btf_gemm_f32_noalloc", "btf_chain_program_bytes", "btf_chain_encode", "btf_chain_run", "btf_stamp_next",
     "btf_gemm_idot", "btf_decoder_prefill", "btf_gemm_wm", "btf_gemm_wm_idot", "btf_gemv_mma", "btf_gemv_mma_idot",
     "btf_rope_table", "btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample",
+    "btf_decoder_step_sampled", "btf_decoder_run_sampled", "btf_decoder_verify", "btf_decoder_accept",
 )
 
 
@@ -124,6 +125,13 @@ class DecoderInfoC(ctypes.Structure):
     _fields_ = [("dims", DecoderDimsC), ("pos", ctypes.c_int), ("stream", ctypes.c_void_p),
                 ("weight_bytes", ctypes.c_uint64), ("state_bytes", ctypes.c_uint64),
                 ("kv_bytes_per_token", ctypes.c_uint64), ("logits", ctypes.c_void_p), ("device_bytes", ctypes.c_uint64)]
+
+
+class SamplingC(ctypes.Structure):
+    """btf_sampling: the parameters of a drawn token."""
+
+    _fields_ = [("temperature", ctypes.c_float), ("top_k", ctypes.c_int), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float)]
 
 
 class StepStatsC(ctypes.Structure):
@@ -251,6 +259,11 @@ def lib() -> ctypes.CDLL:
         "btf_decoder_stats": (i32, [vp, ctypes.POINTER(StepStatsC)]),
         "btf_decoder_reset_stats": (i32, [vp]),
         "btf_plan_memory": (i32, [ctypes.c_char_p, ctypes.POINTER(DecoderOptsC), i32, i32, ctypes.POINTER(MemoryPlanC)]),
+        "btf_decoder_step_sampled": (i32, [vp, ctypes.c_int32, ctypes.POINTER(SamplingC), ctypes.c_float, vp,
+                                           ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_float)]),
+        "btf_decoder_run_sampled": (i32, [vp, i32, ctypes.POINTER(SamplingC), vp]),
+        "btf_decoder_verify": (i32, [vp, vp, vp, i32, ctypes.POINTER(SamplingC), vp, vp, vp]),
+        "btf_decoder_accept": (i32, [vp, i32]),
         "btf_rope_table": (i32, [ctypes.POINTER(RopeCfgC), vp, ctypes.POINTER(ctypes.c_float)]),
         "btf_rope": (i32, [vp, i32, i32, i32, i32, vp, ctypes.c_float, i32, i32, ctypes.c_float,
                            vp, vp]),
@@ -1048,6 +1061,52 @@ class Decoder:
     def run(self, steps: int) -> None:
         """`steps` greedy steps on the device (asynchronous on the decoder's stream)."""
         check(lib().btf_decoder_run(self.h, steps), "btf_decoder_run")
+
+    def step_sampled(self, token: int, u: float, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                     min_p: float = 0.0, logits: bool = False):
+        """One token -> (next token drawn with u in [0, 1), its log-probability, logits or None)
+        (btf_decoder_step_sampled; the parameters are sample()'s)."""
+        import numpy as np
+
+        out = np.empty(self.info()["n_vocab"], dtype=np.float32) if logits else None
+        nxt, lp = ctypes.c_int32(), ctypes.c_float()
+        check(lib().btf_decoder_step_sampled(self.h, token, ctypes.byref(SamplingC(temperature, top_k, top_p, min_p)), u,
+                                             out.ctypes.data if logits else None, ctypes.byref(nxt), ctypes.byref(lp)),
+              "btf_decoder_step_sampled")
+        return nxt.value, lp.value, out
+
+    def run_sampled(self, us, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0) -> None:
+        """len(us) steps on the device, each drawing its token with its u (asynchronous on the decoder's stream)."""
+        import numpy as np
+
+        u = np.ascontiguousarray(np.asarray(us, dtype=np.float32))
+        check(lib().btf_decoder_run_sampled(self.h, len(u), ctypes.byref(SamplingC(temperature, top_k, top_p, min_p)),
+                                            u.ctypes.data), "btf_decoder_run_sampled")
+
+    def verify(self, tokens, parents, sampling: Optional[dict] = None, us=None, logits: bool = False):
+        """Checks a tree of drafted tokens in one pass over the weights (btf_decoder_verify): node j follows node
+        parents[j], or the decoded tokens (-1). Returns (the token after each node: greedy, or drawn with us[j] and
+        sampling = dict(temperature=, top_k=, top_p=, min_p=); logits [n][n_vocab] or None). accept() takes a path."""
+        import numpy as np
+
+        t, p = (np.ascontiguousarray(np.asarray(a, dtype=np.int32)) for a in (tokens, parents))
+        n = len(t)
+        if p.shape != t.shape or (sampling is not None and (us is None or len(us) != n)):
+            raise RuntimeError("verify: a parent per token, and a random number per token to draw with")
+        nxt = np.empty(n, dtype=np.int32)
+        out = np.empty((n, self.info()["n_vocab"]), dtype=np.float32) if logits else None
+        s, u = None, None
+        if sampling is not None:
+            s = SamplingC(**{"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0, **sampling})
+            u = np.ascontiguousarray(np.asarray(us, dtype=np.float32))
+        check(lib().btf_decoder_verify(self.h, t.ctypes.data, p.ctypes.data, n, None if s is None else ctypes.byref(s),
+                                       None if u is None else u.ctypes.data, out.ctypes.data if logits else None,
+                                       nxt.ctypes.data), "btf_decoder_verify")
+        return nxt, out
+
+    def accept(self, node: int) -> None:
+        """Takes over the path down to `node` of the last verify() (btf_decoder_accept)."""
+        check(lib().btf_decoder_accept(self.h, node), "btf_decoder_accept")
 
     def reset(self) -> None:
         check(lib().btf_decoder_reset(self.h), "btf_decoder_reset")

@@ -189,6 +189,7 @@ struct GdnParams {
   float eps;
   const int32_t* pos;
   float* o;           // [DI]
+  const float *ring_from, *state_from;  // read instead of ring and state (the same, or a parent's)
 };
 __global__ void gdn_mix_kernel(const __grid_constant__ GdnParams p) {
   extern __shared__ float sm[];  // q[DK], k[DK], v[DV], out[DV]
@@ -223,10 +224,12 @@ __global__ void gdn_mix_kernel(const __grid_constant__ GdnParams p) {
   // flight during the dots, the conv and the norms below
   const int j = tid / kTpc, part = tid % kTpc;
   const int nt = p.DK / (4 * kTpc);
-  float4* col = reinterpret_cast<float4*>(p.state + ((int64_t)h * p.DV + j) * p.DK) + part;
+  const int64_t col0 = ((int64_t)h * p.DV + j) * p.DK;
+  float4* col = reinterpret_cast<float4*>(p.state + col0) + part;
+  const float4* from = reinterpret_cast<const float4*>(p.state_from + col0) + part;
   float4 st[8];
 #pragma unroll
-  for (int t = 0; t < 8; ++t) st[t] = t < nt ? col[t * kTpc] : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int t = 0; t < 8; ++t) st[t] = t < nt ? from[t * kTpc] : make_float4(0.f, 0.f, 0.f, 0.f);
   // alpha / beta dots
   double sa = 0.0, sb = 0.0;
   {
@@ -257,7 +260,9 @@ __global__ void gdn_mix_kernel(const __grid_constant__ GdnParams p) {
     float sum = 0.f;
     for (int i = 0; i < p.K - 1; ++i) {
       const int slot = ((pos - (p.K - 1) + i) % p.K + p.K) % p.K;
-      sum = __fadd_rn(sum, __fmul_rn(p.ring[(int64_t)slot * p.C + c], p.conv_w[(int64_t)c * p.K + i]));
+      const float tap = p.ring_from[(int64_t)slot * p.C + c];
+      if (p.ring_from != p.ring) p.ring[(int64_t)slot * p.C + c] = tap;
+      sum = __fadd_rn(sum, __fmul_rn(tap, p.conv_w[(int64_t)c * p.K + i]));
     }
     const float xin = p.qkv[c];
     sum = __fadd_rn(sum, __fmul_rn(xin, p.conv_w[(int64_t)c * p.K + p.K - 1]));
@@ -497,6 +502,16 @@ __global__ void attn_fused_kernel(const __grid_constant__ AttnParams p) {
   if (tid == 0) p.cnt[h] = 0;
 }
 
+// The output gate of M rows of attention outputs, one element per thread.
+__global__ void gate_kernel(const __half* a, const float* qf, int M, int H, int D, float* o) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= (int64_t)M * H * D) return;
+  const int64_t mh = i / D;  // row m's head h: its q and gate lie at mh * 2 D
+  o[i] = __half2float(a[i]) * sigmoidf_(qf[mh * 2 * D + D + (i - mh * D)]);
+}
+
 // ------------------------------------------------------------------ argmax
 // Stage 1: CTA b takes a contiguous range; (value, index) with the lowest
 // index among equal maxima. NaN counts as -inf (the emulator's
@@ -624,7 +639,8 @@ cudaError_t launch_embed(const uint8_t* pan, int V, int E, const int32_t* tok, i
 }
 cudaError_t launch_gdn_mix(const GdnArgs& g, cudaStream_t st) {
   const GdnParams p{g.xn, g.aw, g.bw, g.dt, g.a, g.E, g.bf16_in, g.qkv, g.ring, g.conv_w, g.K, g.C, g.z, g.state,
-                    g.norm_w, g.NK, g.DK, g.DV, g.QK, g.eps, g.pos, g.o};
+                    g.norm_w, g.NK, g.DK, g.DV, g.QK, g.eps, g.pos, g.o, g.ring_from ? g.ring_from : g.ring,
+                    g.state_from ? g.state_from : g.state};
   return launch_pdl(gdn_mix_kernel, dim3(g.NV), dim3(g.DV * kTpc), (size_t)(2 * g.DK + 2 * g.DV) * sizeof(float), st,
                     p);
 }
@@ -637,6 +653,11 @@ cudaError_t launch_attention_fused(const float* qf, const float* k, const float*
                (n_ctx + splits - 1) / splits, static_cast<__half*>(kc), static_cast<__half*>(vc), part, cnt, o};
   const size_t smem = (size_t)(4 * D + (threads / 32) * (D + 2)) * sizeof(float);
   return launch_pdl(attn_fused_kernel, dim3(H, splits), dim3(threads), smem, st, p);
+}
+cudaError_t launch_gate(const void* a, const float* qf, int M, int H, int D, float* o, cudaStream_t st) {
+  const int64_t n = (int64_t)M * H * D;
+  return launch_pdl(gate_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, static_cast<const __half*>(a), qf,
+                    M, H, D, o);
 }
 cudaError_t launch_argmax(const float* x, int n, float* pv, int* pi, int parts, int32_t* out, int32_t* tok_next,
                           int32_t* pos, cudaStream_t st) {

@@ -28,6 +28,9 @@ struct GdnArgs {
   const int32_t* pos;
   float* o;
   int NV;
+  // where the ring and the state are read from, when not from where they are written
+  // (a drafted token's own copies follow its parent's)
+  const float *ring_from = nullptr, *state_from = nullptr;
 };
 cudaError_t launch_gdn_mix(const GdnArgs& args, cudaStream_t st);
 // The attention of one layer at position *pos, one launch: q/k RMSNorm + RoPE
@@ -40,6 +43,9 @@ cudaError_t launch_attention_fused(const float* qf, const float* k, const float*
                                    int H, int HK, int D, int R, float theta_scale, float eps, const int32_t* pos,
                                    int round_q, void* kc, void* vc, int n_ctx, int splits, float* part, int* cnt,
                                    float* o, cudaStream_t st);
+// o[m][H * D] = a[m][H * D] * sigmoid(gate of qf[m][H][2 D]) for M rows (the output
+// gate of the attention, applied to btf_tree_attention's fp16 outputs).
+cudaError_t launch_gate(const void* a, const float* qf, int M, int H, int D, float* o, cudaStream_t st);
 // Greedy argmax of x[n] (lowest index on ties) -> *out; also *tok_next = token and
 // *pos += 1 when those are non-null. pv/pi: `parts` partials.
 cudaError_t launch_argmax(const float* x, int n, float* pv, int* pi, int parts, int32_t* out, int32_t* tok_next,

@@ -29,6 +29,7 @@
 #include "common.cuh"
 #include "decode.h"
 #include "gguf_meta.h"
+#include "sample.h"
 
 namespace btf {
 namespace {
@@ -61,6 +62,7 @@ struct Layer {
         *ssm_norm = nullptr;
   int ab_bf16 = 0;
   float *conv_state = nullptr, *ssm_state = nullptr;
+  float *node_ring = nullptr, *node_state = nullptr;  // the drafted nodes' own, kMaxChunk of them
   // attention
   Mat wq, wk, wv, wo;
   float *q_norm = nullptr, *k_norm = nullptr;
@@ -93,6 +95,19 @@ struct Decoder {
   static constexpr int kMaxChunk = 8;
   int32_t *d_ptok = nullptr, *d_ppos = nullptr;
   int32_t* h_io = nullptr;  // pinned: [0] token in, [1] token out
+  // sampled steps: {temperature, top_p, min_p, top_k} of every row, then random
+  // numbers and log-probabilities (allocated by the first)
+  static constexpr int kMaxRandom = 4096;
+  float* d_rows[4] = {};  // [kMaxChunk] each
+  float *d_u = nullptr, *d_lp = nullptr;
+  // drafted tokens (allocated by the first btf_decoder_verify)
+  double* rope_turns = nullptr;
+  __half *q16 = nullptr, *o16 = nullptr;
+  float* node_logits = nullptr;
+  int32_t *d_parents = nullptr, *d_rows_of = nullptr, *d_nexts = nullptr;
+  uint8_t* tree_work = nullptr;
+  int64_t tree_work_bytes = 0;
+  int draft_n = 0, draft_parent[kMaxChunk] = {};  // the draft that btf_decoder_accept may take from
   int pos = 0;
   cudaGraph_t graph = nullptr;
   cudaGraphExec_t exec = nullptr;
@@ -222,6 +237,7 @@ int make_buffers(Decoder& D) {
 
 int reset_state(Decoder& D) {
   cudaError_t e = cudaSuccess;
+  D.draft_n = 0;
   for (Layer& l : D.L) {
     if (l.rec) {
       if (e == cudaSuccess)
@@ -368,6 +384,143 @@ int enqueue_chunk(Decoder& D, int M) {
   return BTF_OK;
 }
 
+// ---------------------------------------------------------------- sampled steps
+// The parameters (the same for every row) and n_u random numbers go to the device, in stream order.
+int set_sampling(Decoder& D, const btf_sampling& s, const float* u, int n_u) {
+  constexpr int R = Decoder::kMaxChunk;
+  if (!D.d_u) {
+    int rc = BTF_OK;
+    float* p = D.alloc<float>(4 * R + Decoder::kMaxRandom + R, &rc);
+    if (rc) return rc;
+    for (int i = 0; i < 4; ++i) D.d_rows[i] = p + i * R;
+    D.d_lp = p + 4 * R;
+    D.d_u = p + 5 * R;
+  }
+  float h[4 * R];
+  for (int i = 0; i < R; ++i) {
+    h[i] = s.temperature;
+    h[R + i] = s.top_p;
+    h[2 * R + i] = s.min_p;
+    std::memcpy(&h[3 * R + i], &s.top_k, 4);
+  }
+  cudaError_t e = cudaMemcpyAsync(D.d_rows[0], h, sizeof h, cudaMemcpyHostToDevice, D.st);  // (pageable: staged at once)
+  if (e == cudaSuccess && n_u) e = cudaMemcpyAsync(D.d_u, u, n_u * sizeof(float), cudaMemcpyHostToDevice, D.st);
+  return e == cudaSuccess ? BTF_OK : cuda_fail(e, "btf_decoder: sampling parameters");
+}
+cudaError_t sample_rows(Decoder& D, const float* logits, int n, const float* u, int32_t* tokens, int32_t* tokens2) {
+  const SampleArgs a{logits, BTF_F32, D.d.n_vocab, n, D.d.n_vocab, u, D.d_rows[0], reinterpret_cast<int32_t*>(D.d_rows[3]),
+                     D.d_rows[1], D.d_rows[2], tokens, tokens2, D.d_lp};
+  return launch_sample(a, D.st);
+}
+int check_sampling(const Decoder& D, const btf_sampling* s, const char* who) {
+  if (!s) return fail(BTF_ERR_ARG, "%s: null sampling", who);
+  if (D.d.n_vocab > BTF_SAMPLE_MAX_V)
+    return fail(BTF_ERR_UNSUPPORTED, "%s: n_vocab above %d", who, BTF_SAMPLE_MAX_V);
+  return BTF_OK;
+}
+
+// ---------------------------------------------------------------- drafted tokens
+int make_draft_buffers(Decoder& D) {
+  if (D.node_logits) return BTF_OK;
+  const btf_decoder_dims& d = D.d;
+  const int R = Decoder::kMaxChunk, H = d.n_head, HK = d.n_head_kv, HD = d.head_dim;
+  int rc = BTF_OK;
+  bool attn = false;
+  for (Layer& l : D.L) {
+    attn |= !l.rec;
+    if (!l.rec || l.node_state) continue;
+    l.node_ring = D.alloc<float>((size_t)R * d.conv_kernel * D.C, &rc, Decoder::kState);
+    l.node_state = D.alloc<float>((size_t)R * D.NV * D.DV * D.DK, &rc, Decoder::kState);
+    if (rc) return rc;
+  }
+  if (attn && !D.tree_work) {
+    if (d.n_rot) {
+      double turns[128];  // n_rot <= head_dim <= 256
+      const btf_rope_cfg cfg{d.n_rot, BTF_ROPE_NONE, d.rope_base, 1.0, 0.0, 0.0, 0};
+      float m = 1.0f;
+      BTF_TRY(btf_rope_table(&cfg, turns, &m));
+      D.rope_turns = D.alloc<double>(d.n_rot / 2, &rc);
+      if (rc) return rc;
+      const cudaError_t e = cudaMemcpy(D.rope_turns, turns, d.n_rot / 2 * sizeof(double), cudaMemcpyHostToDevice);
+      if (e != cudaSuccess) return cuda_fail(e, "btf_decoder_verify: rotary table");
+    }
+    D.q16 = D.alloc<__half>((size_t)R * H * HD, &rc);
+    D.o16 = D.alloc<__half>((size_t)R * H * HD, &rc);
+    if (rc) return rc;
+    // the workspace for any number of nodes up to R: the largest of them
+    for (int n = 1; n <= std::min(R, D.o.n_ctx); ++n) {
+      const int64_t b = btf_tree_attention_work(1, n, H, HK, HD, D.o.n_ctx);
+      if (b < 0) return BTF_ERR_UNSUPPORTED;
+      D.tree_work_bytes = std::max(D.tree_work_bytes, b);
+    }
+    D.tree_work = D.alloc<uint8_t>(D.tree_work_bytes, &rc);
+  }
+  if (!D.d_parents) {
+    D.d_parents = D.alloc<int32_t>(3 * R, &rc);
+    if (rc) return rc;
+    D.d_rows_of = D.d_parents + R;
+    D.d_nexts = D.d_parents + 2 * R;
+  }
+  D.node_logits = D.alloc<float>((size_t)R * d.n_vocab, &rc);
+  return rc;
+}
+
+// Enqueues the forward pass of a draft of n nodes (d_ptok, their positions d_ppos, their rows of the caches
+// d_rows_of, d_parents): enqueue_chunk's order, with every node's recurrent state following its parent's and the
+// attention of all nodes in one launch over the cache and each node's ancestors. Ends with the logits of all nodes.
+int enqueue_draft(Decoder& D, int n, const int* parent) {
+  const btf_decoder_dims& d = D.d;
+  const int E = d.n_embd, F = d.n_ff, H = d.n_head, HK = d.n_head_kv, HD = d.head_dim;
+  for (int m = 0; m < n; ++m)
+    BTF_TRYC(launch_embed(D.embd.pan, d.n_vocab, E, D.d_ptok + m, D.inv_block, D.inv_signs, D.x + (size_t)m * E, D.st));
+  for (Layer& l : D.L) {
+    if (l.rec) {
+      const int C = l.qkv.N, Z = l.zg.N;
+      const size_t ring = (size_t)d.conv_kernel * D.C, state = (size_t)D.NV * D.DV * D.DK;
+      BTF_TRY(prep(D, D.x, E, l.attn_norm, l.qkv.hx, D.xn, n));
+      BTF_TRY(gemv(D, {{&l.qkv, D.bA}, {&l.zg, D.bB}}, E, BTF_STORE, n));
+      for (int m = 0; m < n; ++m) {
+        GdnArgs ga{D.xn + (size_t)m * E, l.alpha_w, l.beta_w, l.ssm_dt, l.ssm_a, E, l.ab_bf16, D.bA + (size_t)m * C,
+                   l.node_ring + m * ring, l.conv_w, d.conv_kernel, D.C, D.bB + (size_t)m * Z, l.node_state + m * state,
+                   l.ssm_norm, D.NK, D.DK, D.DV, D.QK, d.rms_eps, D.d_ppos + m, D.bO + (size_t)m * D.DI, D.NV};
+        ga.ring_from = parent[m] < 0 ? l.conv_state : l.node_ring + parent[m] * ring;
+        ga.state_from = parent[m] < 0 ? l.ssm_state : l.node_state + parent[m] * state;
+        BTF_TRYC(launch_gdn_mix(ga, D.st));
+      }
+      BTF_TRY(prep(D, D.bO, D.DI, nullptr, l.out.hx, nullptr, n));
+      BTF_TRY(gemv(D, {{&l.out, D.x}}, D.DI, BTF_ADD, n));
+    } else {
+      const int NQ = l.wq.N, NKV = l.wk.N, HO = H * HD;
+      BTF_TRY(prep(D, D.x, E, l.attn_norm, l.wq.hx, nullptr, n));
+      BTF_TRY(gemv(D, {{&l.wq, D.bA}, {&l.wk, D.bB}, {&l.wv, D.bC}}, E, BTF_STORE, n));
+      const btf_rope_seg segs[3] = {
+          {D.bA, D.q16, BTF_F32, BTF_F16, H, 1, NQ, 2 * HD, HO, HD, l.q_norm, nullptr, 0},
+          {D.bB, l.kc, BTF_F32, BTF_F16, HK, 1, NKV, HD, HK * HD, HD, l.k_norm, D.d_rows_of, D.o.n_ctx},
+          {D.bC, l.vc, BTF_F32, BTF_F16, HK, 0, NKV, HD, HK * HD, HD, nullptr, D.d_rows_of, D.o.n_ctx}};
+      BTF_TRY(btf_rope(segs, 3, n, HD, d.n_rot, D.rope_turns, 1.0f, 0, 0, d.rms_eps, D.d_ppos, D.st));
+      btf_tree_attn a{};
+      a.q = D.q16, a.q_batch = (int64_t)n * HO, a.q_node = HO, a.q_head = HD;
+      a.k = l.kc, a.v = l.vc, a.kv_batch = (int64_t)D.o.n_ctx * HK * HD, a.kv_row = (int64_t)HK * HD, a.kv_head = HD;
+      a.o = D.o16, a.o_batch = a.q_batch, a.o_node = HO, a.o_head = HD;
+      a.type = BTF_F16;
+      a.B = 1, a.n = n, a.H = H, a.HK = HK, a.D = HD, a.n_ctx = D.o.n_ctx;
+      a.lens = D.d_pos, a.parents = D.d_parents;
+      a.scale = 1.0f / std::sqrt((float)HD);
+      a.work = D.tree_work, a.work_bytes = D.tree_work_bytes;
+      BTF_TRY(btf_tree_attention(&a, D.st));
+      BTF_TRYC(launch_gate(D.o16, D.bA, n, H, HD, D.bO, D.st));
+      BTF_TRY(prep(D, D.bO, HO, nullptr, l.wo.hx, nullptr, n));
+      BTF_TRY(gemv(D, {{&l.wo, D.x}}, HO, BTF_ADD, n));
+    }
+    BTF_TRY(prep(D, D.x, E, l.post_norm, l.gate.hx, nullptr, n));
+    BTF_TRY(gemv(D, {{&l.gate, D.bG}, {&l.up, nullptr}}, E, BTF_SWIGLU, n));
+    BTF_TRY(prep(D, D.bG, F, nullptr, l.down.hx, nullptr, n));
+    BTF_TRY(gemv(D, {{&l.down, D.x}}, F, BTF_ADD, n));
+  }
+  BTF_TRY(prep(D, D.x, E, D.out_norm, D.output.hx, nullptr, n));
+  return gemv(D, {{&D.output, D.node_logits}}, E, BTF_STORE, n);
+}
+
 int capture(Decoder& D) {
   cudaError_t e = cudaStreamBeginCapture(D.st, cudaStreamCaptureModeThreadLocal);
   if (e != cudaSuccess) return cuda_fail(e, "btf_decoder: begin capture");
@@ -386,6 +539,7 @@ int capture(Decoder& D) {
 
 // Runs one step (graph replay or eager) on D.st, no host synchronisation.
 int run_step(Decoder& D) {
+  D.draft_n = 0;  // what was drafted was not accepted
   if (D.pos >= D.o.n_ctx) return fail(BTF_ERR_ARG, "btf_decoder: context full (n_ctx %d)", D.o.n_ctx);
   if (D.world > 1 && !D.connected) return fail(BTF_ERR_STATE, "btf_decoder: tensor-parallel decoder not connected");
   if (D.o.cuda_graph) {
@@ -948,19 +1102,23 @@ int btf_decoder_connect(void* handle, void* const* peer_arenas) {
   return BTF_OK;
 }
 
-int btf_decoder_step(void* handle, int32_t token, float* logits, int32_t* next) {
-  if (!handle) return fail(BTF_ERR_ARG, "btf_decoder_step: null handle");
-  Decoder& D = *static_cast<Decoder*>(handle);
+namespace {
+int step(Decoder& D, int32_t token, const btf_sampling* sampling, float u, float* logits, int32_t* next,
+         float* logprob) {
   if (token < 0 || token >= D.d.n_vocab) return fail(BTF_ERR_ARG, "btf_decoder_step: token %d out of range", token);
   const auto t0 = std::chrono::steady_clock::now();
   BTF_TRY(settle(D));
+  if (sampling) BTF_TRY(set_sampling(D, *sampling, &u, 1));
   D.h_io[0] = token;
   cudaError_t e = cudaMemcpyAsync(D.d_tok, D.h_io, sizeof(int32_t), cudaMemcpyHostToDevice, D.st);
   if (e == cudaSuccess) e = cudaEventRecord(D.ev[0], D.st);
   if (e != cudaSuccess) return cuda_fail(e, "btf_decoder_step: token");
   BTF_TRY(run_step(D));
-  e = cudaEventRecord(D.ev[1], D.st);
+  if (sampling) e = sample_rows(D, D.logits, 1, D.d_u, D.d_next, D.d_tok);  // in place of the greedy token
+  if (e == cudaSuccess) e = cudaEventRecord(D.ev[1], D.st);
   if (e == cudaSuccess) e = cudaMemcpyAsync(D.h_io + 1, D.d_next, sizeof(int32_t), cudaMemcpyDeviceToHost, D.st);
+  if (e == cudaSuccess && sampling)
+    e = cudaMemcpyAsync(D.h_io + 2, D.d_lp, sizeof(float), cudaMemcpyDeviceToHost, D.st);
   if (e == cudaSuccess && logits)
     e = cudaMemcpyAsync(logits, D.logits, (size_t)D.d.n_vocab * sizeof(float), cudaMemcpyDeviceToHost, D.st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(D.st);
@@ -970,6 +1128,126 @@ int btf_decoder_step(void* handle, int32_t token, float* logits, int32_t* next) 
   D.n_steps += 1;
   D.wall_s += seconds_since(t0);
   if (next) *next = D.h_io[1];
+  if (sampling && logprob) std::memcpy(logprob, D.h_io + 2, sizeof(float));
+  return BTF_OK;
+}
+
+int run(Decoder& D, int steps, const btf_sampling* sampling, const float* u) {
+  const auto t0 = std::chrono::steady_clock::now();
+  BTF_TRY(settle(D));
+  cudaError_t e = cudaEventRecord(D.ev[0], D.st);
+  if (e != cudaSuccess) return cuda_fail(e, "btf_decoder_run: event");
+  int done = 0, rc = BTF_OK;
+  for (; done < steps && rc == BTF_OK; ++done) {
+    const int at = done % Decoder::kMaxRandom;
+    if (sampling && at == 0) rc = set_sampling(D, *sampling, u + done, std::min(steps - done, Decoder::kMaxRandom));
+    if (rc == BTF_OK) rc = run_step(D);
+    if (rc == BTF_OK && sampling && (e = sample_rows(D, D.logits, 1, D.d_u + at, D.d_next, D.d_tok)) != cudaSuccess)
+      rc = cuda_fail(e, "btf_decoder_run_sampled");
+  }
+  if (rc) --done;
+  D.n_steps += done;
+  if ((e = cudaEventRecord(D.ev[1], D.st)) != cudaSuccess && rc == BTF_OK) rc = cuda_fail(e, "btf_decoder_run: event");
+  D.ev_pending = e == cudaSuccess;
+  D.wall_s += seconds_since(t0);
+  return rc;
+}
+}  // namespace
+
+int btf_decoder_step(void* handle, int32_t token, float* logits, int32_t* next) {
+  if (!handle) return fail(BTF_ERR_ARG, "btf_decoder_step: null handle");
+  return step(*static_cast<Decoder*>(handle), token, nullptr, 0.0f, logits, next, nullptr);
+}
+
+int btf_decoder_step_sampled(void* handle, int32_t token, const btf_sampling* sampling, float u, float* logits,
+                             int32_t* next, float* logprob) {
+  if (!handle) return fail(BTF_ERR_ARG, "btf_decoder_step_sampled: null handle");
+  Decoder& D = *static_cast<Decoder*>(handle);
+  BTF_TRY(check_sampling(D, sampling, "btf_decoder_step_sampled"));
+  return step(D, token, sampling, u, logits, next, logprob);
+}
+
+int btf_decoder_verify(void* handle, const int32_t* tokens_host, const int32_t* parents_host, int n,
+                       const btf_sampling* sampling, const float* u_host, float* logits, int32_t* next_host) {
+  constexpr int R = Decoder::kMaxChunk;
+  static_assert(R == BTF_DECODER_MAX_DRAFT);
+  if (!handle || !tokens_host || !parents_host || !next_host || (sampling && !u_host))
+    return fail(BTF_ERR_ARG, "btf_decoder_verify: null argument");
+  Decoder& D = *static_cast<Decoder*>(handle);
+  if (n < 1 || n > R) return fail(BTF_ERR_ARG, "btf_decoder_verify: 1..%d nodes (got %d)", R, n);
+  if (D.world > 1) return fail(BTF_ERR_UNSUPPORTED, "btf_decoder_verify: one GPU only");
+  const btf_sampling greedy{0.0f, 0, 1.0f, 0.0f};
+  BTF_TRY(check_sampling(D, sampling ? sampling : &greedy, "btf_decoder_verify"));
+  if (D.pos + n > D.o.n_ctx) return fail(BTF_ERR_ARG, "btf_decoder_verify: context full (n_ctx %d)", D.o.n_ctx);
+  int32_t h[4 * R] = {};  // tokens, positions (as btf_decoder_prefill lays them out), parents, rows
+  int parent[R] = {};
+  for (int j = 0; j < n; ++j) {
+    if (tokens_host[j] < 0 || tokens_host[j] >= D.d.n_vocab)
+      return fail(BTF_ERR_ARG, "btf_decoder_verify: token %d out of range", tokens_host[j]);
+    if (parents_host[j] < -1 || parents_host[j] >= j)
+      return fail(BTF_ERR_ARG, "btf_decoder_verify: node %d must follow an earlier node or -1 (got %d)", j, parents_host[j]);
+    parent[j] = parents_host[j];
+    h[j] = tokens_host[j];
+    h[R + j] = parent[j] < 0 ? D.pos : h[R + parent[j]] + 1;
+    h[2 * R + j] = parent[j];
+    h[3 * R + j] = D.pos + j;
+  }
+  BTF_TRY(settle(D));
+  D.draft_n = 0;
+  BTF_TRY(make_draft_buffers(D));
+  const float none[R] = {};
+  cudaError_t e = cudaStreamSynchronize(D.st);  // nothing reads the arrays any more
+  if (e == cudaSuccess) e = cudaMemcpy(D.d_ptok, h, 2 * R * sizeof(int32_t), cudaMemcpyHostToDevice);
+  if (e == cudaSuccess) e = cudaMemcpy(D.d_parents, h + 2 * R, 2 * R * sizeof(int32_t), cudaMemcpyHostToDevice);
+  if (e != cudaSuccess) return cuda_fail(e, "btf_decoder_verify: tokens");
+  BTF_TRY(set_sampling(D, sampling ? *sampling : greedy, sampling ? u_host : none, n));
+  BTF_TRY(enqueue_draft(D, n, parent));
+  e = sample_rows(D, D.node_logits, n, D.d_u, D.d_nexts, nullptr);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(D.st);
+  if (e == cudaSuccess) e = cudaMemcpy(next_host, D.d_nexts, n * sizeof(int32_t), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess && logits)
+    e = cudaMemcpy(logits, D.node_logits, (size_t)n * D.d.n_vocab * sizeof(float), cudaMemcpyDeviceToHost);
+  if (e != cudaSuccess) return cuda_fail(e, "btf_decoder_verify");
+  std::copy(parent, parent + n, D.draft_parent);
+  D.draft_n = n;
+  return BTF_OK;
+}
+
+int btf_decoder_accept(void* handle, int node) {
+  if (!handle) return fail(BTF_ERR_ARG, "btf_decoder_accept: null handle");
+  Decoder& D = *static_cast<Decoder*>(handle);
+  if (!D.draft_n) return fail(BTF_ERR_STATE, "btf_decoder_accept: no draft since the last step, prompt or reset");
+  if (node < 0 || node >= D.draft_n) return fail(BTF_ERR_ARG, "btf_decoder_accept: node %d of %d", node, D.draft_n);
+  int path[Decoder::kMaxChunk], len = 0;
+  for (int j = node; j >= 0; j = D.draft_parent[j]) path[len++] = j;
+  std::reverse(path, path + len);
+  const size_t row = (size_t)D.d.n_head_kv * D.d.head_dim, ring = (size_t)D.d.conv_kernel * D.C,
+               state = (size_t)D.NV * D.DV * D.DK;
+  cudaError_t e = cudaSuccess;
+  auto copy = [&](void* to, const void* from, size_t bytes) {
+    if (e == cudaSuccess) e = cudaMemcpyAsync(to, from, bytes, cudaMemcpyDeviceToDevice, D.st);
+  };
+  for (Layer& l : D.L) {
+    if (l.rec) {
+      copy(l.conv_state, l.node_ring + node * ring, ring * sizeof(float));
+      copy(l.ssm_state, l.node_state + node * state, state * sizeof(float));
+      continue;
+    }
+    // a path's nodes are in ascending order and node path[i] >= i: no row is overwritten before it has moved
+    for (int i = 0; i < len; ++i) {
+      if (path[i] == i) continue;
+      copy(l.kc + (D.pos + i) * row, l.kc + (size_t)(D.pos + path[i]) * row, row * sizeof(__half));
+      copy(l.vc + (D.pos + i) * row, l.vc + (size_t)(D.pos + path[i]) * row, row * sizeof(__half));
+    }
+  }
+  copy(D.d_tok, D.d_nexts + node, sizeof(int32_t));
+  copy(D.d_next, D.d_nexts + node, sizeof(int32_t));
+  const int32_t pos = D.pos + len;
+  if (e == cudaSuccess) e = cudaStreamSynchronize(D.st);
+  if (e == cudaSuccess) e = cudaMemcpy(D.d_pos, &pos, sizeof(int32_t), cudaMemcpyHostToDevice);
+  if (e != cudaSuccess) return cuda_fail(e, "btf_decoder_accept");
+  D.pos = pos;
+  D.draft_n = 0;
   return BTF_OK;
 }
 
@@ -987,6 +1265,7 @@ int btf_decoder_prefill(void* handle, const int32_t* tokens_host, int n, int max
     if (tokens_host[i] < 0 || tokens_host[i] >= D.d.n_vocab)
       return fail(BTF_ERR_ARG, "btf_decoder_prefill: token %d out of range", tokens_host[i]);
   BTF_TRY(settle(D));
+  D.draft_n = 0;
   for (int i = 0; i < n; i += max_chunk) {
     const int M = std::min(max_chunk, n - i);
     int32_t tp[2 * Decoder::kMaxChunk] = {};
@@ -1015,19 +1294,14 @@ int btf_decoder_prefill(void* handle, const int32_t* tokens_host, int n, int max
 
 int btf_decoder_run(void* handle, int steps) {
   if (!handle || steps < 0) return fail(BTF_ERR_ARG, "btf_decoder_run: bad argument");
+  return run(*static_cast<Decoder*>(handle), steps, nullptr, nullptr);
+}
+
+int btf_decoder_run_sampled(void* handle, int steps, const btf_sampling* sampling, const float* u_host) {
+  if (!handle || steps < 0 || (steps && !u_host)) return fail(BTF_ERR_ARG, "btf_decoder_run_sampled: bad argument");
   Decoder& D = *static_cast<Decoder*>(handle);
-  const auto t0 = std::chrono::steady_clock::now();
-  BTF_TRY(settle(D));
-  cudaError_t e = cudaEventRecord(D.ev[0], D.st);
-  if (e != cudaSuccess) return cuda_fail(e, "btf_decoder_run: event");
-  int done = 0, rc = BTF_OK;
-  for (; done < steps && rc == BTF_OK; ++done) rc = run_step(D);
-  if (rc) --done;
-  D.n_steps += done;
-  if ((e = cudaEventRecord(D.ev[1], D.st)) != cudaSuccess && rc == BTF_OK) rc = cuda_fail(e, "btf_decoder_run: event");
-  D.ev_pending = e == cudaSuccess;
-  D.wall_s += seconds_since(t0);
-  return rc;
+  BTF_TRY(check_sampling(D, sampling, "btf_decoder_run_sampled"));
+  return run(D, steps, sampling, u_host);
 }
 
 int btf_decoder_stats(void* handle, btf_step_stats* out) {

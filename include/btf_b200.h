@@ -446,6 +446,35 @@ int btf_decoder_reset(void* handle);
 int btf_decoder_close(void* handle);
 int btf_decoder_get_info(void* handle, btf_decoder_info* out);
 
+/* ---- a decoder's answers: sampled tokens, drafted tokens */
+typedef struct btf_sampling { /* btf_sample's parameters of one row; 0, 0, 0, 0 is greedy */
+  float temperature;
+  int top_k;
+  float top_p, min_p;
+} btf_sampling;
+/* btf_decoder_step with the next token drawn by btf_sample from the step's logits and u in [0, 1): it goes to *next,
+ * its log-probability to *logprob when non-NULL, and a btf_decoder_run / run_sampled would continue from it. */
+int btf_decoder_step_sampled(void* handle, int32_t token, const btf_sampling* sampling, float u, float* logits,
+                             int32_t* next, float* logprob);
+/* btf_decoder_run with drawn tokens: step i draws with u_host[i]. The numbers are copied before it returns. */
+int btf_decoder_run_sampled(void* handle, int steps, const btf_sampling* sampling, const float* u_host);
+
+/* Checks a tree of n drafted tokens in one pass over the weights: node j holds tokens_host[j] and follows node
+ * parents_host[j] < j, or the decoded tokens when that is -1. Node j sits at position pos + its depth; every ternary
+ * matmul runs once over the n rows, the attention is btf_rope + btf_tree_attention over the layer's cache, and every
+ * node has a recurrent state of its own, which starts from its parent's. next_host[j] is the token after node j:
+ * greedy (sampling NULL), or drawn with u_host[j]; logits (host, [n][n_vocab]) when non-NULL. The decoder's position
+ * and state stay: btf_decoder_accept takes over a path, any other call drops the draft. Synchronous, eager. The first
+ * call allocates the nodes' states (btf_decoder_info.device_bytes then counts them; btf_plan_memory does not).
+ * One GPU only; pos + n <= n_ctx; n_vocab <= BTF_SAMPLE_MAX_V. */
+#define BTF_DECODER_MAX_DRAFT 8
+int btf_decoder_verify(void* handle, const int32_t* tokens_host, const int32_t* parents_host, int n,
+                       const btf_sampling* sampling, const float* u_host, float* logits, int32_t* next_host);
+/* Takes over the path from a node without a parent down to `node` of the last btf_decoder_verify: the path's rows of
+ * the caches move behind the decoded tokens, the node's recurrent state becomes the decoder's, pos += the path's
+ * length, and the token after `node` is the one that a btf_decoder_run continues from. */
+int btf_decoder_accept(void* handle, int node);
+
 /* Per-step accounting since the last reset_stats (FastDecoder::stats /
  * reset_stats and StepStats, include/btf/fast.hpp:72-96). Kept across
  * btf_decoder_reset. Reading the stats waits for a pending btf_decoder_run. */
