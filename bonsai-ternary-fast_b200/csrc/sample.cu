@@ -43,6 +43,7 @@ constexpr int kGroups = 64;    // of bins, summed for the whole cluster's use
 constexpr int kCand = 512;     // elements that one CTA ranks exactly, one per thread
 constexpr int kMaxCluster = 16;
 constexpr int kHeld = 16384;   // logits that a CTA keeps in shared memory at most
+constexpr int kLeast = 4096;   // and at least, while there are SMs without a CTA
 constexpr float kSpan = 32.0f;  // exponents below -kSpan have mass 0: e^-32 < 2^-46
 
 struct SampleParams {
@@ -113,6 +114,7 @@ struct Shared {
   uint64_t cmass[kCand];
   uint32_t ckey[kCand], cidx[kCand];
   uint32_t ncand;
+  float queue[kWarps][32 + 4 * 32];  // logits whose masses a warp works out, 32 at a time
 };
 // A histogram of counts, or an exact one of counts or masses.
 union Hist {
@@ -137,7 +139,8 @@ struct Row {
   // NaN, has no mass.
   __device__ __forceinline__ float place(float v) const { return v == top ? 0.0f : (top - v) * bin_scale; }
   // rint(2^S e^x) for -33 < x <= 0 by a table of 2^(i / 64) and the Taylor polynomial of the rest (Tang's method):
-  // x = n ln2 / 64 + r, |r| <= ln2 / 128, e^r to r^5 / 120 (the rest below 2^-54), in all within 2^-48 relative.
+  // x = n ln2 / 64 + r, |r| <= ln2 / 128, e^r to r^5 / 120 (the rest below 2^-54), in all within 2^-48 relative. (16
+  // entries, whose lookups do not conflict, and one term more: the same time.)
   __device__ __forceinline__ uint64_t weight_of(double x) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
     const double big = fma(x, 92.332482616893656877, kRound);  // 64 / ln 2
@@ -231,9 +234,11 @@ __device__ __forceinline__ uint64_t block_scan(Shared& sh, uint64_t v, uint64_t*
 
 // A CTA's part of the row, in fours of neighbours as fp32: in shared memory (HELD), or where it lies. A warp owns a
 // contiguous block of `blk` fours, its lanes one after another. What pads the last four is -inf.
+constexpr int kGroup = 4;
 template <typename T, bool HELD>
 struct Part {
   float4* held;
+  __nv_bfloat16* peak;  // or the largest of every lane's kGroup fours, rounded up
   const T* x;
   int n, blk;     // logits; fours per warp
   bool whole;     // whether fours are aligned
@@ -257,33 +262,48 @@ struct Part {
     if constexpr (HELD) return held[i];
     else return raw(i);
   }
-  // fn(logit, position in the part) for this thread's fours that hold a logit >= from
+  // fn(four, position in the part) with the whole warp, for the fours of which a lane's holds a logit >= from
   template <typename Fn>
-  __device__ __forceinline__ void each(float from, Fn fn) const {
+  __device__ __forceinline__ void fours(float from, Fn fn) const {
     const bool none = !(largest >= from);
     if (__all_sync(0xffffffffu, none)) return;
-    const int i0 = (threadIdx.x >> 5) * blk, lane = threadIdx.x & 31;
-    constexpr int kAhead = HELD ? 2 : 1;
+    const int i0 = (threadIdx.x >> 5) * blk, i1 = i0 + blk, lane = threadIdx.x & 31;
+    constexpr int kAhead = 2;
+    static_assert(kGroup % kAhead == 0);
     const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
 #pragma unroll 1
-    for (int i = i0 + lane; i < i0 + blk; i += 32 * kAhead) {
+    for (int i = i0 + lane; i < i1; i += 32 * kAhead) {
+      bool any = !none;
+      if (!HELD) any = any && __bfloat162float(*peak_at(i - i0 - lane)) >= from;
+      if (__all_sync(0xffffffffu, !any)) continue;
       float4 q[kAhead];
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a) q[a] = !none && i + 32 * a < i0 + blk ? four(i + 32 * a) : nothing;
+      for (int a = 0; a < kAhead; ++a) q[a] = any && i + 32 * a < i1 ? four(i + 32 * a) : nothing;
       // one copy of fn for all of them: the code stays small
 #pragma unroll 1
       for (int a = 0; a < kAhead; ++a) {
         const float4 f = q[0];
 #pragma unroll
         for (int b = 0; b + 1 < kAhead; ++b) q[b] = q[b + 1];
-        if (!(fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)) >= from)) continue;
-        const int at = 4 * (i + 32 * a);
-        fn(f.x, at);
-        fn(f.y, at + 1);
-        fn(f.z, at + 2);
-        fn(f.w, at + 3);
+        if (__any_sync(0xffffffffu, fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)) >= from)) fn(f, 4 * (i + 32 * a));
       }
     }
+  }
+  // fn(logit, position in the part) for this thread's fours that hold a logit >= from
+  template <typename Fn>
+  __device__ __forceinline__ void each(float from, Fn fn) const {
+    fours(from, [&](const float4& f, int at) {
+      if (!(fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)) >= from)) return;
+      fn(f.x, at);
+      fn(f.y, at + 1);
+      fn(f.z, at + 2);
+      fn(f.w, at + 3);
+    });
+  }
+  // this lane's place in the summary for its fours from `first` of its warp's on
+  __device__ __forceinline__ __nv_bfloat16* peak_at(int first) const {
+    const int groups = (blk + 32 * kGroup - 1) / (32 * kGroup);
+    return peak + ((threadIdx.x >> 5) * groups + first / (32 * kGroup)) * 32 + (threadIdx.x & 31);
   }
 };
 
@@ -820,6 +840,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   {
     const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.ld;
     part.held = reinterpret_cast<float4*>(dynamic + (hist ? sizeof(Hist) : 0));
+    part.peak = reinterpret_cast<__nv_bfloat16*>(part.held);
     part.x = x + idx0;
     part.n = (int)min((int64_t)p.chunk, max((int64_t)0, (int64_t)p.V - idx0));
     part.blk = p.chunk / 4 / kWarps;
@@ -838,7 +859,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const int end = (w + 1) * part.blk;
     float top = -INFINITY;
     uint32_t at = idx0 + 4 * (w * part.blk + lane);
-    constexpr int kAtOnce = 4;
+    constexpr int kAtOnce = kGroup;
     const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     float4 q[kAtOnce], next[kAtOnce];
     auto load = [&](float4(&to)[kAtOnce], int i0) {
@@ -850,16 +871,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 #pragma unroll
       for (int a = 0; a < kAtOnce; ++a) q[a] = next[a];
       load(next, i0 + 32 * kAtOnce);
+      float peak = -INFINITY;
 #pragma unroll
       for (int a = 0; a < kAtOnce; ++a) {
         const int i = i0 + 32 * a;
         if (HELD && i < end) part.held[i] = q[a];
         const float m = fmaxf(fmaxf(q[a].x, q[a].y), fmaxf(q[a].z, q[a].w));
+        peak = fmaxf(peak, m);
         if (m > top) {  // (equal ones come later in the row)
           top = m;
           at = idx0 + 4 * i + (q[a].x == m ? 0 : q[a].y == m ? 1 : q[a].z == m ? 2 : 3);
         }
       }
+      if (!HELD) *part.peak_at(i0 - w * part.blk - lane) = __float2bfloat16_ru(peak);
     }
     part.largest = top;
     best = ((uint64_t)key_of(top) << 32) | (uint32_t)~at;
@@ -935,59 +959,107 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     return e >= row.min_e ? row.weight_of(e) : 0ull;
   };
   uint64_t mine = lane == 0 ? above : 0;
-  part.each(least, [&](float v, int i) {
-    if (!(v >= upto)) mine += kept(v, i);
-  });
+  if (least == row.alive && row.cut == -INFINITY) {  // no filter: nearly all of them
+    part.each(least, [&](float v, int) { mine += row.weight(v); });
+  } else {  // few of them, in few lanes at a time: the others' lanes help
+    float* queue = sh.queue[w];
+    int n = 0;  // in the queue, the same in every lane
+    auto take = [&] {
+      __syncwarp();
+      n -= 32;
+      if (n + lane >= 0) {
+        const double e = row.exponent(queue[n + lane]);
+        if (e >= row.min_e) mine += row.weight_of(e);
+      }
+      __syncwarp();
+    };
+    part.fours(least, [&](const float4& f, int at) {
+      const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool is = v[e] >= least && !(v[e] >= upto) && row.inside(v[e], idx0 + at + e);
+        const unsigned are = __ballot_sync(0xffffffffu, is);
+        if (is) queue[n + __popc(are & ((1u << lane) - 1))] = v[e];
+        n += __popc(are);
+      }
+#pragma unroll 1
+      while (n >= 32) take();
+    });
+    if (n > 0) take();
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   __syncthreads();
   if (lane == 0) sh.warp[w][0] = mine;
   __syncthreads();
-  uint64_t cta = 0, pre = 0;
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < w) pre += sh.warp[i][0];
-    cta += sh.warp[i][0];
-  }
+  uint64_t cta = 0;
+  for (int i = 0; i < kWarps; ++i) cta += sh.warp[i][0];
   const auto s = c.exchange(cta, 0);
-  uint64_t z = 0;
+  uint64_t z = 0, run = 0;
   for (int r = 0; r < c.size; ++r) {
-    if (r < c.rank) pre += s[r][0];
+    if (r < c.rank) run += s[r][0];
     z += s[r][0];
   }
   const uint64_t goal = goal_of_u(p.u[b], z);
-  if (pre <= goal && goal < pre + mine) {
-    // the warp that holds the token walks its block
-    for (int i0 = w * part.blk; i0 < (w + 1) * part.blk; i0 += 32) {
-      const int i = i0 + lane;
-      const float4 q = part.four(i);
-      const float logit[4] = {q.x, q.y, q.z, q.w};
-      uint64_t v[4], inc = 0;
+  // the warp whose block holds the token; its rounds of 32 fours are shared out among all warps, and the one that has
+  // the token in its rounds walks them
+  if (!(run <= goal && goal < run + cta)) return;
+  int of = 0;
+  while (of + 1 < kWarps && goal >= run + sh.warp[of][0]) run += sh.warp[of++][0];
+  const int rounds = part.blk / 32, each = (rounds + kWarps - 1) / kWarps;
+  const int r0 = min(w * each, rounds), r1 = min(r0 + each, rounds);
+  auto masses = [&](int r, float4& q, uint64_t(&v)[4]) {
+    const int i = of * part.blk + 32 * r + lane;
+    q = part.four(i);
+    v[0] = kept(q.x, 4 * i);
+    v[1] = kept(q.y, 4 * i + 1);
+    v[2] = kept(q.z, 4 * i + 2);
+    v[3] = kept(q.w, 4 * i + 3);
+  };
+  float4 q;
+  uint64_t v[4], sum = 0;
+#pragma unroll 1
+  for (int r = r0; r < r1; ++r) {
+    masses(r, q, v);
+    sum += v[0] + v[1] + v[2] + v[3];
+  }
+  uint64_t inc = sum;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = kept(logit[e], 4 * i + e), inc += v[e];
-      const uint64_t four = inc;
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sh.warp[w][1] = sum;
+  __syncthreads();
+  for (int i = 0; i < w; ++i) run += sh.warp[i][1];
+  if (!(run <= goal && goal < run + sum)) return;
+#pragma unroll 1
+  for (int r = r0; r < r1; ++r) {
+    if (each > 1) {  // (else they are at hand)
+      masses(r, q, v);
+      inc = v[0] + v[1] + v[2] + v[3];
+    }
+    const uint64_t four = inc;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, pre + inc > goal);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          uint64_t run = pre + inc - four;
-          bool done = false;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, run + inc > goal);
+    if (hit) {
+      if (lane == __ffs(hit) - 1) {
+        const float logit[4] = {q.x, q.y, q.z, q.w};
+        run += inc - four;
+        bool done = false;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            run += v[e];
-            if (!done && run > goal) {
-              put_token(p, b, row, logit[e], idx0 + 4 * i + e, z);
-              done = true;
-            }
+        for (int e = 0; e < 4; ++e) {
+          run += v[e];
+          if (!done && run > goal) {
+            put_token(p, b, row, logit[e], idx0 + 4 * (of * part.blk + 32 * r + lane) + e, z);
+            done = true;
           }
         }
-        break;
       }
-      pre += __shfl_sync(0xffffffffu, inc, 31);
+      return;
     }
+    run += __shfl_sync(0xffffffffu, inc, 31);
   }
 }
 
@@ -1012,12 +1084,17 @@ cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
   int lg = 0;
   while ((1ll << lg) < a.V) ++lg;
   p.S = std::min(44, 62 - lg);
-  // few rows: a CTA per kHeld logits or less, whose keys stay in shared memory; more
-  // CTAs than are resident at once (2 per SM): fewer and larger parts, read again
+  // few rows: a CTA per kHeld logits or less, which stay in shared memory, and further
+  // ones down to kLeast as long as every CTA has an SM of its own (one row of 128003:
+  // top-p 27.1 -> 23.0 us with 16 CTAs for 8, no filter 15.1 -> 10.7; below 4096 the
+  // barriers cost what is saved); more CTAs than are resident at once (2 per SM):
+  // fewer and larger parts, read again
   const DeviceInfo* dev = current_device();
   const int slots = 2 * (dev ? dev->sm_count : 148);
   int size = 1;
-  while (size < kMaxCluster && (a.V + size - 1) / size > kHeld) size *= 2;
+  while (size < kMaxCluster && ((a.V + size - 1) / size > kHeld ||
+                               ((a.V + size - 1) / size > kLeast && a.B * size <= slots / 4)))
+    size *= 2;
   bool held = (a.V + size - 1) / size <= kHeld;
   if ((int64_t)a.B * size > slots && size > 1) {
     held = false;
@@ -1025,7 +1102,9 @@ cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
   }
   constexpr int kStep = 4 * kThreads;
   p.chunk = ((a.V + size - 1) / size + kStep - 1) / kStep * kStep;
-  const size_t smem = (held ? (size_t)p.chunk * 4 : 0) + (a.top_k || a.top_p ? sizeof(Hist) : 0);
+  const int groups = (p.chunk / 4 / kWarps + 32 * kGroup - 1) / (32 * kGroup);
+  const size_t smem = (held ? (size_t)p.chunk * 4 : (size_t)groups * kThreads * sizeof(__nv_bfloat16)) +
+                      (a.top_k || a.top_p ? sizeof(Hist) : 0);
   const auto kernel =
       a.type == BTF_F32   ? (held ? sample_kernel<float, true> : sample_kernel<float, false>)
       : a.type == BTF_F16 ? (held ? sample_kernel<__half, true> : sample_kernel<__half, false>)
