@@ -586,7 +586,7 @@ typedef struct btf_rope_seg {
 /* Rotates up to 3 tensors by their tokens' positions pos[T] in one launch: pairs (i, i + n_rot / 2) of the
  * first n_rot dims, or (2 i, 2 i + 1) when interleaved, by pos * f_i; the other dims are copied. Angles are
  * reduced in 64 bits, so any int32 position keeps fp32 accuracy. inverse: the transposed map, which is the
- * gradient (normw must be NULL). 1 <= D <= BTF_ROPE_MAX_D, n_rot even, 0..D (0: turns may be NULL).
+ * gradient (normw must be NULL). 1 <= D <= BTF_ROPE_MAX_D, n_rot even, 0..D (0: turns may be NULL), T <= 2^30.
  * Replaces the RoPE of src/emu_decoder.cpp:307-338 for many tokens and other layouts. */
 int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const double* turns, float mscale,
              int interleaved, int inverse, float eps, const int32_t* pos, void* stream);

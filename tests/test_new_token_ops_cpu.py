@@ -153,3 +153,7 @@ def test_packed_arguments_are_the_structs(btf):
     assert btf.TreeAttnC.from_buffer_copy(a).work_bytes == 26 and len(a) == ctypes.sizeof(b)
     for name, _ in btf.TreeAttnC._fields_:
         assert getattr(btf.TreeAttnC.from_buffer_copy(a), name) == getattr(b, name), name
+
+
+def test_rope_refuses_more_tokens_than_it_counts(btf):
+    assert _rope(btf, T=(1 << 30) + 1) == 1

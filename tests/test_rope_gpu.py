@@ -230,3 +230,23 @@ def test_refusals(cuda, btf):
     for fn in bad:
         with pytest.raises(RuntimeError):
             fn()
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("t", [torch.float16, torch.float32])
+def test_many_tokens(cuda, btf, t, inter):
+    """Enough of them that a thread takes several batches of heads, the last one short; rows checked here and there."""
+    T, H, D = 16001, 41, 128
+    g = torch.Generator(device=cuda).manual_seed(5)
+    x = torch.randn(T, H, D, generator=g, device=cuda).to(t)
+    y = torch.empty_like(x)
+    pos = torch.arange(70000, 70000 + T, dtype=torch.int32, device=cuda)
+    table = btf.RopeTable(D, base=1e6, interleaved=inter)
+    btf.rope([btf.RopeSeg(x, y)], table, pos)
+    at = torch.cat([torch.arange(0, T, 97), torch.tensor([T - 2, T - 1])]).to(cuda)
+    ref, size = _reference(x[at], table.host, 1.0, pos[at], inter)
+    _check(y[at], ref, size)
+    # every row keeps its length: an element is off by (|a| + |b|) 8 * 2^-24 + |y| eps / 2 at most, and |a| + |b| is
+    # at most sqrt 2 of its pair's length, so the square by 2 sqrt 2 * 8 * 2^-24 + eps of it, below 2^-19 + 2 eps
+    a, b = x.double().square().sum(-1), y.double().square().sum(-1)
+    assert float(((a - b).abs() / a).max()) <= 2 * torch.finfo(t).eps + 2.0 ** -19
