@@ -31,6 +31,7 @@ struct DeviceInfo {
   int smem_per_sm = 0;
   int l2_bytes = 0;
   int* err_word = nullptr;  // device address of the error word (bounded-wait time-outs)
+  int sample_clusters[5] = {};  // of 1, 2, 4, 8, 16 sampling CTAs that are resident at once, an SM each
 };
 // State of the current device, or nullptr (and a recorded error) if btf_init
 // was not called for it.

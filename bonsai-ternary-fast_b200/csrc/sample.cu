@@ -114,13 +114,16 @@ struct Shared {
   uint64_t cmass[kCand];
   uint32_t ckey[kCand], cidx[kCand];
   uint32_t ncand;
-  float queue[kWarps][32 + 4 * 32];  // logits whose masses a warp works out, 32 at a time
 };
 // A histogram of counts, or an exact one of counts or masses.
 union Hist {
   uint32_t cnt[kFine];
   unsigned long long bin[kBins];
 };
+struct Queue {  // logits whose masses a warp works out, 32 at a time (in the histogram's place: that is done by then)
+  float of[kWarps][32 + 4 * 32];
+};
+static_assert(sizeof(Queue) <= sizeof(Hist));
 
 // One row's state, the same in every thread of the cluster.
 struct Row {
@@ -235,10 +238,12 @@ __device__ __forceinline__ uint64_t block_scan(Shared& sh, uint64_t v, uint64_t*
 // A CTA's part of the row, in fours of neighbours as fp32: in shared memory (HELD), or where it lies. A warp owns a
 // contiguous block of `blk` fours, its lanes one after another. What pads the last four is -inf.
 constexpr int kGroup = 4;
+constexpr int kHits = 256;  // of a warp's groups, 8 rounds of 32, that are listed at a time
 template <typename T, bool HELD>
 struct Part {
   float4* held;
-  __nv_bfloat16* peak;  // or the largest of every lane's kGroup fours, rounded up
+  __nv_bfloat16* peak;  // or the largest of every lane's kGroup fours, rounded up,
+  uint16_t* hits;       // and this warp's list of those that a pass has to read
   const T* x;
   int n, blk;     // logits; fours per warp
   bool whole;     // whether fours are aligned
@@ -268,24 +273,46 @@ struct Part {
     const bool none = !(largest >= from);
     if (__all_sync(0xffffffffu, none)) return;
     const int i0 = (threadIdx.x >> 5) * blk, i1 = i0 + blk, lane = threadIdx.x & 31;
+    const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    // this lane's fours i, i + 32, ...; one copy of fn for all of them: the code stays small
     constexpr int kAhead = 2;
     static_assert(kGroup % kAhead == 0);
-    const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-#pragma unroll 1
-    for (int i = i0 + lane; i < i1; i += 32 * kAhead) {
-      bool any = !none;
-      if (!HELD) any = any && __bfloat162float(*peak_at(i - i0 - lane)) >= from;
-      if (__all_sync(0xffffffffu, !any)) continue;
+    auto some = [&](int i, bool any) {
       float4 q[kAhead];
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) q[a] = any && i + 32 * a < i1 ? four(i + 32 * a) : nothing;
-      // one copy of fn for all of them: the code stays small
 #pragma unroll 1
       for (int a = 0; a < kAhead; ++a) {
         const float4 f = q[0];
 #pragma unroll
         for (int b = 0; b + 1 < kAhead; ++b) q[b] = q[b + 1];
         if (__any_sync(0xffffffffu, fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)) >= from)) fn(f, 4 * (i + 32 * a));
+      }
+    };
+    if constexpr (HELD) {
+#pragma unroll 1
+      for (int i = i0 + lane; i < i1; i += 32 * kAhead) some(i, !none);
+    } else {
+      // the groups with something to read are listed and read a lane each: few of them take one trip to memory
+      const int groups = (blk + 32 * kGroup - 1) / (32 * kGroup);
+#pragma unroll 1
+      for (int g0 = 0; g0 < groups; g0 += kHits / 32) {
+        int n = 0;
+#pragma unroll 1
+        for (int g = g0; g < min(g0 + kHits / 32, groups); ++g) {
+          const bool is = __bfloat162float(peak[g * 32 + lane]) >= from;
+          const unsigned are = __ballot_sync(0xffffffffu, is);
+          if (is) hits[n + __popc(are & ((1u << lane) - 1))] = (uint16_t)(g * 32 + lane);
+          n += __popc(are);
+        }
+        __syncwarp();
+#pragma unroll 1
+        for (int h = lane; h < n + lane; h += 32) {
+          const int e = h < n ? hits[h] : 0;
+#pragma unroll 1
+          for (int a = 0; a < kGroup; a += kAhead) some(i0 + e / 32 * (32 * kGroup) + e % 32 + 32 * a, h < n);
+        }
+        __syncwarp();
       }
     }
   }
@@ -299,11 +326,6 @@ struct Part {
       fn(f.z, at + 2);
       fn(f.w, at + 3);
     });
-  }
-  // this lane's place in the summary for its fours from `first` of its warp's on
-  __device__ __forceinline__ __nv_bfloat16* peak_at(int first) const {
-    const int groups = (blk + 32 * kGroup - 1) / (32 * kGroup);
-    return peak + ((threadIdx.x >> 5) * groups + first / (32 * kGroup)) * 32 + (threadIdx.x & 31);
   }
 };
 
@@ -839,11 +861,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   Part<T, HELD> part;
   {
     const T* x = static_cast<const T*>(p.x) + (int64_t)b * p.ld;
-    part.held = reinterpret_cast<float4*>(dynamic + (hist ? sizeof(Hist) : 0));
-    part.peak = reinterpret_cast<__nv_bfloat16*>(part.held);
+    part.held = reinterpret_cast<float4*>(dynamic + (hist ? sizeof(Hist) : sizeof(Queue)));
     part.x = x + idx0;
     part.n = (int)min((int64_t)p.chunk, max((int64_t)0, (int64_t)p.V - idx0));
     part.blk = p.chunk / 4 / kWarps;
+    const int groups = (part.blk + 32 * kGroup - 1) / (32 * kGroup);
+    part.peak = reinterpret_cast<__nv_bfloat16*>(part.held) + w * groups * 32;
+    part.hits = reinterpret_cast<uint16_t*>(part.held) + kThreads * groups + w * kHits;
     part.whole = reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0;  // (idx0 is a multiple of 4)
   }
   if (tid < 64) sh.exp2_64[tid] = exp2(tid / 64.0);
@@ -883,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           at = idx0 + 4 * i + (q[a].x == m ? 0 : q[a].y == m ? 1 : q[a].z == m ? 2 : 3);
         }
       }
-      if (!HELD) *part.peak_at(i0 - w * part.blk - lane) = __float2bfloat16_ru(peak);
+      if (!HELD) part.peak[(i0 - w * part.blk - lane) / kGroup + lane] = __float2bfloat16_ru(peak);
     }
     part.largest = top;
     best = ((uint64_t)key_of(top) << 32) | (uint32_t)~at;
@@ -962,7 +986,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (least == row.alive && row.cut == -INFINITY) {  // no filter: nearly all of them
     part.each(least, [&](float v, int) { mine += row.weight(v); });
   } else {  // few of them, in few lanes at a time: the others' lanes help
-    float* queue = sh.queue[w];
+    float* queue = reinterpret_cast<Queue*>(dynamic)->of[w];
     int n = 0;  // in the queue, the same in every lane
     auto take = [&] {
       __syncwarp();
@@ -1063,10 +1087,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
 }
 
+// dynamic shared memory with which a CTA has an SM to itself
+constexpr int kAlone = 114 * 1024 - (int)sizeof(Shared);
 }  // namespace
 
 int sample_setup(DeviceInfo& d) {
-  constexpr int kMost = kHeld * 4 + (int)sizeof(Hist);  // a held part and the histogram
+  // a held part or the summary of the longest row, and the histogram
+  constexpr int kMost = kHeld * 4 + kWarps * kHits * 2 + (int)sizeof(Hist);
+  static_assert(BTF_SAMPLE_MAX_V / (4 * kGroup) * 2 <= kHeld * 4);
   if (kMost + (int)sizeof(Shared) + 1024 > d.optin_smem)
     return fail(BTF_ERR_UNSUPPORTED, "sample_kernel needs %d bytes of shared memory", kMost + (int)sizeof(Shared));
   for (const auto f : {sample_kernel<float, true>, sample_kernel<__half, true>, sample_kernel<__nv_bfloat16, true>,
@@ -1074,6 +1102,22 @@ int sample_setup(DeviceInfo& d) {
     cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return cuda_fail(e, "sample_kernel attributes");
+  }
+  for (int i = 0; i < 5; ++i) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1u << i);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kAlone;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 1u << i;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&d.sample_clusters[i], sample_kernel<float, true>, &cfg) != cudaSuccess) {
+      d.sample_clusters[i] = 0;
+      cudaGetLastError();
+    }
   }
   return BTF_OK;
 }
@@ -1087,24 +1131,28 @@ cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st) {
   // few rows: a CTA per kHeld logits or less, which stay in shared memory, and further
   // ones down to kLeast as long as every CTA has an SM of its own (one row of 128003:
   // top-p 27.1 -> 23.0 us with 16 CTAs for 8, no filter 15.1 -> 10.7; below 4096 the
-  // barriers cost what is saved); more CTAs than are resident at once (2 per SM):
-  // fewer and larger parts, read again
+  // barriers cost what is saved), which they then ask for (33 rows of 50257 with every
+  // filter: 18.6 us, 23.3 two to an SM with others idle); more CTAs than are resident at
+  // once (2 per SM): fewer and larger parts, read again
   const DeviceInfo* dev = current_device();
-  const int slots = 2 * (dev ? dev->sm_count : 148);
-  int size = 1;
+  if (!dev) return cudaErrorInitializationError;
+  const int slots = 2 * dev->sm_count;
+  auto alone = [&](int i) { return i < 5 && a.B <= dev->sample_clusters[i]; };  // 2^i CTAs a row, an SM each
+  int size = 1, lg_size = 0;
   while (size < kMaxCluster && ((a.V + size - 1) / size > kHeld ||
-                               ((a.V + size - 1) / size > kLeast && a.B * size <= slots / 4)))
-    size *= 2;
+                                ((a.V + size - 1) / size > kLeast && alone(lg_size + 1))))
+    size *= 2, ++lg_size;
   bool held = (a.V + size - 1) / size <= kHeld;
   if ((int64_t)a.B * size > slots && size > 1) {
     held = false;
-    while (size > 1 && (int64_t)a.B * size > slots) size /= 2;
+    while (size > 1 && (int64_t)a.B * size > slots) size /= 2, --lg_size;
   }
   constexpr int kStep = 4 * kThreads;
   p.chunk = ((a.V + size - 1) / size + kStep - 1) / kStep * kStep;
   const int groups = (p.chunk / 4 / kWarps + 32 * kGroup - 1) / (32 * kGroup);
-  const size_t smem = (held ? (size_t)p.chunk * 4 : (size_t)groups * kThreads * sizeof(__nv_bfloat16)) +
-                      (a.top_k || a.top_p ? sizeof(Hist) : 0);
+  size_t smem = (held ? (size_t)p.chunk * 4 : ((size_t)groups * kThreads + kWarps * kHits) * 2) +
+                      (a.top_k || a.top_p ? sizeof(Hist) : sizeof(Queue));
+  if (alone(lg_size)) smem = std::max(smem, (size_t)kAlone);
   const auto kernel =
       a.type == BTF_F32   ? (held ? sample_kernel<float, true> : sample_kernel<float, false>)
       : a.type == BTF_F16 ? (held ? sample_kernel<__half, true> : sample_kernel<__half, false>)
