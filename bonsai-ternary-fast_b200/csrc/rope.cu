@@ -7,6 +7,13 @@
 // t in turns is pos * (f_i / 2 pi) in 64 bits; its fraction is exact to 2^-50 of
 // a turn at any int32 position, so cos and sin of it in fp32 are good to 2^-23
 // whatever the position (pos * f_i in fp32 loses 2^-24 pos radians: 0.06 at 10^6).
+//
+// What bounds it: bytes, each read and written once, for prompts and gradients (see
+// rope_heads; 7001 tokens of 40 fp32 heads of 80 in 32.2 us, 5.6 TB/s); the launch for
+// a few tokens (1 token of 24 + 4 + 4 heads of 256 with norm and append: 3.1 us, 61
+// tokens of 32 + 8 + 8 heads of 128: 4.4). So the angles are worked out once per token
+// and thread and used for all heads that the thread takes, whole 16-byte words move,
+// and q, k and v share a launch.
 #include <cmath>
 
 #include "elem.cuh"

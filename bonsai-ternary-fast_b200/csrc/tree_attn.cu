@@ -31,6 +31,15 @@
 // 128 x 64 x 16 MMA of Q K^T reads 6 KB in the 32 cycles that it takes, more than the
 // 4 KB that shared memory gives, and S of tile j + 2 need not wait for P V of tile j.
 //
+// Measured (device time): 16 nodes x 24 heads of 256 over 4096 fp16 rows of 4
+// kv-heads: 19.3 us (17 MB; the floor of a call, 1 node over 513 rows, is 12.0: two
+// launches, lengths, q, K, V and the parts' way through memory one after another);
+// 16 sequences of up to 8203 rows, 24 nodes, 32 and 8 heads of 128: 29.8 us, 3.2 TB/s;
+// 1 node over 131072 rows 5.9 TB/s of K and V, 16 nodes 5.4; 64 nodes (three M tiles):
+// 195 us, 1055 TFLOP/s. There a 64-row tile takes 1560 cycles, in which each SM gets its
+// 64 KB of K and V (8.3 TB/s out of L2 for all) and moves 160 KB in shared memory; the
+// MMAs alone take 1024. Two softmax threads per row gained nothing (202 us).
+//
 // p is rounded to the type of V (the MMA takes one type): eps / 2 per term, as much
 // as the output's own rounding at most. fp16 p carry a factor 2^7, so that those
 // down to 2^-32 of the largest still count. Scores, maxima, sums and O are fp32.
