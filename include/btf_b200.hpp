@@ -127,6 +127,24 @@ class Decoder {
     throw_if(btf_decoder_prefill(h_, tokens, n, max_batch, logits, &next), "btf_decoder_prefill");
     return next;
   }
+  // the next token drawn with u in [0, 1) instead of the greedy one
+  int step_sampled(int32_t token, const btf_sampling& sampling, float u, float* logits = nullptr,
+                   float* logprob = nullptr) {
+    int32_t next = -1;
+    throw_if(btf_decoder_step_sampled(h_, token, &sampling, u, logits, &next, logprob), "btf_decoder_step_sampled");
+    return next;
+  }
+  // a tree of drafted tokens -> the token after each of them (greedy without `sampling`); accept takes a path
+  std::vector<int32_t> verify(const std::vector<int32_t>& tokens, const std::vector<int32_t>& parents,
+                              const btf_sampling* sampling = nullptr, const float* u = nullptr,
+                              float* logits = nullptr) {
+    if (tokens.size() != parents.size()) throw std::runtime_error("verify: a parent per token");
+    std::vector<int32_t> next(tokens.size());
+    throw_if(btf_decoder_verify(h_, tokens.data(), parents.data(), (int)tokens.size(), sampling, u, logits, next.data()),
+             "btf_decoder_verify");
+    return next;
+  }
+  void accept(int node) { throw_if(btf_decoder_accept(h_, node), "btf_decoder_accept"); }
   void reset() { throw_if(btf_decoder_reset(h_), "btf_decoder_reset"); }
   // FastDecoder::stats / reset_stats / device_bytes (fast.hpp:90-95)
   btf_step_stats stats() const {

@@ -3,6 +3,8 @@ table against its formulas, and the argument checks of the C ABI. Nothing is
 launched: every refused call returns before it looks for a device."""
 import ctypes
 import math
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -157,3 +159,11 @@ def test_packed_arguments_are_the_structs(btf):
 
 def test_rope_refuses_more_tokens_than_it_counts(btf):
     assert _rope(btf, T=(1 << 30) + 1) == 1
+
+
+def test_cpp_mirror_of_drafts_compiles():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run(["g++", "-std=c++17", "-fsyntax-only", "-I", os.path.join(root, "include"),
+                        "-I", "/usr/local/cuda/include", os.path.join(root, "tests", "shim_draft.cpp")],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr

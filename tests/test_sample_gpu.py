@@ -210,3 +210,37 @@ def test_refusals(cuda, btf):
         with pytest.raises(RuntimeError):
             fn()
     assert btf.sample(x[:0], u[:0])[0].shape == (0,)
+
+
+@pytest.mark.parametrize("f", [dict(), dict(k=50), dict(k=3000, p=0.9), dict(p=0.9), dict(p=0.9999), dict(m=0.05), dict(m=1e-9),
+                               dict(k=200, p=0.95, m=0.01)], ids=str)
+@pytest.mark.parametrize("B,V,off,t", [(100, 60001, 0, torch.float32), (100, 60001, 1, torch.float16),
+                                       (20, 248321, 3, torch.bfloat16), (310, 20000, 0, torch.float16),
+                                       (75, 8192, 0, torch.float32), (300, 524288, 0, torch.bfloat16)])
+def test_many_rows(cuda, btf, B, V, off, t, f):
+    """More rows than the card holds in shared memory: the token and the log-probability of a row are those that it has
+    in a call of its own, to the last bit, and those of the plain form."""
+    g = torch.Generator(device=cuda).manual_seed(V + B)
+    x = (torch.randn(B, V + off, generator=g, device=cuda) * 2.2).to(t)[:, off:]
+    x[1] = -3.0
+    x[2, ::3] = float("nan")
+    x[3] = float("-inf")
+    x[4, V // 2:] = float("-inf")
+    x[5] = x[5].round()
+    x[6, :V - 1] = -100.0
+    x[7, V // 3] = float("inf")
+    x[8] *= 0.01
+    rng = np.random.default_rng(B)
+    u, T = rng.random(B, dtype=np.float32), rng.choice([0.0, 0.5, 1.0, 1.3], B).astype(np.float32)
+    T[1:9] = 1.0
+    a = {n: np.full(B, v) for n, v in f.items()}
+    tok, lp = _run(btf, cuda, x, u, T, **a)
+    rows = list(range(12)) + [B // 2, B - 2, B - 1]
+    for b in rows:
+        one, lpo = _run(btf, cuda, x[b:b + 1], u[b:b + 1], T[b:b + 1], **{n: v[b:b + 1] for n, v in a.items()})
+        assert tok[b] == one[0] and np.array_equal(lp[b:b + 1], lpo, equal_nan=True), b
+    for b in [1, 2, 4, 5, 8, 10, B - 1]:
+        r, l = _reference(x[b].float().cpu().numpy(), u[b], T[b], f.get("k", 0), np.float32(f.get("p", 1.0)),
+                          np.float32(f.get("m", 0.0)))
+        assert tok[b] == r, b
+        np.testing.assert_allclose(lp[b], l, rtol=2.0 ** -23, atol=2.0 ** -15, err_msg=str(b))
