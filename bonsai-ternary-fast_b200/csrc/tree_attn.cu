@@ -834,6 +834,21 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   auto at = [&](int s) { return base + (2 * s + (s == 0 && second)) * kRowsM; };
   const float2* ml = reinterpret_cast<const float2*>(p.ml);
   T* out = static_cast<T*>(p.o) + b * p.o_batch + node * p.o_node + head * p.o_head;
+  // the first parts are on their way while the weights are worked out
+  const int words = p.D / 4;
+  constexpr int kEarly = WARPS == 1 ? 3 : 8;
+  const int ways = WARPS == 1 ? 1 : kJoinThreads / words, way = WARPS == 1 ? 0 : tid / words, w0 = WARPS == 1 ? lane : tid % words;
+  constexpr int kPer = WARPS == 1 ? 2 : 1;  // 16-byte words of a row per thread
+  float4 early[kEarly][kPer];
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) {
+    const int s = way + k * ways;
+#pragma unroll
+    for (int x = 0; x < kPer; ++x)
+      early[k][x] = way < ways && s < parts && w0 + 32 * x < words
+                        ? *reinterpret_cast<const float4*>(p.part + at(s) * p.D + (w0 + 32 * x) * 4)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   const float2 own = lane < parts ? ml[at(lane)] : make_float2(-INFINITY, 0.f);
   float M = own.x;  // every warp for itself
   for (int s = lane + 32; s < parts; s += 32) M = fmaxf(M, ml[at(s)].x);
@@ -851,7 +866,6 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
       if (tid < 32) weight[s] = f;
   }
   L = warp_sum(L);
-  const int words = p.D / 4;
   auto add = [](float4& a, float f, const float4& v) {
     a.x = fmaf(v.x, f, a.x);
     a.y = fmaf(v.y, f, a.y);
@@ -864,8 +878,13 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   };
   if constexpr (WARPS == 1) {
     float4 a[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k) {
+      const float f = __shfl_sync(0xffffffffu, wown, k);
+      if (k < parts) add(a[0], f, early[k][0]), add(a[1], f, early[k][1]);
+    }
 #pragma unroll 4
-    for (int s = 0; s < parts; ++s) {
+    for (int s = kEarly; s < parts; ++s) {
       const float f = s < 32 ? __shfl_sync(0xffffffffu, wown, s & 31) : ex2(ml[at(s)].x - M);
       const float4* v = reinterpret_cast<const float4*>(p.part + at(s) * p.D);
       if (lane < words) add(a[0], f, v[lane]);
@@ -875,12 +894,14 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
     if (lane + 32 < words) store(lane + 32, a[1]);
   } else {
     __syncthreads();
-    const int ways = kJoinThreads / words, w = tid % words, way = tid / words;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     if (way < ways) {
+#pragma unroll
+      for (int k = 0; k < kEarly; ++k)
+        if (way + k * ways < parts) add(a, weight[way + k * ways], early[k][0]);
 #pragma unroll 8
-      for (int s = way; s < parts; s += ways)
-        add(a, weight[s], *reinterpret_cast<const float4*>(p.part + at(s) * p.D + w * 4));
+      for (int s = way + kEarly * ways; s < parts; s += ways)
+        add(a, weight[s], *reinterpret_cast<const float4*>(p.part + at(s) * p.D + w0 * 4));
     }
     sum[tid] = a;
     __syncthreads();
