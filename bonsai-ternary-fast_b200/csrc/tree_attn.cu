@@ -32,9 +32,9 @@
 // 4 KB that shared memory gives, and S of tile j + 2 need not wait for P V of tile j.
 //
 // Measured (device time): 16 nodes x 24 heads of 256 over 4096 fp16 rows of 4
-// kv-heads: 19.3 us (17 MB; the floor of a call, 1 node over 513 rows, is 12.0: two
+// kv-heads: 16.4 us (17 MB; the floor of a call, 1 node over 513 rows, is 11.1: two
 // launches, lengths, q, K, V and the parts' way through memory one after another);
-// 16 sequences of up to 8203 rows, 24 nodes, 32 and 8 heads of 128: 29.8 us, 3.2 TB/s;
+// 16 sequences of up to 8203 rows, 24 nodes, 32 and 8 heads of 128: 29.2 us, 3.3 TB/s;
 // 1 node over 131072 rows 5.9 TB/s of K and V, 16 nodes 5.4; 64 nodes (three M tiles):
 // 195 us, 1055 TFLOP/s. There a 64-row tile takes 1560 cycles, in which each SM gets its
 // 64 KB of K and V (8.3 TB/s out of L2 for all) and moves 160 KB in shared memory; the
@@ -114,7 +114,7 @@ struct Seq {
 // Up to 32 sequences with fewer pairs than ranges: every pair is cut into its own
 // number of equal ranges, n_b = ceil(tiles / per) with the least `per` that fits, and a
 // CTA has one segment (a second one costs its q and its way out again, about 5 tiles
-// of time: 1 x 1 node over 513 rows took 15.5 us with ranges across pairs, 11.1
+// of time: 1 x 1 node over 513 rows took 15.5 us with ranges across pairs, 12.0
 // without). Otherwise the line of all tiles is cut into equal ranges.
 struct Segments {
   const TreeParams& p;
@@ -803,7 +803,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kPerSm)
 // Joins a row's parts: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. WARPS = 1:
 // a warp per row, for many rows; 8: a CTA per row, whose threads share the parts
 // (4 ways at D = 256) over the 16-byte words of the row, so that few rows of many
-// parts take few round trips to memory.
+// parts take few round trips to memory. The first parts are loaded before the weights
+// are known (16 nodes x 24 heads of 37 parts: 19.3 -> 16.4 us with the kernel above).
 constexpr int kJoinThreads = 256, kMaxParts = 1024;
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeParams p) {

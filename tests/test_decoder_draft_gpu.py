@@ -220,3 +220,21 @@ def test_refusals(cuda, btf):
         d.reset()
         with pytest.raises(RuntimeError):
             d.accept(0)
+
+
+def test_a_long_drawn_run(cuda, btf):
+    """More steps than random numbers are copied at a time: the run ends where as many drawn steps end."""
+    dims = dict(SMALL, n_layer=3)
+    us = np.random.default_rng(8).random(4100, dtype=np.float32)
+    params = dict(temperature=1.1, top_k=30)
+    with btf.Decoder(dims=dims, seed=5, n_ctx=4200) as d, btf.Decoder(dims=dims, seed=5, n_ctx=4200) as steps:
+        t = d.step_sampled(3, 0.5, **params)[0]
+        d.run_sampled(us, **params)
+        assert t == steps.step_sampled(3, 0.5, **params)[0]
+        for u in us:
+            t = steps.step_sampled(t, float(u), **params)[0]
+        assert np.array_equal(_device_logits(btf, d), _device_logits(btf, steps))
+        assert d.info()["pos"] == steps.info()["pos"] == 4101
+        with pytest.raises(RuntimeError):
+            d.run_sampled(us[:100], **params)  # past the context
+    assert btf.device_error() == 0
