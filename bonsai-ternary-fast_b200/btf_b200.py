@@ -314,6 +314,7 @@ def kernels_init(device: int = 0) -> None:
     """Per-device set-up (btf_init); kernels_init in src/cuda/kernels.cuh:17."""
     check(lib().btf_init(device), "btf_init")
     _initialised.add(device)
+    _bind_calls()
 
 
 def ensure_init(device: int) -> None:
@@ -643,6 +644,27 @@ SAMPLE_MAX_V = 524288  # BTF_SAMPLE_MAX_V
 _ELEM: dict = {}  # torch dtype -> element type id
 
 
+# The ordinary calls of rope, tree_attention and sample (tensors of the expected types on the current device and its
+# current stream) go through bind/calls.cpp: None from it, and all else, is for the Python below.
+_calls = None
+
+
+def _bind_calls() -> None:
+    global _calls
+    path = os.path.join(HERE, "btf_b200_calls.so")
+    if _calls is not None or not os.path.exists(path):
+        return
+    import importlib.util
+
+    _torch()
+    spec = importlib.util.spec_from_file_location("btf_b200_calls", path)
+    calls = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(calls)
+    calls.bind(*(ctypes.cast(getattr(lib(), n), ctypes.c_void_p).value
+                 for n in ("btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample")))
+    _calls = calls
+
+
 def _elem(t, what: str) -> int:
     if not _ELEM:
         torch = _torch()
@@ -736,6 +758,8 @@ class RopeSeg:
 def rope(segs: Sequence[RopeSeg], table: RopeTable, pos, inverse: bool = False, eps: float = 1e-6, stream=None) -> None:
     """Rotates up to 3 tensors of the same tokens by their positions pos [T] (int32) in one launch (btf_rope).
     inverse: the transposed map, the gradient of the rotation."""
+    if stream is None and _calls is not None and _calls.rope(segs, table, pos, inverse, eps):
+        return
     torch = _torch()
     n = len(segs)
     if not 1 <= n <= 3:
@@ -802,6 +826,10 @@ def tree_attention(q, k, v, lens, parents, counts=None, scale: Optional[float] =
     """Attention of a tree of drafted tokens over a cache (btf_tree_attention): q [B][n][H][D]; k and v
     [B][n_ctx][HK][D] hold lens[b] cached tokens and the nodes behind them; node i sees the cache, itself and its
     ancestors by parents [B][n] (int32, -1: hangs on the cache). counts [B]: nodes of each sequence (None: n)."""
+    if stream is None and _calls is not None:
+        done = _calls.tree_attention(q, k, v, lens, parents, counts, scale, out, work)
+        if done is not None:
+            return done
     torch = _torch()
     qs, ks = q.shape, k.shape
     if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[0] != qs[0] or ks[3] != qs[3]:
@@ -850,6 +878,10 @@ def _tree_call(st, args):
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprobs=None, stream=None):
     """Draws a token of each row of logits [B][V] from the random numbers u [B] in [0, 1) (btf_sample); temperature,
     top_p, min_p (float32) and top_k (int32) are [B] or None. Returns (tokens int32 [B], logprobs float32 [B])."""
+    if stream is None and _calls is not None:
+        done = _calls.sample(logits, u, temperature, top_k, top_p, min_p, tokens, logprobs)
+        if done is not None:
+            return done
     torch = _torch()
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise RuntimeError("sample: logits [B][V] with contiguous rows expected")

@@ -75,3 +75,78 @@ def test_rope_attention_sampling(cuda, btf, t):
             assert int(tok[j]) == want
             assert abs(float(lp[j]) - wlp) <= 2.0 ** -15
     assert btf.device_error() == 0
+
+
+def test_short_and_long_way_of_a_call_agree(cuda, btf, monkeypatch):
+    """The binding of ordinary calls does them itself, on the current stream too; what it leaves to the Python mirror
+    (another type, a stream that is given, an error) ends the same way."""
+    import gc
+
+    g = torch.Generator(device=cuda).manual_seed(4)
+    rn = lambda *s: torch.randn(*s, generator=g, device=cuda)  # noqa: E731
+    T, H, HK, D, ctx = 5, 6, 2, 64, 40
+    q, k, kc, w = rn(T, H, 2 * D)[..., :D], rn(T, HK, D), rn(ctx, HK, D).half(), rn(D)
+    pos, rows = torch.arange(7, 7 + T, dtype=torch.int32, device=cuda), torch.arange(3, 3 + T, dtype=torch.int32, device=cuda)
+    table = btf.RopeTable(32, base=1e5, scaling="linear", factor=2.0, interleaved=True)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    tq, tk, tv = rn(2, 3, H, D).half(), rn(2, ctx, HK, D).half(), rn(2, ctx, HK, D).half()
+    lens, parents, counts = i32(37, 5), torch.tensor([[-1, 0, 1], [-1, -1, 0]], dtype=torch.int32, device=cuda), i32(3, 2)
+    x, u = rn(4, 999), torch.rand(4, generator=g, device=cuda)
+    par = dict(temperature=torch.full((4,), 0.7, device=cuda), top_k=i32(9, 0, 30, 1), top_p=torch.full((4,), 0.9, device=cuda))
+
+    def all_calls(**kw):
+        y, c = torch.zeros(T, H, D, device=cuda), kc.clone()
+        btf.rope([btf.RopeSeg(q, y, normw=w), btf.RopeSeg(k, c, rows=rows, rotate=False)], table, pos, **kw)
+        z = y.clone()
+        btf.rope([btf.RopeSeg(z)], table, pos, True, **kw)
+        o = btf.tree_attention(tq, tk, tv, lens, parents, counts, scale=0.3, **kw)
+        o2 = btf.tree_attention(tq, tk, tv, lens, parents, out=torch.zeros_like(tq), **kw)
+        return [y, c, z, o, o2, *btf.sample(x, u, **par, **kw), *btf.sample(x, u, **kw)]
+
+    btf.ensure_init(0)
+    assert btf._calls is not None
+    taken = []
+    calls = btf._calls
+
+    class Seen:
+        def __getattr__(self, name):
+            def call(*a):
+                r = getattr(calls, name)(*a)
+                taken.append(r is not None)
+                return r
+            return call
+
+    monkeypatch.setattr(btf, "_calls", Seen())
+    short = all_calls()
+    assert len(taken) == 6 and all(taken)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = all_calls()
+    side.synchronize()
+    given = all_calls(stream=side)
+    side.synchronize()
+    assert len(taken) == 12 and all(taken)
+    for bad in (lambda: btf.rope([btf.RopeSeg(x)], table, pos), lambda: btf.sample(x.double(), u),
+                lambda: btf.sample(x, u[:3]), lambda: btf.tree_attention(tq, tk.float(), tv, lens, parents),
+                lambda: btf.rope([btf.RopeSeg(k.cpu())], table, pos), lambda: btf.rope([], table, pos),
+                lambda: btf.tree_attention(tq, tk, tv, lens, parents, work=torch.empty(256, dtype=torch.uint8, device=cuda)),
+                lambda: btf.sample(x, u, tokens=torch.zeros(4, device=cuda))):
+        with pytest.raises(RuntimeError):
+            bad()
+    assert not any(taken[12:])
+    monkeypatch.setattr(btf, "_calls", None)
+    long = all_calls()
+    for other in (on_side, given, long):
+        for a, b in zip(short, other):
+            assert a.dtype == b.dtype and torch.equal(a, b)
+    # the short way keeps no reference
+    monkeypatch.setattr(btf, "_calls", calls)
+    torch.cuda.synchronize()
+    del short, on_side, given, long, other, a, b
+    gc.collect()
+    before = torch.cuda.memory_allocated()
+    for _ in range(50):
+        all_calls()
+    gc.collect()
+    assert torch.cuda.memory_allocated() == before
