@@ -32,7 +32,7 @@
 // 4 KB that shared memory gives, and S of tile j + 2 need not wait for P V of tile j.
 //
 // Measured (device time): 16 nodes x 24 heads of 256 over 4096 fp16 rows of 4
-// kv-heads: 16.4 us (17 MB; the floor of a call, 1 node over 513 rows, is 11.1: two
+// kv-heads: 16.4 us (17 MB; the floor of a call, 1 node over 513 rows, is 10.1: two
 // launches, lengths, q, K, V and the parts' way through memory one after another);
 // 16 sequences of up to 8203 rows, 24 nodes, 32 and 8 heads of 128: 29.2 us, 3.3 TB/s;
 // 1 node over 131072 rows 5.9 TB/s of K and V, 16 nodes 5.4; 64 nodes (three M tiles):
@@ -115,7 +115,7 @@ struct Seq {
 // number of equal ranges, n_b = ceil(tiles / per) with the least `per` that fits, and a
 // CTA has one segment (a second one costs its q and its way out again, about 5 tiles
 // of time: 1 x 1 node over 513 rows took 15.5 us with ranges across pairs, 12.0
-// without). Otherwise the line of all tiles is cut into equal ranges.
+// without; the search for `per` is 0.4 us of it, and left out for equal lengths). Otherwise the line of all tiles is cut into equal ranges.
 struct Segments {
   const TreeParams& p;
   int b, kvh, tile, nt, index;  // the present one; index: in the CTA
@@ -153,14 +153,21 @@ struct Segments {
     load(0);
     const int pairs = p.HK * __popc(__ballot_sync(0xffffffffu, mine.tiles > 0));
     if (p.B <= 32 && pairs <= p.ranges) {
-      const int total = p.HK * __reduce_add_sync(0xffffffffu, mine.tiles);
-      int per = max(1, (total + p.ranges - 1) / p.ranges);
-      // sum ceil(tiles / per) <= total / per + pairs
-      int most = pairs < p.ranges ? max(per, (total + p.ranges - pairs - 1) / (p.ranges - pairs)) : max(1, total);
-      while (per < most) {
-        const int mid = (per + most) / 2;
-        if (p.HK * __reduce_add_sync(0xffffffffu, (mine.tiles + mid - 1) / mid) <= p.ranges) most = mid;
-        else per = mid + 1;
+      const int longest = __reduce_max_sync(0xffffffffu, mine.tiles);
+      int per = 1;
+      if (__all_sync(0xffffffffu, mine.tiles == 0 || mine.tiles == longest)) {  // (all of one length: no search)
+        const int each = p.ranges / max(pairs, 1);
+        per = max(1, (longest + each - 1) / each);
+      } else {
+        const int total = p.HK * __reduce_add_sync(0xffffffffu, mine.tiles);
+        per = max(1, (total + p.ranges - 1) / p.ranges);
+        // sum ceil(tiles / per) <= total / per + pairs
+        int most = pairs < p.ranges ? max(per, (total + p.ranges - pairs - 1) / (p.ranges - pairs)) : max(1, total);
+        while (per < most) {
+          const int mid = (per + most) / 2;
+          if (p.HK * __reduce_add_sync(0xffffffffu, (mine.tiles + mid - 1) / mid) <= p.ranges) most = mid;
+          else per = mid + 1;
+        }
       }
       const int n = (mine.tiles + per - 1) / per, t = up_to(n * p.HK);
       if (table && lane < p.B) p.first[lane] = t - n * p.HK;
@@ -778,12 +785,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<DP>::kPerSm)
             for (int k = 0; k < 8; ++k) st_if(to4 + k * 4 * p.D, v[k], k * 4 < left4 && (lane & 7) * 4 < cols);
           }
         };
+        // few rows' parts: a lane's own row goes out as it is, with less code (which is cold) and no way through
+        // shared memory
+        const bool few = !whole && rows - warp * 32 <= 8 && !__any_sync(0xffffffffu, bad != 0);
+        float* own = p.part + (slot * kRowsM + r) * p.D;
 #pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(tmem + c * 32 + lanes, o);
           tmem_wait_ld(o);
-          emit(c, o);
+          if (few) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              st_if(own + c * 32 + i * 4, make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]),
+                    live && c * 32 + i * 4 < p.D);
+          } else {
+            emit(c, o);
+          }
         }
         if (live && !whole) reinterpret_cast<float2*>(p.ml)[slot * kRowsM + r] = make_float2(m, l);
       }

@@ -280,3 +280,32 @@ def test_refusals(cuda, btf):
         with pytest.raises(RuntimeError):
             fn()
     assert btf.tree_attention(q[:0], k[:0], v[:0], i[:0], par[:0]).shape == (0, 4, 4, 64)
+
+
+@pytest.mark.parametrize("B,n,ctx", [(1, 1, 700), (3, 4, 2100), (40, 2, 600)])
+def test_lengths_that_change_from_call_to_call(cuda, btf, B, n, ctx):
+    """Calls one after another without a synchronisation, the lengths and counts rewritten in between by a kernel on the
+    same stream: each call's outputs are those of a call by itself."""
+    H, HK, D = 4, 2, 128
+    g = torch.Generator(device=cuda).manual_seed(B)
+    q, k, v = (torch.randn(s, generator=g, device=cuda).half() for s in ((B, n, H, D), (B, ctx, HK, D), (B, ctx, HK, D)))
+    parents = (torch.arange(n, dtype=torch.int32, device=cuda) - 1).repeat(B, 1)
+    calls = 40
+    all_lens = torch.randint(0, ctx - n + 1, (calls, B), generator=g, device=cuda).int()
+    all_counts = torch.randint(0, n + 1, (calls, B), generator=g, device=cuda).int()
+    want = []
+    for i in range(calls):
+        torch.cuda.synchronize()
+        want.append(btf.tree_attention(q, k, v, all_lens[i].clone(), parents, all_counts[i].clone()))
+        torch.cuda.synchronize()
+    lens, counts = torch.zeros(B, dtype=torch.int32, device=cuda), torch.zeros(B, dtype=torch.int32, device=cuda)
+    work = btf.tree_attention_work(q, k)
+    got = [torch.zeros_like(q) for _ in range(calls)]
+    torch.cuda.synchronize()
+    for i in range(calls):
+        torch.add(all_lens[i], 0, out=lens)
+        torch.add(all_counts[i], 0, out=counts)
+        btf.tree_attention(q, k, v, lens, parents, counts, out=got[i], work=work)
+    for i in range(calls):
+        assert torch.equal(got[i], want[i]), i
+    assert btf.device_error() == 0
