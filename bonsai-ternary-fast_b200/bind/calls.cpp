@@ -171,6 +171,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     if (args[8] != Py_None) {
       work = on(args[8], dev);
+      if (!work.is_contiguous()) throw Other{};
     } else {
       const int64_t bytes = lib.tree_work((int)B, (int)n, (int)H, (int)HK, (int)D, (int)ctx);
       if (bytes < 0) throw Other{};

@@ -798,6 +798,8 @@ def rope(segs: Sequence[RopeSeg], table: RopeTable, pos, inverse: bool = False, 
     turns = table.turns
     if turns is None or turns.device != dev:
         raise RuntimeError(f"rope: the table must be on {dev}")
+    if table.n_rot > 2 * turns.numel() or turns.dtype != torch.float64 or not turns.is_contiguous():
+        raise RuntimeError(f"rope: the table's turns must hold n_rot / 2 = {table.n_rot // 2} contiguous float64 values")
     _launch(dev, stream, _rope_call, (packed, n, T, D, table.n_rot, turns.data_ptr(), table.mscale, table.interleaved,
                                       inverse, eps, pos_ptr))
 
@@ -861,6 +863,8 @@ def _tree_call(st, args):
         work = tree_attention_work(q, k)
     elif work.device != dev:
         raise RuntimeError(f"tree_attention: work is on {work.device}, not on {dev}")
+    elif not work.is_contiguous():
+        raise RuntimeError("tree_attention: the workspace must be contiguous")
     q0, q1, q2, qd = _strides(q)
     k0, k1, k2, kd = kv = _strides(k)
     o0, o1, o2, od = _strides(out)

@@ -159,10 +159,18 @@ struct Decoder {
     if (dry) return nullptr;
     const cudaError_t e = cudaMalloc(&p, bytes);
     if (e != cudaSuccess) {
+      dev_bytes[kind] -= bytes;
       *rc = cuda_fail(e, "btf_decoder: cudaMalloc");
       return nullptr;
     }
-    allocs.push_back(p);
+    try {
+      allocs.push_back(p);
+    } catch (...) {  // nothing may leave a C entry
+      cudaFree(p);
+      dev_bytes[kind] -= bytes;
+      *rc = fail(BTF_ERR_CUDA, "btf_decoder: out of host memory");
+      return nullptr;
+    }
     return static_cast<T*>(p);
   }
   uint64_t device_total() const {
@@ -428,9 +436,10 @@ int make_draft_buffers(Decoder& D) {
   bool attn = false;
   for (Layer& l : D.L) {
     attn |= !l.rec;
-    if (!l.rec || l.node_state) continue;
-    l.node_ring = D.alloc<float>((size_t)R * d.conv_kernel * D.C, &rc, Decoder::kState);
-    l.node_state = D.alloc<float>((size_t)R * D.NV * D.DV * D.DK, &rc, Decoder::kState);
+    if (!l.rec) continue;
+    // (a call that ran out of memory goes on from there)
+    if (!l.node_ring) l.node_ring = D.alloc<float>((size_t)R * d.conv_kernel * D.C, &rc, Decoder::kState);
+    if (!l.node_state) l.node_state = D.alloc<float>((size_t)R * D.NV * D.DV * D.DK, &rc, Decoder::kState);
     if (rc) return rc;
   }
   if (attn && !D.tree_work) {

@@ -150,3 +150,17 @@ def test_short_and_long_way_of_a_call_agree(cuda, btf, monkeypatch):
         all_calls()
     gc.collect()
     assert torch.cuda.memory_allocated() == before
+
+
+def test_tables_and_workspaces_that_are_too_small(cuda, btf):
+    """A table with fewer frequencies than it says, and a workspace whose bytes are one byte over and over."""
+    x, pos = torch.zeros(2, 1, 64, device=cuda), torch.zeros(2, dtype=torch.int32, device=cuda)
+    table = btf.RopeTable(16)
+    table.n_rot = 64
+    with pytest.raises(RuntimeError):
+        btf.rope([btf.RopeSeg(x)], table, pos)
+    q, k = torch.zeros(1, 1, 2, 64, device=cuda).half(), torch.zeros(1, 300, 2, 64, device=cuda).half()
+    work = btf.tree_attention_work(q, k)
+    for bad in (work[:1].expand(len(work)), torch.empty(2 * len(work), dtype=torch.uint8, device=cuda)[::2]):
+        with pytest.raises(RuntimeError):
+            btf.tree_attention(q, k, k, pos[:1], pos[:1, None], work=bad)
