@@ -167,3 +167,21 @@ def test_cpp_mirror_of_drafts_compiles():
                         "-I", "/usr/local/cuda/include", os.path.join(root, "tests", "shim_draft.cpp")],
                        capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_binding_leaves_what_is_not_ordinary(btf):
+    """Without CUDA tensors the binding of ordinary calls declines, whatever it is given."""
+    torch = pytest.importorskip("torch")
+    if not os.path.exists(os.path.join(btf.HERE, "btf_b200_calls.so")):
+        pytest.skip("built without torch")
+    btf.lib()
+    btf._bind_calls()
+    x, v = torch.zeros(2, 3, 8), torch.zeros(2, dtype=torch.int32)
+    table = btf.RopeTable(8, device=None)
+    for segs in ([], [btf.RopeSeg(x)], [btf.RopeSeg(None)], [None], (btf.RopeSeg(x),), [btf.RopeSeg(x)] * 4, None):
+        assert btf._calls.rope(segs, table, v, False, 1e-6) is None
+    q = torch.zeros(1, 1, 2, 64).half()
+    for a in (q, None, 3):
+        assert btf._calls.tree_attention(a, q, q, v, v, None, None, None, None) is None
+        assert btf._calls.sample(a, v, None, None, None, None, None, None) is None
+    assert btf._calls.sample(x) is None  # (too few arguments)
