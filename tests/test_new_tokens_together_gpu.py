@@ -149,7 +149,7 @@ def test_short_and_long_way_of_a_call_agree(cuda, btf, monkeypatch):
     for _ in range(50):
         all_calls()
     gc.collect()
-    assert torch.cuda.memory_allocated() == before
+    assert torch.cuda.memory_allocated() <= before
 
 
 def test_tables_and_workspaces_that_are_too_small(cuda, btf):
