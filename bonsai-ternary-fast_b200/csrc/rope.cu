@@ -22,6 +22,9 @@ namespace btf {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMaxHeads = 16;  // per thread
+// NORM: none; a token's lanes hold a whole head; or they take several rounds for one
+constexpr int kOneRound = 1, kRounds = 2;
 
 struct RopeSeg {
   const void* x;
@@ -42,7 +45,13 @@ struct RopeParams {
   float mscale, eps;
 };
 
-// One token's heads [h0, h1) of one tensor. A thread owns the C pairs of its
+// 1 / sqrt(mean square + eps) of a head from its lanes' sums of squares.
+__device__ __forceinline__ float norm_scale(const RopeParams& p, unsigned mask, float ss) {
+  for (int o = p.lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+  return 1.0f / sqrtf(ss / (float)p.D + p.eps);
+}
+
+// One token's heads [h0, h1) of one tensor; scales: the token's place for their norms. A thread owns the C pairs of its
 // item (and item + lanes, ... when a head has more items than lanes) and keeps
 // their cos and sin over the heads. The loads of kBatch heads are issued before
 // the first store: x and y may be one tensor, so the compiler would keep each
@@ -50,9 +59,9 @@ struct RopeParams {
 // heads of 128, 336 MB: 100 us a head at a time, 67 with 4, 60 with 8, 57 (5870
 // GB/s, 0.90 of a plain copy's rate) with 16 heads a thread for 8; loads ahead of
 // the angles too keep more registers and lose.
-template <typename TX, typename TY, int C, bool NORM>
+template <typename TX, typename TY, int C, int NORM>
 __device__ __forceinline__ void rope_heads(const RopeParams& p, const RopeSeg& s, int t, int64_t row, int h0, int h1,
-                                           int lane) {
+                                           int lane, float* scales) {
   constexpr int kBatch = NORM ? 1 : C * (int)sizeof(TX) >= 32 ? 2 : C == 8 ? 8 : 4;
   const int R = s.rotate ? p.R : 0, half = R / 2, D = p.D;
   const int nrot = half / C;                               // rotated items: C pairs each
@@ -61,7 +70,24 @@ __device__ __forceinline__ void rope_heads(const RopeParams& p, const RopeSeg& s
   TY* y = static_cast<TY*>(s.y) + row * s.y_token;
   // with a norm: the lanes of this token, which take the same branches
   const unsigned mask = p.lanes == 32 ? 0xffffffffu : ((1u << p.lanes) - 1) << (threadIdx.x & 31 & ~(p.lanes - 1));
-  for (int it0 = 0; it0 < items; it0 += p.lanes) {
+  // in place, a round's stores replace values that the next one's sum would read: every head's scale is taken before
+  // the first store (such a token has a warp). Once a head, not once a round: 4000 tokens of 16 fp16 heads of 1024 take
+  // 194 us for 357.
+  if (NORM == kRounds && s.normw) {
+#pragma unroll 1
+    for (int h = h0; h < h1; ++h) {
+      const TX* xh = x + (int64_t)h * s.x_head;
+      float ss = 0.f;
+      for (int e = lane; e < D; e += p.lanes) {
+        const float v = to_f32(xh[e]);
+        ss = fmaf(v, v, ss);
+      }
+      const float scale = norm_scale(p, mask, ss);
+      if (lane == 0) scales[h - h0] = scale;
+    }
+    __syncwarp(mask);
+  }
+  for (int it0 = 0; it0 < (NORM == kOneRound ? 1 : items); it0 += p.lanes) {  // rounds
     const int it = it0 + lane;
     const bool active = it < items, rot = it < nrot;
     if (!NORM && !active) return;
@@ -106,19 +132,15 @@ __device__ __forceinline__ void rope_heads(const RopeParams& p, const RopeSeg& s
 #pragma unroll
         for (int j = 0; j < C; ++j) fa[j] = a[k].get(j), fb[j] = b[k].get(j);
         if (NORM && s.normw) {
-          float ss = 0.f;
-          if (items <= p.lanes) {  // the token's lanes hold the whole head
+          float scale;
+          if constexpr (NORM == kRounds) {
+            scale = scales[hb - h0];
+          } else {  // the token's lanes hold the whole head
+            float ss = 0.f;
 #pragma unroll
             for (int j = 0; j < C; ++j) ss = fmaf(fa[j], fa[j], fmaf(fb[j], fb[j], ss));
-          } else {
-            const TX* xh = x + (int64_t)hb * s.x_head;
-            for (int e = lane; e < D; e += p.lanes) {
-              const float v = to_f32(xh[e]);
-              ss = fmaf(v, v, ss);
-            }
+            scale = norm_scale(p, mask, ss);
           }
-          for (int o = p.lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-          const float scale = 1.0f / sqrtf(ss / (float)D + p.eps);
 #pragma unroll
           for (int j = 0; j < C; ++j) fa[j] *= scale * wa[j], fb[j] *= scale * wb[j];
         }
@@ -153,16 +175,18 @@ __device__ __forceinline__ void rope_heads(const RopeParams& p, const RopeSeg& s
   }
 }
 
-template <typename TX, int C, bool NORM>
+template <typename TX, int C, int NORM>
 __device__ __forceinline__ void rope_to(const RopeParams& p, const RopeSeg& s, int t, int64_t row, int h0, int h1,
-                                        int lane) {
-  if (s.y_type == BTF_F32) rope_heads<TX, float, C, NORM>(p, s, t, row, h0, h1, lane);
-  else if (s.y_type == BTF_F16) rope_heads<TX, __half, C, NORM>(p, s, t, row, h0, h1, lane);
-  else rope_heads<TX, __nv_bfloat16, C, NORM>(p, s, t, row, h0, h1, lane);
+                                        int lane, float* scales) {
+  if (s.y_type == BTF_F32) rope_heads<TX, float, C, NORM>(p, s, t, row, h0, h1, lane, scales);
+  else if (s.y_type == BTF_F16) rope_heads<TX, __half, C, NORM>(p, s, t, row, h0, h1, lane, scales);
+  else rope_heads<TX, __nv_bfloat16, C, NORM>(p, s, t, row, h0, h1, lane, scales);
 }
 
-template <int C, bool NORM>
+template <int C, int NORM>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p) {
+  __shared__ float scales_of[NORM == kRounds ? kThreads / 32 : 1][kMaxHeads];
+  float* scales = scales_of[NORM == kRounds ? threadIdx.x >> 5 : 0];
   pdl_launch_dependents();
   pdl_wait();
   const int per = kThreads / p.lanes, in = threadIdx.x / p.lanes;
@@ -177,9 +201,9 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
     row = s.rows[t];
     if (row < 0 || row >= s.n_rows) return;
   }
-  if (s.x_type == BTF_F32) rope_to<float, C, NORM>(p, s, t, row, h0, h1, lane);
-  else if (s.x_type == BTF_F16) rope_to<__half, C, NORM>(p, s, t, row, h0, h1, lane);
-  else rope_to<__nv_bfloat16, C, NORM>(p, s, t, row, h0, h1, lane);
+  if (s.x_type == BTF_F32) rope_to<float, C, NORM>(p, s, t, row, h0, h1, lane, scales);
+  else if (s.x_type == BTF_F16) rope_to<__half, C, NORM>(p, s, t, row, h0, h1, lane, scales);
+  else rope_to<__nv_bfloat16, C, NORM>(p, s, t, row, h0, h1, lane, scales);
 }
 
 bool aligned_for(const btf_rope_seg& s, int C) {
@@ -286,7 +310,7 @@ int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const 
   // stays full; 16 pay where 8 are in flight at once (7001 tokens of 40 fp32 heads
   // of 80: 32.5 us with 8, 34.7 with 16)
   const int64_t full = (int64_t)dev->sm_count * 2048;
-  p.hl = (int)std::max<int64_t>(1, std::min<int64_t>(C == 8 && narrow ? 16 : 8, (int64_t)T * heads * p.lanes / full));
+  p.hl = (int)std::max<int64_t>(1, std::min<int64_t>(C == 8 && narrow ? kMaxHeads : 8, (int64_t)T * heads * p.lanes / full));
   int blocks = 0;
   for (int i = 0; i < nseg; ++i) {
     const btf_rope_seg& s = segs[i];
@@ -299,8 +323,10 @@ int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const 
   const int per = kThreads / p.lanes;
   const dim3 grid((T + per - 1) / per, blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const auto kernel = norm ? (C == 8 ? rope_kernel<8, true> : C == 4 ? rope_kernel<4, true> : rope_kernel<1, true>)
-                           : (C == 8 ? rope_kernel<8, false> : C == 4 ? rope_kernel<4, false> : rope_kernel<1, false>);
+  const auto pick = [C](auto c8, auto c4, auto c1) { return C == 8 ? c8 : C == 4 ? c4 : c1; };
+  const auto kernel = !norm             ? pick(rope_kernel<8, 0>, rope_kernel<4, 0>, rope_kernel<1, 0>)
+                      : items > p.lanes ? pick(rope_kernel<8, kRounds>, rope_kernel<4, kRounds>, rope_kernel<1, kRounds>)
+                                        : pick(rope_kernel<8, kOneRound>, rope_kernel<4, kOneRound>, rope_kernel<1, kOneRound>);
   const cudaError_t e = launch_pdl(kernel, grid, dim3(kThreads), 0, st, p);
   return e == cudaSuccess ? BTF_OK : cuda_fail(e, "btf_rope");
 }

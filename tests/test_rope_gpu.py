@@ -250,3 +250,27 @@ def test_many_tokens(cuda, btf, t, inter):
     # at most sqrt 2 of its pair's length, so the square by 2 sqrt 2 * 8 * 2^-24 + eps of it, below 2^-19 + 2 eps
     a, b = x.double().square().sum(-1), y.double().square().sum(-1)
     assert float(((a - b).abs() / a).max()) <= 2 * torch.finfo(t).eps + 2.0 ** -19
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T,H,D,R,off", [(5, 3, 100, 100, 0), (5, 3, 100, 50, 0), (4, 2, 80, 20, 0), (3, 5, 72, 36, 0),
+                                         (2, 3, 1024, 512, 0), (6, 2, 128, 128, 1), (3, 2, 65, 0, 0), (4, 3, 256, 64, 0),
+                                         (3001, 33, 100, 100, 0), (1201, 33, 1024, 1024, 0)])
+def test_norm_in_place(cuda, btf, T, H, D, R, off, t, inter):
+    """A head's norm is that of its values before any of them is replaced, however many rounds of lanes it takes: the
+    same bits as a call into another tensor of the same layout, and the formula's values."""
+    g = torch.Generator(device=cuda).manual_seed(T + D + R)
+    x = (torch.randn(T * H * D + off, generator=g, device=cuda) * 2).to(t)[off:].view(T, H, D)
+    w = torch.rand(D, generator=g, device=cuda) + 0.5
+    pos = torch.randint(0, 5000, (T,), generator=g, device=cuda, dtype=torch.int32)
+    table = btf.RopeTable(max(R, 2), base=1e6, interleaved=inter)
+    table.n_rot = R
+    y = torch.zeros(T * H * D + off, dtype=t, device=cuda)[off:].view(T, H, D)
+    btf.rope([btf.RopeSeg(x, y, normw=w)], table, pos)
+    given = x.cpu()
+    btf.rope([btf.RopeSeg(x, normw=w)], table, pos)
+    assert torch.equal(x, y)
+    at = list(range(T))[:: max(1, T // 50)]
+    ref, size = _reference(given[at], table.host[: R // 2], 1.0, pos[at], inter, normw=w)
+    _check(x[at], ref, size, normed_D=D)
