@@ -862,6 +862,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   // the histogram when there are top_k or top_p, then the logits [chunk] when they are held
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Shared sh;
+  cluster_arrive_relaxed();  // matched by the wait before the first remote store
   uint32_t size;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
   const bool hist = p.top_k || p.top_p;
@@ -930,6 +931,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if ((tid & 31) == 0) sh.warp[tid >> 5][0] = best;
   __syncthreads();
   for (int i = 0; i < kWarps; ++i) best = sh.warp[i][0] > best ? sh.warp[i][0] : best;
+  // every CTA of the cluster is running: its shared memory may be written (one that has no logits comes here at once)
+  __syncwarp();
+  cluster_wait_acquire();
   {
     const auto s = c.exchange(best, 0);
     for (int r = 0; r < c.size; ++r) best = s[r][0] > best ? s[r][0] : best;

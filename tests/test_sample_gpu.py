@@ -244,3 +244,21 @@ def test_many_rows(cuda, btf, B, V, off, t, f):
                           np.float32(f.get("m", 0.0)))
         assert tok[b] == r, b
         np.testing.assert_allclose(lp[b], l, rtol=2.0 ** -23, atol=2.0 ** -15, err_msg=str(b))
+
+
+@pytest.mark.parametrize("f", FILTERS[:5], ids=str)
+@pytest.mark.parametrize("B,V", [(1, 70000), (2, 131073), (3, 33000), (9, 66000), (1, 4097)])
+def test_ctas_without_logits(cuda, btf, B, V, f):
+    """Rows whose last CTAs of the cluster have nothing to read (70000 values: 12 parts of 6144 for 16 CTAs), launched
+    back to back: those CTAs reach the cluster's first exchange before the others have begun to read."""
+    rng = np.random.default_rng(V)
+    x, u, T = _logits(B, V, V), rng.random(B, dtype=np.float32), rng.uniform(0.3, 1.5, B)
+    a = {n: np.full(B, v) for n, v in f.items()}
+    _compare(btf, cuda, x, u, T=T, **a)
+    xd, ud, t = x.to(cuda), torch.from_numpy(u).to(cuda), torch.from_numpy(T.astype(np.float32)).to(cuda)
+    par = {dict(k="top_k", p="top_p", m="min_p")[n]: torch.as_tensor(v, dtype=torch.int32 if n == "k" else torch.float32).to(cuda)
+           for n, v in a.items()}
+    outs = [btf.sample(xd, ud, temperature=t, **par) for _ in range(50)]
+    for tok, lp in outs[1:]:
+        assert torch.equal(tok, outs[0][0]) and torch.equal(lp, outs[0][1])
+    assert btf.device_error() == 0
