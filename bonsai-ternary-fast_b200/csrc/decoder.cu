@@ -393,7 +393,9 @@ int enqueue_chunk(Decoder& D, int M) {
 }
 
 // ---------------------------------------------------------------- sampled steps
-// The parameters (the same for every row) and n_u random numbers go to the device, in stream order.
+// The parameters (the same for every row) and n_u <= kMaxRandom random numbers go to the device, in stream order. They
+// are copied from this function's own memory: a copy from pageable memory has read it when the call returns, one from
+// memory that the caller pinned would read it behind the steps that are queued.
 int set_sampling(Decoder& D, const btf_sampling& s, const float* u, int n_u) {
   constexpr int R = Decoder::kMaxChunk;
   if (!D.d_u) {
@@ -401,18 +403,18 @@ int set_sampling(Decoder& D, const btf_sampling& s, const float* u, int n_u) {
     float* p = D.alloc<float>(4 * R + Decoder::kMaxRandom + R, &rc);
     if (rc) return rc;
     for (int i = 0; i < 4; ++i) D.d_rows[i] = p + i * R;
-    D.d_lp = p + 4 * R;
-    D.d_u = p + 5 * R;
+    D.d_u = p + 4 * R;
+    D.d_lp = D.d_u + Decoder::kMaxRandom;
   }
-  float h[4 * R];
+  float h[4 * R + Decoder::kMaxRandom];
   for (int i = 0; i < R; ++i) {
     h[i] = s.temperature;
     h[R + i] = s.top_p;
     h[2 * R + i] = s.min_p;
     std::memcpy(&h[3 * R + i], &s.top_k, 4);
   }
-  cudaError_t e = cudaMemcpyAsync(D.d_rows[0], h, sizeof h, cudaMemcpyHostToDevice, D.st);  // (pageable: staged at once)
-  if (e == cudaSuccess && n_u) e = cudaMemcpyAsync(D.d_u, u, n_u * sizeof(float), cudaMemcpyHostToDevice, D.st);
+  std::copy(u, u + n_u, h + 4 * R);
+  const cudaError_t e = cudaMemcpyAsync(D.d_rows[0], h, (4 * R + n_u) * sizeof(float), cudaMemcpyHostToDevice, D.st);
   return e == cudaSuccess ? BTF_OK : cuda_fail(e, "btf_decoder: sampling parameters");
 }
 cudaError_t sample_rows(Decoder& D, const float* logits, int n, const float* u, int32_t* tokens, int32_t* tokens2) {

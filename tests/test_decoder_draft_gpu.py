@@ -238,3 +238,20 @@ def test_a_long_drawn_run(cuda, btf):
         with pytest.raises(RuntimeError):
             d.run_sampled(us[:100], **params)  # past the context
     assert btf.device_error() == 0
+
+
+def test_a_drawn_run_copies_its_numbers(cuda, btf):
+    """The random numbers belong to the caller again when run_sampled returns, in pinned memory too."""
+    import torch
+
+    dims = dict(SMALL, n_layer=3)
+    params = dict(temperature=1.1, top_k=30)
+    us = torch.rand(4300, generator=torch.Generator().manual_seed(8)).pin_memory()
+    kept = us.numpy().copy()
+    with btf.Decoder(dims=dims, seed=5, n_ctx=4400) as d, btf.Decoder(dims=dims, seed=5, n_ctx=4400) as other:
+        for x, u in ((d, us.numpy()), (other, kept)):
+            x.step_sampled(3, 0.5, **params)
+            x.run_sampled(u, **params)
+            us.zero_()
+        assert np.array_equal(_device_logits(btf, d), _device_logits(btf, other))
+    assert btf.device_error() == 0
