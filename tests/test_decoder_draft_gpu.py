@@ -255,3 +255,38 @@ def test_a_drawn_run_copies_its_numbers(cuda, btf):
             us.zero_()
         assert np.array_equal(_device_logits(btf, d), _device_logits(btf, other))
     assert btf.device_error() == 0
+
+
+TREE = ([5, 17, 18, 19, 256, 257, 3, 640], [-1, 0, 0, 1, 1, 4, -1, 6])
+
+
+@pytest.mark.parametrize("node", [0, 2, 4, 7])
+def test_run_continues_from_the_accepted_node(cuda, btf, dims, node):
+    """btf_decoder_run takes the token after the accepted node of a branching tree, whichever node that is."""
+    tokens, parents = TREE
+    path, j = [], node
+    while j >= 0:
+        path.insert(0, tokens[j])
+        j = parents[j]
+    with _open(btf, dims) as d:
+        d.prefill(PROMPT)
+        nxt, _ = d.verify(tokens, parents)
+        assert len(set(nxt.tolist())) > 1
+        d.accept(node)
+        d.run(1)
+        got = _device_logits(btf, d)
+        assert d.info()["pos"] == len(PROMPT) + len(path) + 1
+    want = _along(btf, dims, path + [int(nxt[node])])[-1]
+    assert rel_rms(got, want) <= _tol(dims), rel_rms(got, want)
+    if dims["n_layer"] == 3:  # to 1e-5: a token from another node would be seen, and so is a run of several steps
+        with _open(btf, dims) as a, _open(btf, dims) as b:
+            a.prefill(PROMPT)
+            b.prefill(PROMPT)
+            for t in path:
+                a.step(t)
+            b.verify(tokens, parents)
+            b.accept(node)
+            a.run(3)
+            b.run(3)
+            la, lb = _device_logits(btf, a), _device_logits(btf, b)
+            assert rel_rms(lb, la) <= _tol(dims), rel_rms(lb, la)
