@@ -1253,6 +1253,7 @@ int btf_decoder_accept(void* handle, int node) {
   }
   copy(D.d_tok, D.d_nexts + node, sizeof(int32_t));
   copy(D.d_next, D.d_nexts + node, sizeof(int32_t));
+  copy(D.logits, D.node_logits + (size_t)node * D.d.n_vocab, (size_t)D.d.n_vocab * sizeof(float));
   const int32_t pos = D.pos + len;
   if (e == cudaSuccess) e = cudaStreamSynchronize(D.st);
   if (e == cudaSuccess) e = cudaMemcpy(D.d_pos, &pos, sizeof(int32_t), cudaMemcpyHostToDevice);

@@ -423,7 +423,7 @@ typedef struct btf_decoder_info {
   uint64_t weight_bytes;       /* resident weights one step reads (one embedding row) */
   uint64_t state_bytes;        /* recurrent state read + written per step */
   uint64_t kv_bytes_per_token; /* KV cache bytes read per step per cached token */
-  const float* logits;         /* device [n_vocab] of the last step */
+  const float* logits;         /* device [n_vocab]: behind the last token (of a step, a prompt or an accepted draft) */
   uint64_t device_bytes;       /* every device allocation the decoder holds (btf_plan_memory's device_bytes) */
 } btf_decoder_info;
 
@@ -471,8 +471,8 @@ int btf_decoder_run_sampled(void* handle, int steps, const btf_sampling* samplin
 int btf_decoder_verify(void* handle, const int32_t* tokens_host, const int32_t* parents_host, int n,
                        const btf_sampling* sampling, const float* u_host, float* logits, int32_t* next_host);
 /* Takes over the path from a node without a parent down to `node` of the last btf_decoder_verify: the path's rows of
- * the caches move behind the decoded tokens, the node's recurrent state becomes the decoder's, pos += the path's
- * length, and the token after `node` is the one that a btf_decoder_run continues from. */
+ * the caches move behind the decoded tokens, the node's recurrent state and logits become the decoder's, pos += the
+ * path's length, and the token after `node` is the one that a btf_decoder_run continues from. */
 int btf_decoder_accept(void* handle, int node);
 
 /* Per-step accounting since the last reset_stats (FastDecoder::stats /

@@ -290,3 +290,13 @@ def test_run_continues_from_the_accepted_node(cuda, btf, dims, node):
             b.run(3)
             la, lb = _device_logits(btf, a), _device_logits(btf, b)
             assert rel_rms(lb, la) <= _tol(dims), rel_rms(lb, la)
+
+
+@pytest.mark.parametrize("node", [0, 3, 7])
+def test_accepted_node_has_the_decoders_logits(cuda, btf, dims, node):
+    """After an acceptance the decoder's logits are those behind its last token, as after a step."""
+    with _open(btf, dims) as d:
+        d.prefill(PROMPT)
+        _, lg = d.verify(*TREE, logits=True)
+        d.accept(node)
+        assert np.array_equal(_device_logits(btf, d), lg[node])
