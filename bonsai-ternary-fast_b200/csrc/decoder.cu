@@ -436,10 +436,10 @@ int make_draft_buffers(Decoder& D) {
   const int R = Decoder::kMaxChunk, H = d.n_head, HK = d.n_head_kv, HD = d.head_dim;
   int rc = BTF_OK;
   bool attn = false;
+  // (a call that ran out of memory goes on from there: nothing is allocated twice)
   for (Layer& l : D.L) {
     attn |= !l.rec;
     if (!l.rec) continue;
-    // (a call that ran out of memory goes on from there)
     if (!l.node_ring) l.node_ring = D.alloc<float>((size_t)R * d.conv_kernel * D.C, &rc, Decoder::kState);
     if (!l.node_state) l.node_state = D.alloc<float>((size_t)R * D.NV * D.DV * D.DK, &rc, Decoder::kState);
     if (rc) return rc;
@@ -450,13 +450,13 @@ int make_draft_buffers(Decoder& D) {
       const btf_rope_cfg cfg{d.n_rot, BTF_ROPE_NONE, d.rope_base, 1.0, 0.0, 0.0, 0};
       float m = 1.0f;
       BTF_TRY(btf_rope_table(&cfg, turns, &m));
-      D.rope_turns = D.alloc<double>(d.n_rot / 2, &rc);
+      if (!D.rope_turns) D.rope_turns = D.alloc<double>(d.n_rot / 2, &rc);
       if (rc) return rc;
       const cudaError_t e = cudaMemcpy(D.rope_turns, turns, d.n_rot / 2 * sizeof(double), cudaMemcpyHostToDevice);
       if (e != cudaSuccess) return cuda_fail(e, "btf_decoder_verify: rotary table");
     }
-    D.q16 = D.alloc<__half>((size_t)R * H * HD, &rc);
-    D.o16 = D.alloc<__half>((size_t)R * H * HD, &rc);
+    if (!D.q16) D.q16 = D.alloc<__half>((size_t)R * H * HD, &rc);
+    if (!D.o16) D.o16 = D.alloc<__half>((size_t)R * H * HD, &rc);
     if (rc) return rc;
     // the workspace for any number of nodes up to R: the largest of them
     for (int n = 1; n <= std::min(R, D.o.n_ctx); ++n) {

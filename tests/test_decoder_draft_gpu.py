@@ -300,3 +300,47 @@ def test_accepted_node_has_the_decoders_logits(cuda, btf, dims, node):
         _, lg = d.verify(*TREE, logits=True)
         d.accept(node)
         assert np.array_equal(_device_logits(btf, d), lg[node])
+
+
+def test_a_draft_that_found_no_memory_leaves_none_behind(cuda, btf):
+    """A decoder whose first draft fails for want of device memory holds after the next one what it would have held."""
+    import ctypes
+
+    dims = DIMS["model heads"]  # a draft allocates 13 MB of states, the attention's small buffers, its workspace of 39 MB
+
+    def opened():
+        return btf.Decoder(dims=dims, seed=5, n_ctx=9600)
+
+    def take(size, held):
+        p = ctypes.c_void_p()
+        if btf.lib().btf_alloc(size, ctypes.byref(p)):
+            return False
+        held.append(p)
+        return True
+
+    def give(held):
+        while held:
+            assert btf.lib().btf_free(held.pop()) == 0
+
+    with opened() as plain:
+        plain.verify([1], [-1])
+        want = plain.info()["device_bytes"]
+    with opened() as d:
+        spare, rest, size = [], [], 1 << 38
+        try:
+            for _ in range(12):
+                assert take(2 << 20, spare)
+            while size >= 2 << 20:
+                if not take(size, rest):
+                    size //= 2
+            give(spare)  # 24 MB, and less than 2 beside them
+            with pytest.raises(RuntimeError, match="memory"):
+                d.verify([1], [-1])
+            # the workspace, 148 ranges x 2 x 128 rows x (256 + 2) floats, is what was not to be had
+            assert want - d.info()["device_bytes"] > 39 * 10 ** 6
+        finally:
+            give(spare)
+            give(rest)
+        d.verify([1], [-1])
+        assert d.info()["device_bytes"] == want
+    assert btf.device_error() == 0
