@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include "btf_b200.h"
 
@@ -268,5 +269,10 @@ PyMODINIT_FUNC PyInit_btf_b200_calls() {
   s_n_rot = PyUnicode_InternFromString("n_rot");
   s_mscale = PyUnicode_InternFromString("mscale");
   s_interleaved = PyUnicode_InternFromString("interleaved");
-  return PyModule_Create(&module);
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION)) {  // the mirror binds it to no other
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
 }

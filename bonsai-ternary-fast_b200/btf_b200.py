@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import sys
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -314,7 +315,8 @@ def kernels_init(device: int = 0) -> None:
     """Per-device set-up (btf_init); kernels_init in src/cuda/kernels.cuh:17."""
     check(lib().btf_init(device), "btf_init")
     _initialised.add(device)
-    _bind_calls()
+    if "torch" in sys.modules:  # (else with the first call that takes torch tensors)
+        _bind_calls()
 
 
 def ensure_init(device: int) -> None:
@@ -645,24 +647,31 @@ _ELEM: dict = {}  # torch dtype -> element type id
 
 
 # The ordinary calls of rope, tree_attention and sample (tensors of the expected types on the current device and its
-# current stream) go through bind/calls.cpp: None from it, and all else, is for the Python below.
+# current stream) go through bind/calls.cpp: None from it, and all else, is for the Python below. Without it, or with one
+# that does not load here or was built for another torch, that does every call.
 _calls = None
+_bind_tried = False
 
 
 def _bind_calls() -> None:
-    global _calls
+    global _calls, _bind_tried
+    _bind_tried = True
     path = os.path.join(HERE, "btf_b200_calls.so")
     if _calls is not None or not os.path.exists(path):
         return
-    import importlib.util
+    try:
+        import importlib.util
 
-    _torch()
-    spec = importlib.util.spec_from_file_location("btf_b200_calls", path)
-    calls = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(calls)
-    calls.bind(*(ctypes.cast(getattr(lib(), n), ctypes.c_void_p).value
-                 for n in ("btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample")))
-    _calls = calls
+        torch = _torch()
+        spec = importlib.util.spec_from_file_location("btf_b200_calls", path)
+        calls = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(calls)
+        if calls.torch_version == torch.__version__.split("+")[0]:
+            calls.bind(*(ctypes.cast(getattr(lib(), n), ctypes.c_void_p).value
+                         for n in ("btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample")))
+            _calls = calls
+    except Exception:  # whatever keeps it from loading
+        pass
 
 
 def _elem(t, what: str) -> int:
@@ -705,6 +714,8 @@ def _launch(dev, stream, fn, args):
     torch = _torch()
     if dev.index not in _initialised:
         ensure_init(dev.index)
+    if not _bind_tried:
+        _bind_calls()
     if stream is None:
         if torch.cuda.current_device() == dev.index:
             return fn(torch._C._cuda_getCurrentRawStream(dev.index), args)

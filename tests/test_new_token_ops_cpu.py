@@ -5,6 +5,7 @@ import ctypes
 import math
 import os
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -185,3 +186,48 @@ def test_binding_leaves_what_is_not_ordinary(btf):
         assert btf._calls.tree_attention(a, q, q, v, v, None, None, None, None) is None
         assert btf._calls.sample(a, v, None, None, None, None, None, None) is None
     assert btf._calls.sample(x) is None  # (too few arguments)
+
+
+def _rebound(btf, monkeypatch, here):
+    monkeypatch.setattr(btf, "HERE", str(here))
+    monkeypatch.setattr(btf, "_calls", None)
+    monkeypatch.setattr(btf, "_bind_tried", False)
+    btf._bind_calls()
+    return btf._calls
+
+
+def test_a_binding_that_does_not_load_leaves_the_mirror(btf, tmp_path, monkeypatch):
+    """A library of another torch, or no library at all, is no reason for set-up or a call to fail."""
+    btf.lib()
+    assert _rebound(btf, monkeypatch, tmp_path) is None  # none there
+    (tmp_path / "btf_b200_calls.so").write_bytes(b"not a shared object")
+    assert _rebound(btf, monkeypatch, tmp_path) is None
+    src = tmp_path / "m.c"  # loads, and is not the module; then one that wants a symbol that is not there
+    for code in ("int x;", "extern int no_such_symbol(void); int (*f)(void) = no_such_symbol;"):
+        src.write_text(code)
+        so = tmp_path / "other" / "btf_b200_calls.so"
+        so.parent.mkdir(exist_ok=True)
+        subprocess.run(["gcc", "-shared", "-fPIC", str(src), "-o", str(so)], check=True)
+        assert _rebound(btf, monkeypatch, so.parent) is None
+    torch = pytest.importorskip("torch")
+    with pytest.raises(RuntimeError, match="CUDA"):  # the mirror does the call
+        btf.sample(torch.zeros(2, 10), torch.zeros(2))
+
+
+def test_a_binding_of_another_torch_is_not_used(btf, monkeypatch):
+    torch = pytest.importorskip("torch")
+    if not os.path.exists(os.path.join(btf.HERE, "btf_b200_calls.so")):
+        pytest.skip("built without torch")
+    assert _rebound(btf, monkeypatch, btf.HERE) is not None
+    monkeypatch.setattr(torch, "__version__", "1.0.0+cu1")
+    assert _rebound(btf, monkeypatch, btf.HERE) is None
+
+
+@pytest.mark.parametrize("before", ["", "sys.modules['torch'] = None"], ids=["installed", "not to be had"])
+def test_set_up_needs_no_torch(before):
+    """kernels_init neither imports torch nor needs it (the device is not looked for here)."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = ["import sys", "sys.path.insert(0, 'bonsai-ternary-fast_b200')", before, "import btf_b200 as b",
+            "b.check = lambda *a: None", "b.kernels_init(0)", "assert not sys.modules.get('torch') and b._calls is None"]
+    r = subprocess.run([sys.executable, "-c", "\n".join(code)], cwd=root, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
