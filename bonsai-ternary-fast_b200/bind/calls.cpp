@@ -9,10 +9,12 @@
 
 #include <cmath>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/util/SmallVector.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
@@ -39,6 +41,15 @@ const at::Tensor& on(PyObject* o, int dev) {
   const at::Tensor& t = tensor(o);
   if (!t.is_cuda() || t.get_device() != dev) throw Other{};
   return t;
+}
+// A tensor of a call that records no graph; the mirror refuses one that wants a gradient.
+const at::Tensor& plain(const at::Tensor& t) {
+  if (t.requires_grad() && at::GradMode::is_enabled()) throw Other{};
+  return t;
+}
+// Autograd learns that a kernel has written it.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 int elem(const at::Tensor& t) {
   switch (t.scalar_type()) {
@@ -113,12 +124,14 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (n < 1 || n > 3) throw Other{};
     const int dev = device();
     btf_rope_seg segs[3];
+    c10::SmallVector<at::Tensor, 3> to;
     int64_t T = 0, D = 0;
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* s = PyList_GET_ITEM(args[0], i);
       const Attr ax(s, s_x), ay(s, s_y), aw(s, s_normw), at(s, s_rotate), ar(s, s_rows);
-      const at::Tensor& x = on(ax.o, dev);
-      const at::Tensor& y = ay.o == Py_None ? x : on(ay.o, dev);
+      const at::Tensor& x = plain(on(ax.o, dev));
+      const at::Tensor& y = ay.o == Py_None ? x : plain(on(ay.o, dev));
+      if (aw.o != Py_None) plain(on(aw.o, dev));
       if (x.dim() != 3 || y.dim() != 3) throw Other{};
       if (i == 0) T = x.size(0), D = x.size(2);
       if (x.size(0) != T || x.size(2) != D || y.size(2) != D || y.size(1) != x.size(1) || T > INT32_MAX || D > INT32_MAX ||
@@ -128,6 +141,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       segs[i] = {x.data_ptr(), y.data_ptr(), elem(x), elem(y), (int)x.size(1), flag(at.o),
                  stride(x, 0), stride(x, 1), stride(y, 0), stride(y, 1), vec<float>(aw.o, dev, at::kFloat, D),
                  vec<int32_t>(ar.o, dev, at::kInt, T), y.size(0)};
+      to.push_back(y);
     }
     const Attr turns(args[1], s_turns), n_rot(args[1], s_n_rot), mscale(args[1], s_mscale), inter(args[1], s_interleaved);
     if (args[2] == Py_None || turns.o == Py_None || !PyLong_Check(n_rot.o)) throw Other{};
@@ -142,6 +156,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (lib.rope(segs, (int)n, (int)T, (int)D, (int)rot, static_cast<const double*>(f.data_ptr()),
                  (float)number(mscale.o), flag(inter.o), flag(args[3]), (float)number(args[4]), pos, stream_of(dev)))
       throw Other{};
+    for (const at::Tensor& y : to) written(y);
     Py_RETURN_TRUE;
   });
 }
@@ -151,7 +166,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return attempt([&]() -> PyObject* {
     if (nargs != 9) throw Other{};
     const int dev = device();
-    const at::Tensor &q = on(args[0], dev), &k = on(args[1], dev), &v = on(args[2], dev);
+    const at::Tensor &q = plain(on(args[0], dev)), &k = plain(on(args[1], dev)), &v = plain(on(args[2], dev));
     if (q.dim() != 4 || k.dim() != 4 || v.sizes() != k.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3) ||
         k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
       throw Other{};
@@ -165,7 +180,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.counts = vec<int32_t>(args[5], dev, at::kInt, B);
     at::Tensor out, work;
     if (args[7] != Py_None) {
-      out = on(args[7], dev);
+      out = plain(on(args[7], dev));
       if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type()) throw Other{};
     } else {
       out = a.counts ? at::zeros(q.sizes(), q.options()) : at::empty(q.sizes(), q.options());
@@ -190,6 +205,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.scale = args[6] == Py_None ? (float)(1.0 / std::sqrt((double)D)) : (float)number(args[6]);
     a.work = work.data_ptr(), a.work_bytes = (int64_t)work.nbytes();
     if (lib.tree(&a, stream_of(dev))) throw Other{};
+    written(out);
     if (args[7] != Py_None) {
       Py_INCREF(args[7]);
       return args[7];
@@ -215,19 +231,21 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     at::Tensor tokens, logprobs;
     if (args[6] != Py_None) {
       vec(args[6], dev, at::kInt, B);
-      tokens = tensor(args[6]);
+      tokens = plain(tensor(args[6]));
     } else {
       tokens = at::empty({B}, x.options().dtype(at::kInt));
     }
     if (args[7] != Py_None) {
       vec(args[7], dev, at::kFloat, B);
-      logprobs = tensor(args[7]);
+      logprobs = plain(tensor(args[7]));
     } else {
       logprobs = at::empty({B}, x.options().dtype(at::kFloat));
     }
     if (lib.sample(x.data_ptr(), elem(x), B > 1 ? x.stride(0) : V, (int)B, (int)V, u, temp, top_k, top_p, min_p,
                    static_cast<int32_t*>(tokens.data_ptr()), static_cast<float*>(logprobs.data_ptr()), stream_of(dev)))
       throw Other{};
+    written(tokens);
+    written(logprobs);
     PyObject* t = args[6];
     PyObject* l = args[7];
     if (t != Py_None) Py_INCREF(t);

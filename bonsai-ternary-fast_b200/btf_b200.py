@@ -696,6 +696,19 @@ def _on(what: str, dev, name: str, t) -> None:
         raise RuntimeError(f"{what}: {name} is on {t.device}, not on {dev}")
 
 
+def _no_graph(what: str, *tensors) -> None:
+    """These calls record no graph, as torch's own calls with out= do not: inputs that want a gradient are refused while
+    one would be recorded."""
+    if _torch().is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what}: the call records no gradient, but a tensor requires one: detach it, or call under "
+                           "torch.no_grad()")
+
+
+def _written(*tensors) -> None:
+    """Tells autograd that these were written, so that a backward pass that saved one of them notices."""
+    _torch().autograd.graph.increment_version(tensors)
+
+
 def _vector(what: str, dev, name: str, t, dtype, shape) -> Optional[int]:
     """Address of a parameter tensor of the call (None: null): on dev, contiguous, of this type and shape."""
     if t is None:
@@ -768,13 +781,16 @@ class RopeSeg:
 
 def rope(segs: Sequence[RopeSeg], table: RopeTable, pos, inverse: bool = False, eps: float = 1e-6, stream=None) -> None:
     """Rotates up to 3 tensors of the same tokens by their positions pos [T] (int32) in one launch (btf_rope).
-    inverse: the transposed map, the gradient of the rotation."""
+    inverse: the transposed map, the gradient of the rotation. No graph is recorded: tensors that require a gradient are
+    refused outside torch.no_grad()."""
     if stream is None and _calls is not None and _calls.rope(segs, table, pos, inverse, eps):
         return
     torch = _torch()
     n = len(segs)
     if not 1 <= n <= 3:
         raise RuntimeError(f"rope: 1..3 tensors expected, got {n}")
+    for s in segs:
+        _no_graph("rope", s.x, s.y, s.normw)
     x0 = segs[0].x
     T, D, dev = x0.shape[0], x0.shape[-1], _cuda_device("rope", x0)
     i32, f32, packed = torch.int32, torch.float32, b""
@@ -813,6 +829,7 @@ def rope(segs: Sequence[RopeSeg], table: RopeTable, pos, inverse: bool = False, 
         raise RuntimeError(f"rope: the table's turns must hold n_rot / 2 = {table.n_rot // 2} contiguous float64 values")
     _launch(dev, stream, _rope_call, (packed, n, T, D, table.n_rot, turns.data_ptr(), table.mscale, table.interleaved,
                                       inverse, eps, pos_ptr))
+    _written(*(s.x if s.y is None else s.y for s in segs))
 
 
 def _rope_call(st, args) -> None:
@@ -838,7 +855,8 @@ def tree_attention(q, k, v, lens, parents, counts=None, scale: Optional[float] =
                    stream=None):
     """Attention of a tree of drafted tokens over a cache (btf_tree_attention): q [B][n][H][D]; k and v
     [B][n_ctx][HK][D] hold lens[b] cached tokens and the nodes behind them; node i sees the cache, itself and its
-    ancestors by parents [B][n] (int32, -1: hangs on the cache). counts [B]: nodes of each sequence (None: n)."""
+    ancestors by parents [B][n] (int32, -1: hangs on the cache). counts [B]: nodes of each sequence (None: n). No graph is
+    recorded: tensors that require a gradient are refused outside torch.no_grad()."""
     if stream is None and _calls is not None:
         done = _calls.tree_attention(q, k, v, lens, parents, counts, scale, out, work)
         if done is not None:
@@ -848,6 +866,7 @@ def tree_attention(q, k, v, lens, parents, counts=None, scale: Optional[float] =
     if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[0] != qs[0] or ks[3] != qs[3]:
         raise RuntimeError(f"tree_attention: q [B][n][H][D] and k, v [B][n_ctx][HK][D] expected, got {tuple(qs)}, "
                            f"{tuple(ks)}, {tuple(v.shape)}")
+    _no_graph("tree_attention", q, k, v, out)
     B, n, H, D = qs
     dev, dtype, i32 = _cuda_device("tree_attention", q), q.dtype, torch.int32
     if k.device != dev or v.device != dev:
@@ -887,12 +906,14 @@ def _tree_call(st, args):
     status = _lib.btf_tree_attention(packed, st)
     if status:
         check(status, "btf_tree_attention")
+    _written(out)
     return out
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprobs=None, stream=None):
     """Draws a token of each row of logits [B][V] from the random numbers u [B] in [0, 1) (btf_sample); temperature,
-    top_p, min_p (float32) and top_k (int32) are [B] or None. Returns (tokens int32 [B], logprobs float32 [B])."""
+    top_p, min_p (float32) and top_k (int32) are [B] or None. Returns (tokens int32 [B], logprobs float32 [B]), values
+    without a graph whatever the logits require."""
     if stream is None and _calls is not None:
         done = _calls.sample(logits, u, temperature, top_k, top_p, min_p, tokens, logprobs)
         if done is not None:
@@ -900,6 +921,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     torch = _torch()
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise RuntimeError("sample: logits [B][V] with contiguous rows expected")
+    _no_graph("sample", tokens, logprobs)
     B, V = logits.shape
     dev, f32, i32, rows = _cuda_device("sample", logits), torch.float32, torch.int32, (B,)
     pu = _vector("sample", dev, "u", u, f32, rows)
@@ -922,6 +944,7 @@ def _sample_call(st, args):
                              _vector("sample", dev, "logprobs", logprobs, torch.float32, (B,)), st)
     if status:
         check(status, "btf_sample")
+    _written(tokens, logprobs)
     return tokens, logprobs
 
 

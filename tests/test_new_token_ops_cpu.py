@@ -231,3 +231,24 @@ def test_set_up_needs_no_torch(before):
             "b.check = lambda *a: None", "b.kernels_init(0)", "assert not sys.modules.get('torch') and b._calls is None"]
     r = subprocess.run([sys.executable, "-c", "\n".join(code)], cwd=root, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_tensors_that_want_a_gradient_are_refused(btf):
+    """The calls record no graph, so a gradient would be missing in silence: refused as torch's own out= calls are."""
+    torch = pytest.importorskip("torch")
+    t, p = btf.RopeTable(64, device="cpu"), torch.zeros(2, dtype=torch.int32)
+    x, w = torch.zeros(2, 1, 64), torch.ones(64)
+    g = lambda a: a.clone().requires_grad_()  # noqa: E731
+    q, k = torch.zeros(1, 2, 4, 64).half(), torch.zeros(1, 9, 2, 64).half()
+    b = torch.zeros(2, 10)
+    calls = [lambda: btf.rope([btf.RopeSeg(g(x))], t, p), lambda: btf.rope([btf.RopeSeg(x, g(x))], t, p),
+             lambda: btf.rope([btf.RopeSeg(x), btf.RopeSeg(x, x, normw=g(w))], t, p),
+             lambda: btf.tree_attention(g(q), k, k, p[:1], p[None]), lambda: btf.tree_attention(q, g(k), k, p[:1], p[None]),
+             lambda: btf.tree_attention(q, k, g(k), p[:1], p[None]),
+             lambda: btf.tree_attention(q, k, k, p[:1], p[None], out=g(q)),
+             lambda: btf.sample(b, b[:, 0], logprobs=g(b[:, 0]))]
+    for fn in calls:
+        with pytest.raises(RuntimeError, match="gradient"):
+            fn()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            fn()

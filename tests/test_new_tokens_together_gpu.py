@@ -164,3 +164,47 @@ def test_tables_and_workspaces_that_are_too_small(cuda, btf):
     for bad in (work[:1].expand(len(work)), torch.empty(2 * len(work), dtype=torch.uint8, device=cuda)[::2]):
         with pytest.raises(RuntimeError):
             btf.tree_attention(q, k, k, pos[:1], pos[:1, None], work=bad)
+
+
+@pytest.mark.parametrize("short", [True, False])
+def test_autograd_learns_what_is_written(cuda, btf, monkeypatch, short):
+    """No graph is recorded: what wants a gradient is refused while one would be, and what a call writes counts as
+    changed in place, so that a backward pass that saved it says so."""
+    if not short:
+        monkeypatch.setattr(btf, "_calls", None)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    table, pos = btf.RopeTable(64), i32(3, 4)
+    x = torch.randn(2, 3, 64, device=cuda, requires_grad=True)
+    q, k = (torch.randn(*s, device=cuda).half() for s in ((1, 2, 4, 64), (1, 9, 2, 64)))
+    logits, u = torch.randn(2, 50, device=cuda, requires_grad=True), torch.rand(2, device=cuda)
+
+    def each(a, ka, lp):
+        yield lambda: btf.rope([btf.RopeSeg(a)], table, pos)
+        yield lambda: btf.tree_attention(q, ka, k, i32(7), i32(-1, 0)[None])
+        yield lambda: btf.sample(logits.detach(), u, logprobs=lp)
+
+    wants = (x * 1, k.clone().requires_grad_(), torch.zeros(2, device=cuda, requires_grad=True))
+    for fn in each(*wants):
+        with pytest.raises(RuntimeError, match="gradient"):
+            fn()
+    with torch.no_grad():
+        for fn in each(*wants):
+            fn()
+    with torch.inference_mode():
+        for fn in each(x.clone(), k.clone(), torch.zeros(2, device=cuda)):
+            fn()
+    tok, lp = btf.sample(logits, u)  # drawing has no gradient: values
+    assert not lp.requires_grad
+    h = x * 2
+    y = (h * h).sum()  # saves h
+    with torch.no_grad():
+        btf.rope([btf.RopeSeg(h)], table, pos)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    out, cache = torch.zeros_like(q), torch.zeros(5, 3, 64, device=cuda)
+    tok, lp = torch.zeros(2, dtype=torch.int32, device=cuda), torch.zeros(2, device=cuda)
+    versions = [t._version for t in (out, cache, tok, lp, k)]
+    btf.tree_attention(q, k, k, i32(7), i32(-1, 0)[None], out=out)
+    btf.rope([btf.RopeSeg(x.detach(), cache, rows=i32(1, 2))], table, pos)
+    btf.sample(logits, u, tokens=tok, logprobs=lp)
+    assert [t._version for t in (out, cache, tok, lp, k)] == [v + 1 for v in versions[:4]] + versions[4:]
