@@ -280,6 +280,8 @@ int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const 
     if (s.heads && (reinterpret_cast<uintptr_t>(s.x) % elem_bytes(s.x_type) ||
                     reinterpret_cast<uintptr_t>(s.y) % elem_bytes(s.y_type)))
       return fail(BTF_ERR_ARG, "btf_rope: a tensor is not aligned to its type");
+    if (s.heads && ((s.heads > 1 && s.y_head == 0) || (T > 1 && s.y_token == 0 && !(s.rows && s.n_rows == 1))))
+      return fail(BTF_ERR_ARG, "btf_rope: the heads and rows of y need strides");
     if (s.normw && inverse) return fail(BTF_ERR_ARG, "btf_rope: the inverse has no norm");
     if (s.rows && s.n_rows < 1) return fail(BTF_ERR_ARG, "btf_rope: rows without n_rows");
     if (s.heads && s.x == s.y &&

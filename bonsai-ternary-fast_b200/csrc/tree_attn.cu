@@ -1051,6 +1051,8 @@ int btf_tree_attention(const btf_tree_attn* a, void* stream) {
   for (int64_t s : {a->q_batch, a->q_node, a->q_head, a->kv_batch, a->kv_row, a->kv_head, a->o_batch, a->o_node,
                     a->o_head})
     if (s < 0 || s % 8) return fail(BTF_ERR_ARG, "btf_tree_attention: strides must be multiples of 8 elements, >= 0");
+  if ((a->B > 1 && a->o_batch == 0) || (a->n > 1 && a->o_node == 0) || (a->H > 1 && a->o_head == 0))
+    return fail(BTF_ERR_ARG, "btf_tree_attention: the rows of o need strides");
   if (a->n_ctx > 1 && a->kv_row == 0) return fail(BTF_ERR_ARG, "btf_tree_attention: the rows of k and v need a stride");
   if (!std::isfinite(a->scale)) return fail(BTF_ERR_ARG, "btf_tree_attention: scale must be finite");
   if (!a->work || reinterpret_cast<uintptr_t>(a->work) % 256 || a->work_bytes < 256)

@@ -570,7 +570,8 @@ typedef struct btf_rope_cfg {
 int btf_rope_table(const btf_rope_cfg* cfg, double* turns_host, float* mscale);
 
 /* One tensor [T][heads][D] of a btf_rope call; strides in elements, the D dims of a head contiguous.
- * x and y may be the same tensor (same pointer, type and strides, rows NULL), else they must not overlap. */
+ * x and y may be the same tensor (same pointer, type and strides, rows NULL), else they must not overlap.
+ * Heads and rows of y lie apart (no stride of 0 where there are several). */
 typedef struct btf_rope_seg {
   const void* x;
   void* y;
@@ -604,7 +605,7 @@ typedef struct btf_tree_attn {
   const void* k;               /* [B][n_ctx][HK][D], as the decoder's caches */
   const void* v;
   int64_t kv_batch, kv_row, kv_head;
-  void* o;                     /* [B][n][H][D] */
+  void* o;                     /* [B][n][H][D]; no stride of 0 where there are several */
   int64_t o_batch, o_node, o_head;
   int type;                    /* BTF_F16 or BTF_BF16: q, k, v and o */
   int B, n, H, HK, D;          /* 1 <= n <= BTF_TREE_MAX_NODES; H % HK == 0; D % 8 == 0, 8..256 */

@@ -252,3 +252,16 @@ def test_tensors_that_want_a_gradient_are_refused(btf):
             fn()
         with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
             fn()
+
+
+@pytest.mark.parametrize("seg", [dict(heads=2, y_head=0), dict(y_token=0), dict(y_token=0, rows=P, n_rows=2)])
+def test_rope_refuses_rows_that_share_their_memory(btf, seg):
+    """An expanded output, whose rows would overwrite one another."""
+    assert _rope(btf, seg=seg) == 1
+    assert b"strides" in btf.lib().btf_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(B=2, o_batch=0), dict(o_node=0), dict(o_head=0)])
+def test_tree_attention_refuses_rows_that_share_their_memory(btf, kw):
+    assert _tree(btf, **kw) == 1
+    assert b"strides" in btf.lib().btf_last_error()
