@@ -984,10 +984,10 @@ cudaError_t launch_tree_d(const CUtensorMap& mk, const CUtensorMap& mv, const Tr
                         : p.D <= 192 ? launch_tree<T, 192>(mk, mv, p, st)
                                      : launch_tree<T, 256>(mk, mv, p, st);
   if (e != cudaSuccess || p.ranges == 1) return e;
-  const int rows = p.B * p.n * p.H;
+  const int64_t rows = (int64_t)p.B * p.n * p.H;  // at most INT32_MAX
   // a CTA per row while all of them are resident at once
-  if (rows <= 8 * sms) return launch_pdl(tree_join_kernel<T, 8>, dim3(rows), dim3(kJoinThreads), 0, st, p);
-  return launch_pdl(tree_join_kernel<T, 1>, dim3((rows + 7) / 8), dim3(kJoinThreads), 0, st, p);
+  if (rows <= 8 * sms) return launch_pdl(tree_join_kernel<T, 8>, dim3((unsigned)rows), dim3(kJoinThreads), 0, st, p);
+  return launch_pdl(tree_join_kernel<T, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(kJoinThreads), 0, st, p);
 }
 
 // The join runs between two launches that take all of shared memory: it asks for
