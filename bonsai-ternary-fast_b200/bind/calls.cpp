@@ -14,7 +14,6 @@
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
-#include <c10/util/SmallVector.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
@@ -124,7 +123,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (n < 1 || n > 3) throw Other{};
     const int dev = device();
     btf_rope_seg segs[3];
-    c10::SmallVector<at::Tensor, 3> to;
+    const at::Tensor* to[3];  // (the segments keep them)
     int64_t T = 0, D = 0;
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* s = PyList_GET_ITEM(args[0], i);
@@ -141,7 +140,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       segs[i] = {x.data_ptr(), y.data_ptr(), elem(x), elem(y), (int)x.size(1), flag(at.o),
                  stride(x, 0), stride(x, 1), stride(y, 0), stride(y, 1), vec<float>(aw.o, dev, at::kFloat, D),
                  vec<int32_t>(ar.o, dev, at::kInt, T), y.size(0)};
-      to.push_back(y);
+      to[i] = &y;
     }
     const Attr turns(args[1], s_turns), n_rot(args[1], s_n_rot), mscale(args[1], s_mscale), inter(args[1], s_interleaved);
     if (args[2] == Py_None || turns.o == Py_None || !PyLong_Check(n_rot.o)) throw Other{};
@@ -156,7 +155,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (lib.rope(segs, (int)n, (int)T, (int)D, (int)rot, static_cast<const double*>(f.data_ptr()),
                  (float)number(mscale.o), flag(inter.o), flag(args[3]), (float)number(args[4]), pos, stream_of(dev)))
       throw Other{};
-    for (const at::Tensor& y : to) written(y);
+    for (Py_ssize_t i = 0; i < n; ++i) written(*to[i]);
     Py_RETURN_TRUE;
   });
 }
