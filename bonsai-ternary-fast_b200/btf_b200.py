@@ -1154,7 +1154,7 @@ class Decoder:
                                             u.ctypes.data), "btf_decoder_run_sampled")
 
     def verify(self, tokens, parents, sampling: Optional[dict] = None, us=None, logits: bool = False):
-        """Checks a tree of drafted tokens in one pass over the weights (btf_decoder_verify): node j follows node
+        """Checks a tree of drafted tokens in one pass through the layers (btf_decoder_verify): node j follows node
         parents[j], or the decoded tokens (-1). Returns (the token after each node: greedy, or drawn with us[j] and
         sampling = dict(temperature=, top_k=, top_p=, min_p=); logits [n][n_vocab] or None). accept() takes a path."""
         import numpy as np

@@ -4,9 +4,11 @@
 //
 //   (a, b) -> m (a cos t - b sin t, a sin t + b cos t),  t = pos * f_i
 //
-// t in turns is pos * (f_i / 2 pi) in 64 bits; its fraction is exact to 2^-50 of
-// a turn at any int32 position, so cos and sin of it in fp32 are good to 2^-23
-// whatever the position (pos * f_i in fp32 loses 2^-24 pos radians: 0.06 at 10^6).
+// t in turns is pos * (f_i / 2 pi) in 64 bits: off by |turns| 2^-52 or so (the
+// frequency's rounding and the product's). Its fraction is rounded to fp32 (2^-26 of a
+// turn), so cos and sin are good to 2^-22 while the former is the smaller, up to 2^26
+// turns (positions of 4 10^8 at f = 1); at 2^31 they are off by 2^-24 of a turn, 4e-7,
+// more. (pos * f_i in fp32 loses 2^-24 pos radians: 0.06 at 10^6.)
 //
 // What bounds it: bytes, each read and written once, for prompts and gradients (see
 // rope_heads; 7001 tokens of 40 fp32 heads of 80 in 32.2 us, 5.6 TB/s); the launch for

@@ -36,12 +36,13 @@
 // launches, lengths, q, K, V and the parts' way through memory one after another);
 // 16 sequences of up to 8203 rows, 24 nodes, 32 and 8 heads of 128: 29.2 us, 3.3 TB/s;
 // 1 node over 131072 rows 5.9 TB/s of K and V, 16 nodes 5.4; 64 nodes (three M tiles):
-// 195 us, 1055 TFLOP/s. There a 64-row tile takes 1560 cycles, in which each SM gets its
+// 195 us, 1055 TFLOP/s (233 us, 883 TFLOP/s, call after call under the power cap). There a 64-row tile takes 1560 cycles, in which each SM gets its
 // 64 KB of K and V (8.3 TB/s out of L2 for all) and moves 160 KB in shared memory; the
 // MMAs alone take 1024. Two softmax threads per row gained nothing (202 us).
 //
 // p is rounded to the type of V (the MMA takes one type): eps / 2 per term, as much
-// as the output's own rounding at most. fp16 p carry a factor 2^7, so that those
+// as the output's own rounding at most (the error against 64 bits of the cases above, of
+// which the output's rounding is nearly all, grows by 1 to 10 %). fp16 p carry a factor 2^7, so that those
 // down to 2^-32 of the largest still count. Scores, maxima, sums and O are fp32.
 #include <algorithm>
 #include <cmath>
@@ -116,6 +117,11 @@ struct Seq {
 // CTA has one segment (a second one costs its q and its way out again, about 5 tiles
 // of time: 1 x 1 node over 513 rows took 15.5 us with ranges across pairs, 12.0
 // without; the search for `per` is 0.4 us of it, and left out for equal lengths). Otherwise the line of all tiles is cut into equal ranges.
+// Both sides, own ranges and the line, in us for 8 nodes of 32 q-heads over 8 kv-heads: D = 128, 512 rows 11.8 and 11.8
+// (40 pairs), 12.6 and 15.7 (80), 15.9 and 19.8 (240); 8192 rows 59 and 63 (80), 127 and 112 (160), 156 and 167 (240).
+// D = 256, 512 rows 21.9 and 24.2 (80), 22.5 and 26.4 (128); 8192 rows 60 and 66 (40), 133 and 116 (80), 164 and 175 (128).
+// So the line is up to 13 % ahead just above half as many pairs as ranges over long caches, where each pair has one
+// range and nearly half of the CTAs none, and behind elsewhere.
 struct Segments {
   const TreeParams& p;
   int b, kvh, tile, nt, index;  // the present one; index: in the CTA

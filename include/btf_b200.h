@@ -459,10 +459,12 @@ int btf_decoder_step_sampled(void* handle, int32_t token, const btf_sampling* sa
 /* btf_decoder_run with drawn tokens: step i draws with u_host[i]. The numbers are copied before it returns. */
 int btf_decoder_run_sampled(void* handle, int steps, const btf_sampling* sampling, const float* u_host);
 
-/* Checks a tree of n drafted tokens in one pass over the weights: node j holds tokens_host[j] and follows node
+/* Checks a tree of n drafted tokens in one pass through the layers: node j holds tokens_host[j] and follows node
  * parents_host[j] < j, or the decoded tokens when that is -1. Node j sits at position pos + its depth; every ternary
- * matmul runs once over the n rows, the attention is btf_rope + btf_tree_attention over the layer's cache, and every
- * node has a recurrent state of its own, which starts from its parent's. next_host[j] is the token after node j:
+ * matmul is one call over the n rows (which reads most matrices once for up to 4 rows, twice for 5 to 8), the attention
+ * is btf_rope + btf_tree_attention over the layer's cache, and every node has a recurrent state of its own, which
+ * starts from its parent's. q and the attention's outputs are rounded to fp16, whatever btf_decoder_opts.round_q_f16
+ * says: with round_q_f16 = 0 a step keeps both in fp32, and a draft is checked that much less precisely. next_host[j] is the token after node j:
  * greedy (sampling NULL), or drawn with u_host[j]; logits (host, [n][n_vocab]) when non-NULL. The decoder's position
  * and state stay: btf_decoder_accept takes over a path, any other call drops the draft. Synchronous, eager. The first
  * call allocates the nodes' states (btf_decoder_info.device_bytes then counts them; btf_plan_memory does not).
@@ -586,8 +588,8 @@ typedef struct btf_rope_seg {
 } btf_rope_seg;
 /* Rotates up to 3 tensors by their tokens' positions pos[T] in one launch: pairs (i, i + n_rot / 2) of the
  * first n_rot dims, or (2 i, 2 i + 1) when interleaved, by pos * f_i; the other dims are copied. Angles are
- * reduced in 64 bits, so any int32 position keeps fp32 accuracy. inverse: the transposed map, which is the
- * gradient (normw must be NULL). 1 <= D <= BTF_ROPE_MAX_D, n_rot even, 0..D (0: turns may be NULL), T <= 2^30.
+ * reduced in 64 bits: fp32 accuracy up to 2^26 turns (positions of 4 10^8 at f = 1), another 4e-7 rad at 2^31.
+ * inverse: the transposed map, which is the gradient (normw must be NULL). 1 <= D <= BTF_ROPE_MAX_D, n_rot even, 0..D (0: turns may be NULL), T <= 2^30.
  * Replaces the RoPE of src/emu_decoder.cpp:307-338 for many tokens and other layouts. */
 int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const double* turns, float mscale,
              int interleaved, int inverse, float eps, const int32_t* pos, void* stream);
