@@ -344,3 +344,21 @@ def test_a_draft_that_found_no_memory_leaves_none_behind(cuda, btf):
         d.verify([1], [-1])
         assert d.info()["device_bytes"] == want
     assert btf.device_error() == 0
+
+
+@pytest.mark.parametrize("n_layer", [4, 8])
+def test_a_draft_rounds_q_whatever_a_step_does(cuda, btf, n_layer):
+    """The tree attention's q is fp16: a decoder opened with round_q_f16 = 0 checks the same tree to the same bits, and
+    to the bounds above against its own steps, whose q is fp32 (2^-12 of it, beside the 2 * 2^-11.5 there)."""
+    dims = dict(SMALL, n_layer=n_layer)
+    with _open(btf, dims) as a, _open(btf, dims, round_q_f16=False) as b, _open(btf, dims, round_q_f16=False) as steps:
+        got = []
+        for d in (a, b):
+            for t in PROMPT[:1]:  # one token: attention to itself alone, the same states and rows in both
+                d.step(t)
+            got.append(d.verify(*TREE, logits=True)[1])
+        assert np.array_equal(*got)
+        steps.step(PROMPT[0])
+        for j, t in ((0, 5), (1, 17), (3, 19)):
+            want = steps.step(t, logits=True)[1]
+            assert rel_rms(got[1][j], want) <= _tol(dims), (j, rel_rms(got[1][j], want))

@@ -309,3 +309,17 @@ def test_lengths_that_change_from_call_to_call(cuda, btf, B, n, ctx):
     for i in range(calls):
         assert torch.equal(got[i], want[i]), i
     assert btf.device_error() == 0
+
+
+@pytest.mark.parametrize("lengths", ["equal", "ragged", "short"])
+@pytest.mark.parametrize("B,HK,D", [(10, 8, 256), (25, 3, 256), (18, 8, 200), (32, 4, 256), (31, 5, 256), (20, 8, 128), (32, 5, 64),
+                                    (32, 8, 128), (33, 1, 128), (33, 8, 72)])
+def test_pairs_beside_the_ranges(cuda, btf, B, HK, D, lengths):
+    """About half as many, nearly as many and a few more (sequence, kv-head) pairs as the card takes ranges (148 above 128
+    dims, 296 below), and more sequences than a warp has lanes."""
+    n, rng = 3, np.random.default_rng(B * HK)
+    lens = {"equal": [700] * B, "short": [int(x) for x in rng.integers(0, 70, B)],
+            "ragged": [int(x) for x in np.exp(rng.uniform(0, np.log(900), B))]}[lengths]
+    counts = [n] * B if lengths == "equal" else [int(x) for x in rng.integers(0, n + 1, B)]
+    _case(btf, cuda, B, n, 2 * HK, HK, D, torch.float16, lens, [random_tree(rng, n) for _ in range(B)], counts,
+          ctx=max(lens) + n + 1, seed=B)
