@@ -15,7 +15,6 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
-#include <torch/version.h>
 
 #include "btf_b200.h"
 
@@ -287,7 +286,7 @@ PyMODINIT_FUNC PyInit_btf_b200_calls() {
   s_mscale = PyUnicode_InternFromString("mscale");
   s_interleaved = PyUnicode_InternFromString("interleaved");
   PyObject* m = PyModule_Create(&module);
-  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION)) {  // the mirror binds it to no other
+  if (m && PyModule_AddStringConstant(m, "torch_version", BTF_TORCH_VERSION)) {  // the mirror binds it to no other
     Py_DECREF(m);
     return nullptr;
   }

@@ -666,7 +666,7 @@ def _bind_calls() -> None:
         spec = importlib.util.spec_from_file_location("btf_b200_calls", path)
         calls = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(calls)
-        if calls.torch_version == torch.__version__.split("+")[0]:
+        if calls.torch_version == torch.__version__:
             calls.bind(*(ctypes.cast(getattr(lib(), n), ctypes.c_void_p).value
                          for n in ("btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample")))
             _calls = calls
