@@ -634,7 +634,8 @@ int btf_tree_attention(const btf_tree_attn* args, void* stream);
  * tokens[b] gets it, logprobs[b] the log of its share of the kept mass. A NaN logit counts as -inf; a row with
  * nothing above -inf gives token 0 and a NaN logprob. Each parameter is [B] on the device or NULL (1, off, off,
  * off); top_k <= 0, top_p >= 1 and min_p <= 0 are off for their row. u in [0, 1). Masses are 2^-44 fixed point
- * (coarser for V > 2^18), so results do not depend on an order of summation; V <= BTF_SAMPLE_MAX_V.
+ * (coarser for V > 2^18), so results do not depend on an order of summation; a token of less than 2^-45 of the largest
+ * mass has none and is not drawn, by u = 0 neither. V <= BTF_SAMPLE_MAX_V.
  * Beside the greedy token of src/emu_decoder.cpp:214-217. */
 #define BTF_SAMPLE_MAX_V 524288
 int btf_sample(const void* logits, int type, int64_t ld, int B, int V, const float* u, const float* temperature,

@@ -262,3 +262,15 @@ def test_ctas_without_logits(cuda, btf, B, V, f):
     for tok, lp in outs[1:]:
         assert torch.equal(tok, outs[0][0]) and torch.equal(lp, outs[0][1])
     assert btf.device_error() == 0
+
+
+@pytest.mark.parametrize("V", [4, 4099, 248320])
+def test_tokens_without_mass_are_not_drawn(cuda, btf, V):
+    """Masses are 2^-44 fixed point: e^-30 of the largest is 1.6 of a unit, e^-31.5 is 0.4 and rounds to none, so u = 0
+    draws the first token that has one."""
+    x = torch.full((3, V), -100.0)
+    x[:, 1], x[:, 2], x[:, 3] = -31.5, torch.tensor([-30.0, -31.5, -30.0]), 0.0
+    x[2, 0] = -30.0
+    tok, lp = _run(btf, cuda, x.to(cuda), np.zeros(3, np.float32))
+    assert tok.tolist() == [2, 3, 0]
+    np.testing.assert_allclose(lp, [-30.0, 0.0, -30.0], atol=1e-9, rtol=2.0 ** -23)
