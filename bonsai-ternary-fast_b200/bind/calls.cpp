@@ -70,16 +70,27 @@ template <typename T>
 const T* vec(PyObject* o, int dev, at::ScalarType type, int64_t n, int64_t m = -1) {
   return static_cast<const T*>(vec(o, dev, type, n, m));
 }
-struct Attr {  // a new reference
-  PyObject* o;
-  Attr(PyObject* from, PyObject* name) : o(PyObject_GetAttr(from, name)) {
+// References of a call, kept to its end (an attribute may be made anew each time it is read).
+struct Kept {
+  PyObject* of[3 * 6 + 4];
+  int n = 0;
+  Kept() = default;
+  Kept(const Kept&) = delete;
+  PyObject* keep(PyObject* o) {
+    Py_INCREF(o);
+    return of[n++] = o;
+  }
+  PyObject* attr(PyObject* from, PyObject* name) {
+    PyObject* o = PyObject_GetAttr(from, name);
     if (!o) {
       PyErr_Clear();
       throw Other{};
     }
+    return of[n++] = o;
   }
-  ~Attr() { Py_DECREF(o); }
-  Attr(const Attr&) = delete;
+  ~Kept() {
+    while (n) Py_DECREF(of[--n]);
+  }
 };
 int flag(PyObject* o) {
   const int v = PyObject_IsTrue(o);
@@ -122,37 +133,41 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (n < 1 || n > 3) throw Other{};
     const int dev = device();
     btf_rope_seg segs[3];
-    const at::Tensor* to[3];  // (the segments keep them)
+    const at::Tensor* to[3];
+    Kept kept;
     int64_t T = 0, D = 0;
     for (Py_ssize_t i = 0; i < n; ++i) {
-      PyObject* s = PyList_GET_ITEM(args[0], i);
-      const Attr ax(s, s_x), ay(s, s_y), aw(s, s_normw), at(s, s_rotate), ar(s, s_rows);
-      const at::Tensor& x = plain(on(ax.o, dev));
-      const at::Tensor& y = ay.o == Py_None ? x : plain(on(ay.o, dev));
-      if (aw.o != Py_None) plain(on(aw.o, dev));
+      if (i >= PyList_GET_SIZE(args[0])) throw Other{};
+      PyObject* s = kept.keep(PyList_GET_ITEM(args[0], i));
+      PyObject *ox = kept.attr(s, s_x), *oy = kept.attr(s, s_y), *ow = kept.attr(s, s_normw);
+      PyObject *orot = kept.attr(s, s_rotate), *orows = kept.attr(s, s_rows);
+      const at::Tensor& x = plain(on(ox, dev));
+      const at::Tensor& y = oy == Py_None ? x : plain(on(oy, dev));
+      if (ow != Py_None) plain(on(ow, dev));
       if (x.dim() != 3 || y.dim() != 3) throw Other{};
       if (i == 0) T = x.size(0), D = x.size(2);
       if (x.size(0) != T || x.size(2) != D || y.size(2) != D || y.size(1) != x.size(1) || T > INT32_MAX || D > INT32_MAX ||
           x.size(1) > INT32_MAX || (D > 1 && (x.stride(2) != 1 || y.stride(2) != 1)) ||
-          (ar.o == Py_None && y.size(0) != T))
+          (orows == Py_None && y.size(0) != T))
         throw Other{};
-      segs[i] = {x.data_ptr(), y.data_ptr(), elem(x), elem(y), (int)x.size(1), flag(at.o),
-                 stride(x, 0), stride(x, 1), stride(y, 0), stride(y, 1), vec<float>(aw.o, dev, at::kFloat, D),
-                 vec<int32_t>(ar.o, dev, at::kInt, T), y.size(0)};
+      segs[i] = {x.data_ptr(), y.data_ptr(), elem(x), elem(y), (int)x.size(1), flag(orot),
+                 stride(x, 0), stride(x, 1), stride(y, 0), stride(y, 1), vec<float>(ow, dev, at::kFloat, D),
+                 vec<int32_t>(orows, dev, at::kInt, T), y.size(0)};
       to[i] = &y;
     }
-    const Attr turns(args[1], s_turns), n_rot(args[1], s_n_rot), mscale(args[1], s_mscale), inter(args[1], s_interleaved);
-    if (args[2] == Py_None || turns.o == Py_None || !PyLong_Check(n_rot.o)) throw Other{};
-    const at::Tensor& f = on(turns.o, dev);
+    PyObject *turns = kept.attr(args[1], s_turns), *n_rot = kept.attr(args[1], s_n_rot);
+    PyObject *mscale = kept.attr(args[1], s_mscale), *inter = kept.attr(args[1], s_interleaved);
+    if (args[2] == Py_None || turns == Py_None || !PyLong_Check(n_rot)) throw Other{};
+    const at::Tensor& f = on(turns, dev);
     if (f.scalar_type() != at::kDouble || !f.is_contiguous()) throw Other{};
     const int32_t* pos = vec<int32_t>(args[2], dev, at::kInt, T);
-    const long rot = PyLong_AsLong(n_rot.o);
+    const long rot = PyLong_AsLong(n_rot);
     if (rot < 0 || rot > 2 * f.numel()) {
       PyErr_Clear();
       throw Other{};
     }
     if (lib.rope(segs, (int)n, (int)T, (int)D, (int)rot, static_cast<const double*>(f.data_ptr()),
-                 (float)number(mscale.o), flag(inter.o), flag(args[3]), (float)number(args[4]), pos, stream_of(dev)))
+                 (float)number(mscale), flag(inter), flag(args[3]), (float)number(args[4]), pos, stream_of(dev)))
       throw Other{};
     for (Py_ssize_t i = 0; i < n; ++i) written(*to[i]);
     Py_RETURN_TRUE;

@@ -208,3 +208,23 @@ def test_autograd_learns_what_is_written(cuda, btf, monkeypatch, short):
     btf.rope([btf.RopeSeg(x.detach(), cache, rows=i32(1, 2))], table, pos)
     btf.sample(logits, u, tokens=tok, logprobs=lp)
     assert [t._version for t in (out, cache, tok, lp, k)] == [v + 1 for v in versions[:4]] + versions[4:]
+
+
+def test_segments_that_make_their_tensors_when_asked(cuda, btf):
+    """Objects with a segment's attributes, each a view made anew when it is read: used to the call's end."""
+    base, out = torch.randn(4, 3, 128, device=cuda), torch.zeros(4, 3, 64, device=cuda)
+    table, pos = btf.RopeTable(64), torch.arange(4, dtype=torch.int32, device=cuda)
+
+    class Seg:
+        x = property(lambda self: base[..., 64:])
+        y = property(lambda self: out[:])
+        normw = rows = None
+        rotate = True
+
+    version = out._version
+    for _ in range(20):
+        btf.rope([Seg(), Seg()], table, pos)
+    assert out._version == version + 40
+    want = torch.empty_like(out)
+    btf.rope([btf.RopeSeg(base[..., 64:], want)], table, pos)
+    assert torch.equal(out, want)
