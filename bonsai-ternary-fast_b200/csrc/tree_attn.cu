@@ -121,7 +121,8 @@ struct Seq {
 // (40 pairs), 12.6 and 15.7 (80), 15.9 and 19.8 (240); 8192 rows 59 and 63 (80), 127 and 112 (160), 156 and 167 (240).
 // D = 256, 512 rows 21.9 and 24.2 (80), 22.5 and 26.4 (128); 8192 rows 60 and 66 (40), 133 and 116 (80), 164 and 175 (128).
 // So the line is up to 13 % ahead just above half as many pairs as ranges over long caches, where each pair has one
-// range and nearly half of the CTAs none, and behind elsewhere.
+// range and nearly half of the CTAs none, and behind elsewhere. 32 sequences are what a warp works out at once, a lane
+// each; what the 33rd of one kv-head costs: D = 128, 4096 rows 19.9 -> 20.6, D = 256 33.5 -> 39.1, 600 rows 15.2 -> 20.2.
 struct Segments {
   const TreeParams& p;
   int b, kvh, tile, nt, index;  // the present one; index: in the CTA
