@@ -26,6 +26,7 @@ struct Library {
   decltype(&btf_tree_attention_work) tree_work = nullptr;
   decltype(&btf_tree_attention) tree = nullptr;
   decltype(&btf_sample) sample = nullptr;
+  decltype(&btf_rope_axes) rope_axes = nullptr;
 } lib;
 
 // A refused fast call: caught below, becomes None.
@@ -72,7 +73,7 @@ const T* vec(PyObject* o, int dev, at::ScalarType type, int64_t n, int64_t m = -
 }
 // References of a call, kept to its end (an attribute may be made anew each time it is read).
 struct Kept {
-  PyObject* of[3 * 6 + 4];
+  PyObject* of[3 * 6 + 6];
   int n = 0;
   Kept() = default;
   Kept(const Kept&) = delete;
@@ -123,7 +124,7 @@ PyObject* attempt(Fn fn) {
   Py_RETURN_NONE;
 }
 
-PyObject *s_x, *s_y, *s_normw, *s_rotate, *s_rows, *s_turns, *s_n_rot, *s_mscale, *s_interleaved;
+PyObject *s_x, *s_y, *s_normw, *s_rotate, *s_rows, *s_turns, *s_n_rot, *s_mscale, *s_interleaved, *s_axis, *s_n_axes;
 
 // rope(segs, table, pos, inverse, eps) -> True, or None
 PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -160,15 +161,30 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (args[2] == Py_None || turns == Py_None || !PyLong_Check(n_rot)) throw Other{};
     const at::Tensor& f = on(turns, dev);
     if (f.scalar_type() != at::kDouble || !f.is_contiguous()) throw Other{};
-    const int32_t* pos = vec<int32_t>(args[2], dev, at::kInt, T);
     const long rot = PyLong_AsLong(n_rot);
     if (rot < 0 || rot > 2 * f.numel()) {
       PyErr_Clear();
       throw Other{};
     }
-    if (lib.rope(segs, (int)n, (int)T, (int)D, (int)rot, static_cast<const double*>(f.data_ptr()),
-                 (float)number(mscale), flag(inter), flag(args[3]), (float)number(args[4]), pos, stream_of(dev)))
-      throw Other{};
+    const double* freq = static_cast<const double*>(f.data_ptr());
+    PyObject* oaxis = kept.attr(args[1], s_axis);
+    if (oaxis == Py_None) {
+      if (lib.rope(segs, (int)n, (int)T, (int)D, (int)rot, freq, (float)number(mscale), flag(inter), flag(args[3]),
+                   (float)number(args[4]), vec<int32_t>(args[2], dev, at::kInt, T), stream_of(dev)))
+        throw Other{};
+    } else {
+      const at::Tensor& axis = on(oaxis, dev);
+      const long axes = PyLong_AsLong(kept.attr(args[1], s_n_axes));
+      if (axes < 1 || axes > BTF_ROPE_MAX_AXES || axis.scalar_type() != at::kByte || !axis.is_contiguous() ||
+          rot > 2 * axis.numel()) {
+        PyErr_Clear();
+        throw Other{};
+      }
+      if (lib.rope_axes(segs, (int)n, (int)T, (int)D, (int)rot, freq, static_cast<const uint8_t*>(axis.data_ptr()),
+                        (int)axes, (float)number(mscale), flag(inter), flag(args[3]), (float)number(args[4]),
+                        vec<int32_t>(args[2], dev, at::kInt, axes, T), T, stream_of(dev)))
+        throw Other{};
+    }
     for (Py_ssize_t i = 0; i < n; ++i) written(*to[i]);
     Py_RETURN_TRUE;
   });
@@ -272,12 +288,13 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// bind(rope, tree_attention_work, tree_attention, sample): addresses in the loaded library
+// bind(rope, tree_attention_work, tree_attention, sample, rope_axes): addresses in the loaded library
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[4];
-  if (!PyArg_ParseTuple(args, "KKKK", &a[0], &a[1], &a[2], &a[3])) return nullptr;
+  unsigned long long a[5];
+  if (!PyArg_ParseTuple(args, "KKKKK", &a[0], &a[1], &a[2], &a[3], &a[4])) return nullptr;
   lib = {reinterpret_cast<decltype(lib.rope)>(a[0]), reinterpret_cast<decltype(lib.tree_work)>(a[1]),
-         reinterpret_cast<decltype(lib.tree)>(a[2]), reinterpret_cast<decltype(lib.sample)>(a[3])};
+         reinterpret_cast<decltype(lib.tree)>(a[2]), reinterpret_cast<decltype(lib.sample)>(a[3]),
+         reinterpret_cast<decltype(lib.rope_axes)>(a[4])};
   Py_RETURN_NONE;
 }
 
@@ -300,6 +317,8 @@ PyMODINIT_FUNC PyInit_btf_b200_calls() {
   s_n_rot = PyUnicode_InternFromString("n_rot");
   s_mscale = PyUnicode_InternFromString("mscale");
   s_interleaved = PyUnicode_InternFromString("interleaved");
+  s_axis = PyUnicode_InternFromString("axis");
+  s_n_axes = PyUnicode_InternFromString("n_axes");
   PyObject* m = PyModule_Create(&module);
   if (m && PyModule_AddStringConstant(m, "torch_version", BTF_TORCH_VERSION)) {  // the mirror binds it to no other
     Py_DECREF(m);

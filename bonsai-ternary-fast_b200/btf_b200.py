@@ -45,6 +45,7 @@ EXPORTS = (
     "btf_gemm_idot", "btf_decoder_prefill", "btf_gemm_wm", "btf_gemm_wm_idot", "btf_gemv_mma", "btf_gemv_mma_idot",
     "btf_rope_table", "btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample",
     "btf_decoder_step_sampled", "btf_decoder_run_sampled", "btf_decoder_verify", "btf_decoder_accept",
+    "btf_rope_axes_table", "btf_rope_axes",
 )
 
 
@@ -268,6 +269,9 @@ def lib() -> ctypes.CDLL:
         "btf_rope_table": (i32, [ctypes.POINTER(RopeCfgC), vp, ctypes.POINTER(ctypes.c_float)]),
         "btf_rope": (i32, [vp, i32, i32, i32, i32, vp, ctypes.c_float, i32, i32, ctypes.c_float,
                            vp, vp]),
+        "btf_rope_axes_table": (i32, [ctypes.POINTER(RopeCfgC), vp, i32, i32, vp, vp, ctypes.POINTER(ctypes.c_float)]),
+        "btf_rope_axes": (i32, [vp, i32, i32, i32, i32, vp, vp, i32, ctypes.c_float, i32, i32, ctypes.c_float, vp, i64,
+                                vp]),
         "btf_tree_attention_work": (i64, [i32] * 6),
         "btf_tree_attention": (i32, [vp, vp]),
         "btf_sample": (i32, [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
@@ -639,6 +643,7 @@ def prep(x, normw=None, eps: float = 1e-6, block: int = 0, perm=(0, 0, 0), signs
 # attention for a tree of drafted tokens, sampling
 F32, F16, BF16 = 0, 1, 2  # BTF_F32 / BTF_F16 / BTF_BF16
 ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+ROPE_AXES = {"split": 0, "turns": 1, "own": 2}
 TREE_MAX_NODES = 64  # BTF_TREE_MAX_NODES
 SAMPLE_MAX_V = 524288  # BTF_SAMPLE_MAX_V
 
@@ -668,7 +673,7 @@ def _bind_calls() -> None:
         spec.loader.exec_module(calls)
         if calls.torch_version == torch.__version__:
             calls.bind(*(ctypes.cast(getattr(lib(), n), ctypes.c_void_p).value
-                         for n in ("btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample")))
+                         for n in ("btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample", "btf_rope_axes")))
             _calls = calls
     except Exception:  # whatever keeps it from loading
         pass
@@ -751,10 +756,13 @@ def _strides(t) -> tuple:
 class RopeTable:
     """Rotary frequencies (btf_rope_table) kept on the device: n_rot rotated dims of a head, base, the scaling for
     long contexts ("none", "linear", "ntk", "yarn" with its factor, trained context and betas) and the layout of the
-    pairs (interleaved: (2i, 2i + 1), else (i, i + n_rot / 2)). device=None: host only."""
+    pairs (interleaved: (2i, 2i + 1), else (i, i + n_rot / 2)). With `sections`, positions with several axes
+    (btf_rope_axes_table): each axis's pairs, n_rot / 2 in all, and which they are: `axes` = "split" (one axis's after
+    another's), "turns" (in turn) or "own" (split, with frequencies of its own for every axis). device=None: host only."""
 
     def __init__(self, n_rot: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, orig_ctx: int = 0,
-                 beta_fast: float = 32.0, beta_slow: float = 1.0, interleaved: bool = False, device="cuda"):
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, interleaved: bool = False, device="cuda",
+                 sections: Optional[Sequence[int]] = None, axes: str = "split"):
         import numpy as np
 
         if scaling not in ROPE_SCALINGS:
@@ -762,9 +770,22 @@ class RopeTable:
         cfg = RopeCfgC(n_rot, ROPE_SCALINGS[scaling], base, factor, beta_fast, beta_slow, orig_ctx)
         self.host = np.zeros(max(1, n_rot // 2), dtype=np.float64)
         m = ctypes.c_float()
-        check(lib().btf_rope_table(ctypes.byref(cfg), self.host.ctypes.data, ctypes.byref(m)), "btf_rope_table")
+        self.axis = self.axis_host = None
+        self.n_axes = 1
+        if sections is None:
+            check(lib().btf_rope_table(ctypes.byref(cfg), self.host.ctypes.data, ctypes.byref(m)), "btf_rope_table")
+        else:
+            if axes not in ROPE_AXES:
+                raise RuntimeError(f"RopeTable: axes must be one of {sorted(ROPE_AXES)}, got {axes!r}")
+            self.n_axes = len(sections)
+            self.axis_host = np.zeros(len(self.host), dtype=np.uint8)
+            check(lib().btf_rope_axes_table(ctypes.byref(cfg), (ctypes.c_int * self.n_axes)(*sections), self.n_axes,
+                                            ROPE_AXES[axes], self.host.ctypes.data, self.axis_host.ctypes.data,
+                                            ctypes.byref(m)), "btf_rope_axes_table")
         self.n_rot, self.mscale, self.interleaved = n_rot, m.value, interleaved
         self.turns = None if device is None else _torch().from_numpy(self.host).to(device)
+        if device is not None and sections is not None:
+            self.axis = _torch().from_numpy(self.axis_host).to(device)
 
 
 @dataclass
@@ -780,7 +801,8 @@ class RopeSeg:
 
 
 def rope(segs: Sequence[RopeSeg], table: RopeTable, pos, inverse: bool = False, eps: float = 1e-6, stream=None) -> None:
-    """Rotates up to 3 tensors of the same tokens by their positions pos [T] (int32) in one launch (btf_rope).
+    """Rotates up to 3 tensors of the same tokens by their positions pos [T] (int32) in one launch (btf_rope); with a
+    table of several axes, by pos [axes][T] (btf_rope_axes; rows may be strided or expanded, their tokens contiguous).
     inverse: the transposed map, the gradient of the rotation. No graph is recorded: tensors that require a gradient are
     refused outside torch.no_grad()."""
     if stream is None and _calls is not None and _calls.rope(segs, table, pos, inverse, eps):
@@ -821,14 +843,31 @@ def rope(segs: Sequence[RopeSeg], table: RopeTable, pos, inverse: bool = False, 
             raise RuntimeError(f"rope: y has {n_rows} rows for {T} tokens")
         packed += _ROPE_SEG.pack(x.data_ptr(), y.data_ptr(), _elem(x, "rope"), _elem(y, "rope"), heads, s.rotate, xt, xh,
                                  yt, yh, normw, rows, n_rows)
-    pos_ptr = _vector("rope", dev, "pos", pos, i32, (T,))
+    if getattr(table, "axis_host", None) is None:
+        pos_ptr = _vector("rope", dev, "pos", pos, i32, (T,))
+    else:
+        if pos is None or pos.dtype != i32 or pos.shape != (table.n_axes, T) or (T > 1 and pos.stride(1) != 1):
+            raise RuntimeError(f"rope: pos must be an int32 tensor of shape {(table.n_axes, T)} with contiguous rows, got "
+                               f"{'None' if pos is None else f'{pos.dtype} {tuple(pos.shape)}'}")
+        _on("rope", dev, "pos", pos)
+        axis = table.axis
+        if axis is None or axis.device != dev:
+            raise RuntimeError(f"rope: the table must be on {dev}")
+        if table.n_rot > 2 * axis.numel() or axis.dtype != torch.uint8 or not axis.is_contiguous():
+            raise RuntimeError(f"rope: the table's axis must hold n_rot / 2 = {table.n_rot // 2} contiguous uint8 values")
+        pos_ptr = pos.data_ptr()
     turns = table.turns
     if turns is None or turns.device != dev:
         raise RuntimeError(f"rope: the table must be on {dev}")
     if table.n_rot > 2 * turns.numel() or turns.dtype != torch.float64 or not turns.is_contiguous():
         raise RuntimeError(f"rope: the table's turns must hold n_rot / 2 = {table.n_rot // 2} contiguous float64 values")
-    _launch(dev, stream, _rope_call, (packed, n, T, D, table.n_rot, turns.data_ptr(), table.mscale, table.interleaved,
-                                      inverse, eps, pos_ptr))
+    if getattr(table, "axis_host", None) is None:
+        _launch(dev, stream, _rope_call, (packed, n, T, D, table.n_rot, turns.data_ptr(), table.mscale, table.interleaved,
+                                          inverse, eps, pos_ptr))
+    else:
+        _launch(dev, stream, _rope_axes_call, (packed, n, T, D, table.n_rot, turns.data_ptr(), axis.data_ptr(),
+                                               table.n_axes, table.mscale, table.interleaved, inverse, eps, pos_ptr,
+                                               pos.stride(0) if table.n_axes > 1 else 0))
     _written(*(s.x if s.y is None else s.y for s in segs))
 
 
@@ -836,6 +875,12 @@ def _rope_call(st, args) -> None:
     status = _lib.btf_rope(*args, st)
     if status:
         check(status, "btf_rope")
+
+
+def _rope_axes_call(st, args) -> None:
+    status = _lib.btf_rope_axes(*args, st)
+    if status:
+        check(status, "btf_rope_axes")
 
 
 def tree_attention_work(q, k):

@@ -17,6 +17,7 @@
 // and thread and used for all heads that the thread takes, whole 16-byte words move,
 // and q, k and v share a launch.
 #include <cmath>
+#include <type_traits>
 
 #include "elem.cuh"
 
@@ -45,6 +46,10 @@ struct RopeParams {
   const double* turns;
   const int32_t* pos;
   float mscale, eps;
+  // several axes: each pair's axis, and the elements from one axis's positions to the next's
+  const uint8_t* axis;
+  int64_t pos_axis;
+  int n_axes;
 };
 
 // 1 / sqrt(mean square + eps) of a head from its lanes' sums of squares.
@@ -61,7 +66,10 @@ __device__ __forceinline__ float norm_scale(const RopeParams& p, unsigned mask, 
 // heads of 128, 336 MB: 100 us a head at a time, 67 with 4, 60 with 8, 57 (5870
 // GB/s, 0.90 of a plain copy's rate) with 16 heads a thread for 8; loads ahead of
 // the angles too keep more registers and lose.
-template <typename TX, typename TY, int C, int NORM>
+//
+// AXES: pair i turns by the token's position on its axis. All positions of the token (at most four) are read at once
+// and picked from, so that no read waits for the axis.
+template <typename TX, typename TY, int C, int NORM, bool AXES>
 __device__ __forceinline__ void rope_heads(const RopeParams& p, const RopeSeg& s, int t, int64_t row, int h0, int h1,
                                            int lane, float* scales) {
   constexpr int kBatch = NORM ? 1 : C * (int)sizeof(TX) >= 32 ? 2 : C == 8 ? 8 : 4;
@@ -99,10 +107,21 @@ __device__ __forceinline__ void rope_heads(const RopeParams& p, const RopeSeg& s
     const bool hasb = active && cb < D;
     float cs[C], sn[C];
     if (rot) {
-      const double ps = (double)p.pos[t];
+      int at[AXES ? BTF_ROPE_MAX_AXES : 1];
+      at[0] = p.pos[t];
+      if constexpr (AXES) {
+#pragma unroll
+        for (int a = 1; a < BTF_ROPE_MAX_AXES; ++a) at[a] = a < p.n_axes ? p.pos[a * p.pos_axis + t] : at[0];
+      }
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        const double turn = ps * p.turns[i + j];
+        int on = at[0];
+        if constexpr (AXES) {
+          const int ax = p.axis[i + j];
+#pragma unroll
+          for (int a = 1; a < BTF_ROPE_MAX_AXES; ++a) on = ax == a ? at[a] : on;
+        }
+        const double turn = (double)on * p.turns[i + j];
         const float f = (float)(turn - rint(turn));
         float sv, cv;
         sincospif(2.0f * f, &sv, &cv);
@@ -177,15 +196,15 @@ __device__ __forceinline__ void rope_heads(const RopeParams& p, const RopeSeg& s
   }
 }
 
-template <typename TX, int C, int NORM>
+template <typename TX, int C, int NORM, bool AXES>
 __device__ __forceinline__ void rope_to(const RopeParams& p, const RopeSeg& s, int t, int64_t row, int h0, int h1,
                                         int lane, float* scales) {
-  if (s.y_type == BTF_F32) rope_heads<TX, float, C, NORM>(p, s, t, row, h0, h1, lane, scales);
-  else if (s.y_type == BTF_F16) rope_heads<TX, __half, C, NORM>(p, s, t, row, h0, h1, lane, scales);
-  else rope_heads<TX, __nv_bfloat16, C, NORM>(p, s, t, row, h0, h1, lane, scales);
+  if (s.y_type == BTF_F32) rope_heads<TX, float, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
+  else if (s.y_type == BTF_F16) rope_heads<TX, __half, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
+  else rope_heads<TX, __nv_bfloat16, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
 }
 
-template <int C, int NORM>
+template <int C, int NORM, bool AXES>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p) {
   __shared__ float scales_of[NORM == kRounds ? kThreads / 32 : 1][kMaxHeads];
   float* scales = scales_of[NORM == kRounds ? threadIdx.x >> 5 : 0];
@@ -203,9 +222,9 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
     row = s.rows[t];
     if (row < 0 || row >= s.n_rows) return;
   }
-  if (s.x_type == BTF_F32) rope_to<float, C, NORM>(p, s, t, row, h0, h1, lane, scales);
-  else if (s.x_type == BTF_F16) rope_to<__half, C, NORM>(p, s, t, row, h0, h1, lane, scales);
-  else rope_to<__nv_bfloat16, C, NORM>(p, s, t, row, h0, h1, lane, scales);
+  if (s.x_type == BTF_F32) rope_to<float, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
+  else if (s.x_type == BTF_F16) rope_to<__half, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
+  else rope_to<__nv_bfloat16, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
 }
 
 bool aligned_for(const btf_rope_seg& s, int C) {
@@ -261,8 +280,47 @@ int btf_rope_table(const btf_rope_cfg* c, double* turns, float* mscale) {
   return BTF_OK;
 }
 
-int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const double* turns, float mscale,
-             int interleaved, int inverse, float eps, const int32_t* pos, void* stream) {
+int btf_rope_axes_table(const btf_rope_cfg* c, const int* sections, int n_axes, int layout, double* turns, uint8_t* axis,
+                        float* mscale) {
+  if (!c || !sections || !turns || !axis || !mscale) return fail(BTF_ERR_ARG, "btf_rope_axes_table: null argument");
+  if (n_axes < 1 || n_axes > BTF_ROPE_MAX_AXES)
+    return fail(BTF_ERR_ARG, "btf_rope_axes_table: 1..%d axes (got %d)", BTF_ROPE_MAX_AXES, n_axes);
+  if (layout < BTF_AXES_SPLIT || layout > BTF_AXES_OWN)
+    return fail(BTF_ERR_ARG, "btf_rope_axes_table: unknown layout %d", layout);
+  int64_t pairs = 0;
+  for (int a = 0; a < n_axes; ++a) {
+    if (sections[a] < 0 || sections[a] > BTF_ROPE_MAX_D / 2)
+      return fail(BTF_ERR_ARG, "btf_rope_axes_table: an axis has 0..%d pairs (got %d)", BTF_ROPE_MAX_D / 2, sections[a]);
+    pairs += sections[a];
+  }
+  if (2 * pairs != c->n_rot)
+    return fail(BTF_ERR_ARG, "btf_rope_axes_table: the axes have %lld pairs, n_rot is %d", (long long)pairs, c->n_rot);
+  btf_rope_cfg own = *c;
+  if (layout != BTF_AXES_OWN) {
+    if (int rc = btf_rope_table(c, turns, mscale)) return rc;
+  }
+  int left[BTF_ROPE_MAX_AXES], at = 0;
+  for (int a = 0; a < n_axes; ++a) {
+    left[a] = sections[a];
+    if (layout == BTF_AXES_TURNS) continue;
+    own.n_rot = 2 * sections[a];
+    if (layout == BTF_AXES_OWN && sections[a])
+      if (int rc = btf_rope_table(&own, turns + at, mscale)) return rc;
+    for (int j = 0; j < sections[a]; ++j) axis[at++] = (uint8_t)a;
+  }
+  for (int a = 0; at < pairs; a = (a + 1) % n_axes)  // in turn
+    if (left[a]) --left[a], axis[at++] = (uint8_t)a;
+  return BTF_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// Both calls; axis NULL: one position per token.
+int rope_call(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const double* turns, float mscale,
+              int interleaved, int inverse, float eps, const int32_t* pos, const uint8_t* axis, int n_axes,
+              int64_t pos_axis, void* stream) {
   if (!segs || nseg < 1 || nseg > 3) return fail(BTF_ERR_ARG, "btf_rope: 1..3 tensors (got %d)", nseg);
   if (T < 0 || T > 1 << 30) return fail(BTF_ERR_ARG, "btf_rope: T must be 0..2^30 (got %d)", T);
   if (D < 1 || D > BTF_ROPE_MAX_D || n_rot < 0 || n_rot % 2 || n_rot > D)
@@ -301,6 +359,7 @@ int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const 
   p.nseg = 0;
   p.T = T, p.D = D, p.R = n_rot, p.inter = interleaved != 0, p.inverse = inverse != 0;
   p.turns = turns, p.pos = pos, p.mscale = mscale, p.eps = eps;
+  p.axis = axis, p.n_axes = n_axes, p.pos_axis = pos_axis;
   const int items = std::max(n_rot / 2 / C + (D - n_rot + 2 * C - 1) / (2 * C), (D + 2 * C - 1) / (2 * C));
   bool norm = false, narrow = true;
   for (int i = 0; i < nseg; ++i) {
@@ -328,11 +387,35 @@ int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const 
   const dim3 grid((T + per - 1) / per, blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const auto pick = [C](auto c8, auto c4, auto c1) { return C == 8 ? c8 : C == 4 ? c4 : c1; };
-  const auto kernel = !norm             ? pick(rope_kernel<8, 0>, rope_kernel<4, 0>, rope_kernel<1, 0>)
-                      : items > p.lanes ? pick(rope_kernel<8, kRounds>, rope_kernel<4, kRounds>, rope_kernel<1, kRounds>)
-                                        : pick(rope_kernel<8, kOneRound>, rope_kernel<4, kOneRound>, rope_kernel<1, kOneRound>);
+  const auto kernel_of = [&](auto axes) {
+    constexpr bool A = decltype(axes)::value;
+    return !norm             ? pick(rope_kernel<8, 0, A>, rope_kernel<4, 0, A>, rope_kernel<1, 0, A>)
+           : items > p.lanes ? pick(rope_kernel<8, kRounds, A>, rope_kernel<4, kRounds, A>, rope_kernel<1, kRounds, A>)
+                             : pick(rope_kernel<8, kOneRound, A>, rope_kernel<4, kOneRound, A>, rope_kernel<1, kOneRound, A>);
+  };
+  const auto kernel = axis ? kernel_of(std::true_type{}) : kernel_of(std::false_type{});
   const cudaError_t e = launch_pdl(kernel, grid, dim3(kThreads), 0, st, p);
   return e == cudaSuccess ? BTF_OK : cuda_fail(e, "btf_rope");
+}
+
+}  // namespace
+
+extern "C" {
+
+int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const double* turns, float mscale,
+             int interleaved, int inverse, float eps, const int32_t* pos, void* stream) {
+  return rope_call(segs, nseg, T, D, n_rot, turns, mscale, interleaved, inverse, eps, pos, nullptr, 1, 0, stream);
+}
+
+int btf_rope_axes(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const double* turns, const uint8_t* axis,
+                  int n_axes, float mscale, int interleaved, int inverse, float eps, const int32_t* pos,
+                  int64_t pos_axis, void* stream) {
+  if (n_axes < 1 || n_axes > BTF_ROPE_MAX_AXES)
+    return fail(BTF_ERR_ARG, "btf_rope_axes: 1..%d axes (got %d)", BTF_ROPE_MAX_AXES, n_axes);
+  if (n_rot > 0 && T > 0 && !axis) return fail(BTF_ERR_ARG, "btf_rope_axes: null axis");
+  if (n_axes > 1 && pos_axis < 0) return fail(BTF_ERR_ARG, "btf_rope_axes: the stride between the axes' positions is negative");
+  return rope_call(segs, nseg, T, D, n_rot, turns, mscale, interleaved, inverse, eps, pos, n_rot > 0 ? axis : nullptr,
+                   n_axes, pos_axis, stream);
 }
 
 }  // extern "C"

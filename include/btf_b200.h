@@ -594,6 +594,27 @@ typedef struct btf_rope_seg {
 int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const double* turns, float mscale,
              int interleaved, int inverse, float eps, const int32_t* pos, void* stream);
 
+/* Rotary positions with several axes (time, height and width of images and video): pair i of a head turns by the
+ * token's position on the pair's own axis, pos[axis[i]][t] * f_i. `sections` has each axis's pairs, n_rot / 2 in all:
+ *   BTF_AXES_SPLIT  the first sections[0] pairs are axis 0's, the next sections[1] axis 1's, ...; f_i as btf_rope_table's
+ *   BTF_AXES_TURNS  the pairs go to the axes in turn (0, 1, 2, 0, 1, 2, ...; an axis without pairs left is passed
+ *                   over); f_i as btf_rope_table's
+ *   BTF_AXES_OWN    as BTF_AXES_SPLIT, and every axis has frequencies of its own: those of btf_rope_table with n_rot = 2
+ *                   sections[a]
+ * An axis may have no pairs. Host only: fills turns_host[n_rot / 2] and axis_host[n_rot / 2], and *mscale. */
+#define BTF_ROPE_MAX_AXES 4
+#define BTF_AXES_SPLIT 0
+#define BTF_AXES_TURNS 1
+#define BTF_AXES_OWN 2
+int btf_rope_axes_table(const btf_rope_cfg* cfg, const int* sections, int n_axes, int layout, double* turns_host,
+                        uint8_t* axis_host, float* mscale);
+/* btf_rope with n_axes positions per token: axis a's lie at pos + a * pos_axis (elements), one per token; axis[n_rot / 2]
+ * is on the device (values >= n_axes count as axis 0). Text, whose tokens have one position on every axis, may share one row
+ * of positions (pos_axis 0). The rest as btf_rope, its limits and its inverse (the gradient) among it. */
+int btf_rope_axes(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const double* turns, const uint8_t* axis,
+                  int n_axes, float mscale, int interleaved, int inverse, float eps, const int32_t* pos,
+                  int64_t pos_axis, void* stream);
+
 /* Attention for a tree of drafted tokens over a cache. Sequence b has lens[b] cached tokens in rows
  * [0, lens[b]) of k and v, and its counts[b] <= n drafted nodes' k and v in the rows behind them (node j in row
  * lens[b] + j). Node i attends to every cached row, to itself and to its ancestors: parents[b][j] < j is the
