@@ -45,7 +45,8 @@ EXPORTS = (
     "btf_gemm_idot", "btf_decoder_prefill", "btf_gemm_wm", "btf_gemm_wm_idot", "btf_gemv_mma", "btf_gemv_mma_idot",
     "btf_rope_table", "btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample",
     "btf_decoder_step_sampled", "btf_decoder_run_sampled", "btf_decoder_verify", "btf_decoder_accept",
-    "btf_rope_axes_table", "btf_rope_axes",
+    "btf_rope_axes_table", "btf_rope_axes", "btf_adapter_plan_bytes", "btf_adapter_plan", "btf_adapters_work",
+    "btf_adapters",
 )
 
 
@@ -187,6 +188,23 @@ class TreeAttnC(ctypes.Structure):
 _TREE_ATTN = struct.Struct("@PqqqPPqqqPqqqiiiiiiiPPPfPq")  # a btf_tree_attn
 
 
+class AdapterSegC(ctypes.Structure):
+    """btf_adapter_seg: one projection of a btf_adapters call."""
+
+    _fields_ = [("a", ctypes.c_void_p), ("a_adapter", ctypes.c_int64), ("a_row", ctypes.c_int64), ("b", ctypes.c_void_p),
+                ("b_adapter", ctypes.c_int64), ("b_row", ctypes.c_int64), ("N", ctypes.c_int), ("base", ctypes.c_void_p),
+                ("base_row", ctypes.c_int64), ("y", ctypes.c_void_p), ("y_row", ctypes.c_int64)]
+
+
+class AdaptersArgsC(ctypes.Structure):
+    """btf_adapters_args: low-rank adapters of many requests."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("x_row", ctypes.c_int64)] + [
+        (f, ctypes.c_int) for f in ("x_type", "w_type", "y_type", "T", "K", "R", "n_adapters", "nseg")] + [
+        ("segs", AdapterSegC * 3), ("ranks", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("plan", ctypes.c_void_p),
+        ("plan_bytes", ctypes.c_int64), ("work", ctypes.c_void_p), ("work_bytes", ctypes.c_int64)]
+
+
 def lib() -> ctypes.CDLL:
     """Loads libbtf_b200.so (raises if it was not built)."""
     global _lib
@@ -272,6 +290,10 @@ def lib() -> ctypes.CDLL:
         "btf_rope_axes_table": (i32, [ctypes.POINTER(RopeCfgC), vp, i32, i32, vp, vp, ctypes.POINTER(ctypes.c_float)]),
         "btf_rope_axes": (i32, [vp, i32, i32, i32, i32, vp, vp, i32, ctypes.c_float, i32, i32, ctypes.c_float, vp, i64,
                                 vp]),
+        "btf_adapter_plan_bytes": (i64, [i32, i32]),
+        "btf_adapter_plan": (i32, [vp, i32, i32, vp, i64, vp]),
+        "btf_adapters_work": (i64, [i32] * 5),
+        "btf_adapters": (i32, [vp, vp]),
         "btf_tree_attention_work": (i64, [i32] * 6),
         "btf_tree_attention": (i32, [vp, vp]),
         "btf_sample": (i32, [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
@@ -881,6 +903,132 @@ def _rope_axes_call(st, args) -> None:
     status = _lib.btf_rope_axes(*args, st)
     if status:
         check(status, "btf_rope_axes")
+
+
+ADAPTERS_MAX, ADAPTERS_MAX_RANK = 1024, 128  # BTF_ADAPTERS_MAX, BTF_ADAPTERS_MAX_RANK
+
+
+class AdapterPlan:
+    """Which rows of a batch belong to which adapter (btf_adapter_plan), sorted on the device for every adapters() call of
+    a step: index [T] (int32 on the device; -1: a row without adapter) of n_adapters."""
+
+    def __init__(self, index, n_adapters: int, stream=None):
+        torch = _torch()
+        dev = _cuda_device("AdapterPlan", index)
+        self.T, self.n_adapters = index.numel(), n_adapters
+        size = lib().btf_adapter_plan_bytes(self.T, n_adapters)
+        if size < 0:
+            check(1, "btf_adapter_plan_bytes")
+        self.plan = torch.empty(size, dtype=torch.uint8, device=dev)
+        self.update(index, stream)
+
+    def update(self, index, stream=None) -> None:
+        """Sorts the rows of another step, as many as before, into the same plan (in stream order)."""
+        ptr = _vector("AdapterPlan", self.plan.device, "index", index, _torch().int32, (self.T,))
+        if ptr is None:
+            raise RuntimeError("AdapterPlan: index must be a tensor")
+        _launch(self.plan.device, stream, self._call, ptr)
+
+    def _call(self, st, ptr) -> None:
+        check(lib().btf_adapter_plan(ptr, self.T, self.n_adapters, self.plan.data_ptr(), self.plan.nbytes, st),
+              "btf_adapter_plan")
+        _written(self.plan)
+
+
+@dataclass
+class AdapterSeg:
+    """One projection of an adapters() call: a [n_adapters][R][K], b [n_adapters][N][R] (float16 or bfloat16), y [T][N] (None:
+    a new tensor) and base [T][N] of y's type (None: 0; y itself: in place)."""
+
+    a: object
+    b: object
+    y: object = None
+    base: object = None
+
+
+def adapters_work(x, segs: Sequence[AdapterSeg], plan: AdapterPlan):
+    """A workspace for adapters() calls of these shapes. Calls that may run at the same time need one each."""
+    torch = _torch()
+    dev = _cuda_device("adapters_work", x)
+    ensure_init(dev.index)
+    with torch.cuda.device(dev):
+        size = lib().btf_adapters_work(x.shape[0], x.shape[1], segs[0].a.shape[1], len(segs), plan.n_adapters)
+    if size < 0:
+        check(1, "btf_adapters_work")
+    return torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
+
+
+def adapters(x, segs: Sequence[AdapterSeg], plan: AdapterPlan, ranks=None, scales=None, work=None, stream=None) -> list:
+    """Low-rank adapters of many requests beside up to 3 projections of the same rows x [T][K] (btf_adapters): y = base +
+    scales[a] (x A_a^T) B_a^T with each row's adapter a of the plan, by the first ranks[a] (int32 [n_adapters], None: R) of
+    its rank; scales float32 [n_adapters] or None. Returns the y. No graph is recorded: tensors that require a gradient
+    are refused outside torch.no_grad()."""
+    torch = _torch()
+    if not 1 <= len(segs) <= 3:
+        raise RuntimeError(f"adapters: 1..3 projections expected, got {len(segs)}")
+    dev = _cuda_device("adapters", x)
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise RuntimeError("adapters: x [T][K] with contiguous rows expected")
+    (T, K), a0 = x.shape, segs[0].a
+    if plan.T != T or plan.plan.device != dev:
+        raise RuntimeError(f"adapters: a plan of {plan.T} rows on {plan.plan.device} for {T} rows on {dev}")
+    n, R = plan.n_adapters, a0.shape[1] if a0.dim() == 3 else -1
+    _no_graph("adapters", x, scales)
+    y_type = None
+    for s in segs:
+        _no_graph("adapters", s.a, s.b, s.y, s.base)
+        if s.a.dim() != 3 or s.b.dim() != 3 or tuple(s.a.shape) != (n, R, K) or s.b.shape[0] != n or s.b.shape[2] != R:
+            raise RuntimeError(f"adapters: a [{n}][{R}][{K}] and b [{n}][N][{R}] expected, got {tuple(s.a.shape)} and "
+                               f"{tuple(s.b.shape)}")
+        if s.a.stride(2) != 1 or s.b.stride(2) != 1:
+            raise RuntimeError("adapters: the rows of a and b must be contiguous")
+        if s.a.dtype != a0.dtype or s.b.dtype != a0.dtype:
+            raise RuntimeError("adapters: every a and b must have one type")
+        for name, t in (("a", s.a), ("b", s.b), ("y", s.y), ("base", s.base)):
+            if t is not None:
+                _on("adapters", dev, name, t)
+        for t in (s.y, s.base):
+            if t is not None:
+                if tuple(t.shape) != (T, s.b.shape[1]) or (t.shape[1] > 1 and t.stride(1) != 1):
+                    raise RuntimeError(f"adapters: y and base {(T, s.b.shape[1])} with contiguous rows expected, got "
+                                       f"{tuple(t.shape)}")
+                if y_type not in (None, t.dtype):
+                    raise RuntimeError("adapters: every y and base must have one type")
+                y_type = t.dtype
+    rp = _vector("adapters", dev, "ranks", ranks, torch.int32, (n,))
+    sp = _vector("adapters", dev, "scales", scales, torch.float32, (n,))
+    return _launch(dev, stream, _adapters_call, (x, segs, plan, y_type or x.dtype, rp, sp, work))
+
+
+_ADAPTERS_HEAD, _ADAPTER_SEG = struct.Struct("@Pqiiiiiiii"), struct.Struct("@PqqPqqiPqPq")
+_ADAPTERS_TAIL = struct.Struct("@PPPqPq")  # with 3 segments between: a btf_adapters_args
+
+
+def _adapters_call(st, args) -> list:
+    x, segs, plan, y_type, rp, sp, work = args
+    torch = _torch()
+    (T, K), dev, a0 = x.shape, x.device, segs[0].a
+    out = [torch.empty((T, s.b.shape[1]), dtype=y_type, device=dev) if s.y is None else s.y for s in segs]
+    if T == 0:
+        return out
+    if work is None:
+        work = adapters_work(x, segs, plan)
+    elif work.device != dev or not work.is_contiguous():
+        raise RuntimeError(f"adapters: the workspace must be contiguous, on {dev}")
+    packed = _ADAPTERS_HEAD.pack(x.data_ptr(), x.stride(0), _elem(x, "adapters"), _elem(a0, "adapters"),
+                                 _elem(out[0], "adapters"), T, K, a0.shape[1], plan.n_adapters, len(segs))
+    for s, y in zip(segs, out):
+        base = s.base
+        packed += _ADAPTER_SEG.pack(s.a.data_ptr(), s.a.stride(0), s.a.stride(1), s.b.data_ptr(), s.b.stride(0),
+                                    s.b.stride(1), s.b.shape[1], 0 if base is None else base.data_ptr(),
+                                    0 if base is None else base.stride(0), y.data_ptr(), y.stride(0))
+    packed += bytes(_ADAPTER_SEG.size * (3 - len(segs))) + _ADAPTERS_TAIL.pack(
+        rp or 0, sp or 0, plan.plan.data_ptr(), plan.plan.nbytes, work.data_ptr(), work.nbytes)
+    status = _lib.btf_adapters(packed, st)
+    if status:
+        check(status, "btf_adapters")
+    _written(*out)
+    return out
 
 
 def tree_attention_work(q, k):

@@ -154,7 +154,8 @@ int btf_gemv(const btf_gemv_seg* segs, int nseg, int K, int M, btf_q8act act, in
 int btf_gemv_f32(const btf_gemv_seg* segs, int nseg, int K, int M, const float* x, int ldx, int mode, void* stream);
 
 /* Device error word of the current device: nonzero after a bounded device-side
- * wait gave up (the kernel then returned early instead of hanging). Synchronous;
+ * wait gave up (1; the kernel then returned early instead of hanging) or btf_adapters
+ * met a plan of other sizes (2). Synchronous;
  * not for use inside stream capture. clear != 0 resets it. Returns -1 on failure. */
 int btf_device_error(int clear);
 
@@ -614,6 +615,52 @@ int btf_rope_axes_table(const btf_rope_cfg* cfg, const int* sections, int n_axes
 int btf_rope_axes(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const double* turns, const uint8_t* axis,
                   int n_axes, float mscale, int interleaved, int inverse, float eps, const int32_t* pos,
                   int64_t pos_axis, void* stream);
+
+/* Low-rank adapters of many requests at once, beside a shared projection: for each of up to 3 projections of the same
+ * rows x_t (q, k and v; gate and up),
+ *   y_t = base_t + scales[a] * B_a (A_a x_t),  a = index[t] of the plan,
+ * with A_a the first ranks[a] of R rows of K, and B_a the first ranks[a] of R columns of N rows (what lies behind an
+ * adapter's rank is never part of a result). A row whose index is no adapter (-1, or any other number outside 0 ..
+ * n_adapters - 1) is y_t = base_t. base is what the shared projection gave (btf_gemv's y) and may be y itself (same
+ * stride), or NULL (0). Products are summed in fp32, and an fp32 x or y is served to fp32: see csrc/adapters.cu. The
+ * reference has no adapters; the call stands beside launch_gemv (src/cuda/kernels.cuh:56). */
+#define BTF_ADAPTERS_MAX 1024         /* adapters of a call */
+#define BTF_ADAPTERS_MAX_RANK 128     /* R */
+#define BTF_ADAPTERS_MAX_ROWS 1048576 /* T */
+/* Which rows belong to which adapter, for every call of a step with these rows: index[T] on the device, sorted on the
+ * device into `plan` (btf_adapter_plan_bytes bytes, 16-byte aligned). Asynchronous; the calls that use it come behind it. */
+int64_t btf_adapter_plan_bytes(int T, int n_adapters);
+int btf_adapter_plan(const int32_t* index, int T, int n_adapters, void* plan, int64_t plan_bytes, void* stream);
+typedef struct btf_adapter_seg { /* one projection; strides in elements, rows contiguous */
+  const void* a;               /* [n_adapters][R][K], 16-byte aligned, strides multiples of 8 */
+  int64_t a_adapter, a_row;
+  const void* b;               /* [n_adapters][N][R], as a */
+  int64_t b_adapter, b_row;
+  int N;
+  const void* base;            /* [T][N] of y's type, y itself, or NULL; must not overlap y otherwise */
+  int64_t base_row;
+  void* y;                     /* [T][N], rows apart (y_row >= N) */
+  int64_t y_row;
+} btf_adapter_seg;
+typedef struct btf_adapters_args {
+  const void* x;               /* [T][K], 16-byte aligned as its rows; must not overlap a y */
+  int64_t x_row;
+  int x_type, w_type, y_type;  /* a and b: BTF_F16 or BTF_BF16; x and y: that or BTF_F32 */
+  int T, K, R, n_adapters;     /* K % 8 == 0, R % 8 == 0 */
+  int nseg;                    /* 1..3 */
+  btf_adapter_seg segs[3];
+  const int32_t* ranks;        /* [n_adapters] on the device (taken as 0 .. R), or NULL: R each */
+  const float* scales;         /* [n_adapters] on the device, or NULL: 1 each */
+  const void* plan;            /* of btf_adapter_plan with the same T and n_adapters (btf_device_error tells 2 after a
+                                  call whose plan says others; its y is then left as it was) */
+  int64_t plan_bytes;
+  void* work;                  /* btf_adapters_work(...) bytes, 16-byte aligned; calls that may run at the same time need
+                                  one each */
+  int64_t work_bytes;
+} btf_adapters_args;
+/* Workspace bytes of a call with these sizes on the current device (host only; -1 on bad sizes). */
+int64_t btf_adapters_work(int T, int K, int R, int nseg, int n_adapters);
+int btf_adapters(const btf_adapters_args* args, void* stream);
 
 /* Attention for a tree of drafted tokens over a cache. Sequence b has lens[b] cached tokens in rows
  * [0, lens[b]) of k and v, and its counts[b] <= n drafted nodes' k and v in the rows behind them (node j in row

@@ -64,3 +64,43 @@ def test_rope_axes_refuses(btf, kw):
 
 def test_rope_axes_of_nothing_is_done(btf):
     assert _axes(btf, T=0, axis=None) == 0 and _axes(btf, seg=dict(heads=0)) == 0
+
+
+# ---------------------------------------------------------------- low-rank adapters
+def _adapters(btf, seg=None, **kw):
+    s = dict(a=P, a_adapter=8 * 64, a_row=64, b=P, b_adapter=16 * 8, b_row=8, N=16, base=P, base_row=16, y=P + 1024, y_row=16)
+    s.update(seg or {})
+    a = dict(x=P, x_row=64, x_type=0, w_type=1, y_type=0, T=4, K=64, R=8, n_adapters=2, nseg=1, ranks=None, scales=None,
+             plan=P, plan_bytes=1 << 40, work=P, work_bytes=1 << 40)
+    a.update(kw)
+    args = btf.AdaptersArgsC(**a)
+    for i in range(3):
+        args.segs[i] = btf.AdapterSegC(**s)
+    return btf.lib().btf_adapters(ctypes.byref(args), None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(T=-1), dict(T=(1 << 20) + 1), dict(K=0), dict(K=60), dict(R=0), dict(R=12), dict(R=136), dict(n_adapters=0),
+    dict(n_adapters=1025), dict(nseg=0), dict(nseg=4), dict(w_type=0), dict(w_type=3), dict(x_type=2), dict(y_type=2),
+    dict(y_type=3), dict(x=None), dict(x=P + 8), dict(x_row=62), dict(x_row=-64), dict(x_type=1, x_row=68), dict(plan=None),
+    dict(plan=P + 8), dict(plan_bytes=64),
+    dict(seg=dict(a=None)), dict(seg=dict(b=None)), dict(seg=dict(y=None)), dict(seg=dict(a=P + 8)), dict(seg=dict(b=P + 4)),
+    dict(seg=dict(a_row=60)), dict(seg=dict(b_row=-8)), dict(seg=dict(a_adapter=4)), dict(seg=dict(N=0)), dict(seg=dict(y=P + 2)),
+    dict(seg=dict(base=P + 1)), dict(seg=dict(y_row=15)), dict(seg=dict(base_row=-1)), dict(seg=dict(base=P + 1024, base_row=32)),
+])
+def test_adapters_refuses(btf, kw):
+    assert _adapters(btf, **kw) == 1, kw
+    assert btf.lib().btf_last_error()
+
+
+def test_adapters_of_no_row_are_done_and_plans_refuse(btf):
+    L = btf.lib()
+    assert _adapters(btf, T=0) == 0
+    assert L.btf_adapters(None, None) == 1
+    for T, n in ((-1, 1), (1, 0), (1, 1025), ((1 << 20) + 1, 1)):
+        assert L.btf_adapter_plan_bytes(T, n) == -1 and L.btf_adapter_plan(P, T, n, P, 1 << 40, None) == 1
+    size = L.btf_adapter_plan_bytes(100, 7)
+    assert size > 400
+    for args in ((None, 100, 7, P, size), (P, 100, 7, None, size), (P, 100, 7, P + 8, size), (P, 100, 7, P, size - 1)):
+        assert L.btf_adapter_plan(*args, None) == 1
+    assert L.btf_adapters_work(4, 60, 8, 1, 2) == -1
