@@ -46,7 +46,7 @@ EXPORTS = (
     "btf_rope_table", "btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample",
     "btf_decoder_step_sampled", "btf_decoder_run_sampled", "btf_decoder_verify", "btf_decoder_accept",
     "btf_rope_axes_table", "btf_rope_axes", "btf_adapter_plan_bytes", "btf_adapter_plan", "btf_adapters_work",
-    "btf_adapters",
+    "btf_adapters", "btf_prefix_attention_work", "btf_prefix_attention",
 )
 
 
@@ -188,6 +188,16 @@ class TreeAttnC(ctypes.Structure):
 _TREE_ATTN = struct.Struct("@PqqqPPqqqPqqqiiiiiiiPPPfPq")  # a btf_tree_attn
 
 
+class PrefixC(ctypes.Structure):
+    """btf_prefix: the rows that a batch's sequences share."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("row", ctypes.c_int64), ("head", ctypes.c_int64),
+                ("rows", ctypes.c_int), ("len", ctypes.c_void_p)]
+
+
+_PREFIX = struct.Struct("@PPqqiP")  # a btf_prefix
+
+
 class AdapterSegC(ctypes.Structure):
     """btf_adapter_seg: one projection of a btf_adapters call."""
 
@@ -296,6 +306,8 @@ def lib() -> ctypes.CDLL:
         "btf_adapters": (i32, [vp, vp]),
         "btf_tree_attention_work": (i64, [i32] * 6),
         "btf_tree_attention": (i32, [vp, vp]),
+        "btf_prefix_attention_work": (i64, [i32] * 7),
+        "btf_prefix_attention": (i32, [vp, vp, vp]),
         "btf_sample": (i32, [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
         "btf_plan_memory_synthetic": (i32, [ctypes.POINTER(DecoderDimsC), ctypes.POINTER(DecoderOptsC), i32, i32,
                                             ctypes.POINTER(MemoryPlanC)]),
@@ -1054,53 +1066,98 @@ def tree_attention(q, k, v, lens, parents, counts=None, scale: Optional[float] =
         done = _calls.tree_attention(q, k, v, lens, parents, counts, scale, out, work)
         if done is not None:
             return done
+    return _tree("tree_attention", q, k, v, lens, parents, counts, scale, out, work, None, stream)
+
+
+def _tree(what, q, k, v, lens, parents, counts, scale, out, work, prefix, stream):
+    """tree_attention, and prefix_attention with prefix = (pk, pv, prefix_len)."""
     torch = _torch()
     qs, ks = q.shape, k.shape
     if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[0] != qs[0] or ks[3] != qs[3]:
-        raise RuntimeError(f"tree_attention: q [B][n][H][D] and k, v [B][n_ctx][HK][D] expected, got {tuple(qs)}, "
+        raise RuntimeError(f"{what}: q [B][n][H][D] and k, v [B][n_ctx][HK][D] expected, got {tuple(qs)}, "
                            f"{tuple(ks)}, {tuple(v.shape)}")
-    _no_graph("tree_attention", q, k, v, out)
+    _no_graph(what, q, k, v, out)
     B, n, H, D = qs
-    dev, dtype, i32 = _cuda_device("tree_attention", q), q.dtype, torch.int32
+    dev, dtype, i32 = _cuda_device(what, q), q.dtype, torch.int32
     if k.device != dev or v.device != dev:
-        raise RuntimeError(f"tree_attention: k and v must be on {dev}, got {k.device} and {v.device}")
+        raise RuntimeError(f"{what}: k and v must be on {dev}, got {k.device} and {v.device}")
     if k.dtype != dtype or v.dtype != dtype:
-        raise RuntimeError("tree_attention: q, k and v must have one type")
-    vectors = (_vector("tree_attention", dev, "lens", lens, i32, (B,)),
-               _vector("tree_attention", dev, "parents", parents, i32, (B, n)),
-               0 if counts is None else _vector("tree_attention", dev, "counts", counts, i32, (B,)))
-    return _launch(dev, stream, _tree_call, (q, k, v, vectors, D ** -0.5 if scale is None else scale, out, work))
+        raise RuntimeError(f"{what}: q, k and v must have one type")
+    vectors = (_vector(what, dev, "lens", lens, i32, (B,)) or 0,
+               _vector(what, dev, "parents", parents, i32, (B, n)) or 0,
+               0 if counts is None else _vector(what, dev, "counts", counts, i32, (B,)))
+    if prefix is not None:
+        pk, pv, plen = prefix
+        _no_graph(what, pk, pv)
+        if pk.dim() != 3 or pv.shape != pk.shape or tuple(pk.shape[1:]) != tuple(ks[2:]):
+            raise RuntimeError(f"{what}: pk and pv [rows][{ks[2]}][{D}] expected, got {tuple(pk.shape)}, {tuple(pv.shape)}")
+        if pk.dtype != dtype or pv.dtype != dtype:
+            raise RuntimeError(f"{what}: pk and pv must have q's type")
+        _on(what, dev, "pk", pk)
+        _on(what, dev, "pv", pv)
+        s0, s1, sd = _strides(pk)
+        if (s0, s1, sd) != _strides(pv) or (D > 1 and sd != 1):
+            raise RuntimeError(f"{what}: the dims of a head must be contiguous, and pk and pv strided alike")
+        prefix = (pk.data_ptr(), pv.data_ptr(), s0, s1, pk.shape[0], _vector(what, dev, "prefix_len", plen, i32, (1,)) or 0)
+    return _launch(dev, stream, _tree_call, (what, q, k, v, vectors, D ** -0.5 if scale is None else scale, out, work,
+                                             prefix))
 
 
 def _tree_call(st, args):
-    q, k, v, vectors, scale, out, work = args
+    what, q, k, v, vectors, scale, out, work, prefix = args
     torch = _torch()
     (B, n, H, D), ks, dev = q.shape, k.shape, q.device
     if out is None:
         out = (torch.zeros if vectors[2] else torch.empty)(q.shape, dtype=q.dtype, device=dev)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
-        raise RuntimeError("tree_attention: out must be as q")
+        raise RuntimeError(f"{what}: out must be as q")
     if B == 0:
         return out
     if work is None:
-        work = tree_attention_work(q, k)
+        work = tree_attention_work(q, k) if prefix is None else _prefix_work(q, k, prefix[4])
     elif work.device != dev:
-        raise RuntimeError(f"tree_attention: work is on {work.device}, not on {dev}")
+        raise RuntimeError(f"{what}: work is on {work.device}, not on {dev}")
     elif not work.is_contiguous():
-        raise RuntimeError("tree_attention: the workspace must be contiguous")
+        raise RuntimeError(f"{what}: the workspace must be contiguous")
     q0, q1, q2, qd = _strides(q)
     k0, k1, k2, kd = kv = _strides(k)
     o0, o1, o2, od = _strides(out)
     if kv != _strides(v) or (D > 1 and not qd == kd == od == 1):
-        raise RuntimeError("tree_attention: the dims of a head must be contiguous, and k and v strided alike")
+        raise RuntimeError(f"{what}: the dims of a head must be contiguous, and k and v strided alike")
     packed = _TREE_ATTN.pack(q.data_ptr(), q0, q1, q2, k.data_ptr(), v.data_ptr(), k0, k1, k2, out.data_ptr(), o0, o1, o2,
-                             _elem(q, "tree_attention"), B, n, H, ks[2], D, ks[1], *vectors, scale, work.data_ptr(),
+                             _elem(q, what), B, n, H, ks[2], D, ks[1], *vectors, scale, work.data_ptr(),
                              work.nbytes)
-    status = _lib.btf_tree_attention(packed, st)
+    status = _lib.btf_tree_attention(packed, st) if prefix is None else _lib.btf_prefix_attention(
+        packed, _PREFIX.pack(*prefix), st)
     if status:
-        check(status, "btf_tree_attention")
+        check(status, f"btf_{what}")
     _written(out)
     return out
+
+
+def _prefix_work(q, k, rows):
+    B, n, H, D = q.shape
+    ensure_init(_cuda_device("prefix_attention_work", q).index)
+    torch = _torch()
+    with torch.cuda.device(q.device):
+        size = lib().btf_prefix_attention_work(B, n, H, k.shape[2], D, k.shape[1], rows)
+    if size < 0:
+        check(1, "btf_prefix_attention_work")
+    return torch.empty(size, dtype=torch.uint8, device=q.device)
+
+
+def prefix_attention_work(q, pk, k):
+    """A workspace for prefix_attention calls of these shapes (q [B][n][H][D], pk [rows][HK][D], k [B][n_ctx][HK][D]).
+    Calls that may run at the same time need one each."""
+    return _prefix_work(q, k, pk.shape[0])
+
+
+def prefix_attention(q, pk, pv, k, v, lens, parents, prefix_len=None, counts=None, scale: Optional[float] = None, out=None,
+                     work=None, stream=None):
+    """tree_attention for a batch whose sequences share their first rows (btf_prefix_attention): pk and pv [rows][HK][D]
+    lie in front of every sequence's own k and v, the first prefix_len (int32 [1] on the device; None: all) of them. They
+    are read once for the whole batch. The rest, and its limits, as tree_attention."""
+    return _tree("prefix_attention", q, k, v, lens, parents, counts, scale, out, work, (pk, pv, prefix_len), stream)
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprobs=None, stream=None):

@@ -58,6 +58,7 @@ int gemv_mma_setup(DeviceInfo& d);
 int chain_setup(DeviceInfo& d);
 int sample_setup(DeviceInfo& d);
 int tree_attn_setup(DeviceInfo& d);
+int prefix_attn_setup(DeviceInfo& d);
 int adapters_setup(DeviceInfo& d);
 
 }  // namespace btf
@@ -115,7 +116,8 @@ int btf_init(int device) {
   } else if ((st = gemv_setup(d)) == BTF_OK && (st = gemm_setup(d)) == BTF_OK && (st = gemm_wm_setup(d)) == BTF_OK &&
              (st = gemv_mma_setup(d)) == BTF_OK && (st = chain_setup(d)) == BTF_OK &&
              (st = sample_setup(d)) == BTF_OK &&
-             (st = tree_attn_setup(d)) == BTF_OK && (st = adapters_setup(d)) == BTF_OK) {
+             (st = tree_attn_setup(d)) == BTF_OK && (st = prefix_attn_setup(d)) == BTF_OK &&
+             (st = adapters_setup(d)) == BTF_OK) {
     d.ready = true;
     g_dev[device] = d;
   }

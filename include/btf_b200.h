@@ -694,6 +694,23 @@ int64_t btf_tree_attention_work(int B, int n, int H, int HK, int D, int n_ctx);
 /* q, k, v and o 16-byte aligned, their strides multiples of 8 elements. */
 int btf_tree_attention(const btf_tree_attn* args, void* stream);
 
+/* Attention for a batch whose sequences share their first rows (a system prompt, a document, the prompt of several
+ * answers), which are read once for all of them: btf_tree_attention's sequences, trees and own caches, and in front of
+ * every sequence's own rows the same shared ones. Node i of sequence b attends to the shared rows [0, *len), to the
+ * lens[b] own cached rows, to itself and to its ancestors. Lengths are read on the device: one captured graph serves a
+ * growing batch. What is behind a length is never part of a result. */
+typedef struct btf_prefix {
+  const void* k;       /* [rows][HK][D] of the call's type, 16-byte aligned; NULL when rows is 0 */
+  const void* v;
+  int64_t row, head;   /* strides in elements, multiples of 8 */
+  int rows;            /* 0 .. 2^30 */
+  const int32_t* len;  /* [1] on the device, taken as 0 .. rows; NULL: all rows */
+} btf_prefix;
+/* Workspace bytes of a call with these sizes on the current device (host only; -1 on bad sizes). */
+int64_t btf_prefix_attention_work(int B, int n, int H, int HK, int D, int n_ctx, int prefix_rows);
+/* args as btf_tree_attention's, work of btf_prefix_attention_work(...) bytes. */
+int btf_prefix_attention(const btf_tree_attn* args, const btf_prefix* prefix, void* stream);
+
 /* Draws one token of each of B rows of logits [B][ld] (V values each) from given random numbers. Per row:
  *   w_i = exp((l_i - max l) / temperature)  (temperature <= 0: the first largest logit, as the argmax);
  *   order by (l descending, i ascending); keep the first top_k; of these the shortest prefix whose mass is

@@ -104,3 +104,32 @@ def test_adapters_of_no_row_are_done_and_plans_refuse(btf):
     for args in ((None, 100, 7, P, size), (P, 100, 7, None, size), (P, 100, 7, P + 8, size), (P, 100, 7, P, size - 1)):
         assert L.btf_adapter_plan(*args, None) == 1
     assert L.btf_adapters_work(4, 60, 8, 1, 2) == -1
+
+
+# ---------------------------------------------------------------- attention behind shared rows
+def _prefix(btf, tree=None, **kw):
+    a = dict(q=P, q_batch=1024, q_node=512, q_head=64, k=P, v=P, kv_batch=4096, kv_row=64, kv_head=64, o=P, o_batch=1024,
+             o_node=512, o_head=64, type=1, B=1, n=2, H=8, HK=1, D=64, n_ctx=64, lens=P, parents=P, counts=None,
+             scale=0.125, work=P, work_bytes=1 << 40)
+    a.update(tree or {})
+    s = dict(k=P, v=P, row=64, head=64, rows=100, len=None)
+    s.update(kw)
+    return btf.lib().btf_prefix_attention(ctypes.byref(btf.TreeAttnC(**a)), ctypes.byref(btf.PrefixC(**s)), None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(k=None), dict(v=None), dict(k=P + 8), dict(v=P + 2), dict(row=63), dict(row=-64), dict(row=0), dict(head=4),
+    dict(rows=-1), dict(rows=(1 << 30) + 1), dict(tree=dict(n=65)), dict(tree=dict(q=None)), dict(tree=dict(type=0)),
+    dict(tree=dict(lens=None)), dict(tree=dict(o_head=0)), dict(tree=dict(kv_row=60)), dict(tree=dict(work=None)),
+])
+def test_prefix_attention_refuses(btf, kw):
+    assert _prefix(btf, **kw) == 1, kw
+    assert btf.lib().btf_last_error()
+
+
+def test_prefix_attention_of_no_sequence_is_done(btf):
+    assert _prefix(btf, tree=dict(B=0)) == 0
+    assert btf.lib().btf_prefix_attention(None, None, None) == 1
+    assert btf.lib().btf_prefix_attention_work(1, 65, 8, 1, 64, 64, 10) == -1
+    assert btf.lib().btf_prefix_attention_work(1, 1, 8, 1, 64, 64, -1) == -1
+    assert ctypes.sizeof(btf.PrefixC) == btf._PREFIX.size
