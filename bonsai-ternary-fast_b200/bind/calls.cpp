@@ -1,6 +1,6 @@
-// The ordinary calls of btf_b200.rope, tree_attention and sample, from torch tensors
-// straight to the C ABI: a call of the ctypes mirror spends 6 to 10 us on reading the
-// tensors and packing arguments, more than most of these kernels run. Only what needs no
+// The ordinary calls of btf_b200.rope, tree_attention, prefix_attention, adapters and sample,
+// from torch tensors straight to the C ABI: a call of the ctypes mirror spends 6 to 15 us on
+// reading the tensors and packing arguments, more than most of these kernels run. Only what needs no
 // thought is done here: tensors of the expected types and shapes on the current
 // device, its current stream. Everything else, errors among it, returns None, and the
 // mirror does the call (nothing has been launched then).
@@ -27,6 +27,10 @@ struct Library {
   decltype(&btf_tree_attention) tree = nullptr;
   decltype(&btf_sample) sample = nullptr;
   decltype(&btf_rope_axes) rope_axes = nullptr;
+  decltype(&btf_prefix_attention_work) prefix_work = nullptr;
+  decltype(&btf_prefix_attention) prefix = nullptr;
+  decltype(&btf_adapters_work) adapters_work = nullptr;
+  decltype(&btf_adapters) adapters = nullptr;
 } lib;
 
 // A refused fast call: caught below, becomes None.
@@ -125,6 +129,7 @@ PyObject* attempt(Fn fn) {
 }
 
 PyObject *s_x, *s_y, *s_normw, *s_rotate, *s_rows, *s_turns, *s_n_rot, *s_mscale, *s_interleaved, *s_axis, *s_n_axes;
+PyObject *s_a, *s_b, *s_base, *s_plan, *s_T, *s_n_adapters;
 
 // rope(segs, table, pos, inverse, eps) -> True, or None
 PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -190,10 +195,9 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// tree_attention(q, k, v, lens, parents, counts, scale, out, work) -> the output, or None
-PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+// Both attentions. args: q, k, v, lens, parents, counts, scale, out, work; shared: pk, pv, prefix_len or null.
+PyObject* attention(PyObject* const* args, PyObject* const* shared) {
   return attempt([&]() -> PyObject* {
-    if (nargs != 9) throw Other{};
     const int dev = device();
     const at::Tensor &q = plain(on(args[0], dev)), &k = plain(on(args[1], dev)), &v = plain(on(args[2], dev));
     if (q.dim() != 4 || k.dim() != 4 || v.sizes() != k.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3) ||
@@ -203,6 +207,15 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     for (int64_t s : {B, n, H, D, ctx, HK})
       if (s < 1 || s > INT32_MAX) throw Other{};
     if (args[3] == Py_None || args[4] == Py_None) throw Other{};
+    btf_prefix s{};
+    if (shared) {
+      const at::Tensor &pk = plain(on(shared[0], dev)), &pv = plain(on(shared[1], dev));
+      if (pk.dim() != 3 || pv.sizes() != pk.sizes() || pk.size(1) != HK || pk.size(2) != D || pk.size(0) > INT32_MAX ||
+          pk.scalar_type() != q.scalar_type() || pv.scalar_type() != q.scalar_type() ||
+          stride(pk, 0) != stride(pv, 0) || stride(pk, 1) != stride(pv, 1) || (D > 1 && (pk.stride(2) != 1 || pv.stride(2) != 1)))
+        throw Other{};
+      s = {pk.data_ptr(), pv.data_ptr(), stride(pk, 0), stride(pk, 1), (int)pk.size(0), vec<int32_t>(shared[2], dev, at::kInt, 1)};
+    }
     btf_tree_attn a{};
     a.lens = vec<int32_t>(args[3], dev, at::kInt, B);
     a.parents = vec<int32_t>(args[4], dev, at::kInt, B, n);
@@ -218,7 +231,8 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       work = on(args[8], dev);
       if (!work.is_contiguous()) throw Other{};
     } else {
-      const int64_t bytes = lib.tree_work((int)B, (int)n, (int)H, (int)HK, (int)D, (int)ctx);
+      const int64_t bytes = shared ? lib.prefix_work((int)B, (int)n, (int)H, (int)HK, (int)D, (int)ctx, s.rows)
+                                   : lib.tree_work((int)B, (int)n, (int)H, (int)HK, (int)D, (int)ctx);
       if (bytes < 0) throw Other{};
       work = at::empty({bytes}, q.options().dtype(at::kByte));
     }
@@ -233,13 +247,110 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.B = (int)B, a.n = (int)n, a.H = (int)H, a.HK = (int)HK, a.D = (int)D, a.n_ctx = (int)ctx;
     a.scale = args[6] == Py_None ? (float)(1.0 / std::sqrt((double)D)) : (float)number(args[6]);
     a.work = work.data_ptr(), a.work_bytes = (int64_t)work.nbytes();
-    if (lib.tree(&a, stream_of(dev))) throw Other{};
+    if (shared ? lib.prefix(&a, &s, stream_of(dev)) : lib.tree(&a, stream_of(dev))) throw Other{};
     written(out);
     if (args[7] != Py_None) {
       Py_INCREF(args[7]);
       return args[7];
     }
     return THPVariable_Wrap(out);
+  });
+}
+// tree_attention(q, k, v, lens, parents, counts, scale, out, work) -> the output, or None
+PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 9) Py_RETURN_NONE;
+  return attention(args, nullptr);
+}
+// prefix_attention(q, k, v, lens, parents, counts, scale, out, work, pk, pv, prefix_len) -> the output, or None
+PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 12) Py_RETURN_NONE;
+  return attention(args, args + 9);
+}
+
+// adapters(x, segs, plan, ranks, scales, work) -> the list of y, or None
+PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return attempt([&]() -> PyObject* {
+    if (nargs != 6 || !PyList_Check(args[1])) throw Other{};
+    const Py_ssize_t nseg = PyList_GET_SIZE(args[1]);
+    if (nseg < 1 || nseg > 3) throw Other{};
+    const int dev = device();
+    const at::Tensor& x = plain(on(args[0], dev));
+    if (x.dim() != 2 || x.size(0) < 1 || x.size(0) > INT32_MAX || x.size(1) > INT32_MAX || (x.size(1) > 1 && x.stride(1) != 1))
+      throw Other{};
+    Kept kept;
+    PyObject* oT = kept.attr(args[2], s_T);
+    PyObject* on_ = kept.attr(args[2], s_n_adapters);
+    const long T = PyLong_AsLong(oT), n = PyLong_AsLong(on_);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      throw Other{};
+    }
+    const at::Tensor& plan = on(kept.attr(args[2], s_plan), dev);
+    if (T != x.size(0) || n < 1 || n > INT32_MAX || !plan.is_contiguous()) throw Other{};
+    btf_adapters_args a{};
+    at::Tensor out[3];
+    PyObject* given[3];
+    int64_t R = 0;
+    bool typed = false;
+    at::ScalarType y_type = x.scalar_type(), w_type = y_type;
+    for (Py_ssize_t i = 0; i < nseg; ++i) {
+      if (i >= PyList_GET_SIZE(args[1])) throw Other{};
+      PyObject* s = kept.keep(PyList_GET_ITEM(args[1], i));
+      PyObject *oa = kept.attr(s, s_a), *ob = kept.attr(s, s_b), *oy = kept.attr(s, s_y), *obase = kept.attr(s, s_base);
+      const at::Tensor &wa = plain(on(oa, dev)), &wb = plain(on(ob, dev));
+      if (wa.dim() != 3 || wb.dim() != 3) throw Other{};
+      if (i == 0) R = wa.size(1), w_type = wa.scalar_type();
+      const int64_t N = wb.size(1);
+      if (wa.size(0) != n || wa.size(1) != R || wa.size(2) != x.size(1) || wb.size(0) != n || wb.size(2) != R ||
+          wa.stride(2) != 1 || wb.stride(2) != 1 || wa.scalar_type() != w_type || wb.scalar_type() != w_type || R > INT32_MAX ||
+          N < 1 || N > INT32_MAX)
+        throw Other{};
+      const at::Tensor* two[2] = {oy == Py_None ? nullptr : &plain(on(oy, dev)), obase == Py_None ? nullptr : &plain(on(obase, dev))};
+      for (const at::Tensor* t : two) {
+        if (!t) continue;
+        if (t->dim() != 2 || t->size(0) != T || t->size(1) != N || (N > 1 && t->stride(1) != 1)) throw Other{};
+        if (typed && t->scalar_type() != y_type) throw Other{};
+        typed = true, y_type = t->scalar_type();
+      }
+      given[i] = oy;
+      if (two[0]) out[i] = *two[0];
+      btf_adapter_seg& c = a.segs[i];
+      c = {wa.data_ptr(), wa.stride(0), wa.stride(1), wb.data_ptr(), wb.stride(0), wb.stride(1), (int)N,
+           two[1] ? two[1]->data_ptr() : nullptr, two[1] ? two[1]->stride(0) : 0, nullptr, 0};
+    }
+    for (Py_ssize_t i = 0; i < nseg; ++i) {
+      if (!out[i].defined()) out[i] = at::empty({T, a.segs[i].N}, x.options().dtype(y_type));
+      a.segs[i].y = out[i].data_ptr(), a.segs[i].y_row = out[i].stride(0);
+    }
+    a.x = x.data_ptr(), a.x_row = x.stride(0);
+    a.x_type = elem(x), a.w_type = w_type == at::kHalf ? BTF_F16 : w_type == at::kBFloat16 ? BTF_BF16 : BTF_F32;
+    a.y_type = elem(out[0]);
+    a.T = (int)T, a.K = (int)x.size(1), a.R = (int)R, a.n_adapters = (int)n, a.nseg = (int)nseg;
+    a.ranks = vec<int32_t>(args[3], dev, at::kInt, n);
+    a.scales = vec<float>(args[4], dev, at::kFloat, n);
+    if (args[4] != Py_None) plain(tensor(args[4]));
+    a.plan = plan.data_ptr(), a.plan_bytes = (int64_t)plan.nbytes();
+    at::Tensor work;
+    if (args[5] != Py_None) {
+      work = on(args[5], dev);
+      if (!work.is_contiguous()) throw Other{};
+    } else {
+      const int64_t bytes = lib.adapters_work(a.T, a.K, a.R, a.nseg, a.n_adapters);
+      if (bytes < 0) throw Other{};
+      work = at::empty({bytes}, x.options().dtype(at::kByte));
+    }
+    a.work = work.data_ptr(), a.work_bytes = (int64_t)work.nbytes();
+    if (lib.adapters(&a, stream_of(dev))) throw Other{};
+    PyObject* r = PyList_New(nseg);
+    if (!r) return nullptr;
+    for (Py_ssize_t i = 0; i < nseg; ++i) {
+      written(out[i]);
+      PyObject* y = given[i];
+      if (y != Py_None) Py_INCREF(y);
+      else y = THPVariable_Wrap(out[i]);
+      PyList_SET_ITEM(r, i, y);
+    }
+    return r;
   });
 }
 
@@ -288,19 +399,24 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// bind(rope, tree_attention_work, tree_attention, sample, rope_axes): addresses in the loaded library
+// bind(rope, tree_attention_work, tree_attention, sample, rope_axes, prefix_attention_work, prefix_attention,
+// adapters_work, adapters): addresses in the loaded library
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[5];
-  if (!PyArg_ParseTuple(args, "KKKKK", &a[0], &a[1], &a[2], &a[3], &a[4])) return nullptr;
-  lib = {reinterpret_cast<decltype(lib.rope)>(a[0]), reinterpret_cast<decltype(lib.tree_work)>(a[1]),
-         reinterpret_cast<decltype(lib.tree)>(a[2]), reinterpret_cast<decltype(lib.sample)>(a[3]),
-         reinterpret_cast<decltype(lib.rope_axes)>(a[4])};
+  unsigned long long a[9];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8])) return nullptr;
+  lib = {reinterpret_cast<decltype(lib.rope)>(a[0]),         reinterpret_cast<decltype(lib.tree_work)>(a[1]),
+         reinterpret_cast<decltype(lib.tree)>(a[2]),         reinterpret_cast<decltype(lib.sample)>(a[3]),
+         reinterpret_cast<decltype(lib.rope_axes)>(a[4]),    reinterpret_cast<decltype(lib.prefix_work)>(a[5]),
+         reinterpret_cast<decltype(lib.prefix)>(a[6]),       reinterpret_cast<decltype(lib.adapters_work)>(a[7]),
+         reinterpret_cast<decltype(lib.adapters)>(a[8])};
   Py_RETURN_NONE;
 }
 
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
                          {"rope", (PyCFunction)(void (*)(void))rope, METH_FASTCALL, nullptr},
                          {"tree_attention", (PyCFunction)(void (*)(void))tree_attention, METH_FASTCALL, nullptr},
+                         {"prefix_attention", (PyCFunction)(void (*)(void))prefix_attention, METH_FASTCALL, nullptr},
+                         {"adapters", (PyCFunction)(void (*)(void))adapters, METH_FASTCALL, nullptr},
                          {"sample", (PyCFunction)(void (*)(void))sample, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "btf_b200_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -319,6 +435,12 @@ PyMODINIT_FUNC PyInit_btf_b200_calls() {
   s_interleaved = PyUnicode_InternFromString("interleaved");
   s_axis = PyUnicode_InternFromString("axis");
   s_n_axes = PyUnicode_InternFromString("n_axes");
+  s_a = PyUnicode_InternFromString("a");
+  s_b = PyUnicode_InternFromString("b");
+  s_base = PyUnicode_InternFromString("base");
+  s_plan = PyUnicode_InternFromString("plan");
+  s_T = PyUnicode_InternFromString("T");
+  s_n_adapters = PyUnicode_InternFromString("n_adapters");
   PyObject* m = PyModule_Create(&module);
   if (m && PyModule_AddStringConstant(m, "torch_version", BTF_TORCH_VERSION)) {  // the mirror binds it to no other
     Py_DECREF(m);

@@ -707,7 +707,8 @@ def _bind_calls() -> None:
         spec.loader.exec_module(calls)
         if calls.torch_version == torch.__version__:
             calls.bind(*(ctypes.cast(getattr(lib(), n), ctypes.c_void_p).value
-                         for n in ("btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample", "btf_rope_axes")))
+                         for n in ("btf_rope", "btf_tree_attention_work", "btf_tree_attention", "btf_sample", "btf_rope_axes",
+                                   "btf_prefix_attention_work", "btf_prefix_attention", "btf_adapters_work", "btf_adapters")))
             _calls = calls
     except Exception:  # whatever keeps it from loading
         pass
@@ -975,6 +976,10 @@ def adapters(x, segs: Sequence[AdapterSeg], plan: AdapterPlan, ranks=None, scale
     scales[a] (x A_a^T) B_a^T with each row's adapter a of the plan, by the first ranks[a] (int32 [n_adapters], None: R) of
     its rank; scales float32 [n_adapters] or None. Returns the y. No graph is recorded: tensors that require a gradient
     are refused outside torch.no_grad()."""
+    if stream is None and _calls is not None:
+        done = _calls.adapters(x, segs, plan, ranks, scales, work)
+        if done is not None:
+            return done
     torch = _torch()
     if not 1 <= len(segs) <= 3:
         raise RuntimeError(f"adapters: 1..3 projections expected, got {len(segs)}")
@@ -1157,6 +1162,10 @@ def prefix_attention(q, pk, pv, k, v, lens, parents, prefix_len=None, counts=Non
     """tree_attention for a batch whose sequences share their first rows (btf_prefix_attention): pk and pv [rows][HK][D]
     lie in front of every sequence's own k and v, the first prefix_len (int32 [1] on the device; None: all) of them. They
     are read once for the whole batch. The rest, and its limits, as tree_attention."""
+    if stream is None and _calls is not None:
+        done = _calls.prefix_attention(q, k, v, lens, parents, counts, scale, out, work, pk, pv, prefix_len)
+        if done is not None:
+            return done
     return _tree("prefix_attention", q, k, v, lens, parents, counts, scale, out, work, (pk, pv, prefix_len), stream)
 
 
