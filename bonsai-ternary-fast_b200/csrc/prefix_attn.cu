@@ -36,7 +36,8 @@ struct Split {
   int ranges;                // of the own rows
   __device__ __forceinline__ explicit Split(const PrefixParams& p) {
     const int lane = threadIdx.x & 31;
-    int own = 0;
+    len = p.prefix_len ? min(max(*p.prefix_len, 0), p.prefix_rows) : p.prefix_rows;
+    int own = 0, pairs = 0;  // tiles of the own rows of a kv-head, sequences with any
     nodes = 0;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
       Seq s;
@@ -44,22 +45,28 @@ struct Split {
       if (b0 + lane < p.B) s = Seq(p, b0 + lane);
       nodes += __reduce_add_sync(0xffffffffu, s.count);
       own += __reduce_add_sync(0xffffffffu, s.tiles);
+      pairs += __popc(__ballot_sync(0xffffffffu, s.tiles > 0));
     }
-    len = p.prefix_len ? min(max(*p.prefix_len, 0), p.prefix_rows) : p.prefix_rows;
     tiles = (len + kTile - 1) / kTile;
     mtiles = (int)(((int64_t)nodes * (p.H / p.HK) + kRowsM - 1) / kRowsM);
     chunks = ctas = 0;
     ranges = p.ctas / p.mtiles;
     if (tiles == 0 || mtiles == 0) return;
     // lane i: the shared rows of each (kv-head, M tile) in i + 1 stretches
-    const float streams = (float)p.HK * (float)mtiles, shared = streams * (float)tiles, mine = (float)p.HK * (float)p.mtiles * (float)own;
+    const float streams = (float)p.HK * (float)mtiles;
+    const float mine = (float)p.HK * (float)p.mtiles * ((float)own + kSegTiles * (float)pairs);
+    // and what the slowest CTA then has, with the CTAs shared out so that both kinds end together: in w turns over
+    // the shared rows' items, rounded down or up
     const int n = min(lane + 1, min(p.most_chunks, tiles));
     const float items = streams * (float)n, each = ceilf((float)tiles / (float)n) + kSegTiles;
-    const float most = (float)(p.ctas - p.mtiles);
-    const float ideal = fminf(most, fmaxf(1.0f, (float)p.ctas * shared / (shared + mine)));
-    const float turns = fmaxf(1.0f, rintf(items / ideal));
-    const float take = fminf(most, ceilf(items / turns));
-    const float cost = fmaxf(ceilf(items / take) * each, ceilf(mine / ((float)p.ctas - take)) + kSegTiles);
+    const float most = (float)(p.ctas - p.mtiles), w = floorf((mine + items * each) / (each * (float)p.ctas));
+    float take = 0.f, cost = INFINITY;
+#pragma unroll
+    for (int up = 0; up < 2; ++up) {
+      const float t = fminf(most, ceilf(items / fmaxf(1.0f, w + (float)up)));
+      const float c = fmaxf(ceilf(items / t) * each, mine / ((float)p.ctas - t));
+      if (c < cost) cost = c, take = t;
+    }
     const uint32_t best = __reduce_min_sync(0xffffffffu, __float_as_uint(cost));
     const int l = __ffs(__ballot_sync(0xffffffffu, __float_as_uint(cost) == best)) - 1;
     chunks = __shfl_sync(0xffffffffu, n, l);
