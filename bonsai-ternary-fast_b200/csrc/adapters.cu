@@ -27,31 +27,14 @@
 // of two of its row, which keeps fp16's range.
 #include <algorithm>
 
-#include "elem.cuh"
+#include "adapters_tc.cuh"
 
 namespace btf {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kSmall = 16, kLarge = 64;  // rows of a tile
-constexpr int kMaxSplits = 16;
-constexpr int kErrPlan = 2;  // device error word: a plan of other sizes
+using namespace adapt;
 
-struct Tile {
-  int adapter, begin, count, unused;  // adapter -1: rows without one
-};
-// The plan in memory: 8 words {T, adapters, small tiles, large tiles, rows with an
-// adapter}, the rows in order, then both lists of tiles.
-struct PlanLayout {
-  int64_t order, small, large, bytes;
-  PlanLayout(int64_t T, int64_t n) {
-    const int64_t lists = std::min(n + 1, T) + 1;
-    order = 32;
-    small = (order + 4 * T + 15) / 16 * 16;
-    large = small + 16 * (T / kSmall + lists);
-    bytes = large + 16 * (T / kLarge + lists);
-  }
-};
+constexpr int kThreads = 256, kExpand = 64;
 
 // ------------------------------------------------------------------ plan
 // One CTA. Warp w counts and later places its own stretch of the rows, so that the
@@ -128,35 +111,6 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t* index
   });
 }
 
-// ------------------------------------------------------------------ the call
-struct Seg {
-  const void *a, *b, *base;
-  void* y;
-  int64_t a_adapter, a_row, b_adapter, b_row, base_row, y_row;
-  int N;
-  int vec;  // y (and base) take whole 16-byte words
-};
-struct Params {
-  Seg seg[3];
-  const void* x;
-  int64_t x_row;
-  int T, K, R, n, nseg, splits, ranges;
-  const int32_t* ranks;
-  const float* scales;
-  const int32_t *head, *order;
-  const Tile* tiles;
-  int which;  // the plan's word with the number of tiles
-  float* h;   // [splits][nseg][T][R]
-  int* err;
-};
-
-__device__ __forceinline__ bool plan_ok(const Params& p) {
-  if (p.head[0] == p.T && p.head[1] == p.n) return true;
-  if (blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.err, 0, kErrPlan);
-  return false;
-}
-__device__ __forceinline__ int rank_of(const Params& p, int a) { return p.ranks ? min(max(p.ranks[a], 0), p.R) : p.R; }
-
 template <typename T>
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                       uint32_t b1) {
@@ -178,34 +132,6 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1
 __device__ __forceinline__ uint4 ld16(const void* p, bool on) {
   return on ? __ldg(static_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
 }
-// What `shrink` wrote: never from L1, and in its place behind the wait.
-__device__ __forceinline__ float4 ld_cg(const float* p) {
-  float4 v;
-  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, __half>) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if constexpr (std::is_same_v<T, __half>) {
-    const __half2 h = *reinterpret_cast<const __half2*>(&w);
-    return __half22float2(h);
-  } else {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  }
-}
-// What is left of v behind its first term (0 behind an infinity, not inf - inf).
-__device__ __forceinline__ float rest(float v, float term) { return v == term ? 0.f : v - term; }
-
 // 8 consecutive elements of x as the B operands of a step: TERMS x 4 words of 16-bit pairs, or (fp32 x, fp16 weights)
 // 2 x 8 tf32 values.
 template <typename TX, typename TW>
@@ -230,10 +156,14 @@ __global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XFrag<TX, TW>
   pdl_wait();
   pdl_launch_dependents();  // (behind the wait: `expand` reads the plan before its own)
   if (!plan_ok(p)) return;
-  const int split = blockIdx.x % p.splits, seg = blockIdx.x / p.splits % p.nseg, ti = blockIdx.x / (p.splits * p.nseg);
+  constexpr int kParts = RG == 1 ? 1 : kLarge / kRows;  // of a tile
+  const int split = blockIdx.x % p.splits, seg = blockIdx.x / p.splits % p.nseg, part = blockIdx.x / (p.splits * p.nseg);
+  const int ti = part / kParts;
   if (ti >= p.head[p.which]) return;
-  const Tile tile = p.tiles[ti];
-  if (tile.adapter < 0) return;
+  Tile tile = p.tiles[ti];
+  tile.begin += part % kParts * kRows;
+  tile.count = min(tile.count - part % kParts * kRows, kRows);
+  if (tile.adapter < 0 || tile.count <= 0) return;
   const int rank = rank_of(p, tile.adapter);
   if (rank == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -359,16 +289,16 @@ __global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XFrag<TX, TW>
 }
 
 // ------------------------------------------------------------------ expand
-// A CTA takes a tile's rows, one projection and a stretch of its N outputs, 32 at a time per warp (and group of MT x
-// 16 rows). h's terms lie in shared memory as the MMA's A operands, 16 bytes a lane; the weights are its 8-wide side,
-// with the rows of B so assigned that a lane ends up with 8 consecutive outputs of a row.
-template <typename TW, typename TY, int MT, int RG, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) adapter_expand_kernel(const __grid_constant__ Params p) {
+// Few rows: a CTA takes a tile's 16 rows and a stretch of the outputs of all projections, 32 at a time per warp. h's
+// terms lie in shared memory as the MMA's A operands, 16 bytes a lane; the weights are its 8-wide side, with the rows of
+// B so assigned that a lane ends up with 8 consecutive outputs of a row. (Prompts: adapters_tc.cu.)
+template <typename TW, typename TY>
+__global__ void __launch_bounds__(kExpand, 8) adapter_expand_kernel(const __grid_constant__ Params p) {
   constexpr bool kHalf = std::is_same_v<TW, __half>, kY32 = std::is_same_v<TY, float>;
   constexpr int kTerms = !kHalf && kY32 ? 3 : 2;
-  constexpr int kWidth = WARPS * 32 / RG, kRows = RG * MT * 16, kThr = WARPS * 32;  // kWidth: outputs of a piece
+  constexpr int kRows = kSmall;
   constexpr int kYWords = 8 * (int)sizeof(TY) / 16;  // 16-byte words of a lane's 8 outputs
-  extern __shared__ uint4 frag[];  // [RG * MT][k32 blocks][2][terms][32]
+  extern __shared__ uint4 frag[];  // [k32 blocks][2][terms][32]
   __shared__ float mul[kRows];
   __shared__ int top[kRows];
   // The plan, the weights and base were complete before `shrink` let this grid start.
@@ -386,27 +316,22 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) adapter_expand_kernel(
   const Tile tile = p.tiles[ti];
   const int rank = tile.adapter < 0 ? 0 : rank_of(p, tile.adapter);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int rg = warp % RG, nw = warp / RG, blocks = (rank + 31) / 32;
+  const int blocks = (rank + 31) / 32;
   // the CTA's pieces, of all projections in a line
-  auto pieces = [&](int i) { return (p.seg[i].N + kWidth - 1) / kWidth; };
+  auto pieces = [&](int i) { return (p.seg[i].N + kExpand - 1) / kExpand; };
   int total = 0;
   for (int i = 0; i < p.nseg; ++i) total += pieces(i);
   const int first = (int)((int64_t)range * total / p.ranges), last = (int)((int64_t)(range + 1) * total / p.ranges);
   int seg = 0, before = 0;  // pieces of the projections before seg
-  int row[MT][2];
+  int row[2];
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = (rg * MT + m) * 16 + e * 8 + g;
-      row[m][e] = r < tile.count ? p.order[tile.begin + r] : -1;
-    }
+  for (int e = 0; e < 2; ++e) row[e] = e * 8 + g < tile.count ? p.order[tile.begin + e * 8 + g] : -1;
   bool waited = false;
   int have = -1;  // the projection whose h lies in shared memory
   for (int piece = first; piece < last; ++piece) {
     for (int k; piece - before >= (k = pieces(seg)); ++seg) before += k;
     const Seg& s = p.seg[seg];
-    const int n0 = (piece - before) * kWidth + nw * 32;
+    const int n0 = (piece - before) * kExpand + warp * 32;
     const bool copy = rank == 0;
     if (copy && s.base == s.y && s.base_row == s.y_row) continue;  // in place: stays
     // weights of the first k32 block and base on their way before h is looked at
@@ -428,17 +353,15 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) adapter_expand_kernel(
     uint4 wb[4];
     load_b(wb, 0);
     const int n8 = n0 + 8 * t;  // the lane's outputs
-    uint4 bv[MT][2][kYWords];
+    uint4 bv[2][kYWords];
     const bool vec = s.vec && n8 + 8 <= s.N;
     if (s.base && vec) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int w = 0; w < kYWords; ++w)
-            bv[m][e][w] = row[m][e] >= 0 ? *(reinterpret_cast<const uint4*>(static_cast<const TY*>(s.base) + row[m][e] * s.base_row + n8) + w)
-                                         : make_uint4(0, 0, 0, 0);
+        for (int w = 0; w < kYWords; ++w)
+          bv[e][w] = row[e] >= 0 ? *(reinterpret_cast<const uint4*>(static_cast<const TY*>(s.base) + row[e] * s.base_row + n8) + w)
+                                 : make_uint4(0, 0, 0, 0);
     }
     if (!waited) {
       pdl_wait();
@@ -467,9 +390,9 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) adapter_expand_kernel(
           if (k + i >= rank) v[i] = 0.f;
       };
       if constexpr (kHalf) {  // each row over a power of two: its largest in [2^14, 2^15)
-        for (int r = threadIdx.x; r < kRows; r += kThr) top[r] = 0;
+        for (int r = threadIdx.x; r < kRows; r += kExpand) top[r] = 0;
         __syncthreads();
-        for (int u = threadIdx.x; u < kRows * chunks; u += kThr) {
+        for (int u = threadIdx.x; u < kRows * chunks; u += kExpand) {
           float v[8];
           sum(u, v);
           float m = 0.f;
@@ -480,7 +403,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) adapter_expand_kernel(
         __syncthreads();
       }
       const float scale = p.scales ? p.scales[tile.adapter] : 1.f;
-      for (int r = threadIdx.x; r < kRows; r += kThr) {
+      for (int r = threadIdx.x; r < kRows; r += kExpand) {
         if constexpr (kHalf) {
           const int e = (top[r] >> 23) - 127;  // of the largest; 0, denormal and infinite rows stay as they are
           mul[r] = e >= -112 && e < 128 ? scale * __int_as_float((e - 14 + 127) << 23) : scale;
@@ -488,7 +411,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) adapter_expand_kernel(
           mul[r] = scale;
         }
       }
-      for (int u = threadIdx.x; u < kRows * chunks; u += kThr) {
+      for (int u = threadIdx.x; u < kRows * chunks; u += kExpand) {
         float v[8];
         sum(u, v);
         const int r = u / chunks, k = u % chunks;
@@ -499,8 +422,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) adapter_expand_kernel(
           for (int i = 0; i < 8; ++i) v[i] *= f;
         }
         // row r of its 16: g = r % 8, words 0 and 2 (r < 8) or 1 and 3
-        uint32_t* to = reinterpret_cast<uint32_t*>(frag + ((int64_t)((r >> 4) * blocks + (k >> 2)) * 2 * kTerms) * 32 +
-                                                   (r & 7) * 4 + (k & 3)) + ((r >> 3) & 1);
+        uint32_t* to = reinterpret_cast<uint32_t*>(frag + (k >> 2) * 2 * kTerms * 32 + (r & 7) * 4 + (k & 3)) + (r >> 3);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v0 = v[2 * i], v1 = v[2 * i + 1];
@@ -515,73 +437,62 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) adapter_expand_kernel(
       }
       __syncthreads();
     }
-    float c[MT][4][4];
+    float c[4][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) c[m][j][0] = c[m][j][1] = c[m][j][2] = c[m][j][3] = 0.f;
+    for (int j = 0; j < 4; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
 #pragma unroll 1
     for (int kb = 0; kb < blocks; ++kb) {
       uint4 wn[4];
-      if (MT == 1 && kb + 1 < blocks) load_b(wn, kb + 1);
+      if (kb + 1 < blocks) load_b(wn, kb + 1);
+      const uint4* f = frag + (int64_t)kb * 2 * kTerms * 32 + lane;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint4* f = frag + ((int64_t)((rg * MT + m) * blocks + kb) * 2 * kTerms) * 32 + lane;
+      for (int e = kTerms - 1; e >= 0; --e) {
+        const uint4 a0 = f[e * 32], a1 = f[(kTerms + e) * 32];
 #pragma unroll
-        for (int e = kTerms - 1; e >= 0; --e) {
-          const uint4 a0 = f[e * 32], a1 = f[(kTerms + e) * 32];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mma16<TW>(c[m][j], a0.x, a0.y, a0.z, a0.w, wb[j].x, wb[j].y);
-            mma16<TW>(c[m][j], a1.x, a1.y, a1.z, a1.w, wb[j].z, wb[j].w);
-          }
+        for (int j = 0; j < 4; ++j) {
+          mma16<TW>(c[j], a0.x, a0.y, a0.z, a0.w, wb[j].x, wb[j].y);
+          mma16<TW>(c[j], a1.x, a1.y, a1.z, a1.w, wb[j].z, wb[j].w);
         }
       }
-      if constexpr (MT == 1) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) wb[j] = wn[j];
-      } else if (kb + 1 < blocks) {  // (no registers for the next weights beside these)
-        load_b(wb, kb + 1);
-      }
+      for (int j = 0; j < 4; ++j) wb[j] = wn[j];
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int e = 0; e < 2; ++e) {
+      if (row[e] < 0) continue;
+      const float f = copy ? 0.f : mul[e * 8 + g];
+      float v[8];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (row[m][e] < 0) continue;
-        const float f = copy ? 0.f : mul[(rg * MT + m) * 16 + e * 8 + g];
-        float v[8];
+      for (int j = 0; j < 4; ++j) v[2 * j] = c[j][2 * e] * f, v[2 * j + 1] = c[j][2 * e + 1] * f;
+      TY* y = static_cast<TY*>(s.y) + row[e] * s.y_row + n8;
+      if (vec) {
+        if (s.base) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[2 * j] = c[m][j][2 * e] * f, v[2 * j + 1] = c[m][j][2 * e + 1] * f;
-        TY* y = static_cast<TY*>(s.y) + row[m][e] * s.y_row + n8;
-        if (vec) {
-          if (s.base) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if constexpr (kY32) {
-                const uint4 w = bv[m][e][i >> 1];
-                v[2 * i] += __uint_as_float(i & 1 ? w.z : w.x), v[2 * i + 1] += __uint_as_float(i & 1 ? w.w : w.y);
-              } else {
-                const uint4 w = bv[m][e][0];
-                const float2 q = unpack2<TY>(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w);
-                v[2 * i] += q.x, v[2 * i + 1] += q.y;
-              }
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (kY32) {
+              const uint4 w = bv[e][i >> 1];
+              v[2 * i] += __uint_as_float(i & 1 ? w.z : w.x), v[2 * i + 1] += __uint_as_float(i & 1 ? w.w : w.y);
+            } else {
+              const uint4 w = bv[e][0];
+              const float2 q = unpack2<TY>(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w);
+              v[2 * i] += q.x, v[2 * i + 1] += q.y;
             }
           }
-          if constexpr (kY32) {
-            reinterpret_cast<float4*>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
-          } else {
-            *reinterpret_cast<uint4*>(y) = make_uint4(pack2<TY>(v[0], v[1]), pack2<TY>(v[2], v[3]), pack2<TY>(v[4], v[5]),
-                                                      pack2<TY>(v[6], v[7]));
-          }
-        } else {
-          const TY* base = s.base ? static_cast<const TY*>(s.base) + row[m][e] * s.base_row + n8 : nullptr;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (n8 + i < s.N) y[i] = from_f32<TY>(base ? v[i] + to_f32(base[i]) : v[i]);
         }
+        if constexpr (kY32) {
+          reinterpret_cast<float4*>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4*>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          *reinterpret_cast<uint4*>(y) = make_uint4(pack2<TY>(v[0], v[1]), pack2<TY>(v[2], v[3]), pack2<TY>(v[4], v[5]),
+                                                    pack2<TY>(v[6], v[7]));
+        }
+      } else {
+        const TY* base = s.base ? static_cast<const TY*>(s.base) + row[e] * s.base_row + n8 : nullptr;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (n8 + i < s.N) y[i] = from_f32<TY>(base ? v[i] + to_f32(base[i]) : v[i]);
       }
+    }
   }
   if (!waited) pdl_wait();
 }
@@ -592,7 +503,7 @@ bool sizes_ok(int T, int K, int R, int nseg, int n) {
          R <= BTF_ADAPTERS_MAX_RANK && nseg >= 1 && nseg <= 3 && n >= 1 && n <= BTF_ADAPTERS_MAX;
 }
 
-// Tiles of 16 rows while the adapters' rows are few, of 64 for prompts.
+// Tiles of 16 rows while the adapters' rows are few, of 128 for prompts.
 struct Shape {
   bool large;
   int tiles;   // at most
@@ -604,7 +515,7 @@ Shape shape_of(const DeviceInfo& d, int T, int K, int nseg, int n) {
   const int rows = s.large ? kLarge : kSmall;
   s.tiles = T / rows + std::min(n + 1, T);
   const int steps = (K + 31) / 32, warps = s.large ? 4 : 8;  // that share a CTA's stretch
-  const int want = 2 * d.sm_count / (s.tiles * nseg);
+  const int want = 2 * d.sm_count / (s.tiles * nseg * (s.large ? 2 : 1));
   s.splits = std::max(1, std::min({want, kMaxSplits, (steps + warps - 1) / warps}));
   return s;
 }
@@ -615,7 +526,7 @@ cudaError_t shrink(const Params& p, int tiles, cudaStream_t st, bool setup) {
   constexpr int smem = 8 / RG * (RG * NT * 8) * (RT * 16 + 4) * 4;
   if (setup)
     return cudaFuncSetAttribute(adapter_shrink_kernel<TX, TW, RT, NT, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  return launch_pdl(adapter_shrink_kernel<TX, TW, RT, NT, RG>, dim3((unsigned)(tiles * p.nseg * p.splits)), dim3(kThreads),
+  return launch_pdl(adapter_shrink_kernel<TX, TW, RT, NT, RG>, dim3((unsigned)(tiles * p.nseg * p.splits * (RG == 1 ? 1 : kLarge / (RG * NT * 8)))), dim3(kThreads),
                     smem, st, p);
 }
 template <typename TX, typename TW, int RT>
@@ -642,26 +553,14 @@ cudaError_t shrink_setup() {
   return cudaSuccess;
 }
 
-template <typename TW, typename TY, int MT, int RG, int WARPS>
-cudaError_t expand(Params p, int tiles, int ctas, cudaStream_t st, bool setup) {
-  constexpr int terms = std::is_same_v<TW, __half> || !std::is_same_v<TY, float> ? 2 : 3;
-  auto smem = [&](int R) { return RG * MT * ((R + 31) / 32) * 2 * terms * 512; };
-  if (setup)
-    return cudaFuncSetAttribute(adapter_expand_kernel<TW, TY, MT, RG, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                smem(BTF_ADAPTERS_MAX_RANK));
-  constexpr int width = WARPS * 32 / RG;
-  int64_t pieces = 0;
-  for (int i = 0; i < p.nseg; ++i) pieces += (p.seg[i].N + width - 1) / width;
-  p.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(pieces, (ctas + tiles - 1) / tiles));
-  return launch_pdl(adapter_expand_kernel<TW, TY, MT, RG, WARPS>, dim3((unsigned)(tiles * p.ranges)), dim3(WARPS * 32),
-                    smem(p.R), st, p);
-}
 template <typename TW, typename TY>
-cudaError_t expand_t(const Params& p, bool large, int tiles, int sms, cudaStream_t st, bool setup) {
-  if (setup)
-    if (cudaError_t e = expand<TW, TY, 1, 1, 2>(p, tiles, sms * 8, st, true)) return e;
-  return large || setup ? expand<TW, TY, 2, 2, 8>(p, tiles, sms * 4, st, setup)
-                        : expand<TW, TY, 1, 1, 2>(p, tiles, sms * 8, st, false);
+cudaError_t expand(Params p, int tiles, int sms, cudaStream_t st) {
+  constexpr int terms = std::is_same_v<TW, __half> || !std::is_same_v<TY, float> ? 2 : 3;
+  int64_t pieces = 0;
+  for (int i = 0; i < p.nseg; ++i) pieces += (p.seg[i].N + kExpand - 1) / kExpand;
+  p.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(pieces, (8 * sms + tiles - 1) / tiles));
+  return launch_pdl(adapter_expand_kernel<TW, TY>, dim3((unsigned)(tiles * p.ranges)), dim3(kExpand),
+                    (size_t)(p.R + 31) / 32 * 2 * terms * 512, st, p);
 }
 
 }  // namespace
@@ -672,11 +571,9 @@ int adapters_setup(DeviceInfo& d) {
   for (cudaError_t e :
        {cudaFuncSetAttribute(adapter_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * (BTF_ADAPTERS_MAX + 1) * 4),
         shrink_setup<float, __half>(), shrink_setup<float, __nv_bfloat16>(), shrink_setup<__half, __half>(),
-        shrink_setup<__nv_bfloat16, __nv_bfloat16>(), expand_t<__half, float>(p, true, 1, 1, nullptr, true),
-        expand_t<__half, __half>(p, true, 1, 1, nullptr, true), expand_t<__nv_bfloat16, float>(p, true, 1, 1, nullptr, true),
-        expand_t<__nv_bfloat16, __nv_bfloat16>(p, true, 1, 1, nullptr, true)})
+        shrink_setup<__nv_bfloat16, __nv_bfloat16>()})
     if (e != cudaSuccess) return cuda_fail(e, "adapter kernels' attributes");
-  return BTF_OK;
+  return setup_tc();
 }
 
 }  // namespace btf
@@ -744,6 +641,7 @@ int btf_adapters(const btf_adapters_args* a, void* stream) {
       return fail(BTF_ERR_ARG, "btf_adapters: a, b or y is null, or a or b is not 16-byte aligned");
     for (int64_t v : {s.a_adapter, s.a_row, s.b_adapter, s.b_row})
       if (v < 0 || v % 8) return fail(BTF_ERR_ARG, "btf_adapters: the strides of a and b must be multiples of 8 elements, >= 0");
+    if (s.a_row == 0 || (s.N > 1 && s.b_row == 0)) return fail(BTF_ERR_ARG, "btf_adapters: the rows of a and b need a stride");
     if (reinterpret_cast<uintptr_t>(s.y) % yb || reinterpret_cast<uintptr_t>(s.base) % yb)
       return fail(BTF_ERR_ARG, "btf_adapters: y or base is not aligned to its type");
     if (a->T > 1 && s.y_row < s.N) return fail(BTF_ERR_ARG, "btf_adapters: the rows of y overlap");
@@ -773,11 +671,11 @@ int btf_adapters(const btf_adapters_args* a, void* stream) {
   cudaError_t e = half ? (x32 ? shrink_r<float, __half>(p, sh.large, sh.tiles, st) : shrink_r<__half, __half>(p, sh.large, sh.tiles, st))
                        : (x32 ? shrink_r<float, __nv_bfloat16>(p, sh.large, sh.tiles, st)
                               : shrink_r<__nv_bfloat16, __nv_bfloat16>(p, sh.large, sh.tiles, st));
+  if (e == cudaSuccess && sh.large) return expand_tc(p, half, y32, dev->sm_count, st);
   if (e == cudaSuccess)
-    e = half ? (y32 ? expand_t<__half, float>(p, sh.large, sh.tiles, dev->sm_count, st, false)
-                    : expand_t<__half, __half>(p, sh.large, sh.tiles, dev->sm_count, st, false))
-             : (y32 ? expand_t<__nv_bfloat16, float>(p, sh.large, sh.tiles, dev->sm_count, st, false)
-                    : expand_t<__nv_bfloat16, __nv_bfloat16>(p, sh.large, sh.tiles, dev->sm_count, st, false));
+    e = half ? (y32 ? expand<__half, float>(p, sh.tiles, dev->sm_count, st) : expand<__half, __half>(p, sh.tiles, dev->sm_count, st))
+             : (y32 ? expand<__nv_bfloat16, float>(p, sh.tiles, dev->sm_count, st)
+                    : expand<__nv_bfloat16, __nv_bfloat16>(p, sh.tiles, dev->sm_count, st));
   return e == cudaSuccess ? BTF_OK : cuda_fail(e, "btf_adapters");
 }
 

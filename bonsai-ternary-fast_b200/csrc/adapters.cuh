@@ -1,0 +1,88 @@
+// Shared by the two halves of the low-rank adapters: few rows (adapters.cu) and
+// prompts on tcgen05 (adapters_tc.cu).
+#pragma once
+#include <algorithm>
+
+#include "elem.cuh"
+
+namespace btf {
+namespace adapt {
+
+constexpr int kSmall = 16, kLarge = 128;  // rows of a tile
+constexpr int kMaxSplits = 16;
+constexpr int kErrPlan = 2;  // device error word: a plan of other sizes
+
+struct Tile {
+  int adapter, begin, count, unused;  // adapter -1: rows without one
+};
+// The plan in memory: 8 words {T, adapters, small tiles, large tiles, rows with an
+// adapter}, the rows in order, then both lists of tiles.
+struct PlanLayout {
+  int64_t order, small, large, bytes;
+  PlanLayout(int64_t T, int64_t n) {
+    const int64_t lists = std::min(n + 1, T) + 1;
+    order = 32;
+    small = (order + 4 * T + 15) / 16 * 16;
+    large = small + 16 * (T / kSmall + lists);
+    bytes = large + 16 * (T / kLarge + lists);
+  }
+};
+
+struct Seg {
+  const void *a, *b, *base;
+  void* y;
+  int64_t a_adapter, a_row, b_adapter, b_row, base_row, y_row;
+  int N;
+  int vec;  // y (and base) take whole 16-byte words
+};
+struct Params {
+  Seg seg[3];
+  const void* x;
+  int64_t x_row;
+  int T, K, R, n, nseg, splits, ranges;
+  const int32_t* ranks;
+  const float* scales;
+  const int32_t *head, *order;
+  const Tile* tiles;
+  int which;  // the plan's word with the number of tiles
+  float* h;   // [splits][nseg][T][R]
+  int* err;
+};
+
+__device__ __forceinline__ bool plan_ok(const Params& p) {
+  if (p.head[0] == p.T && p.head[1] == p.n) return true;
+  if (blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.err, 0, kErrPlan);
+  return false;
+}
+__device__ __forceinline__ int rank_of(const Params& p, int a) { return p.ranks ? min(max(p.ranks[a], 0), p.R) : p.R; }
+
+// What `shrink` wrote: never from L1, and in its place behind the wait.
+__device__ __forceinline__ float4 ld_cg(const float* p) {
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
+    return __half22float2(h);
+  } else {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+}
+// What is left of v behind its first term (0 behind an infinity, not inf - inf).
+__device__ __forceinline__ float rest(float v, float term) { return v == term ? 0.f : v - term; }
+
+}  // namespace adapt
+}  // namespace btf

@@ -100,7 +100,7 @@ def test_plan_sorts_the_rows(cuda, btf, T, n):
     assert words[:2].tolist() == [T, n] and int(words[4]) == int((key < n).sum())
     small = (32 + 4 * T + 15) // 16 * 4
     lists = min(n + 1, T) + 1
-    for word, size, first in ((2, 16, small), (3, 64, small + 4 * (T // 16 + lists))):
+    for word, size, first in ((2, 16, small), (3, 128, small + 4 * (T // 16 + lists))):
         tiles = words[first: first + 4 * int(words[word])].view(-1, 4)
         want, at = [], 0
         for j, c in enumerate(torch.bincount(key, minlength=n + 1).tolist()):
@@ -124,7 +124,7 @@ def test_ranks(cuda, btf, R, types):
         _case(btf, cuda, T, 5, 512, R, [96], types, seed=R, ranks=None, scaled=False)
 
 
-@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 63, 64, 65, 255, 256, 257, 1025])
+@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257, 385, 1025])
 def test_rows(cuda, btf, T):
     _case(btf, cuda, T, 4, 128, 16, [64, 8, 129], (F32, F16, F32), seed=T)
     _case(btf, cuda, T, 1, 128, 16, [64], (BF16, BF16, BF16), seed=T, base=False, index=torch.zeros(T, dtype=torch.int32, device=cuda))
