@@ -103,9 +103,9 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t* index
     }
   }
   __syncthreads();
-  int32_t* order = reinterpret_cast<int32_t*>(plan + at.order);
+  int32_t *order = reinterpret_cast<int32_t*>(plan + at.order), *owner = reinterpret_cast<int32_t*>(plan + at.owner);
   each([&](int t, int a, unsigned same, int before) {
-    if (t < t1) order[first[a] + mine[a] + before] = t;
+    if (t < t1) order[first[a] + mine[a] + before] = t, owner[first[a] + mine[a] + before] = a;
     __syncwarp();
     if (t < t1 && before == 0) mine[a] += __popc(same);
   });
@@ -519,7 +519,15 @@ Shape shape_of(const DeviceInfo& d, int T, int K, int nseg, int n) {
   s.splits = std::max(1, std::min({want, kMaxSplits, (steps + warps - 1) / warps}));
   return s;
 }
-int64_t work_of(const Shape& s, int T, int R, int nseg) { return (int64_t)s.splits * nseg * T * R * 4; }
+// The workspace: h, and for prompts its terms and the rows' factors.
+struct Work {
+  int64_t terms, mul, bytes;
+  Work(const Shape& s, int T, int R, int nseg) {
+    terms = ((int64_t)s.splits * nseg * T * R * 4 + 15) / 16 * 16;
+    mul = terms + (s.large ? (int64_t)3 * nseg * T * ((R + 63) / 64 * 64) * 2 : 0);
+    bytes = mul + (s.large ? (int64_t)nseg * T * 4 : 0);
+  }
+};
 
 template <typename TX, typename TW, int RT, int NT, int RG>
 cudaError_t shrink(const Params& p, int tiles, cudaStream_t st, bool setup) {
@@ -612,7 +620,7 @@ int64_t btf_adapters_work(int T, int K, int R, int nseg, int n_adapters) {
   }
   const DeviceInfo* dev = current_device();
   if (!dev) return -1;
-  return T == 0 ? 0 : work_of(shape_of(*dev, T, K, nseg, n_adapters), T, R, nseg);
+  return T == 0 ? 0 : Work(shape_of(*dev, T, K, nseg, n_adapters), T, R, nseg).bytes;
 }
 
 int btf_adapters(const btf_adapters_args* a, void* stream) {
@@ -655,17 +663,21 @@ int btf_adapters(const btf_adapters_args* a, void* stream) {
   const DeviceInfo* dev = current_device();
   if (!dev) return BTF_ERR_STATE;
   const Shape sh = shape_of(*dev, a->T, a->K, a->nseg, a->n_adapters);
-  if (!a->work || !al(a->work) || a->work_bytes < work_of(sh, a->T, a->R, a->nseg))
+  const Work w(sh, a->T, a->R, a->nseg);
+  if (!a->work || !al(a->work) || a->work_bytes < w.bytes)
     return fail(BTF_ERR_ARG, "btf_adapters: workspace null, not 16-byte aligned or too small (%lld bytes, %lld are needed)",
-                (long long)a->work_bytes, (long long)work_of(sh, a->T, a->R, a->nseg));
+                (long long)a->work_bytes, (long long)w.bytes);
   const PlanLayout at(a->T, a->n_adapters);
   const uint8_t* plan = static_cast<const uint8_t*>(a->plan);
   p.x = a->x, p.x_row = a->T > 1 ? a->x_row : 0;
   p.T = a->T, p.K = a->K, p.R = a->R, p.n = a->n_adapters, p.nseg = a->nseg, p.splits = sh.splits, p.ranges = 1;
   p.ranks = a->ranks, p.scales = a->scales;
   p.head = reinterpret_cast<const int32_t*>(plan), p.order = reinterpret_cast<const int32_t*>(plan + at.order);
+  p.owner = reinterpret_cast<const int32_t*>(plan + at.owner);
   p.tiles = reinterpret_cast<const Tile*>(plan + (sh.large ? at.large : at.small)), p.which = sh.large ? 3 : 2;
-  p.h = static_cast<float*>(a->work), p.err = dev->err_word;
+  uint8_t* work = static_cast<uint8_t*>(a->work);
+  p.h = reinterpret_cast<float*>(work), p.terms = reinterpret_cast<uint16_t*>(work + w.terms), p.mul = reinterpret_cast<float*>(work + w.mul);
+  p.err = dev->err_word;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool half = a->w_type == BTF_F16, x32 = a->x_type == BTF_F32, y32 = a->y_type == BTF_F32;
   cudaError_t e = half ? (x32 ? shrink_r<float, __half>(p, sh.large, sh.tiles, st) : shrink_r<__half, __half>(p, sh.large, sh.tiles, st))

@@ -16,13 +16,14 @@ struct Tile {
   int adapter, begin, count, unused;  // adapter -1: rows without one
 };
 // The plan in memory: 8 words {T, adapters, small tiles, large tiles, rows with an
-// adapter}, the rows in order, then both lists of tiles.
+// adapter}, the rows in order, the adapter of each (n: none), then both lists of tiles.
 struct PlanLayout {
-  int64_t order, small, large, bytes;
+  int64_t order, owner, small, large, bytes;
   PlanLayout(int64_t T, int64_t n) {
     const int64_t lists = std::min(n + 1, T) + 1;
     order = 32;
-    small = (order + 4 * T + 15) / 16 * 16;
+    owner = order + 4 * T;
+    small = (owner + 4 * T + 15) / 16 * 16;
     large = small + 16 * (T / kSmall + lists);
     bytes = large + 16 * (T / kLarge + lists);
   }
@@ -42,10 +43,13 @@ struct Params {
   int T, K, R, n, nseg, splits, ranges;
   const int32_t* ranks;
   const float* scales;
-  const int32_t *head, *order;
+  const int32_t *head, *order, *owner;
   const Tile* tiles;
   int which;  // the plan's word with the number of tiles
   float* h;   // [splits][nseg][T][R]
+  // prompts: h as the MMAs take it, [terms][nseg][T][R to whole 64], and each row's factor [nseg][T]
+  uint16_t* terms;
+  float* mul;
   int* err;
 };
 

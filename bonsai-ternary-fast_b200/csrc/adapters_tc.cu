@@ -5,13 +5,15 @@
 // term of h (see adapters.cu), 256 at r = 64 in bf16: 0.06 ns of a card that moves 4 bytes
 // in 0.6. So the MMAs (128 x 128 outputs at a time, four accumulators in tensor memory)
 // run far ahead and the kernel is its way out: 8 warps, each with 32 rows of every other
-// tile, read base two tiles before they need it, whole 32-byte sectors of a row a lane,
-// add and store as many at a time.
+// tile. A lane has a row: copies bring 256 bytes of its base into shared memory ahead of
+// their turn and take the sum from the same place to y: one TMA copy of 32 rows x 128
+// bytes where the rows follow one another (a prompt's do), else 16 bytes a lane, eight
+// lanes a row. (Bulk copies of a row each are issued one after another by a warp: 178 us
+// for what takes XX us.)
 //
 // Work: the tiles of 128 rows times 128 outputs of all projections make a line, cut into
-// equal stretches of one CTA per SM. A stretch begins with the terms of its rows' h in
-// shared memory (the A operand, 128-byte swizzle) and again where it comes to other rows
-// or another projection. Warp 8 brings the weights by TMA, warp 9 issues the MMAs.
+// equal stretches of one CTA per SM. Warp 8 brings the terms of the rows' h (made by a
+// small kernel between) and the weights by TMA, warp 9 issues the MMAs.
 #include <cuda.h>
 
 #include "adapters_tc.cuh"
@@ -26,24 +28,24 @@ using namespace tc;
 constexpr int kCols = 128, kEpi = 8, kThreads = (kEpi + 2) * 32, kBufs = 4;
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr int kBlock = 128 * 128;          // bytes of 128 rows x 64 elements
-constexpr int kStagePitch = 33;            // a warp's 32 x 32 outputs on their way, in words
-constexpr int kStageBytes = kEpi * 32 * kStagePitch * 4;
+constexpr int kUnit = 128;                 // bytes of a row that move at once
+constexpr int kSlot = 32 * kUnit;           // a warp's rows, 128-byte swizzle
 
 struct ExpandMaps {
-  CUtensorMap b[3];
+  CUtensorMap h, b[3], y[3], base[3];
 };
 struct ExpandParams : Params {
   int b_mul[3];  // 0: every adapter has the same B
-  int wide[3];   // y (and base) take whole 32-byte words
-  int blocks, stages;  // 64-wide blocks of R; slots of the ring
+  int wide[3];   // rows of y (and base) take bulk copies
+  int blocks;                    // 64-wide blocks of R
+  int stages, hs, slots;         // slots of the weights, of h, of a warp
 };
 struct Misc {
-  uint64_t full[4], empty[4], acc_full[kBufs], acc_empty[kBufs], h_ready, final;
+  uint64_t full[2], empty[2], acc_full[kBufs], acc_empty[kBufs], h_full[2], h_empty[2], final, base[kEpi][3];
   uint32_t tmem;
   int abort;
-  float mul[2][kLarge];  // of this run's rows, and the next one's
 };
-static_assert(kLarge == 128 && sizeof(Misc) <= 2048);
+static_assert(kLarge == 128 && sizeof(Misc) <= 512);
 
 // The present tile of the line.
 struct Line {
@@ -67,31 +69,106 @@ struct Line {
   }
 };
 
-__device__ __forceinline__ void ld_v8(uint32_t (&v)[8], const void* p) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-               : "l"(p));
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void st_v8(void* p, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "l"(p)
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(src)
                : "memory");
 }
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+__device__ __forceinline__ float ld_cg1(const float* p) {  // behind the wait, as ld_cg
+  float v;
+  asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+
+// ------------------------------------------------------------------ terms
+// h summed over the stretches of K, cut to the adapter's rank and split into terms [TERMS][nseg][T][wide], and the
+// factor of each row: its adapter's scale, over the power of two that fp16 terms carry. Eight lanes a row.
+template <typename TW, int TERMS>
+__global__ void __launch_bounds__(256) adapter_terms_kernel(const __grid_constant__ Params p, uint16_t* terms, int wide) {
+  pdl_wait();
+  pdl_launch_dependents();  // (behind the wait: the next grid reads the plan before its own)
+  const int at = blockIdx.x * 32 + (threadIdx.x >> 3), l = threadIdx.x & 7, seg = blockIdx.y;
+  if (p.head[0] != p.T || p.head[1] != p.n) return;
+  const bool live = at < p.head[4];  // rows with an adapter come first
+  const int a = live ? p.owner[at] : 0, rank = live ? rank_of(p, a) : 0;
+  const int64_t next = (int64_t)p.nseg * p.T * p.R;
+  const float* h = p.h + ((int64_t)seg * p.T + at) * p.R;
+  float v[2][8];  // of a row's 128 at most: elements 8 l .. and 64 + 8 l ..
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int k = b * 64 + l * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[b][i] = 0.f;
+    if (k >= rank) continue;
+    const float* from = h + k;
+#pragma unroll 4
+    for (int q = 0; q < p.splits; ++q, from += next) {
+      const float4 v0 = ld_cg(from), v1 = ld_cg(from + 4);
+      v[b][0] += v0.x, v[b][1] += v0.y, v[b][2] += v0.z, v[b][3] += v0.w;
+      v[b][4] += v1.x, v[b][5] += v1.y, v[b][6] += v1.z, v[b][7] += v1.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i >= rank) v[b][i] = 0.f;
+  }
+  const float scale = live && p.scales ? p.scales[a] : 1.f;
+  float f = 1.f, back = scale;
+  if constexpr (std::is_same_v<TW, __half>) {  // the row over a power of two: its largest in [2^14, 2^15)
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(v[0][i]), fabsf(v[1][i])));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const int e = (__float_as_int(m) >> 23) - 127;  // 0, denormal and infinite rows stay as they are
+    if (e >= -112 && e < 128) f = __int_as_float((14 - e + 127) << 23), back = scale * __int_as_float((e - 14 + 127) << 23);
+  }
+  if (!live) return;
+  if (l == 0) p.mul[(int64_t)seg * p.T + at] = back;
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    if (b * 64 >= wide) break;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[b][i] *= f;
+#pragma unroll
+    for (int e = 0; e < TERMS; ++e) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = pack2<TW>(v[b][2 * i], v[b][2 * i + 1]);
+        const float2 u = unpack2<TW>(w[i]);
+        v[b][2 * i] = rest(v[b][2 * i], u.x), v[b][2 * i + 1] = rest(v[b][2 * i + 1], u.y);
+      }
+      *reinterpret_cast<uint4*>(terms + (((int64_t)e * p.nseg + seg) * p.T + at) * wide + b * 64 + l * 8) =
+          make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ y
 template <typename TW, typename TY>
 __global__ void __launch_bounds__(kThreads, 1)
     adapter_expand_tc_kernel(const __grid_constant__ ExpandMaps maps, const __grid_constant__ ExpandParams p) {
   constexpr bool kHalf = std::is_same_v<TW, __half>, kY32 = std::is_same_v<TY, float>, kBf16 = !kHalf;
   constexpr int kTerms = !kHalf && kY32 ? 3 : 2;
-  constexpr int kWords = 32 / (int)sizeof(TY);      // outputs of a 32-byte word
-  constexpr int kPer = 32 / kWords;                 // of which 32 outputs have so many
-  constexpr int kRing = kY32 ? 2 : 4;               // base: so many 32-wide pieces ahead
+  constexpr int kWidth = kUnit / (int)sizeof(TY), kUnits = kCols / kWidth;  // outputs of a unit, units of a tile's row
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), sbase = (raw + 1023) & ~1023u;
   uint8_t* smem = smem_raw + (sbase - raw);
-  const uint32_t off_ring = kTerms * p.blocks * kBlock, off_misc = off_ring + p.stages * p.blocks * kBlock;
+  const uint32_t h_bytes = kTerms * p.blocks * kBlock, off_ring = p.hs * h_bytes, off_slots = off_ring + p.stages * p.blocks * kBlock;
+  const uint32_t off_misc = off_slots + kEpi * p.slots * kSlot;
   Misc& ms = *reinterpret_cast<Misc*>(smem + off_misc);
-  float* stage = reinterpret_cast<float*>(smem + off_misc + 2048);
   volatile int* abort_flag = &ms.abort;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (warp == kEpi + 1) {
@@ -101,10 +178,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 0) {
-    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&ms.full[i]), 1), mbar_init(smem_u32(&ms.empty[i]), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ms.full[i]), 1), mbar_init(smem_u32(&ms.empty[i]), 1);
+      mbar_init(smem_u32(&ms.h_full[i]), 1), mbar_init(smem_u32(&ms.h_empty[i]), 1);
+    }
     for (int i = 0; i < kBufs; ++i) mbar_init(smem_u32(&ms.acc_full[i]), 1), mbar_init(smem_u32(&ms.acc_empty[i]), 4);
-    mbar_init(smem_u32(&ms.h_ready), kEpi);
     mbar_init(smem_u32(&ms.final), 1);
+    for (int i = 0; i < kEpi; ++i)
+      for (int k = 0; k < 3; ++k) mbar_init(smem_u32(&ms.base[i][k]), 1);
     ms.abort = 0;
     fence_mbar_init();
   }
@@ -112,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, ms.tmem, 0);
-  // The plan, the weights and base were complete before `shrink` let this grid start.
+  // The plan, the weights and base were complete before `terms` let this grid start; h is what the wait is for.
   pdl_launch_dependents();
 
   auto wait = [&](const uint64_t& bar, uint32_t parity) -> bool {  // bounded
@@ -139,6 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------- weights
     if (lane == 0) {
       int sent = 0;
+      bool waited = false;
       for (int at = first; ok && at < last;) {
         int ti, seg, piece, end;
         line.place(at, ti, seg, piece, end);
@@ -149,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           at = end;
           continue;
         }
-        for (; ok && at < end; ++at, ++piece, ++t) {
+        for (int begin = at; ok && at < end; ++at, ++piece, ++t) {
           const int s = t % p.stages;
           if (t >= p.stages && !(ok = wait(ms.empty[s], (uint32_t)((t / p.stages - 1) & 1)))) break;
           const uint32_t bar = smem_u32(&ms.full[s]), dst = sbase + off_ring + s * p.blocks * kBlock;
@@ -157,12 +239,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < blocks; ++k)
             tma_load_3d(dst + k * kBlock, &maps.b[seg], k * 64, piece * kCols, tile.adapter * p.b_mul[seg], bar);
           ++sent;
+          if (at > begin) continue;
+          // with the run's first weights: its rows' h
+          if (!waited) {
+            pdl_wait();
+            asm volatile("fence.proxy.async.global;" ::: "memory");  // h was written as ordinary stores
+          }
+          waited = true;
+          const int hs = run % p.hs;
+          if (run >= p.hs && !(ok = wait(ms.h_empty[hs], (uint32_t)((run / p.hs - 1) & 1)))) break;
+          const uint32_t hbar = smem_u32(&ms.h_full[hs]);
+          mbar_expect_tx(hbar, kTerms * blocks * kBlock);
+          for (int e = 0; e < kTerms; ++e)
+            for (int k = 0; k < blocks; ++k)
+              tma_load_3d(sbase + hs * h_bytes + (e * p.blocks + k) * kBlock, &maps.h, k * 64, tile.begin, e * p.nseg + seg, hbar);
+          ++run;
         }
       }
       // after a time-out, leave no copy in flight into this CTA's shared memory (bounded)
-      if (!ok || *abort_flag)
+      if (!ok || *abort_flag) {
         for (int k = max(0, sent - p.stages); k < sent; ++k)
           mbar_wait_bounded(smem_u32(&ms.full[k % p.stages]), (uint32_t)((k / p.stages) & 1), kWaitNs / 10);
+        for (int k = max(0, run - p.hs); k < run; ++k)
+          mbar_wait_bounded(smem_u32(&ms.h_full[k % p.hs]), (uint32_t)((k / p.hs) & 1), kWaitNs / 10);
+      }
     }
   } else if (warp == kEpi + 1) {
     // ---------------------------------------------------------- MMAs
@@ -177,7 +277,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         at = end;
         continue;
       }
-      ok = warp_wait(ms.h_ready, (uint32_t)(run++ & 1));
+      const int hs = run % p.hs;
+      ok = warp_wait(ms.h_full[hs], (uint32_t)((run++ / p.hs) & 1));
       for (; ok && at < end; ++at, ++t) {
         const int s = t % p.stages, buf = t % kBufs;
         if (!(ok = warp_wait(ms.full[s], (uint32_t)((t / p.stages) & 1)))) break;
@@ -202,8 +303,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t bd = smem_desc_sw128(ws + off);
 #pragma unroll
             for (int e = kTerms - 1; e >= 0; --e)
-              mma_f16_ss(d, smem_desc_sw128(sbase + e * p.blocks * kBlock + off), bd, kDesc, k > 0 || e < kTerms - 1);
+              mma_f16_ss(d, smem_desc_sw128(sbase + hs * h_bytes + e * p.blocks * kBlock + off), bd, kDesc, k > 0 || e < kTerms - 1);
           }
+          if (at + 1 == end) mma_commit(smem_u32(&ms.h_empty[hs]));
           mma_commit(smem_u32(&ms.empty[s]));
           mma_commit(smem_u32(&ms.acc_full[buf]));
         }
@@ -218,8 +320,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------- the way out: 32 rows a warp, every other tile
     const int group = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    float* own = stage + warp * 32 * kStagePitch;
+    const uint32_t own_at = off_slots + warp * p.slots * kSlot;  // the warp's slots
     bool waited = false;
+    int q = 0;        // units so far, of which each has its slot in turn
+    uint32_t loads = 0, pending = 0;  // bit i: the phase of slot i's next load; whether one is under way
     for (int at = first; at < last;) {
       int ti, seg, piece, end;
       line.place(at, ti, seg, piece, end);
@@ -228,92 +332,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int rank = tile.adapter < 0 ? 0 : rank_of(p, tile.adapter);
       const Seg& s = p.seg[seg];
       const bool copy = rank == 0, live = r < tile.count, wide = p.wide[seg];
+      const int rows = min(32, tile.count - (warp & 3) * 32);  // of the warp
       if (copy && s.base == s.y && s.base_row == s.y_row) {  // in place: stays
         at = end;
         continue;
       }
       const int64_t row = live ? p.order[tile.begin + r] : 0;
-      TY* y = static_cast<TY*>(s.y) + row * s.y_row;
-      const TY* base = s.base ? static_cast<const TY*>(s.base) + row * s.base_row : nullptr;
-      auto whole = [&](int pc) { return wide && (pc + 1) * kCols <= s.N; };  // a piece that takes 32-byte words
-      // base of the 32-wide pieces ahead of the group's
-      uint32_t ring[kRing][kPer][8];
-      auto fetch = [&](uint32_t (&v)[kPer][8], int pc, int c) {
-        if (base && live && whole(pc)) {
+      const bool base = s.base != nullptr;
+      const int row0 = (int)__shfl_sync(0xffffffffu, row, 0);
+      const bool tiled = wide && rows >= 32 && __all_sync(0xffffffffu, row == row0 + lane);
+      int rows_at[8];  // of the lane's words where the rows do not follow one another
 #pragma unroll
-          for (int w = 0; w < kPer; ++w) ld_v8(v[w], base + pc * kCols + c * 32 + w * kWords);
-        }
+      for (int i = 0; i < 8; ++i) rows_at[i] = (int)__shfl_sync(0xffffffffu, row, i * 4 + (lane >> 3));
+      // bytes of a row of the unit from output n0 that copies move; 0: rows that begin anywhere, and odd ends
+      auto bytes_of = [&](int n0) {
+        if (tiled) return n0 < s.N ? kUnit : 0;  // (a TMA copy stops at N)
+        const int b = min(kUnit, (s.N - n0) * (int)sizeof(TY));
+        return wide && b > 0 && b % 16 == 0 ? b : 0;
       };
-      const int mine = at + ((at ^ group) & 1);  // the group's first
+      const int start = at + ((at ^ group) & 1), units = start < end ? ((end - start + 1) >> 1) * kUnits : 0;
+      const int first_n = (piece + start - at) * kCols;  // the run's first output of this group
+      auto output = [&](int u) { return first_n + u / kUnits * 2 * kCols + u % kUnits * kWidth; };
+      // base of the run's unit u to its slot, which its last store has been read from
+      auto fetch = [&](int u, int qu) {
+        const int n0 = output(u), b = u < units && base && rows > 0 ? bytes_of(n0) : 0, slot = qu % p.slots;
+        const uint32_t to = sbase + own_at + slot * kSlot;
+        if (b && tiled) {
+          const uint32_t bar = smem_u32(&ms.base[warp][slot]);
+          pending |= 1u << slot;
+          if (lane == 0) {
+            mbar_expect_tx(bar, kSlot);
+            tma_load_2d(to, &maps.base[seg], n0, row0, bar);
+          }
+        } else if (b && (lane & 7) * 16 < b) {
 #pragma unroll
-      for (int c = 0; c < kRing; ++c)
-        if (mine < end) fetch(ring[c], piece + mine - at, c);
+          for (int i = 0; i < 8; ++i) {
+            const int k = i * 4 + (lane >> 3);
+            if (k < rows)
+              cp_async16(to + k * kUnit + (((lane & 7) ^ (k & 7)) << 4),
+                         static_cast<const TY*>(s.base) + rows_at[i] * s.base_row + n0 + (lane & 7) * (16 / (int)sizeof(TY)));
+          }
+        }
+        cp_commit();  // (a group a unit, empty or not)
+      };
+      bulk_wait_read();
+      __syncwarp();
+      for (int u = 0; u < p.slots - 1; ++u) fetch(u, q + u);
       if (!waited) {
         pdl_wait();
         waited = true;
       }
-      float mul = 0.f;
-      if (!copy) {
-        // this run's h, in terms, where the MMAs of the one before are done: two threads a row
-        if (t > 0) ok = ok && warp_wait(ms.acc_full[(t - 1) % kBufs], (uint32_t)(((t - 1) / kBufs) & 1));
-        const int hr = tid >> 1, chunks = (rank + 15) / 16 * 2;  // of 8 elements
-        const float* h = p.h + ((int64_t)seg * p.T + tile.begin + hr) * p.R;
-        const int64_t next = (int64_t)p.nseg * p.T * p.R;
-        auto sum = [&](int k, float (&v)[8]) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 0.f;
-          if (hr >= tile.count || k * 8 >= rank) return;
-          const float* from = h + k * 8;
-#pragma unroll 4
-          for (int q = 0; q < p.splits; ++q, from += next) {
-            const float4 v0 = ld_cg(from), v1 = ld_cg(from + 4);
-            v[0] += v0.x, v[1] += v0.y, v[2] += v0.z, v[3] += v0.w;
-            v[4] += v1.x, v[5] += v1.y, v[6] += v1.z, v[7] += v1.w;
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (k * 8 + i >= rank) v[i] = 0.f;
-        };
-        const float scale = p.scales ? p.scales[tile.adapter] : 1.f;
-        float f = 1.f, back = scale;
-        if constexpr (kHalf) {  // the row over a power of two: its largest in [2^14, 2^15)
-          float m = 0.f;
-          for (int k = tid & 1; k < chunks; k += 2) {
-            float v[8];
-            sum(k, v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
-          }
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          const int e = (__float_as_int(m) >> 23) - 127;  // 0, denormal and infinite rows stay as they are
-          if (e >= -112 && e < 128) f = __int_as_float((14 - e + 127) << 23), back = scale * __int_as_float((e - 14 + 127) << 23);
-        }
-        if ((tid & 1) == 0) ms.mul[run & 1][hr] = back;
-        for (int k = tid & 1; k < chunks; k += 2) {
-          float v[8];
-          sum(k, v);
-          uint8_t* to = smem + (k >> 3) * kBlock + hr * 128 + (((k & 7) ^ (hr & 7)) << 4);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= f;
-#pragma unroll
-          for (int e = 0; e < kTerms; ++e) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              w[i] = pack2<TW>(v[2 * i], v[2 * i + 1]);
-              const float2 u = unpack2<TW>(w[i]);
-              v[2 * i] = rest(v[2 * i], u.x), v[2 * i + 1] = rest(v[2 * i + 1], u.y);
-            }
-            *reinterpret_cast<uint4*>(to + e * p.blocks * kBlock) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ms.h_ready));
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // mul; every run, by every warp of these
-        mul = ms.mul[run++ & 1][r];
-      }
-      for (; at < end; ++at, ++piece) {
+      const float mul = copy || !live ? 0.f : ld_cg1(p.mul + (int64_t)seg * p.T + tile.begin + r);
+      int u = 0;
+      for (; at < end; ++at) {
         const int now = t;
         t += !copy;
         if ((at & 1) != group) continue;
@@ -322,67 +393,105 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = ok && warp_wait(ms.acc_full[buf], (uint32_t)((now / kBufs) & 1));
           tc_fence_after();
         }
-        const bool fast = whole(piece);
 #pragma unroll
-        for (int c = 0; c < kCols / 32; ++c) {
-          uint32_t v[32];
-          if (!copy) {
-            tmem_ld32(tmem + buf * kCols + c * 32 + lanes, v);
-            tmem_wait_ld(v);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0;
+        for (int h = 0; h < kUnits; ++h, ++u, ++q) {
+          const int n0 = output(u), bytes = bytes_of(n0), slot = q % p.slots;
+          uint8_t* own = smem + own_at + slot * kSlot;
+          // into the slot of the unit before, whose store has been read
+          bulk_wait_read();
+          __syncwarp();
+          fetch(u + p.slots - 1, q + p.slots - 1);
+          if (base && bytes && rows > 0) {
+            if (tiled) {
+              ok = ok && warp_wait(ms.base[warp][slot], (loads >> slot) & 1);
+              if (ok) loads ^= 1u << slot, pending &= ~(1u << slot);
+            } else {
+              if (p.slots == 3) cp_wait<2>();
+              else cp_wait<1>();
+              __syncwarp();
+            }
           }
-          if (c == kCols / 32 - 1 && !copy) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&ms.acc_empty[buf]));
-          }
-          if (!ok) continue;
-          if (fast) {
-            uint32_t (&q)[kPer][8] = ring[c % kRing];
-            if (live) {
 #pragma unroll
-              for (int w = 0; w < kPer; ++w) {
-                uint32_t o[8];
-                if constexpr (kY32) {
+          for (int c = 0; c < kWidth / 32; ++c) {
+            uint32_t v[32];
+            if (!copy) {
+              tmem_ld32(tmem + buf * kCols + h * kWidth + c * 32 + lanes, v);
+              tmem_wait_ld(v);
+            } else {
 #pragma unroll
-                  for (int i = 0; i < 8; ++i)
-                    o[i] = __float_as_uint(fmaf(__uint_as_float(v[w * 8 + i]), mul, base ? __uint_as_float(q[w][i]) : 0.f));
-                } else {
+              for (int i = 0; i < 32; ++i) v[i] = 0;
+            }
+            if (c == kWidth / 32 - 1 && h == kUnits - 1 && !copy) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&ms.acc_empty[buf]));
+            }
+            if (!ok || rows <= 0) continue;
+            if (bytes) {
 #pragma unroll
-                  for (int i = 0; i < 8; ++i) {
-                    const float2 b2 = base ? unpack2<TY>(q[w][i]) : make_float2(0.f, 0.f);
-                    o[i] = pack2<TY>(fmaf(__uint_as_float(v[w * 16 + 2 * i]), mul, b2.x),
-                                     fmaf(__uint_as_float(v[w * 16 + 2 * i + 1]), mul, b2.y));
+              for (int w = 0; w < 2 * (int)sizeof(TY); ++w) {
+                const int k = c * 2 * (int)sizeof(TY) + w;  // the row's 16-byte word
+                uint4* mine = reinterpret_cast<uint4*>(own + lane * kUnit + ((k ^ (lane & 7)) << 4));
+                const uint4 b4 = base ? *mine : make_uint4(0, 0, 0, 0);
+                const uint32_t b[4] = {b4.x, b4.y, b4.z, b4.w};
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  if constexpr (kY32) {
+                    o[i] = __float_as_uint(fmaf(__uint_as_float(v[w * 4 + i]), mul, __uint_as_float(b[i])));
+                  } else {
+                    const float2 b2 = unpack2<TY>(b[i]);
+                    o[i] = pack2<TY>(fmaf(__uint_as_float(v[w * 8 + 2 * i]), mul, b2.x),
+                                     fmaf(__uint_as_float(v[w * 8 + 2 * i + 1]), mul, b2.y));
                   }
                 }
-                st_v8(y + piece * kCols + c * 32 + w * kWords, o);
+                *mine = make_uint4(o[0], o[1], o[2], o[3]);
               }
-            }
-          } else {
-            // rows that begin anywhere, and the last outputs: through shared memory, a row at a time for the warp
+            } else {
+              // rows that begin anywhere, and odd ends: a row at a time for the warp
+              float* stage = reinterpret_cast<float*>(own);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) own[lane * kStagePitch + i] = __uint_as_float(v[i]) * mul;
-            __syncwarp();
-            const int n = piece * kCols + c * 32 + lane;
+              for (int i = 0; i < 32; ++i) stage[lane * 32 + (i ^ lane)] = __uint_as_float(v[i]) * mul;
+              __syncwarp();
+              TY* const to = static_cast<TY*>(s.y);
+              const TY* const from = static_cast<const TY*>(s.base);
+              const int n = n0 + c * 32 + lane;
 #pragma unroll 4
-            for (int k = 0; k < 32; ++k) {
-              const int64_t kr = __shfl_sync(0xffffffffu, row, k);
-              if ((warp & 3) * 32 + k < tile.count && n < s.N) {
-                const float o = own[k * kStagePitch + lane];
-                static_cast<TY*>(s.y)[kr * s.y_row + n] =
-                    from_f32<TY>(s.base ? o + to_f32(static_cast<const TY*>(s.base)[kr * s.base_row + n]) : o);
+              for (int k = 0; k < 32; ++k) {
+                const int64_t at_row = __shfl_sync(0xffffffffu, row, k);
+                if (k < rows && n < s.N) {
+                  const float o = stage[k * 32 + (lane ^ k)];
+                  to[at_row * s.y_row + n] = from_f32<TY>(from ? o + to_f32(from[at_row * s.base_row + n]) : o);
+                }
+              }
+              fence_proxy_async_smem();  // (the slot's next content may come by a bulk copy)
+              __syncwarp();
+            }
+          }
+          if (bytes && ok) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (tiled) {
+              if (lane == 0) tma_store_2d(&maps.y[seg], n0, row0, sbase + own_at + slot * kSlot);
+            } else if ((lane & 7) * 16 < bytes) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int k = i * 4 + (lane >> 3);
+                if (k < rows)
+                  *reinterpret_cast<uint4*>(static_cast<TY*>(s.y) + rows_at[i] * s.y_row + n0 + (lane & 7) * (16 / (int)sizeof(TY))) =
+                      *reinterpret_cast<const uint4*>(own + k * kUnit + (((lane & 7) ^ (k & 7)) << 4));
               }
             }
-            __syncwarp();
+            bulk_commit();
           }
-          // the next 32-wide piece that this place of the ring is for
-          const int ahead = c + kRing < kCols / 32 ? 0 : 2;
-          if (at + ahead < end) fetch(ring[c % kRing], piece + ahead, (c + kRing) % (kCols / 32));
         }
       }
     }
+    bulk_wait();
+    cp_wait<0>();
+    // after a time-out, leave no copy in flight into this CTA's shared memory (bounded)
+    for (int i = 0; i < p.slots; ++i)
+      if ((pending >> i) & 1) mbar_wait_bounded(smem_u32(&ms.base[warp][i]), (loads >> i) & 1, kWaitNs / 10);
     if (!waited) pdl_wait();  // (a grid may only end after the one before it)
   }
   tc_fence_before();
@@ -393,33 +502,48 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-int expand_smem(int R, int terms, int* blocks, int* stages) {
-  *blocks = (R + 63) / 64;
-  *stages = *blocks == 1 ? 4 : 2;
-  return 1024 + (terms + *stages) * *blocks * kBlock + 2048 + kStageBytes;
+// What fits: the terms of h twice, two slots of weights and three of each warp, or less where there are three terms or
+// R > 64.
+int expand_smem(int R, int terms, ExpandParams* p) {
+  p->blocks = (R + 63) / 64;
+  p->hs = p->blocks == 1 ? 2 : 1;
+  p->stages = p->blocks == 1 || terms == 2 ? 2 : 1;
+  p->slots = p->blocks == 1 && terms == 2 ? 3 : 2;
+  return 1024 + (p->hs * terms + p->stages) * p->blocks * kBlock + kEpi * p->slots * kSlot + 512;
 }
 
 // b as [adapters][N][R]
 int encode_b(CUtensorMap* m, const Params& p, int seg, bool half, bool one) {
-  const EncodeFn fn = encode_fn();
-  if (!fn) return fail(BTF_ERR_CUDA, "btf_adapters: cuTensorMapEncodeTiled is not available");
   const Seg& s = p.seg[seg];
   const cuuint64_t dims[3] = {(cuuint64_t)p.R, (cuuint64_t)s.N, (cuuint64_t)(one ? 1 : p.n)};
   const cuuint64_t strides[2] = {(cuuint64_t)(s.N > 1 ? s.b_row * 2 : 16), (cuuint64_t)(one ? 16 : s.b_adapter * 2)};
   const cuuint32_t box[3] = {64, kCols, 1}, step[3] = {1, 1, 1};
-  const CUresult r = fn(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(s.b),
+  const CUresult r = encode_fn()(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(s.b),
                         dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? BTF_OK : fail(BTF_ERR_ARG, "btf_adapters: the strides of b make no tensor map (%d)", (int)r);
 }
 
+// y or base as [T][N], 32 rows x 128 bytes at a time
+int encode_y(CUtensorMap* m, const Params& p, const void* at, int64_t row, int N, bool y32, bool half) {
+  const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)p.T}, strides[1] = {(cuuint64_t)(row * (y32 ? 4 : 2))};
+  const cuuint32_t box[2] = {y32 ? 32u : 64u, 32}, step[2] = {1, 1};
+  const CUresult r = encode_fn()(m, y32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                 2, const_cast<void*>(at), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? BTF_OK : fail(BTF_ERR_ARG, "btf_adapters: the strides of y or base make no tensor map (%d)", (int)r);
+}
+
 template <typename TW, typename TY>
 cudaError_t expand(const ExpandMaps& maps, ExpandParams p, int sms, cudaStream_t st, bool setup) {
   constexpr int terms = std::is_same_v<TW, __half> || !std::is_same_v<TY, float> ? 2 : 3;
-  const int smem = expand_smem(setup ? BTF_ADAPTERS_MAX_RANK : p.R, terms, &p.blocks, &p.stages);
   if (setup)
     return cudaFuncSetAttribute(adapter_expand_tc_kernel<TW, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                std::max(smem, expand_smem(64, terms, &p.blocks, &p.stages)));
+                                std::max(expand_smem(BTF_ADAPTERS_MAX_RANK, terms, &p), expand_smem(64, terms, &p)));
+  const int smem = expand_smem(p.R, terms, &p);
+  if (cudaError_t e = launch_pdl(adapter_terms_kernel<TW, terms>, dim3((unsigned)((p.T + 31) / 32), p.nseg), dim3(256), 0, st, p, p.terms,
+                                 p.blocks * 64))
+    return e;
   return launch_pdl(adapter_expand_tc_kernel<TW, TY>, dim3((unsigned)sms), dim3(kThreads), (size_t)smem, st, maps, p);
 }
 
@@ -435,19 +559,37 @@ int setup_tc() {
   return BTF_OK;
 }
 
+// h's terms as [terms x nseg][T][wide]
+int encode_h(CUtensorMap* m, const Params& p, int terms, bool half) {
+  const int wide = (p.R + 63) / 64 * 64;
+  const cuuint64_t dims[3] = {(cuuint64_t)wide, (cuuint64_t)p.T, (cuuint64_t)(terms * p.nseg)};
+  const cuuint64_t strides[2] = {(cuuint64_t)wide * 2, (cuuint64_t)wide * 2 * p.T};
+  const cuuint32_t box[3] = {64, kLarge, 1}, step[3] = {1, 1, 1};
+  const CUresult r = encode_fn()(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p.terms, dims,
+                                 strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? BTF_OK : fail(BTF_ERR_CUDA, "btf_adapters: no tensor map of the workspace (%d)", (int)r);
+}
+
 int expand_tc(const Params& q, bool half, bool y32, int sms, cudaStream_t st) {
+  if (!encode_fn()) return fail(BTF_ERR_CUDA, "btf_adapters: cuTensorMapEncodeTiled is not available");
   ExpandMaps maps{};
   ExpandParams p{};
   static_cast<Params&>(p) = q;
-  const int size = y32 ? 4 : 2;
   for (int i = 0; i < p.nseg; ++i) {
     const Seg& s = p.seg[i];
     const bool one = p.n == 1 || s.b_adapter == 0;
     p.b_mul[i] = !one;
-    p.wide[i] = reinterpret_cast<uintptr_t>(s.y) % 32 == 0 && s.y_row * size % 32 == 0 &&
-                reinterpret_cast<uintptr_t>(s.base) % 32 == 0 && s.base_row * size % 32 == 0;
     if (int rc = encode_b(&maps.b[i], p, i, half, one)) return rc;
+    // one row of base for all rows (stride 0) makes no map, nor do rows that begin anywhere
+    p.wide[i] = s.vec && (!s.base || s.base_row > 0);
+    if (p.wide[i]) {
+      if (int rc = encode_y(&maps.y[i], p, s.y, s.y_row, s.N, y32, half)) return rc;
+      if (s.base)
+        if (int rc = encode_y(&maps.base[i], p, s.base, s.base_row, s.N, y32, half)) return rc;
+    }
   }
+  if (int rc = encode_h(&maps.h, p, half || !y32 ? 2 : 3, half)) return rc;
   const cudaError_t e = half ? (y32 ? expand<__half, float>(maps, p, sms, st, false) : expand<__half, __half>(maps, p, sms, st, false))
                              : (y32 ? expand<__nv_bfloat16, float>(maps, p, sms, st, false)
                                     : expand<__nv_bfloat16, __nv_bfloat16>(maps, p, sms, st, false));

@@ -97,8 +97,9 @@ def test_plan_sorts_the_rows(cuda, btf, T, n):
     key = torch.where((index < 0) | (index >= n), n, index).cpu()
     order = words[8: 8 + T].long()
     assert torch.equal(order, torch.sort(key, stable=True).indices)
+    assert torch.equal(words[8 + T: 8 + 2 * T], key[order])
     assert words[:2].tolist() == [T, n] and int(words[4]) == int((key < n).sum())
-    small = (32 + 4 * T + 15) // 16 * 4
+    small = (32 + 8 * T + 15) // 16 * 4
     lists = min(n + 1, T) + 1
     for word, size, first in ((2, 16, small), (3, 128, small + 4 * (T // 16 + lists))):
         tiles = words[first: first + 4 * int(words[word])].view(-1, 4)
