@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t* index
   int32_t* head = reinterpret_cast<int32_t*>(plan);
   if (warp < 3) {  // running sums over the adapters: rows, small tiles, large tiles
     const int size = warp == 0 ? 1 : warp == 1 ? kSmall : kLarge;
-    Tile* tiles = reinterpret_cast<Tile*>(plan + (warp == 1 ? at.small : at.large));
+    Tile* large = reinterpret_cast<Tile*>(plan + at.large);
+    SmallTile* small = reinterpret_cast<SmallTile*>(plan + at.small);
     int sum = 0, rows = 0;
     for (int b = 0; b < nb; b += 32) {
       const int a = b + lane, c = a < nb ? total[a] : 0, k = (c + size - 1) / size;
@@ -90,8 +91,11 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t* index
         if (warp == 0) {
           first[a] = rows + r - c;
         } else {
-          for (int i = 0; i < k; ++i)
-            tiles[sum + s - k + i] = {a < n ? a : -1, rows + r - c + i * size, min(size, c - i * size), 0};
+          for (int i = 0; i < k; ++i) {
+            const Tile tile{a < n ? a : -1, rows + r - c + i * size, min(size, c - i * size), 0};
+            if (warp == 1) small[sum + s - k + i].tile = tile;
+            else large[sum + s - k + i] = tile;
+          }
         }
       }
       sum += __shfl_sync(0xffffffffu, s, 31);
@@ -103,9 +107,30 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t* index
     }
   }
   __syncthreads();
+  // where each adapter's small tiles begin
+  if (warp == 0) {
+    int sum = 0;
+    for (int b = 0; b < nb; b += 32) {
+      const int a = b + lane, k = a < nb ? (total[a] + kSmall - 1) / kSmall : 0;
+      int s = k;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int q = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += q;
+      }
+      if (a < nb) total[a] = sum + s - k;
+      sum += __shfl_sync(0xffffffffu, s, 31);
+    }
+  }
+  __syncthreads();
+  SmallTile* small = reinterpret_cast<SmallTile*>(plan + at.small);
   int32_t *order = reinterpret_cast<int32_t*>(plan + at.order), *owner = reinterpret_cast<int32_t*>(plan + at.owner);
   each([&](int t, int a, unsigned same, int before) {
-    if (t < t1) order[first[a] + mine[a] + before] = t, owner[first[a] + mine[a] + before] = a;
+    if (t < t1) {
+      const int i = mine[a] + before;  // the row's place among its adapter's
+      order[first[a] + i] = t, owner[first[a] + i] = a;
+      small[total[a] + i / kSmall].rows[i % kSmall] = t;
+    }
     __syncwarp();
     if (t < t1 && before == 0) mine[a] += __popc(same);
   });
@@ -142,130 +167,140 @@ struct XFrag {
   static constexpr int kLoads = kF32 ? 2 : 1;
 };
 
+// c += the products of a 32-wide step: lo and hi the weights' rows g and g + 8 of each 16, xw the rows of x; of the
+// weights' 16s and the rows' 8s only the first ms and ns have anything.
+template <typename TX, typename TW, int RT, int NT>
+__device__ __forceinline__ void products(float (&c)[RT][NT][4], const uint4 (&lo)[RT], const uint4 (&hi)[RT],
+                                         const uint4 (&xw)[NT][XFrag<TX, TW>::kLoads], int ms, int ns) {
+  using F = XFrag<TX, TW>;
+  if constexpr (!F::kF32) {
+#pragma unroll
+    for (int m = 0; m < RT; ++m)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        if (m < ms && j < ns) mma16<TW>(c[m][j], lo[m].x, hi[m].x, lo[m].y, hi[m].y, xw[j][0].x, xw[j][0].y);
+#pragma unroll
+    for (int m = 0; m < RT; ++m)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        if (m < ms && j < ns) mma16<TW>(c[m][j], lo[m].z, hi[m].z, lo[m].w, hi[m].w, xw[j][0].z, xw[j][0].w);
+  } else if constexpr (!F::kTf32) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      if (j >= ns) break;
+      const uint32_t w[8] = {xw[j][0].x, xw[j][0].y, xw[j][0].z, xw[j][0].w,
+                             xw[j][1].x, xw[j][1].y, xw[j][1].z, xw[j][1].w};
+      uint32_t term[3][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float v0 = __uint_as_float(w[2 * i]), v1 = __uint_as_float(w[2 * i + 1]);
+        term[0][i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);  // cut off: never beyond fp32's range
+        const float r0 = rest(v0, __uint_as_float(w[2 * i] & 0xffff0000u));
+        const float r1 = rest(v1, __uint_as_float(w[2 * i + 1] & 0xffff0000u));
+        term[1][i] = pack2<__nv_bfloat16>(r0, r1);
+        const float2 mid = unpack2<__nv_bfloat16>(term[1][i]);
+        term[2][i] = pack2<__nv_bfloat16>(r0 - mid.x, r1 - mid.y);
+      }
+#pragma unroll
+      for (int e = 2; e >= 0; --e) {
+#pragma unroll
+        for (int m = 0; m < RT; ++m)
+          if (m < ms) mma16<TW>(c[m][j], lo[m].x, hi[m].x, lo[m].y, hi[m].y, term[e][0], term[e][1]);
+#pragma unroll
+        for (int m = 0; m < RT; ++m)
+          if (m < ms) mma16<TW>(c[m][j], lo[m].z, hi[m].z, lo[m].w, hi[m].w, term[e][2], term[e][3]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // the lane's elements 2 i and 2 i + 1
+      uint32_t big[NT][2], small[NT][2];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint4 v4 = xw[j][i >> 1];
+          const uint32_t w = i & 1 ? (e ? v4.w : v4.z) : (e ? v4.y : v4.x);
+          big[j][e] = w & 0xffffe000u;
+          const float r = rest(__uint_as_float(w), __uint_as_float(big[j][e]));
+          asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(small[j][e]) : "f"(r));
+        }
+#pragma unroll
+      for (int m = 0; m < RT; ++m) {
+        if (m >= ms) break;
+        const uint32_t wl = i == 0 ? lo[m].x : i == 1 ? lo[m].y : i == 2 ? lo[m].z : lo[m].w;
+        const uint32_t wh = i == 0 ? hi[m].x : i == 1 ? hi[m].y : i == 2 ? hi[m].z : hi[m].w;
+        const float2 fl = unpack2<TW>(wl), fh = unpack2<TW>(wh);
+        const uint32_t a0 = __float_as_uint(fl.x), a1 = __float_as_uint(fh.x), a2 = __float_as_uint(fl.y),
+                       a3 = __float_as_uint(fh.y);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          if (j < ns) mma_tf32(c[m][j], a0, a1, a2, a3, small[j][0], small[j][1]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          if (j < ns) mma_tf32(c[m][j], a0, a1, a2, a3, big[j][0], big[j][1]);
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------ shrink
-// A CTA takes a tile's rows, one projection and one of `splits` stretches of K, which its warps share: RG groups of
-// NT x 8 rows times 8 / RG stretches. The weights are the MMA's 16-row side (RT x 16 of them), the rows of x its 8-wide
-// side. The stretches of K of one CTA meet in shared memory, in order; those of several in `expand`.
-template <typename TX, typename TW, int RT, int NT, int RG>
+// Few rows: a CTA takes a tile's 16 rows, one projection and one of `splits` stretches of K, which its warps share. The
+// weights are the MMA's 16-row side (RT x 16 of them), the rows of x its 8-wide side. The stretches of K of one CTA meet in
+// shared memory, in order; those of several in `expand`.
+template <typename TX, typename TW, int RT>
 __global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XFrag<TX, TW>::kTf32) ? 1 : 2)
     adapter_shrink_kernel(const __grid_constant__ Params p) {
   using F = XFrag<TX, TW>;
-  constexpr int KG = kThreads / 32 / RG, kRows = RG * NT * 8;
+  constexpr int KG = kThreads / 32, NT = 2, kRows = kSmall;
   extern __shared__ float red[];  // [KG][kRows][RT * 16 + 4]
   constexpr int kPitch = RT * 16 + 4;
   pdl_wait();
   pdl_launch_dependents();  // (behind the wait: `expand` reads the plan before its own)
-  if (!plan_ok(p)) return;
-  constexpr int kParts = RG == 1 ? 1 : kLarge / kRows;  // of a tile
-  const int split = blockIdx.x % p.splits, seg = blockIdx.x / p.splits % p.nseg, part = blockIdx.x / (p.splits * p.nseg);
-  const int ti = part / kParts;
-  if (ti >= p.head[p.which]) return;
-  Tile tile = p.tiles[ti];
-  tile.begin += part % kParts * kRows;
-  tile.count = min(tile.count - part % kParts * kRows, kRows);
-  if (tile.adapter < 0 || tile.count <= 0) return;
+  const int split = blockIdx.x % p.splits, seg = blockIdx.x / p.splits % p.nseg, ti = blockIdx.x / (p.splits * p.nseg);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  // head, tile and rows in one round trip (the list has room for every CTA's tile)
+  const SmallTile* st = p.small + ti;
+  const Tile tile = st->tile;
+  const int rows[2] = {st->rows[g], st->rows[8 + g]};
+  if (!plan_ok(p) || ti >= p.head[p.which] || tile.adapter < 0) return;
   const int rank = rank_of(p, tile.adapter);
   if (rank == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int rg = warp % RG, kg = warp / RG;
   const Seg& s = p.seg[seg];
   const int steps = (p.K + 31) / 32, ways = p.splits * KG;
-  const int way = split * KG + kg, k0 = (int)((int64_t)way * steps / ways), k1 = (int)((int64_t)(way + 1) * steps / ways);
+  const int way = split * KG + warp, k0 = (int)((int64_t)way * steps / ways), k1 = (int)((int64_t)(way + 1) * steps / ways);
   const TW* a = static_cast<const TW*>(s.a) + tile.adapter * s.a_adapter + 8 * t;
   const TX* x[NT];
   bool on[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    const int r = (rg * NT + j) * 8 + g;
-    on[j] = r < tile.count;
-    x[j] = static_cast<const TX*>(p.x) + (on[j] ? p.order[tile.begin + r] * p.x_row : 0) + 8 * t;
+    on[j] = j * 8 + g < tile.count;
+    x[j] = static_cast<const TX*>(p.x) + (on[j] ? rows[j] * p.x_row : 0) + 8 * t;
   }
   float c[RT][NT][4];
 #pragma unroll
   for (int m = 0; m < RT; ++m)
 #pragma unroll
     for (int j = 0; j < NT; ++j) c[m][j][0] = c[m][j][1] = c[m][j][2] = c[m][j][3] = 0.f;
-  const int mts = (rank + 15) / 16;
-  if (rg * NT * 8 < tile.count) {
+  const int mts = (rank + 15) / 16, nts = (tile.count + 7) / 8;
 #pragma unroll 1
-    for (int ks = k0; ks < k1; ++ks) {
-      const int k = ks * 32;
-      const bool kin = k + 8 * t < p.K;
-      uint4 xw[NT][F::kLoads], lo[RT], hi[RT];
+  for (int ks = k0; ks < k1; ++ks) {
+    const int k = ks * 32;
+    const bool kin = k + 8 * t < p.K;
+    uint4 xw[NT][F::kLoads], lo[RT], hi[RT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int l = 0; l < F::kLoads; ++l) xw[j][l] = ld16(x[j] + k + 4 * l, kin && on[j]);
+      for (int l = 0; l < F::kLoads; ++l) xw[j][l] = ld16(x[j] + k + 4 * l, kin && on[j]);
 #pragma unroll
-      for (int m = 0; m < RT; ++m) {
-        lo[m] = ld16(a + (int64_t)(m * 16 + g) * s.a_row + k, kin && m < mts && m * 16 + g < p.R);
-        hi[m] = ld16(a + (int64_t)(m * 16 + 8 + g) * s.a_row + k, kin && m < mts && m * 16 + 8 + g < p.R);
-      }
-      if constexpr (!F::kF32) {
-#pragma unroll
-        for (int m = 0; m < RT; ++m)
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            mma16<TW>(c[m][j], lo[m].x, hi[m].x, lo[m].y, hi[m].y, xw[j][0].x, xw[j][0].y);
-            mma16<TW>(c[m][j], lo[m].z, hi[m].z, lo[m].w, hi[m].w, xw[j][0].z, xw[j][0].w);
-          }
-      } else if constexpr (!F::kTf32) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const uint32_t w[8] = {xw[j][0].x, xw[j][0].y, xw[j][0].z, xw[j][0].w,
-                                 xw[j][1].x, xw[j][1].y, xw[j][1].z, xw[j][1].w};
-          uint32_t term[3][4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float v0 = __uint_as_float(w[2 * i]), v1 = __uint_as_float(w[2 * i + 1]);
-            term[0][i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);  // cut off: never beyond fp32's range
-            const float r0 = rest(v0, __uint_as_float(w[2 * i] & 0xffff0000u));
-            const float r1 = rest(v1, __uint_as_float(w[2 * i + 1] & 0xffff0000u));
-            term[1][i] = pack2<__nv_bfloat16>(r0, r1);
-            const float2 mid = unpack2<__nv_bfloat16>(term[1][i]);
-            term[2][i] = pack2<__nv_bfloat16>(r0 - mid.x, r1 - mid.y);
-          }
-#pragma unroll
-          for (int e = 2; e >= 0; --e)
-#pragma unroll
-            for (int m = 0; m < RT; ++m) {
-              mma16<TW>(c[m][j], lo[m].x, hi[m].x, lo[m].y, hi[m].y, term[e][0], term[e][1]);
-              mma16<TW>(c[m][j], lo[m].z, hi[m].z, lo[m].w, hi[m].w, term[e][2], term[e][3]);
-            }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // the lane's elements 2 i and 2 i + 1
-          uint32_t big[NT][2], small[NT][2];
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint4 v4 = xw[j][i >> 1];
-              const uint32_t w = i & 1 ? (e ? v4.w : v4.z) : (e ? v4.y : v4.x);
-              big[j][e] = w & 0xffffe000u;
-              const float r = rest(__uint_as_float(w), __uint_as_float(big[j][e]));
-              asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(small[j][e]) : "f"(r));
-            }
-#pragma unroll
-          for (int m = 0; m < RT; ++m) {
-            const uint32_t wl = i == 0 ? lo[m].x : i == 1 ? lo[m].y : i == 2 ? lo[m].z : lo[m].w;
-            const uint32_t wh = i == 0 ? hi[m].x : i == 1 ? hi[m].y : i == 2 ? hi[m].z : hi[m].w;
-            const float2 fl = unpack2<TW>(wl), fh = unpack2<TW>(wh);
-            const uint32_t a0 = __float_as_uint(fl.x), a1 = __float_as_uint(fh.x), a2 = __float_as_uint(fl.y),
-                           a3 = __float_as_uint(fh.y);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              mma_tf32(c[m][j], a0, a1, a2, a3, small[j][0], small[j][1]);
-              mma_tf32(c[m][j], a0, a1, a2, a3, big[j][0], big[j][1]);
-            }
-          }
-        }
-      }
+    for (int m = 0; m < RT; ++m) {
+      lo[m] = ld16(a + (int64_t)(m * 16 + g) * s.a_row + k, kin && m < mts && m * 16 + g < p.R);
+      hi[m] = ld16(a + (int64_t)(m * 16 + 8 + g) * s.a_row + k, kin && m < mts && m * 16 + 8 + g < p.R);
     }
+    products<TX, TW, RT, NT>(c, lo, hi, xw, mts, nts);
   }
-  // c[m][j]: weight rows 16 m + g and + 8, rows 8 j + 2 t and + 1 of the group
-  float* mine = red + (kg * kRows + rg * NT * 8) * kPitch;
+  // c[m][j]: weight rows 16 m + g and + 8, rows 8 j + 2 t and + 1
+  float* mine = red + warp * kRows * kPitch;
 #pragma unroll
   for (int m = 0; m < RT; ++m)
 #pragma unroll
@@ -288,150 +323,289 @@ __global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XFrag<TX, TW>
   }
 }
 
+// Prompts: a CTA takes a tile's 128 rows, one projection and one of `splits` stretches of K. x and the weights come
+// through a ring in shared memory, 128 bytes of each row of x at a time (64 elements, 32 of fp32), which keeps 16 KB a
+// stage under way: with operands loaded as above a step waits out the memory's latency (6007 rows of 5120 in bf16:
+// 39 us; XX here). The MMAs' rate is not what bounds it: 8 us of it there.
+//
+// Warp (rg, kg) has NT x 8 of the rows and, of two, one 32-wide step of a stage. A word lies at its place ^ f(row), f
+// such that the lanes that read together, four words of two neighbouring rows, meet no bank twice.
+template <typename TX, typename TW, int RT>
+struct Long {
+  static constexpr int NT = RT <= 4 && !std::is_same_v<TX, float> ? 4 : 2;
+  static constexpr int RG = kLarge / (NT * 8), KG = kThreads / 32 / RG;
+  static constexpr int MB = RT < 2 ? RT : 2;
+  static constexpr int kStep = 128 / (int)sizeof(TX), kSteps = kStep / 32;  // elements of a stage; 32-wide steps
+  static constexpr int kXBytes = kLarge * 128, kARow = kStep * 2, kABytes = RT * 16 * kARow;
+  static constexpr int kStage = kXBytes + kABytes, kStages = RT == 8 ? 3 : 4;
+  static constexpr int kPitch = RT * 16 + 4, kRed = KG * kLarge * kPitch * 4;
+  static constexpr int kSmem = kStages * kStage > kRed ? kStages * kStage : kRed;
+};
+__device__ __forceinline__ int spread(int row) { return ((row & 1) << 2) | ((row >> 1) & 3); }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {  // zeros where not on
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+template <typename TX, typename TW, int RT>
+__global__ void __launch_bounds__(kThreads, RT == 8 && XFrag<TX, TW>::kF32 ? 1 : 2)
+    adapter_shrink_long_kernel(const __grid_constant__ Params p) {
+  using F = XFrag<TX, TW>;
+  using L = Long<TX, TW, RT>;
+  constexpr int NT = L::NT, KG = L::KG, kPer = 16 / (int)sizeof(TX);  // elements of x in a 16-byte word
+  extern __shared__ __align__(128) uint8_t smem[];
+  pdl_wait();
+  pdl_launch_dependents();  // (behind the wait: the grids behind this one read the plan before their own)
+  if (!plan_ok(p)) return;
+  const int split = blockIdx.x % p.splits, seg = blockIdx.x / p.splits % p.nseg, ti = blockIdx.x / (p.splits * p.nseg);
+  if (ti >= p.head[p.which]) return;
+  const Tile tile = p.tiles[ti];
+  if (tile.adapter < 0) return;
+  const int rank = rank_of(p, tile.adapter);
+  if (rank == 0) return;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int rg = warp % L::RG, kg = warp / L::RG;
+  const Seg& s = p.seg[seg];
+  const int all = (p.K + L::kStep - 1) / L::kStep;
+  const int s0 = (int)((int64_t)split * all / p.splits), s1 = (int)((int64_t)(split + 1) * all / p.splits);
+  const int mts = (rank + 15) / 16;
+  const uint32_t sbase = smem_u32(smem);
+  // this thread's words of a stage: word tid % 8 of the rows tid / 8 + 32 i of x, and some of the weights
+  int from[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) from[i] = tid / 8 + 32 * i < tile.count ? p.order[tile.begin + tid / 8 + 32 * i] : -1;
+  const TW* a = static_cast<const TW*>(s.a) + tile.adapter * s.a_adapter;
+  constexpr int kAWords = L::kARow / 16;  // of a row of the weights
+  const int arows = min(mts * 16, p.R);
+  auto load = [&](int st) {
+    if (st < s1) {
+      const int k0 = st * L::kStep;
+      const uint32_t to = sbase + (st - s0) % L::kStages * L::kStage;
+      const int k = k0 + tid % 8 * kPer;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = tid / 8 + 32 * i;
+        const bool there = from[i] >= 0 && k < p.K;
+        cp_async16(to + r * 128 + ((tid % 8 ^ spread(r)) << 4),
+                   static_cast<const TX*>(p.x) + (there ? from[i] * p.x_row + k : 0), there);
+      }
+#pragma unroll
+      for (int w = tid; w < RT * 16 * kAWords; w += kThreads) {
+        const int r = w / kAWords, c = w % kAWords;
+        const bool there = r < arows && k0 + c * 8 < p.K;
+        cp_async16(to + L::kXBytes + r * L::kARow + ((kAWords == 8 ? c ^ spread(r) : c) << 4),
+                   there ? a + (int64_t)r * s.a_row + k0 + c * 8 : a, there);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  float c[RT / L::MB][L::MB][NT][4];
+#pragma unroll
+  for (int m = 0; m < RT; ++m)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[m / L::MB][m % L::MB][j][e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < L::kStages - 1; ++i) load(s0 + i);
+#pragma unroll 1
+  for (int st = s0; st < s1; ++st) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+    __syncthreads();  // this stage is there for all, and the one before it has been read by all
+    load(st + L::kStages - 1);
+    const uint8_t* xs = smem + (st - s0) % L::kStages * L::kStage;
+    const uint8_t* as = xs + L::kXBytes;
+    if (rg * NT * 8 >= tile.count) continue;
+#pragma unroll
+    for (int h = 0; h < L::kSteps; ++h) {
+      if (KG > 1 && h != kg) continue;
+      uint4 xw[NT][F::kLoads];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int r = (rg * NT + j) * 8 + g;
+#pragma unroll
+        for (int l = 0; l < F::kLoads; ++l) {
+          const int w = F::kF32 ? 2 * t + l : 4 * h + t;
+          xw[j][l] = *reinterpret_cast<const uint4*>(xs + r * 128 + ((w ^ spread(r)) << 4));
+        }
+      }
+      // (two of the weights' 16 rows at a time: all of them at once leave no registers for a second CTA)
+#pragma unroll
+      for (int m0 = 0; m0 < RT; m0 += L::MB) {
+        if (m0 >= mts) break;
+        uint4 lo[L::MB], hi[L::MB];
+#pragma unroll
+        for (int m = 0; m < L::MB; ++m) {
+          const int r = (m0 + m) * 16 + g, w = kAWords == 8 ? 4 * h + t : t;
+          lo[m] = *reinterpret_cast<const uint4*>(as + r * L::kARow + ((kAWords == 8 ? w ^ spread(r) : w) << 4));
+          hi[m] = *reinterpret_cast<const uint4*>(as + (r + 8) * L::kARow + ((kAWords == 8 ? w ^ spread(r) : w) << 4));
+        }
+        products<TX, TW, L::MB, NT>(c[m0 / L::MB], lo, hi, xw, mts - m0, NT);
+        if (RT > L::MB) asm volatile("" ::: "memory");
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  // c[m][j]: weight rows 16 m + g and + 8, rows 8 j + 2 t and + 1 of the warp's
+  float* red = reinterpret_cast<float*>(smem);
+  float* mine = red + (kg * kLarge + rg * NT * 8) * L::kPitch;
+#pragma unroll
+  for (int m = 0; m < RT; ++m)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[(j * 8 + 2 * t + (e & 1)) * L::kPitch + m * 16 + g + (e >> 1) * 8] = c[m / L::MB][m % L::MB][j][e];
+  __syncthreads();
+  const int quads = p.R / 4, live = min((rank + 3) / 4, quads);
+  float* h = p.h + ((int64_t)(split * p.nseg + seg) * p.T + tile.begin) * p.R;
+  for (int i = tid; i < tile.count * quads; i += kThreads) {
+    const int r = i / quads, q = i % quads;
+    if (q >= live) continue;
+    float4 v = *reinterpret_cast<const float4*>(red + r * L::kPitch + q * 4);
+    if constexpr (KG > 1) {
+      const float4 u = *reinterpret_cast<const float4*>(red + (kLarge + r) * L::kPitch + q * 4);
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    }
+    *reinterpret_cast<float4*>(h + (int64_t)r * p.R + q * 4) = v;
+  }
+}
+
 // ------------------------------------------------------------------ expand
 // Few rows: a CTA takes a tile's 16 rows and a stretch of the outputs of all projections, 32 at a time per warp. h's
 // terms lie in shared memory as the MMA's A operands, 16 bytes a lane; the weights are its 8-wide side, with the rows of
 // B so assigned that a lane ends up with 8 consecutive outputs of a row. (Prompts: adapters_tc.cu.)
-template <typename TW, typename TY>
-__global__ void __launch_bounds__(kExpand, 8) adapter_expand_kernel(const __grid_constant__ Params p) {
+template <typename TW, typename TY, int kBlocks>  // k32 blocks of R at most
+__global__ void __launch_bounds__(kExpand, kBlocks == 4 ? 5 : 6) adapter_expand_kernel(const __grid_constant__ Params p) {
   constexpr bool kHalf = std::is_same_v<TW, __half>, kY32 = std::is_same_v<TY, float>;
   constexpr int kTerms = !kHalf && kY32 ? 3 : 2;
   constexpr int kRows = kSmall;
   constexpr int kYWords = 8 * (int)sizeof(TY) / 16;  // 16-byte words of a lane's 8 outputs
   extern __shared__ uint4 frag[];  // [k32 blocks][2][terms][32]
   __shared__ float mul[kRows];
-  __shared__ int top[kRows];
   // The plan, the weights and base were complete before `shrink` let this grid start.
   // (A grid may only end after the one before it, or the one behind it starts too early: every way out waits.)
   pdl_launch_dependents();
-  if (!plan_ok(p)) {
-    pdl_wait();
-    return;
-  }
   const int range = blockIdx.x % p.ranges, ti = blockIdx.x / p.ranges;
-  if (ti >= p.head[p.which]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const SmallTile* st = p.small + ti;  // (read at once, as above)
+  const Tile tile = st->tile;
+  int row[2] = {st->rows[g], st->rows[8 + g]};
+  if (!plan_ok(p) || ti >= p.head[p.which]) {
     pdl_wait();
     return;
   }
-  const Tile tile = p.tiles[ti];
   const int rank = tile.adapter < 0 ? 0 : rank_of(p, tile.adapter);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int blocks = (rank + 31) / 32;
   // the CTA's pieces, of all projections in a line
   auto pieces = [&](int i) { return (p.seg[i].N + kExpand - 1) / kExpand; };
   int total = 0;
   for (int i = 0; i < p.nseg; ++i) total += pieces(i);
   const int first = (int)((int64_t)range * total / p.ranges), last = (int)((int64_t)(range + 1) * total / p.ranges);
-  int seg = 0, before = 0;  // pieces of the projections before seg
-  int row[2];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) row[e] = e * 8 + g < tile.count ? p.order[tile.begin + e * 8 + g] : -1;
-  bool waited = false;
-  int have = -1;  // the projection whose h lies in shared memory
-  for (int piece = first; piece < last; ++piece) {
-    for (int k; piece - before >= (k = pieces(seg)); ++seg) before += k;
-    const Seg& s = p.seg[seg];
-    const int n0 = (piece - before) * kExpand + warp * 32;
-    const bool copy = rank == 0;
-    if (copy && s.base == s.y && s.base_row == s.y_row) continue;  // in place: stays
-    // weights of the first k32 block and base on their way before h is looked at
+  for (int e = 0; e < 2; ++e)
+    if (e * 8 + g >= tile.count) row[e] = -1;
+  const bool copy = rank == 0;
+  // A piece's projection, the warp's first output of it, and what of it does not depend on h: the weights of the first
+  // k32 block and base.
+  struct Piece {
+    int seg, n0;
+    bool vec;
+    uint4 wb[4], bv[2][kYWords];
+  };
+  auto load_b = [&](const Piece& q, uint4 (&w)[4], int kb) {
+    const Seg& s = p.seg[q.seg];
     const TW* b = static_cast<const TW*>(s.b) + (copy ? 0 : tile.adapter * s.b_adapter) + 8 * t;
-    auto load_b = [&](uint4 (&w)[4], int kb) {
-      const int k = kb * 32 + 8 * t, valid = rank - k;
+    const int k = kb * 32 + 8 * t, valid = rank - k;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
-        w[j] = ld16(b + (int64_t)n * s.b_row + kb * 32, valid > 0 && n < s.N);
-        if (valid > 0 && valid < 8) {  // columns behind the adapter's rank may hold anything
-          uint32_t v[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+    for (int j = 0; j < 4; ++j) {
+      const int n = q.n0 + 8 * (g >> 1) + 2 * j + (g & 1);
+      w[j] = ld16(b + (int64_t)n * s.b_row + kb * 32, valid > 0 && n < s.N);
+      if (valid > 0 && valid < 8) {  // columns behind the adapter's rank may hold anything
+        uint32_t v[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] &= valid >= 2 * i + 2 ? 0xffffffffu : valid == 2 * i + 1 ? 0xffffu : 0u;
-          w[j] = make_uint4(v[0], v[1], v[2], v[3]);
-        }
+        for (int i = 0; i < 4; ++i) v[i] &= valid >= 2 * i + 2 ? 0xffffffffu : valid == 2 * i + 1 ? 0xffffu : 0u;
+        w[j] = make_uint4(v[0], v[1], v[2], v[3]);
       }
-    };
-    uint4 wb[4];
-    load_b(wb, 0);
-    const int n8 = n0 + 8 * t;  // the lane's outputs
-    uint4 bv[2][kYWords];
-    const bool vec = s.vec && n8 + 8 <= s.N;
-    if (s.base && vec) {
+    }
+  };
+  auto fetch = [&](Piece& q, int piece) {
+    if (piece >= last) return;
+    q.seg = 0;
+    for (int k; piece >= (k = pieces(q.seg)); ++q.seg) piece -= k;
+    const Seg& s = p.seg[q.seg];
+    q.n0 = piece * kExpand + warp * 32;
+    load_b(q, q.wb, 0);
+    const int n8 = q.n0 + 8 * t;  // the lane's outputs
+    q.vec = s.vec && n8 + 8 <= s.N;
+    if (!s.base || !q.vec) return;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int w = 0; w < kYWords; ++w)
-          bv[e][w] = row[e] >= 0 ? *(reinterpret_cast<const uint4*>(static_cast<const TY*>(s.base) + row[e] * s.base_row + n8) + w)
+      for (int w = 0; w < kYWords; ++w)
+        q.bv[e][w] = row[e] >= 0 ? *(reinterpret_cast<const uint4*>(static_cast<const TY*>(s.base) + row[e] * s.base_row + n8) + w)
                                  : make_uint4(0, 0, 0, 0);
-    }
-    if (!waited) {
-      pdl_wait();
-      waited = true;
-    }
+  };
+  int have = -1;  // the projection whose h lies in shared memory
+  Piece now, next;
+  fetch(now, first);
+  pdl_wait();
+  for (int piece = first; piece < last; ++piece, now = next) {
+    fetch(next, piece + 1);
+    const int seg = now.seg;
+    const Seg& s = p.seg[seg];
+    if (copy && s.base == s.y && s.base_row == s.y_row) continue;  // in place: stays
     if (have != seg && !copy) {
       __syncthreads();  // nobody reads the one before any more
       have = seg;
-      const int chunks = blocks * 4;  // of 8 elements of h
-      const float* h = p.h + ((int64_t)seg * p.T + tile.begin) * p.R;
-      const int64_t next = (int64_t)p.nseg * p.T * p.R;
-      auto sum = [&](int u, float (&v)[8]) {
-        const int r = u / chunks, k = u % chunks * 8;
+      // four threads a row: each the words that the lane of its place takes, of every k32 block
+      const int r = threadIdx.x >> 2, l = threadIdx.x & 3;
+      const bool there = r < tile.count;
+      const float* h = p.h + ((int64_t)seg * p.T + tile.begin + r) * p.R + l * 8;
+      const int64_t stretch = (int64_t)p.nseg * p.T * p.R;
+      float v[kBlocks][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        if (r >= tile.count || k >= rank) return;
-        const float* from = h + (int64_t)r * p.R + k;
-#pragma unroll 4
-        for (int q = 0; q < p.splits; ++q, from += next) {
-          const float4 v0 = ld_cg(from), v1 = ld_cg(from + 4);
-          v[0] += v0.x, v[1] += v0.y, v[2] += v0.z, v[3] += v0.w;
-          v[4] += v1.x, v[5] += v1.y, v[6] += v1.z, v[7] += v1.w;
-        }
+      for (int kb = 0; kb < kBlocks; ++kb)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (k + i >= rank) v[i] = 0.f;
-      };
-      if constexpr (kHalf) {  // each row over a power of two: its largest in [2^14, 2^15)
-        for (int r = threadIdx.x; r < kRows; r += kExpand) top[r] = 0;
-        __syncthreads();
-        for (int u = threadIdx.x; u < kRows * chunks; u += kExpand) {
-          float v[8];
-          sum(u, v);
-          float m = 0.f;
+        for (int i = 0; i < 8; ++i) v[kb][i] = 0.f;
+#pragma unroll (8 / kBlocks)
+      for (int q = 0; q < p.splits; ++q, h += stretch) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
-          atomicMax(&top[u / chunks], __float_as_int(m));
-        }
-        __syncthreads();
-      }
-      const float scale = p.scales ? p.scales[tile.adapter] : 1.f;
-      for (int r = threadIdx.x; r < kRows; r += kExpand) {
-        if constexpr (kHalf) {
-          const int e = (top[r] >> 23) - 127;  // of the largest; 0, denormal and infinite rows stay as they are
-          mul[r] = e >= -112 && e < 128 ? scale * __int_as_float((e - 14 + 127) << 23) : scale;
-        } else {
-          mul[r] = scale;
+        for (int kb = 0; kb < kBlocks; ++kb) {
+          if (!there || kb * 32 + l * 8 >= rank) continue;
+          const float4 v0 = ld_cg(h + kb * 32), v1 = ld_cg(h + kb * 32 + 4);
+          v[kb][0] += v0.x, v[kb][1] += v0.y, v[kb][2] += v0.z, v[kb][3] += v0.w;
+          v[kb][4] += v1.x, v[kb][5] += v1.y, v[kb][6] += v1.z, v[kb][7] += v1.w;
         }
       }
-      for (int u = threadIdx.x; u < kRows * chunks; u += kExpand) {
-        float v[8];
-        sum(u, v);
-        const int r = u / chunks, k = u % chunks;
-        if constexpr (kHalf) {
-          const int e = (top[r] >> 23) - 127;
-          const float f = e >= -112 && e < 128 ? __int_as_float((14 - e + 127) << 23) : 1.f;
+      float f = 1.f, back = p.scales ? p.scales[tile.adapter] : 1.f, m = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= f;
+      for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (kb * 32 + l * 8 + i >= rank) v[kb][i] = 0.f;
+          m = fmaxf(m, fabsf(v[kb][i]));
         }
+      if constexpr (kHalf) {  // the row over a power of two: its largest in [2^14, 2^15)
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const int e = (__float_as_int(m) >> 23) - 127;  // 0, denormal and infinite rows stay as they are
+        if (e >= -112 && e < 128) f = __int_as_float((14 - e + 127) << 23), back *= __int_as_float((e - 14 + 127) << 23);
+      }
+      if (l == 0) mul[r] = back;
+#pragma unroll
+      for (int kb = 0; kb < kBlocks; ++kb) {
+        if (kb >= blocks) break;
         // row r of its 16: g = r % 8, words 0 and 2 (r < 8) or 1 and 3
-        uint32_t* to = reinterpret_cast<uint32_t*>(frag + (k >> 2) * 2 * kTerms * 32 + (r & 7) * 4 + (k & 3)) + (r >> 3);
+        uint32_t* to = reinterpret_cast<uint32_t*>(frag + kb * 2 * kTerms * 32 + (r & 7) * 4 + l) + (r >> 3);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float v0 = v[2 * i], v1 = v[2 * i + 1];
+          float v0 = v[kb][2 * i] * f, v1 = v[kb][2 * i + 1] * f;
 #pragma unroll
           for (int e = 0; e < kTerms; ++e) {
             const uint32_t w = pack2<TW>(v0, v1);
             to[(((i >> 1) * kTerms + e) * 32) * 4 + (i & 1) * 2] = w;
-            const float2 f = unpack2<TW>(w);
-            v0 = rest(v0, f.x), v1 = rest(v1, f.y);
+            const float2 u = unpack2<TW>(w);
+            v0 = rest(v0, u.x), v1 = rest(v1, u.y);
           }
         }
       }
@@ -443,19 +617,18 @@ __global__ void __launch_bounds__(kExpand, 8) adapter_expand_kernel(const __grid
 #pragma unroll 1
     for (int kb = 0; kb < blocks; ++kb) {
       uint4 wn[4];
-      if (kb + 1 < blocks) load_b(wn, kb + 1);
+      if (kb + 1 < blocks) load_b(now, wn, kb + 1);
       const uint4* f = frag + (int64_t)kb * 2 * kTerms * 32 + lane;
 #pragma unroll
       for (int e = kTerms - 1; e >= 0; --e) {
         const uint4 a0 = f[e * 32], a1 = f[(kTerms + e) * 32];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma16<TW>(c[j], a0.x, a0.y, a0.z, a0.w, wb[j].x, wb[j].y);
-          mma16<TW>(c[j], a1.x, a1.y, a1.z, a1.w, wb[j].z, wb[j].w);
-        }
+        for (int j = 0; j < 4; ++j) mma16<TW>(c[j], a0.x, a0.y, a0.z, a0.w, now.wb[j].x, now.wb[j].y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma16<TW>(c[j], a1.x, a1.y, a1.z, a1.w, now.wb[j].z, now.wb[j].w);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) wb[j] = wn[j];
+      for (int j = 0; j < 4; ++j) now.wb[j] = wn[j];
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -464,16 +637,16 @@ __global__ void __launch_bounds__(kExpand, 8) adapter_expand_kernel(const __grid
       float v[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[2 * j] = c[j][2 * e] * f, v[2 * j + 1] = c[j][2 * e + 1] * f;
-      TY* y = static_cast<TY*>(s.y) + row[e] * s.y_row + n8;
-      if (vec) {
+      TY* y = static_cast<TY*>(s.y) + row[e] * s.y_row + now.n0 + 8 * t;
+      if (now.vec) {
         if (s.base) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if constexpr (kY32) {
-              const uint4 w = bv[e][i >> 1];
+              const uint4 w = now.bv[e][i >> 1];
               v[2 * i] += __uint_as_float(i & 1 ? w.z : w.x), v[2 * i + 1] += __uint_as_float(i & 1 ? w.w : w.y);
             } else {
-              const uint4 w = bv[e][0];
+              const uint4 w = now.bv[e][0];
               const float2 q = unpack2<TY>(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w);
               v[2 * i] += q.x, v[2 * i + 1] += q.y;
             }
@@ -487,14 +660,13 @@ __global__ void __launch_bounds__(kExpand, 8) adapter_expand_kernel(const __grid
                                                     pack2<TY>(v[6], v[7]));
         }
       } else {
-        const TY* base = s.base ? static_cast<const TY*>(s.base) + row[e] * s.base_row + n8 : nullptr;
+        const TY* base = s.base ? static_cast<const TY*>(s.base) + row[e] * s.base_row + now.n0 + 8 * t : nullptr;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (n8 + i < s.N) y[i] = from_f32<TY>(base ? v[i] + to_f32(base[i]) : v[i]);
+          if (now.n0 + 8 * t + i < s.N) y[i] = from_f32<TY>(base ? v[i] + to_f32(base[i]) : v[i]);
       }
     }
   }
-  if (!waited) pdl_wait();
 }
 
 // ------------------------------------------------------------------ launches
@@ -514,9 +686,8 @@ Shape shape_of(const DeviceInfo& d, int T, int K, int nseg, int n) {
   s.large = T > 256;
   const int rows = s.large ? kLarge : kSmall;
   s.tiles = T / rows + std::min(n + 1, T);
-  const int steps = (K + 31) / 32, warps = s.large ? 4 : 8;  // that share a CTA's stretch
-  const int want = 2 * d.sm_count / (s.tiles * nseg * (s.large ? 2 : 1));
-  s.splits = std::max(1, std::min({want, kMaxSplits, (steps + warps - 1) / warps}));
+  const int least = s.large ? 512 : 256;  // of K that a stretch has
+  s.splits = std::max(1, std::min({2 * d.sm_count / (s.tiles * nseg), kMaxSplits, (K + least - 1) / least}));
   return s;
 }
 // The workspace: h, and for prompts its terms and the rows' factors.
@@ -529,21 +700,18 @@ struct Work {
   }
 };
 
-template <typename TX, typename TW, int RT, int NT, int RG>
-cudaError_t shrink(const Params& p, int tiles, cudaStream_t st, bool setup) {
-  constexpr int smem = 8 / RG * (RG * NT * 8) * (RT * 16 + 4) * 4;
-  if (setup)
-    return cudaFuncSetAttribute(adapter_shrink_kernel<TX, TW, RT, NT, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  return launch_pdl(adapter_shrink_kernel<TX, TW, RT, NT, RG>, dim3((unsigned)(tiles * p.nseg * p.splits * (RG == 1 ? 1 : kLarge / (RG * NT * 8)))), dim3(kThreads),
-                    smem, st, p);
-}
 template <typename TX, typename TW, int RT>
 cudaError_t shrink_rt(const Params& p, bool large, int tiles, cudaStream_t st, bool setup) {
-  // 64 rows: 32 a warp where the accumulators leave room for it, else 16
-  constexpr int NT = RT <= 4 && !std::is_same_v<TX, float> ? 4 : 2;
-  if (setup)
-    if (cudaError_t e = shrink<TX, TW, RT, 2, 1>(p, tiles, st, true)) return e;
-  return large || setup ? shrink<TX, TW, RT, NT, 8 / NT>(p, tiles, st, setup) : shrink<TX, TW, RT, 2, 1>(p, tiles, st, false);
+  constexpr int smem = kThreads / 32 * kSmall * (RT * 16 + 4) * 4, smem_long = Long<TX, TW, RT>::kSmem;
+  static_assert(Long<TX, TW, RT>::KG <= 2 && smem_long <= 113 * 1024);
+  if (setup) {
+    if (cudaError_t e = cudaFuncSetAttribute(adapter_shrink_kernel<TX, TW, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
+      return e;
+    return cudaFuncSetAttribute(adapter_shrink_long_kernel<TX, TW, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_long);
+  }
+  const dim3 grid((unsigned)(tiles * p.nseg * p.splits));
+  return large ? launch_pdl(adapter_shrink_long_kernel<TX, TW, RT>, grid, dim3(kThreads), (size_t)smem_long, st, p)
+               : launch_pdl(adapter_shrink_kernel<TX, TW, RT>, grid, dim3(kThreads), (size_t)smem, st, p);
 }
 template <typename TX, typename TW>
 cudaError_t shrink_r(const Params& p, bool large, int tiles, cudaStream_t st) {
@@ -566,9 +734,14 @@ cudaError_t expand(Params p, int tiles, int sms, cudaStream_t st) {
   constexpr int terms = std::is_same_v<TW, __half> || !std::is_same_v<TY, float> ? 2 : 3;
   int64_t pieces = 0;
   for (int i = 0; i < p.nseg; ++i) pieces += (p.seg[i].N + kExpand - 1) / kExpand;
-  p.ranges = (int)std::max<int64_t>(1, std::min<int64_t>(pieces, (8 * sms + tiles - 1) / tiles));
-  return launch_pdl(adapter_expand_kernel<TW, TY>, dim3((unsigned)(tiles * p.ranges)), dim3(kExpand),
-                    (size_t)(p.R + 31) / 32 * 2 * terms * 512, st, p);
+  // as many pieces each as make about one wave of CTAs
+  const int64_t per = std::max<int64_t>(1, (pieces * tiles + 8 * sms - 1) / (8 * sms));
+  p.ranges = (int)((pieces + per - 1) / per);
+  const dim3 grid((unsigned)(tiles * p.ranges));
+  const size_t smem = (size_t)(p.R + 31) / 32 * 2 * terms * 512;
+  return p.R <= 32   ? launch_pdl(adapter_expand_kernel<TW, TY, 1>, grid, dim3(kExpand), smem, st, p)
+         : p.R <= 64 ? launch_pdl(adapter_expand_kernel<TW, TY, 2>, grid, dim3(kExpand), smem, st, p)
+                     : launch_pdl(adapter_expand_kernel<TW, TY, 4>, grid, dim3(kExpand), smem, st, p);
 }
 
 }  // namespace
@@ -674,7 +847,8 @@ int btf_adapters(const btf_adapters_args* a, void* stream) {
   p.ranks = a->ranks, p.scales = a->scales;
   p.head = reinterpret_cast<const int32_t*>(plan), p.order = reinterpret_cast<const int32_t*>(plan + at.order);
   p.owner = reinterpret_cast<const int32_t*>(plan + at.owner);
-  p.tiles = reinterpret_cast<const Tile*>(plan + (sh.large ? at.large : at.small)), p.which = sh.large ? 3 : 2;
+  p.tiles = reinterpret_cast<const Tile*>(plan + at.large), p.small = reinterpret_cast<const SmallTile*>(plan + at.small);
+  p.which = sh.large ? 3 : 2;
   uint8_t* work = static_cast<uint8_t*>(a->work);
   p.h = reinterpret_cast<float*>(work), p.terms = reinterpret_cast<uint16_t*>(work + w.terms), p.mul = reinterpret_cast<float*>(work + w.mul);
   p.err = dev->err_word;

@@ -15,6 +15,10 @@ constexpr int kErrPlan = 2;  // device error word: a plan of other sizes
 struct Tile {
   int adapter, begin, count, unused;  // adapter -1: rows without one
 };
+struct SmallTile {
+  Tile tile;
+  int32_t rows[kSmall];  // the first `count` of them
+};
 // The plan in memory: 8 words {T, adapters, small tiles, large tiles, rows with an
 // adapter}, the rows in order, the adapter of each (n: none), then both lists of tiles.
 struct PlanLayout {
@@ -24,8 +28,8 @@ struct PlanLayout {
     order = 32;
     owner = order + 4 * T;
     small = (owner + 4 * T + 15) / 16 * 16;
-    large = small + 16 * (T / kSmall + lists);
-    bytes = large + 16 * (T / kLarge + lists);
+    large = small + (int64_t)sizeof(SmallTile) * (T / kSmall + lists);
+    bytes = large + (int64_t)sizeof(Tile) * (T / kLarge + lists);
   }
 };
 
@@ -44,7 +48,8 @@ struct Params {
   const int32_t* ranks;
   const float* scales;
   const int32_t *head, *order, *owner;
-  const Tile* tiles;
+  const Tile* tiles;  // the large ones
+  const SmallTile* small;
   int which;  // the plan's word with the number of tiles
   float* h;   // [splits][nseg][T][R]
   // prompts: h as the MMAs take it, [terms][nseg][T][R to whole 64], and each row's factor [nseg][T]

@@ -101,13 +101,15 @@ def test_plan_sorts_the_rows(cuda, btf, T, n):
     assert words[:2].tolist() == [T, n] and int(words[4]) == int((key < n).sum())
     small = (32 + 8 * T + 15) // 16 * 4
     lists = min(n + 1, T) + 1
-    for word, size, first in ((2, 16, small), (3, 128, small + 4 * (T // 16 + lists))):
-        tiles = words[first: first + 4 * int(words[word])].view(-1, 4)
+    for word, size, width, first in ((2, 16, 20, small), (3, 128, 4, small + 20 * (T // 16 + lists))):
+        tiles = words[first: first + width * int(words[word])].view(-1, width)
         want, at = [], 0
         for j, c in enumerate(torch.bincount(key, minlength=n + 1).tolist()):
             want += [[j if j < n else -1, at + i, min(size, c - i)] for i in range(0, c, size)]
             at += c
         assert tiles[:, :3].tolist() == want
+        if size == 16:  # with their rows
+            assert all(t[4: 4 + t[2]] == order[t[1]: t[1] + t[2]].tolist() for t in tiles.tolist())
 
 
 # ---------------------------------------------------------------- the call
