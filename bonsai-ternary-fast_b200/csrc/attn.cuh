@@ -134,18 +134,21 @@ struct RowPlace {
 // range and nearly half of the CTAs none, and behind elsewhere. 32 sequences are what a warp works out at once, a lane
 // each; what the 33rd of one kv-head costs: D = 128, 4096 rows 19.9 -> 20.6, D = 256 33.5 -> 39.1, 600 rows 15.2 -> 20.2.
 //
-// The table for the join: each sequence's first range, or first tile in the line of all tiles; then tiles per range, and
-// which of the two it is.
+// A pair on the line has `over` units in front of its tiles, the time of its q and its way out in tiles (0 where pairs
+// are few and long): with short pairs, equal numbers of tiles alone give one range many pairs and many times the work.
+//
+// The table for the join: each sequence's first range, or first unit on the line; then units per range, and which of the
+// two it is. The parts of a cut pair: two to a range, 1 for the pair whose first tile is in it.
 struct Segments {
   const AttnParams& p;
-  const int ranges, mt, range;
-  int b, kvh, tile, nt, index;  // the present one; index: in the CTA
-  int left;                     // tiles behind it
+  const int ranges, over, mt, range;
+  int b, kvh, tile, nt;         // the present one
+  int left;                     // units behind it
   Seq seq;
   // M tile block % mtiles of range block / mtiles (block < 0: no segment). Warp-uniform; every warp works it out for
   // itself. Writes the workspace's table when `table`.
-  __device__ __forceinline__ Segments(const AttnParams& p_, int block, int ranges_, bool table)
-      : p(p_), ranges(ranges_), mt(block % p_.mtiles), range(block / p_.mtiles), b(0), kvh(0), tile(0), nt(0), index(0), left(0) {
+  __device__ __forceinline__ Segments(const AttnParams& p_, int block, int ranges_, int over_, bool table)
+      : p(p_), ranges(ranges_), over(over_), mt(block % p_.mtiles), range(block / p_.mtiles), b(0), kvh(0), tile(0), nt(0), left(0) {
     if (block < 0) return;
     const int lane = threadIdx.x & 31;
     Seq mine;  // the lane's sequence of the 32 from b0
@@ -203,11 +206,12 @@ struct Segments {
       nt = (int)((int64_t)(part + 1) * seq.tiles / ns) - tile;
       return;
     }
+    auto units = [&]() { return mine.tiles ? (mine.tiles + over) * p.HK : 0; };
     int total = 0, t = 0;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
       load(b0);
-      t = up_to(mine.tiles * p.HK);
-      if (table && b0 + lane < p.B) p.first[b0 + lane] = total + t - mine.tiles * p.HK;
+      t = up_to(units());
+      if (table && b0 + lane < p.B) p.first[b0 + lane] = total + t - units();
       total += __shfl_sync(0xffffffffu, t, 31);
     }
     const int per = max(1, (total + ranges - 1) / ranges);
@@ -217,28 +221,32 @@ struct Segments {
     left = min(per, total - start);
     for (int b0 = 0;; b0 += 32) {  // the sequence that the range starts in
       load(b0);
-      t = up_to(mine.tiles * p.HK);
+      t = up_to(units());
       if (pick(b0, t, &start)) break;
       start -= __shfl_sync(0xffffffffu, t, 31);
     }
-    kvh = start / seq.tiles;
-    tile = start % seq.tiles;
-    nt = min(left, seq.tiles - tile);
-    left -= nt;
+    kvh = start / (seq.tiles + over);
+    take(start % (seq.tiles + over));
+    if (nt == 0) next();  // (the range begins with the end of a pair's units in front)
+  }
+  // The present pair from its unit `at`.
+  __device__ __forceinline__ void take(int at) {
+    const int to = min(at + left, seq.tiles + over);
+    left -= to - at;
+    tile = max(0, at - over);
+    nt = max(0, to - over) - tile;
   }
   __device__ __forceinline__ bool any() const { return nt > 0; }
   __device__ __forceinline__ void next() {
     nt = 0;
-    if (left == 0) return;
-    if (++kvh == p.HK) {
-      kvh = 0;
-      do seq = Seq(p, ++b);
-      while (seq.tiles == 0);
+    while (nt == 0 && left > 0) {
+      if (++kvh == p.HK) {
+        kvh = 0;
+        do seq = Seq(p, ++b);
+        while (seq.tiles == 0);
+      }
+      take(0);
     }
-    ++index;
-    tile = 0;
-    nt = min(left, seq.tiles);
-    left -= nt;
   }
   __device__ __forceinline__ int rows() const { return min(kRowsM, seq.count * (p.H / p.HK) - mt * kRowsM); }
   __device__ __forceinline__ int plane_b() const { return b * p.b_mul; }
@@ -248,18 +256,15 @@ struct Segments {
     const bool live = r < rows();
     return {b, live ? rr / G : 0, kvh * G + (live ? rr % G : 0), live};
   }
-  // By the table: the first range of a (sequence, kv-head), their number, and whether the first one begins with another
-  // pair's tiles.
-  static __device__ __forceinline__ int ranges_of(const AttnParams& p, const Seq& seq, int b, int kvh, int* n, bool* second) {
+  // By the table: the first range of a (sequence, kv-head), and their number.
+  static __device__ __forceinline__ int ranges_of(const AttnParams& p, int over, const Seq& seq, int b, int kvh, int* n) {
     const int per = p.first[p.B], first = p.first[b];
-    *second = false;
     if (p.first[p.B + 1]) {
       *n = (seq.tiles + per - 1) / per;
       return first + kvh * *n;
     }
-    const int t0 = first + kvh * seq.tiles, t1 = t0 + seq.tiles - 1, r0 = t0 / per;
+    const int t0 = first + kvh * (seq.tiles + over) + over, t1 = t0 + seq.tiles - 1, r0 = t0 / per;
     *n = t1 / per - r0 + 1;
-    *second = r0 * per < t0;
     return r0;
   }
 };

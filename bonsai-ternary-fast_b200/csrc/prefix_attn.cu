@@ -19,7 +19,7 @@ namespace btf {
 namespace {
 
 constexpr int kMaxChunks = 32;   // stretches of the shared rows: what a warp compares, a lane each
-constexpr float kSegTiles = 5;   // what a segment costs beside its tiles: q's way in and O's way out
+constexpr int kSegTiles = 5;     // what a segment costs beside its tiles: q's way in and O's way out
 
 struct PrefixParams : AttnParams {
   const int32_t* prefix_len;  // or null: all
@@ -54,7 +54,7 @@ struct Split {
     if (tiles == 0 || mtiles == 0) return;
     // lane i: the shared rows of each (kv-head, M tile) in i + 1 stretches
     const float streams = (float)p.HK * (float)mtiles;
-    const float mine = (float)p.HK * (float)p.mtiles * ((float)own + kSegTiles * (float)pairs);
+    const float mine = (float)p.HK * (float)p.mtiles * ((float)own + (float)(kSegTiles * pairs));
     // and what the slowest CTA then has, with the CTAs shared out so that both kinds end together: in w turns over
     // the shared rows' items, rounded down or up
     const int n = min(lane + 1, min(p.most_chunks, tiles));
@@ -89,7 +89,7 @@ struct PrefixSegments : Segments {
   __device__ __forceinline__ PrefixSegments(const PrefixParams& p_, bool warp0) : PrefixSegments(p_, warp0, Split(p_)) {}
   __device__ __forceinline__ PrefixSegments(const PrefixParams& p_, bool warp0, const Split& s)
       : Segments(p_, (int)blockIdx.x < s.ctas || (int)blockIdx.x >= s.ctas + s.ranges * p_.mtiles ? -1 : (int)blockIdx.x - s.ctas,
-                 s.ranges, warp0 && (int)blockIdx.x == s.ctas),
+                 s.ranges, kSegTiles, warp0 && (int)blockIdx.x == s.ctas),
         pp(p_), sp(s), shared((int)blockIdx.x < s.ctas), item((int)blockIdx.x), chunk(0), pmt(0) {
     if (shared) take();
     if (warp0 && (int)blockIdx.x == sp.ctas) {
@@ -144,7 +144,7 @@ struct PrefixSegments : Segments {
   __device__ __forceinline__ int64_t slot() const {
     if (shared) return shared_slot(pp, chunk, kvh, pmt);
     if (nt == seq.tiles) return pp.own_whole + (((int64_t)b * p.HK + kvh) * p.mtiles + mt) * pp.rpad;
-    return pp.own_part + ((int64_t)mt * 2 * ranges + 2 * range + (index > 0)) * pp.rpad;
+    return pp.own_part + ((int64_t)mt * 2 * ranges + 2 * range + (tile == 0)) * pp.rpad;
   }
   __device__ __forceinline__ RowPlace place(int r, bool on) const {
     if (!shared) return place_of(r);
@@ -182,7 +182,6 @@ struct PrefixSegments : Segments {
 
   struct Parts {
     int n, shared, own;
-    bool second;
     int64_t own_base, own_step, shared_base, shared_step;
     __device__ __forceinline__ Parts(const PrefixParams& p, const Seq& seq, int b, int node, int head) {
       const int G = p.H / p.HK, kvh = head / G, rr = node * G + head % G, mt = rr / kRowsM;
@@ -191,18 +190,16 @@ struct PrefixSegments : Segments {
       const int64_t ps = ((int64_t)p.first[p.B + 4 + b] + node) * G + head % G;
       shared_base = shared_slot(p, 0, kvh, (int)(ps / kRowsM)) + ps % kRowsM;
       shared_step = shared_slot(p, 1, 0, 0);
-      const int r0 = ranges_of(p, seq, b, kvh, &own, &second);
+      const int r0 = ranges_of(p, kSegTiles, seq, b, kvh, &own);
       own_step = 2 * p.rpad;
       own_base = own == 1 ? p.own_whole + (((int64_t)b * p.HK + kvh) * p.mtiles + mt) * p.rpad + rr % kRowsM
                           : p.own_part + ((int64_t)mt * 2 * ranges + 2 * r0) * p.rpad + rr % kRowsM;
-      second = second && own > 1;
-      if (second) own_base += p.rpad;
       n = shared == 0 && own == 1 ? 0 : shared + own;
     }
     __device__ __forceinline__ int64_t operator()(int s) const {
       if (s < shared) return shared_base + s * shared_step;
       s -= shared;
-      return own_base + s * own_step - (second && s > 0 ? own_step / 2 : 0);
+      return own_base + s * own_step + (own > 1 && s == 0 ? own_step / 2 : 0);
     }
   };
 };
@@ -310,7 +307,8 @@ int btf_prefix_attention(const btf_tree_attn* a, const btf_prefix* s, void* stre
   if (a->work_bytes < plan.bytes)
     return fail(BTF_ERR_ARG, "%s: the workspace has %lld bytes, %lld are needed", what, (long long)a->work_bytes,
                 (long long)plan.bytes);
-  if (plan.ctas > 1024 || attn_too_many(*a) || (int64_t)a->HK * plan.most_mtiles * plan.most_chunks > INT32_MAX / 2)
+  if (plan.ctas > 1024 || attn_too_many(*a) || (int64_t)a->HK * plan.most_mtiles * plan.most_chunks > INT32_MAX / 2 ||
+      (int64_t)a->B * a->HK * ((a->n_ctx + kTile - 1) / kTile + kSegTiles) > INT32_MAX / 2)
     return fail(BTF_ERR_UNSUPPORTED, "%s: too many sequences and heads for one launch", what);
   const int heads = s->head == 0 ? 1 : a->HK;
   AttnMaps<4> maps;

@@ -15,25 +15,24 @@ struct TreeSegments : Segments {
   using Place = RowPlace;
   static constexpr int kMaps = 2;
   __device__ __forceinline__ TreeSegments(const AttnParams& p, bool warp0)
-      : Segments(p, blockIdx.x, p.ranges, blockIdx.x == 0 && warp0) {}
+      : Segments(p, blockIdx.x, p.ranges, 0, blockIdx.x == 0 && warp0) {}
   __device__ __forceinline__ bool whole() const { return nt == seq.tiles; }
   __device__ __forceinline__ bool tree() const { return true; }
   __device__ __forceinline__ int map() const { return 0; }
-  __device__ __forceinline__ int64_t slot() const { return ((int64_t)mt * 2 * ranges + 2 * range + (index > 0)) * kRowsM; }
+  __device__ __forceinline__ int64_t slot() const { return ((int64_t)mt * 2 * ranges + 2 * range + (tile == 0)) * kRowsM; }
   __device__ __forceinline__ RowPlace place(int r, bool) const { return place_of(r); }
 
   // Where the parts of an output row lie.
   struct Parts {
     int n;
-    bool second;
     int64_t base;
     __device__ __forceinline__ Parts(const AttnParams& p, const Seq& seq, int b, int node, int head) {
       const int G = p.H / p.HK, rr = node * G + head % G;
-      const int r0 = ranges_of(p, seq, b, head / G, &n, &second);
+      const int r0 = ranges_of(p, 0, seq, b, head / G, &n);
       base = ((int64_t)(rr / kRowsM) * 2 * p.ranges + 2 * r0) * kRowsM + rr % kRowsM;
       if (n == 1) n = 0;  // written whole
     }
-    __device__ __forceinline__ int64_t operator()(int s) const { return base + (2 * s + (s == 0 && second)) * kRowsM; }
+    __device__ __forceinline__ int64_t operator()(int s) const { return base + (2 * s + (s == 0)) * kRowsM; }
   };
 };
 
