@@ -72,7 +72,7 @@ __device__ __forceinline__ float norm_scale(const RopeParams& p, unsigned mask, 
 template <typename TX, typename TY, int C, int NORM, bool AXES>
 __device__ __forceinline__ void rope_heads(const RopeParams& p, const RopeSeg& s, int t, int64_t row, int h0, int h1,
                                            int lane, float* scales) {
-  constexpr int kBatch = NORM ? 1 : C * (int)sizeof(TX) >= 32 ? 2 : C == 8 ? 8 : 4;
+  constexpr int kBatch = NORM ? 1 : C == 8 ? 8 : 4;
   const int R = s.rotate ? p.R : 0, half = R / 2, D = p.D;
   const int nrot = half / C;                               // rotated items: C pairs each
   const int items = nrot + (D - R + 2 * C - 1) / (2 * C);  // copied items: 2 C elements each
@@ -222,8 +222,9 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
     row = s.rows[t];
     if (row < 0 || row >= s.n_rows) return;
   }
-  if (s.x_type == BTF_F32) rope_to<float, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
-  else if (s.x_type == BTF_F16) rope_to<__half, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
+  if constexpr (C != 8 || NORM)  // the host takes 4 for fp32 without a norm
+    if (s.x_type == BTF_F32) return rope_to<float, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
+  if (s.x_type == BTF_F16) rope_to<__half, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
   else rope_to<__nv_bfloat16, C, NORM, AXES>(p, s, t, row, h0, h1, lane, scales);
 }
 
@@ -328,7 +329,7 @@ int rope_call(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const
                 n_rot);
   if (T == 0) return BTF_OK;
   RopeParams p{};
-  bool rotates = false;
+  bool rotates = false, norm = false, wide = false;
   int64_t heads = 0;
   int C = 8;
   if (n_rot % 16 || D % 8) C = n_rot % 8 || D % 4 ? 1 : 4;
@@ -348,6 +349,8 @@ int rope_call(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const
         (s.x_type != s.y_type || s.rows || s.x_token != s.y_token || s.x_head != s.y_head))
       return fail(BTF_ERR_ARG, "btf_rope: in place needs one type, the same strides and no rows");
     rotates |= s.heads > 0 && s.rotate && n_rot > 0;
+    norm |= s.heads && s.normw;
+    wide |= s.heads && s.x_type == BTF_F32;
     heads += s.heads;
     if (C == 8 && !aligned_for(s, 8)) C = 4;
     if (C == 4 && !aligned_for(s, 4)) C = 1;
@@ -360,12 +363,10 @@ int rope_call(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const
   p.T = T, p.D = D, p.R = n_rot, p.inter = interleaved != 0, p.inverse = inverse != 0;
   p.turns = turns, p.pos = pos, p.mscale = mscale, p.eps = eps;
   p.axis = axis, p.n_axes = n_axes, p.pos_axis = pos_axis;
+  // fp32 without a norm: 4 pairs an item, one 16-byte word a load and twice the threads (16384 tokens of
+  // 16 + 16 interleaved heads of 80: 59 us, 76 with 8 pairs, whose words lie 32 bytes apart from lane to lane)
+  if (C == 8 && !norm && wide) C = 4;
   const int items = std::max(n_rot / 2 / C + (D - n_rot + 2 * C - 1) / (2 * C), (D + 2 * C - 1) / (2 * C));
-  bool norm = false, narrow = true;
-  for (int i = 0; i < nseg; ++i) {
-    norm |= segs[i].heads && segs[i].normw;
-    narrow &= !segs[i].heads || segs[i].x_type != BTF_F32;
-  }
   // with a norm a token's lanes sum over a head by shuffles: a power of two of them
   p.lanes = norm ? 1 : std::min(items, kThreads);
   while (norm && p.lanes < items && p.lanes < 32) p.lanes *= 2;
@@ -373,7 +374,7 @@ int rope_call(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const
   // stays full; 16 pay where 8 are in flight at once (7001 tokens of 40 fp32 heads
   // of 80: 32.5 us with 8, 34.7 with 16)
   const int64_t full = (int64_t)dev->sm_count * 2048;
-  p.hl = (int)std::max<int64_t>(1, std::min<int64_t>(C == 8 && narrow ? kMaxHeads : 8, (int64_t)T * heads * p.lanes / full));
+  p.hl = (int)std::max<int64_t>(1, std::min<int64_t>(C == 8 && !wide ? kMaxHeads : 8, (int64_t)T * heads * p.lanes / full));
   int blocks = 0;
   for (int i = 0; i < nseg; ++i) {
     const btf_rope_seg& s = segs[i];
