@@ -2,19 +2,25 @@
 //
 //   y_t = base_t + s_a B_a (A_a x_t),  a = the adapter of row t
 //
-// for up to three projections of the same rows (q, k and v; gate and up). Two
-// launches: `shrink` makes h = A x (fp32), `expand` makes y. The rows are taken in
-// tiles of one adapter, from a plan that sorts them (btf_adapter_plan).
+// for up to three projections of the same rows (q, k and v; gate and up). The rows are
+// taken in tiles of one adapter, from a plan that sorts them (btf_adapter_plan). Few
+// rows: tiles of 16 and two launches, `shrink` makes h = A x (fp32), `expand` makes y.
+// Prompts: tiles of 128 rows, `shrink`, a small kernel that lays h out as operands, and y
+// on tcgen05 (adapters_tc.cu).
 //
 // What bounds it: bytes. A row's x is read once, y written and base read once: with
 // rank r that is 2 r (K + N) multiply-adds for (K + 2 N) elements, 64 a byte at r = 64
 // in 16 bits, where the card has 250 a byte on tcgen05 and 80 on the warp-level MMA.
 // For few rows the weights are what is read, once for the rows of an adapter, and there
-// the time is the latency of one pass through memory after another. So the MMAs are
-// warp-level (m16n8k16), whose operands come from global memory straight into
-// registers, 16 bytes a lane: no shared memory, barrier or transposition lies between
-// a load and its product, N, strides and row order are free, and the accumulators lie
-// where y's rows are stored from.
+// the time is the latency of one pass through memory after another: 1 fp32 row, 6144 to
+// 5120, rank 16: 7.8 us (0.3 MB); 200 fp16 rows over 9 adapters, 1672 to 4091, rank 24:
+// 12 us; 48 fp32 rows over 24 adapters, 5120 to q, k and v, rank 64: 18.7 us (39 MB,
+// 2.1 TB/s). So the MMAs there are warp-level (m16n8k16), whose operands come from
+// global memory straight into registers, 16 bytes a lane: no shared memory, barrier or
+// transposition lies between a load and its product, N, strides and row order are free,
+// and the accumulators lie where y's rows are stored from. `expand` reads what does not
+// depend on h before it waits for it, and a piece's weights and base under the piece
+// before.
 //
 // k is permuted alike in both operands of an MMA: the lane of place t holds the 8
 // consecutive elements 8 t .. 8 t + 7 of a 32-wide step (one 16-byte load), which are
@@ -157,117 +163,111 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1
 __device__ __forceinline__ uint4 ld16(const void* p, bool on) {
   return on ? __ldg(static_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
 }
-// 8 consecutive elements of x as the B operands of a step: TERMS x 4 words of 16-bit pairs, or (fp32 x, fp16 weights)
-// 2 x 8 tf32 values.
-template <typename TX, typename TW>
-struct XFrag {
+// 8 consecutive elements of NT rows of x as the B operands of a 32-wide step: `kTerms` terms of 4 words of 16-bit pairs,
+// or (fp32 x, fp16 weights) 2 terms of 8 tf32 values.
+template <typename TX, typename TW, int NT>
+struct XTerms {
   static constexpr bool kF32 = std::is_same_v<TX, float>;
   static constexpr bool kTf32 = kF32 && std::is_same_v<TW, __half>;
-  static constexpr int kTerms = !kF32 ? 1 : kTf32 ? 2 : 3;
+  static constexpr int kTerms = !kF32 ? 1 : kTf32 ? 2 : 3, kWords = kTf32 ? 8 : 4;
   static constexpr int kLoads = kF32 ? 2 : 1;
-};
+  uint32_t v[NT][kTerms][kWords];
 
-// c += the products of a 32-wide step: lo and hi the weights' rows g and g + 8 of each 16, xw the rows of x; of the
-// weights' 16s and the rows' 8s only the first ms and ns have anything.
-template <typename TX, typename TW, int RT, int NT>
-__device__ __forceinline__ void products(float (&c)[RT][NT][4], const uint4 (&lo)[RT], const uint4 (&hi)[RT],
-                                         const uint4 (&xw)[NT][XFrag<TX, TW>::kLoads], int ms, int ns) {
-  using F = XFrag<TX, TW>;
-  if constexpr (!F::kF32) {
-#pragma unroll
-    for (int m = 0; m < RT; ++m)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        if (m < ms && j < ns) mma16<TW>(c[m][j], lo[m].x, hi[m].x, lo[m].y, hi[m].y, xw[j][0].x, xw[j][0].y);
-#pragma unroll
-    for (int m = 0; m < RT; ++m)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        if (m < ms && j < ns) mma16<TW>(c[m][j], lo[m].z, hi[m].z, lo[m].w, hi[m].w, xw[j][0].z, xw[j][0].w);
-  } else if constexpr (!F::kTf32) {
+  __device__ __forceinline__ explicit XTerms(const uint4 (&xw)[NT][kLoads]) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      if (j >= ns) break;
-      const uint32_t w[8] = {xw[j][0].x, xw[j][0].y, xw[j][0].z, xw[j][0].w,
-                             xw[j][1].x, xw[j][1].y, xw[j][1].z, xw[j][1].w};
-      uint32_t term[3][4];
+      uint32_t w[4 * kLoads];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v0 = __uint_as_float(w[2 * i]), v1 = __uint_as_float(w[2 * i + 1]);
-        term[0][i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);  // cut off: never beyond fp32's range
-        const float r0 = rest(v0, __uint_as_float(w[2 * i] & 0xffff0000u));
-        const float r1 = rest(v1, __uint_as_float(w[2 * i + 1] & 0xffff0000u));
-        term[1][i] = pack2<__nv_bfloat16>(r0, r1);
-        const float2 mid = unpack2<__nv_bfloat16>(term[1][i]);
-        term[2][i] = pack2<__nv_bfloat16>(r0 - mid.x, r1 - mid.y);
-      }
+      for (int l = 0; l < kLoads; ++l) w[4 * l] = xw[j][l].x, w[4 * l + 1] = xw[j][l].y, w[4 * l + 2] = xw[j][l].z, w[4 * l + 3] = xw[j][l].w;
+      if constexpr (!kF32) {
 #pragma unroll
-      for (int e = 2; e >= 0; --e) {
+        for (int i = 0; i < 4; ++i) v[j][0][i] = w[i];
+      } else if constexpr (!kTf32) {
 #pragma unroll
-        for (int m = 0; m < RT; ++m)
-          if (m < ms) mma16<TW>(c[m][j], lo[m].x, hi[m].x, lo[m].y, hi[m].y, term[e][0], term[e][1]);
-#pragma unroll
-        for (int m = 0; m < RT; ++m)
-          if (m < ms) mma16<TW>(c[m][j], lo[m].z, hi[m].z, lo[m].w, hi[m].w, term[e][2], term[e][3]);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // the lane's elements 2 i and 2 i + 1
-      uint32_t big[NT][2], small[NT][2];
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint4 v4 = xw[j][i >> 1];
-          const uint32_t w = i & 1 ? (e ? v4.w : v4.z) : (e ? v4.y : v4.x);
-          big[j][e] = w & 0xffffe000u;
-          const float r = rest(__uint_as_float(w), __uint_as_float(big[j][e]));
-          asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(small[j][e]) : "f"(r));
+        for (int i = 0; i < 4; ++i) {
+          const float v0 = __uint_as_float(w[2 * i]), v1 = __uint_as_float(w[2 * i + 1]);
+          v[j][0][i] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);  // cut off: never beyond fp32's range
+          const float r0 = rest(v0, __uint_as_float(w[2 * i] & 0xffff0000u));
+          const float r1 = rest(v1, __uint_as_float(w[2 * i + 1] & 0xffff0000u));
+          v[j][1][i] = pack2<__nv_bfloat16>(r0, r1);
+          const float2 mid = unpack2<__nv_bfloat16>(v[j][1][i]);
+          v[j][2][i] = pack2<__nv_bfloat16>(r0 - mid.x, r1 - mid.y);
         }
+      } else {
 #pragma unroll
-      for (int m = 0; m < RT; ++m) {
-        if (m >= ms) break;
-        const uint32_t wl = i == 0 ? lo[m].x : i == 1 ? lo[m].y : i == 2 ? lo[m].z : lo[m].w;
-        const uint32_t wh = i == 0 ? hi[m].x : i == 1 ? hi[m].y : i == 2 ? hi[m].z : hi[m].w;
-        const float2 fl = unpack2<TW>(wl), fh = unpack2<TW>(wh);
-        const uint32_t a0 = __float_as_uint(fl.x), a1 = __float_as_uint(fh.x), a2 = __float_as_uint(fl.y),
-                       a3 = __float_as_uint(fh.y);
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          if (j < ns) mma_tf32(c[m][j], a0, a1, a2, a3, small[j][0], small[j][1]);
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          if (j < ns) mma_tf32(c[m][j], a0, a1, a2, a3, big[j][0], big[j][1]);
+        for (int i = 0; i < 8; ++i) {
+          v[j][0][i] = w[i] & 0xffffe000u;
+          const float r = rest(__uint_as_float(w[i]), __uint_as_float(v[j][0][i]));
+          asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(v[j][1][i]) : "f"(r));
+        }
       }
     }
   }
-}
+  // c += the products: lo and hi the weights' rows g and g + 8 of each 16; of the weights' 16s and the rows' 8s only the
+  // first ms and ns have anything.
+  template <int RT>
+  __device__ __forceinline__ void products(float (&c)[RT][NT][4], const uint4 (&lo)[RT], const uint4 (&hi)[RT], int ms, int ns) const {
+    if constexpr (!kTf32) {
+#pragma unroll
+      for (int e = kTerms - 1; e >= 0; --e) {
+#pragma unroll
+        for (int m = 0; m < RT; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            if (m < ms && j < ns) mma16<TW>(c[m][j], lo[m].x, hi[m].x, lo[m].y, hi[m].y, v[j][e][0], v[j][e][1]);
+#pragma unroll
+        for (int m = 0; m < RT; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            if (m < ms && j < ns) mma16<TW>(c[m][j], lo[m].z, hi[m].z, lo[m].w, hi[m].w, v[j][e][2], v[j][e][3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // the lane's elements 2 i and 2 i + 1
+#pragma unroll
+        for (int m = 0; m < RT; ++m) {
+          if (m >= ms) break;
+          const float2 fl = unpack2<TW>(i == 0 ? lo[m].x : i == 1 ? lo[m].y : i == 2 ? lo[m].z : lo[m].w);
+          const float2 fh = unpack2<TW>(i == 0 ? hi[m].x : i == 1 ? hi[m].y : i == 2 ? hi[m].z : hi[m].w);
+#pragma unroll
+          for (int e = 1; e >= 0; --e)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+              if (j < ns)
+                mma_tf32(c[m][j], __float_as_uint(fl.x), __float_as_uint(fh.x), __float_as_uint(fl.y), __float_as_uint(fh.y),
+                         v[j][e][2 * i], v[j][e][2 * i + 1]);
+        }
+    }
+  }
+};
 
 // ------------------------------------------------------------------ shrink
 // Few rows: a CTA takes a tile's 16 rows, one projection and one of `splits` stretches of K, which its warps share. The
 // weights are the MMA's 16-row side (RT x 16 of them), the rows of x its 8-wide side. The stretches of K of one CTA meet in
 // shared memory, in order; those of several in `expand`.
 template <typename TX, typename TW, int RT>
-__global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XFrag<TX, TW>::kTf32) ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XTerms<TX, TW, 2>::kTf32) ? 1 : 2)
     adapter_shrink_kernel(const __grid_constant__ Params p) {
-  using F = XFrag<TX, TW>;
-  constexpr int KG = kThreads / 32, NT = 2, kRows = kSmall;
+  // (fp32: the terms of 8 rows at a time, whose making overlaps the MMAs of the 8 before)
+  constexpr int NT = 2, JT = std::is_same_v<TX, float> ? 1 : 2;
+  using F = XTerms<TX, TW, JT>;
+  constexpr int KG = kThreads / 32, kRows = kSmall;
   extern __shared__ float red[];  // [KG][kRows][RT * 16 + 4]
   constexpr int kPitch = RT * 16 + 4;
   pdl_wait();
   pdl_launch_dependents();  // (behind the wait: `expand` reads the plan before its own)
-  const int split = blockIdx.x % p.splits, seg = blockIdx.x / p.splits % p.nseg, ti = blockIdx.x / (p.splits * p.nseg);
+  const int seg = blockIdx.x % p.nseg, ti = blockIdx.x / p.nseg % p.most, split = blockIdx.x / (p.nseg * p.most);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   // head, tile and rows in one round trip (the list has room for every CTA's tile)
   const SmallTile* st = p.small + ti;
   const Tile tile = st->tile;
   const int rows[2] = {st->rows[g], st->rows[8 + g]};
-  if (!plan_ok(p) || ti >= p.head[p.which] || tile.adapter < 0) return;
+  const int splits = splits_of(p);
+  if (!plan_ok(p) || ti >= p.head[p.which] || tile.adapter < 0 || split >= splits) return;
   const int rank = rank_of(p, tile.adapter);
   if (rank == 0) return;
   const Seg& s = p.seg[seg];
-  const int steps = (p.K + 31) / 32, ways = p.splits * KG;
+  const int steps = (p.K + 31) / 32, ways = splits * KG;
   const int way = split * KG + warp, k0 = (int)((int64_t)way * steps / ways), k1 = (int)((int64_t)(way + 1) * steps / ways);
   const TW* a = static_cast<const TW*>(s.a) + tile.adapter * s.a_adapter + 8 * t;
   const TX* x[NT];
@@ -277,27 +277,31 @@ __global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XFrag<TX, TW>
     on[j] = j * 8 + g < tile.count;
     x[j] = static_cast<const TX*>(p.x) + (on[j] ? rows[j] * p.x_row : 0) + 8 * t;
   }
-  float c[RT][NT][4];
+  float c[NT / JT][RT][JT][4];
 #pragma unroll
-  for (int m = 0; m < RT; ++m)
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) c[m][j][0] = c[m][j][1] = c[m][j][2] = c[m][j][3] = 0.f;
+    for (int m = 0; m < RT; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[j / JT][m][j % JT][e] = 0.f;
   const int mts = (rank + 15) / 16, nts = (tile.count + 7) / 8;
 #pragma unroll 1
   for (int ks = k0; ks < k1; ++ks) {
     const int k = ks * 32;
     const bool kin = k + 8 * t < p.K;
-    uint4 xw[NT][F::kLoads], lo[RT], hi[RT];
+    uint4 xw[NT / JT][JT][F::kLoads], lo[RT], hi[RT];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int l = 0; l < F::kLoads; ++l) xw[j][l] = ld16(x[j] + k + 4 * l, kin && on[j]);
+      for (int l = 0; l < F::kLoads; ++l) xw[j / JT][j % JT][l] = ld16(x[j] + k + 4 * l, kin && on[j]);
 #pragma unroll
     for (int m = 0; m < RT; ++m) {
       lo[m] = ld16(a + (int64_t)(m * 16 + g) * s.a_row + k, kin && m < mts && m * 16 + g < p.R);
       hi[m] = ld16(a + (int64_t)(m * 16 + 8 + g) * s.a_row + k, kin && m < mts && m * 16 + 8 + g < p.R);
     }
-    products<TX, TW, RT, NT>(c, lo, hi, xw, mts, nts);
+#pragma unroll
+    for (int j = 0; j < NT / JT; ++j)
+      if (j * JT < nts) F(xw[j]).products(c[j], lo, hi, mts, nts - j * JT);
   }
   // c[m][j]: weight rows 16 m + g and + 8, rows 8 j + 2 t and + 1
   float* mine = red + warp * kRows * kPitch;
@@ -306,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XFrag<TX, TW>
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mine[(j * 8 + 2 * t + (e & 1)) * kPitch + m * 16 + g + (e >> 1) * 8] = c[m][j][e];
+      for (int e = 0; e < 4; ++e) mine[(j * 8 + 2 * t + (e & 1)) * kPitch + m * 16 + g + (e >> 1) * 8] = c[j / JT][m][j % JT][e];
   __syncthreads();
   const int quads = p.R / 4, live = min((rank + 3) / 4, quads);
   float* h = p.h + ((int64_t)(split * p.nseg + seg) * p.T + tile.begin) * p.R;
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XFrag<TX, TW>
 // Prompts: a CTA takes a tile's 128 rows, one projection and one of `splits` stretches of K. x and the weights come
 // through a ring in shared memory, 128 bytes of each row of x at a time (64 elements, 32 of fp32), which keeps 16 KB a
 // stage under way: with operands loaded as above a step waits out the memory's latency (6007 rows of 5120 in bf16:
-// 39 us; XX here). The MMAs' rate is not what bounds it: 8 us of it there.
+// 39 us, 26 so). The MMAs' rate is not what bounds it: 8 us of it there.
 //
 // Warp (rg, kg) has NT x 8 of the rows and, of two, one 32-wide step of a stage. A word lies at its place ^ f(row), f
 // such that the lanes that read together, four words of two neighbouring rows, meet no bank twice.
@@ -347,17 +351,18 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool o
 }
 
 template <typename TX, typename TW, int RT>
-__global__ void __launch_bounds__(kThreads, RT == 8 && XFrag<TX, TW>::kF32 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, RT == 8 && std::is_same_v<TX, float> ? 1 : 2)
     adapter_shrink_long_kernel(const __grid_constant__ Params p) {
-  using F = XFrag<TX, TW>;
   using L = Long<TX, TW, RT>;
+  using F = XTerms<TX, TW, L::NT>;
   constexpr int NT = L::NT, KG = L::KG, kPer = 16 / (int)sizeof(TX);  // elements of x in a 16-byte word
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_wait();
   pdl_launch_dependents();  // (behind the wait: the grids behind this one read the plan before their own)
   if (!plan_ok(p)) return;
-  const int split = blockIdx.x % p.splits, seg = blockIdx.x / p.splits % p.nseg, ti = blockIdx.x / (p.splits * p.nseg);
-  if (ti >= p.head[p.which]) return;
+  const int tiles = min(p.head[p.which], p.most), splits = long_splits(p);
+  if ((int)blockIdx.x >= tiles * splits * p.nseg) return;
+  const int seg = blockIdx.x % p.nseg, ti = blockIdx.x / p.nseg % tiles, split = blockIdx.x / (p.nseg * tiles);
   const Tile tile = p.tiles[ti];
   if (tile.adapter < 0) return;
   const int rank = rank_of(p, tile.adapter);
@@ -366,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, RT == 8 && XFrag<TX, TW>::kF32 ? 1 :
   const int rg = warp % L::RG, kg = warp / L::RG;
   const Seg& s = p.seg[seg];
   const int all = (p.K + L::kStep - 1) / L::kStep;
-  const int s0 = (int)((int64_t)split * all / p.splits), s1 = (int)((int64_t)(split + 1) * all / p.splits);
+  const int s0 = (int)((int64_t)split * all / splits), s1 = (int)((int64_t)(split + 1) * all / splits);
   const int mts = (rank + 15) / 16;
   const uint32_t sbase = smem_u32(smem);
   // this thread's words of a stage: word tid % 8 of the rows tid / 8 + 32 i of x, and some of the weights
@@ -428,6 +433,7 @@ __global__ void __launch_bounds__(kThreads, RT == 8 && XFrag<TX, TW>::kF32 ? 1 :
           xw[j][l] = *reinterpret_cast<const uint4*>(xs + r * 128 + ((w ^ spread(r)) << 4));
         }
       }
+      const F terms(xw);
       // (two of the weights' 16 rows at a time: all of them at once leave no registers for a second CTA)
 #pragma unroll
       for (int m0 = 0; m0 < RT; m0 += L::MB) {
@@ -439,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, RT == 8 && XFrag<TX, TW>::kF32 ? 1 :
           lo[m] = *reinterpret_cast<const uint4*>(as + r * L::kARow + ((kAWords == 8 ? w ^ spread(r) : w) << 4));
           hi[m] = *reinterpret_cast<const uint4*>(as + (r + 8) * L::kARow + ((kAWords == 8 ? w ^ spread(r) : w) << 4));
         }
-        products<TX, TW, L::MB, NT>(c[m0 / L::MB], lo, hi, xw, mts - m0, NT);
+        terms.products(c[m0 / L::MB], lo, hi, mts - m0, NT);
         if (RT > L::MB) asm volatile("" ::: "memory");
       }
     }
@@ -562,13 +568,14 @@ __global__ void __launch_bounds__(kExpand, kBlocks == 4 ? 5 : 6) adapter_expand_
       const bool there = r < tile.count;
       const float* h = p.h + ((int64_t)seg * p.T + tile.begin + r) * p.R + l * 8;
       const int64_t stretch = (int64_t)p.nseg * p.T * p.R;
+      const int splits = splits_of(p);  // (here: one register less all along)
       float v[kBlocks][8];
 #pragma unroll
       for (int kb = 0; kb < kBlocks; ++kb)
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[kb][i] = 0.f;
 #pragma unroll (8 / kBlocks)
-      for (int q = 0; q < p.splits; ++q, h += stretch) {
+      for (int q = 0; q < splits; ++q, h += stretch) {
 #pragma unroll
         for (int kb = 0; kb < kBlocks; ++kb) {
           if (!there || kb * 32 + l * 8 >= rank) continue;
@@ -675,19 +682,28 @@ bool sizes_ok(int T, int K, int R, int nseg, int n) {
          R <= BTF_ADAPTERS_MAX_RANK && nseg >= 1 && nseg <= 3 && n >= 1 && n <= BTF_ADAPTERS_MAX;
 }
 
-// Tiles of 16 rows while the adapters' rows are few, of 128 for prompts.
+// Tiles of 16 rows while the rows are few, of 128 for prompts: us as few and as prompts, with the rows of 1 request, of 8
+// and each with an adapter of its own. bf16 to 17408, rank 64: 384 rows 20, 26, 27 and 25, 33, 36; 512 rows 32, 29, 39 and
+// 25, 30, 37; 1024 rows 52, 67, 69 and 31, 40, 42. fp32 q, k and v, whose terms cost the more the fewer rows share their
+// weights: 512 rows 29, 41, 45 and 38, 48, 102; 1024 rows 58, 67, 74 and 46, 69, 109; 2048 rows 116, 138, 132 and 71,
+// 107, 136.
 struct Shape {
   bool large;
   int tiles;   // at most
-  int splits;  // stretches of K
+  int splits;  // stretches of K, at most
 };
-Shape shape_of(const DeviceInfo& d, int T, int K, int nseg, int n) {
+Shape shape_of(const DeviceInfo& d, int T, int K, int nseg, int n, bool x32) {
   Shape s;
-  s.large = T > 256;
+  s.large = T > (x32 ? 1024 : 512);
   const int rows = s.large ? kLarge : kSmall;
   s.tiles = T / rows + std::min(n + 1, T);
   const int least = s.large ? 512 : 256;  // of K that a stretch has
-  s.splits = std::max(1, std::min({2 * d.sm_count / (s.tiles * nseg), kMaxSplits, (K + least - 1) / least}));
+  // for prompts up to kTurns turns of the least tiles, for the small tiles' grid, whose CTAs know their place before they
+  // know the plan, at most three quarters of them idle
+  const int room = 2 * d.sm_count, least_tiles = (T + rows - 1) / rows;
+  s.splits = std::min({s.large ? kTurns * room / (least_tiles * nseg) : std::min(room / (least_tiles * nseg), 4 * room / (s.tiles * nseg)),
+                       kMaxSplits, (K + least - 1) / least});
+  s.splits = std::max(1, s.splits);
   return s;
 }
 // The workspace: h, and for prompts its terms and the rows' factors.
@@ -709,7 +725,9 @@ cudaError_t shrink_rt(const Params& p, bool large, int tiles, cudaStream_t st, b
       return e;
     return cudaFuncSetAttribute(adapter_shrink_long_kernel<TX, TW, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_long);
   }
-  const dim3 grid((unsigned)(tiles * p.nseg * p.splits));
+  // what splits_of can come to; CTAs beyond what it takes end at once
+  const int most = tiles * p.nseg;
+  const dim3 grid((unsigned)(large ? std::max(most, std::min(kTurns * p.room, most * p.splits)) : most * p.splits));
   return large ? launch_pdl(adapter_shrink_long_kernel<TX, TW, RT>, grid, dim3(kThreads), (size_t)smem_long, st, p)
                : launch_pdl(adapter_shrink_kernel<TX, TW, RT>, grid, dim3(kThreads), (size_t)smem, st, p);
 }
@@ -747,7 +765,6 @@ cudaError_t expand(Params p, int tiles, int sms, cudaStream_t st) {
 }  // namespace
 
 int adapters_setup(DeviceInfo& d) {
-  const Params p{};
   if (32 * (BTF_ADAPTERS_MAX + 1) * 4 > d.optin_smem) return cuda_fail(cudaErrorInvalidValue, "adapter_plan_kernel attributes");
   for (cudaError_t e :
        {cudaFuncSetAttribute(adapter_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * (BTF_ADAPTERS_MAX + 1) * 4),
@@ -793,7 +810,10 @@ int64_t btf_adapters_work(int T, int K, int R, int nseg, int n_adapters) {
   }
   const DeviceInfo* dev = current_device();
   if (!dev) return -1;
-  return T == 0 ? 0 : Work(shape_of(*dev, T, K, nseg, n_adapters), T, R, nseg).bytes;
+  if (T == 0) return 0;
+  int64_t bytes = 0;  // whatever x's type
+  for (bool x32 : {false, true}) bytes = std::max(bytes, Work(shape_of(*dev, T, K, nseg, n_adapters, x32), T, R, nseg).bytes);
+  return bytes;
 }
 
 int btf_adapters(const btf_adapters_args* a, void* stream) {
@@ -835,7 +855,7 @@ int btf_adapters(const btf_adapters_args* a, void* stream) {
   }
   const DeviceInfo* dev = current_device();
   if (!dev) return BTF_ERR_STATE;
-  const Shape sh = shape_of(*dev, a->T, a->K, a->nseg, a->n_adapters);
+  const Shape sh = shape_of(*dev, a->T, a->K, a->nseg, a->n_adapters, a->x_type == BTF_F32);
   const Work w(sh, a->T, a->R, a->nseg);
   if (!a->work || !al(a->work) || a->work_bytes < w.bytes)
     return fail(BTF_ERR_ARG, "btf_adapters: workspace null, not 16-byte aligned or too small (%lld bytes, %lld are needed)",
@@ -843,7 +863,8 @@ int btf_adapters(const btf_adapters_args* a, void* stream) {
   const PlanLayout at(a->T, a->n_adapters);
   const uint8_t* plan = static_cast<const uint8_t*>(a->plan);
   p.x = a->x, p.x_row = a->T > 1 ? a->x_row : 0;
-  p.T = a->T, p.K = a->K, p.R = a->R, p.n = a->n_adapters, p.nseg = a->nseg, p.splits = sh.splits, p.ranges = 1;
+  p.T = a->T, p.K = a->K, p.R = a->R, p.n = a->n_adapters, p.nseg = a->nseg, p.splits = sh.splits, p.room = 2 * dev->sm_count, p.most = sh.tiles, p.ranges = 1;
+  p.steps = (a->K * elem_bytes(a->x_type) + 127) / 128;
   p.ranks = a->ranks, p.scales = a->scales;
   p.head = reinterpret_cast<const int32_t*>(plan), p.order = reinterpret_cast<const int32_t*>(plan + at.order);
   p.owner = reinterpret_cast<const int32_t*>(plan + at.owner);

@@ -2,6 +2,7 @@
 // prompts on tcgen05 (adapters_tc.cu).
 #pragma once
 #include <algorithm>
+#include <climits>
 
 #include "elem.cuh"
 
@@ -10,6 +11,8 @@ namespace adapt {
 
 constexpr int kSmall = 16, kLarge = 128;  // rows of a tile
 constexpr int kMaxSplits = 16;
+constexpr int kTurns = 4;
+constexpr int kItemSteps = 5;  // what an item costs beside its steps: the ring's filling, h
 constexpr int kErrPlan = 2;  // device error word: a plan of other sizes
 
 struct Tile {
@@ -44,7 +47,9 @@ struct Params {
   Seg seg[3];
   const void* x;
   int64_t x_row;
-  int T, K, R, n, nseg, splits, ranges;
+  int T, K, R, n, nseg, ranges;
+  int splits, room;  // stretches of K at most; CTAs that they may come to
+  int most, steps;   // tiles at most; steps of K (prompts)
   const int32_t* ranks;
   const float* scales;
   const int32_t *head, *order, *owner;
@@ -64,6 +69,19 @@ __device__ __forceinline__ bool plan_ok(const Params& p) {
   return false;
 }
 __device__ __forceinline__ int rank_of(const Params& p, int a) { return p.ranks ? min(max(p.ranks[a], 0), p.R) : p.R; }
+// The stretches of K, by the tiles that there are: 256 rows of one request among 24 adapters are 16 tiles, where up to 41
+// could be (256 fp32 rows, q, k and v: 29 us with the stretches that room for all of them leaves, 23 so).
+__device__ __forceinline__ int splits_of(const Params& p) {
+  return max(1, min(p.splits, p.room / (min(max(p.head[p.which], 1), p.most) * p.nseg)));
+}
+// The same for prompts, by how many turns of how many steps the CTAs then take (whole warps; 6007 fp32 rows of 8
+// requests, 156 items for 296 places: 375 us in one turn, 254 so; 1024 rows of one, 24 items: 114 and 46).
+__device__ __forceinline__ int long_splits(const Params& p) {
+  const int items = min(max(p.head[p.which], 1), p.most) * p.nseg, s = (threadIdx.x & 31) + 1;
+  const int turns = (items * s + p.room - 1) / p.room, each = (p.steps + s - 1) / s + kItemSteps;
+  const int cost = s == 1 || (s <= p.splits && turns <= kTurns) ? turns * each : INT_MAX;
+  return __ffs(__ballot_sync(0xffffffffu, cost == __reduce_min_sync(0xffffffffu, cost)));
+}
 
 // What `shrink` wrote: never from L1, and in its place behind the wait.
 __device__ __forceinline__ float4 ld_cg(const float* p) {

@@ -9,7 +9,7 @@
 // their turn and take the sum from the same place to y: one TMA copy of 32 rows x 128
 // bytes where the rows follow one another (a prompt's do), else 16 bytes a lane, eight
 // lanes a row. (Bulk copies of a row each are issued one after another by a warp: 178 us
-// for what takes XX us.)
+// for what takes 105 so: 6007 rows of 17408 in bf16 on a base, 418 MB, 4 TB/s.)
 //
 // Work: the tiles of 128 rows times 128 outputs of all projections make a line, cut into
 // equal stretches of one CTA per SM. Warp 8 brings the terms of the rows' h (made by a
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(256) adapter_terms_kernel(const __grid_constan
   const int at = blockIdx.x * 32 + (threadIdx.x >> 3), l = threadIdx.x & 7, seg = blockIdx.y;
   if (p.head[0] != p.T || p.head[1] != p.n) return;
   const bool live = at < p.head[4];  // rows with an adapter come first
-  const int a = live ? p.owner[at] : 0, rank = live ? rank_of(p, a) : 0;
+  const int a = live ? p.owner[at] : 0, rank = live ? rank_of(p, a) : 0, splits = long_splits(p);
   const int64_t next = (int64_t)p.nseg * p.T * p.R;
   const float* h = p.h + ((int64_t)seg * p.T + at) * p.R;
   float v[2][8];  // of a row's 128 at most: elements 8 l .. and 64 + 8 l ..
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256) adapter_terms_kernel(const __grid_constan
     if (k >= rank) continue;
     const float* from = h + k;
 #pragma unroll 4
-    for (int q = 0; q < p.splits; ++q, from += next) {
+    for (int q = 0; q < splits; ++q, from += next) {
       const float4 v0 = ld_cg(from), v1 = ld_cg(from + 4);
       v[b][0] += v0.x, v[b][1] += v0.y, v[b][2] += v0.z, v[b][3] += v0.w;
       v[b][4] += v1.x, v[b][5] += v1.y, v[b][6] += v1.z, v[b][7] += v1.w;

@@ -114,7 +114,7 @@ def test_plan_sorts_the_rows(cuda, btf, T, n):
 
 # ---------------------------------------------------------------- the call
 @pytest.mark.parametrize("types", TYPES, ids=str)
-@pytest.mark.parametrize("T", [1, 7, 300])
+@pytest.mark.parametrize("T", [1, 7, 300, 1100])
 def test_types(cuda, btf, types, T):
     _case(btf, cuda, T, 3, 264, 64, [200], types, seed=T)
 
@@ -122,12 +122,12 @@ def test_types(cuda, btf, types, T):
 @pytest.mark.parametrize("types", [(F32, BF16, F32), (F16, F16, F16)], ids=str)
 @pytest.mark.parametrize("R", [8, 16, 24, 32, 40, 64, 72, 96, 128])
 def test_ranks(cuda, btf, R, types):
-    for T in (20, 400):
+    for T in (20, 1100):
         _case(btf, cuda, T, 5, 512, R, [96, 33], types, seed=R)
         _case(btf, cuda, T, 5, 512, R, [96], types, seed=R, ranks=None, scaled=False)
 
 
-@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257, 385, 1025])
+@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257, 385, 511, 512, 513, 1024, 1025, 2111])
 def test_rows(cuda, btf, T):
     _case(btf, cuda, T, 4, 128, 16, [64, 8, 129], (F32, F16, F32), seed=T)
     _case(btf, cuda, T, 1, 128, 16, [64], (BF16, BF16, BF16), seed=T, base=False, index=torch.zeros(T, dtype=torch.int32, device=cuda))
@@ -136,24 +136,35 @@ def test_rows(cuda, btf, T):
 @pytest.mark.parametrize("K", [8, 16, 24, 32, 40, 1000, 5120, 17408])
 def test_depths(cuda, btf, K):
     _case(btf, cuda, 9, 2, K, 32, [72], (F32, BF16, F32), seed=K)
-    _case(btf, cuda, 300, 2, K, 32, [72], (BF16, BF16, BF16), seed=K)
-    _case(btf, cuda, 300, 2, K, 48, [72], (F32, F16, F32), seed=K)
+    _case(btf, cuda, 600, 2, K, 32, [72], (BF16, BF16, BF16), seed=K)
+    _case(btf, cuda, 300, 2, K, 48, [72], (F16, F16, F32), seed=K)
+    _case(btf, cuda, 1100, 2, K, 48, [72], (F32, F16, F32), seed=K)
 
 
 @pytest.mark.parametrize("N", [1, 2, 7, 8, 9, 31, 32, 33, 63, 64, 65, 127, 257, 1000])
 def test_widths(cuda, btf, N):
     _case(btf, cuda, 6, 2, 64, 24, [N, 1, N + 1], (F32, F16, F16), seed=N)
-    _case(btf, cuda, 270, 2, 64, 24, [N], (F16, F16, F16), seed=N, base=False)
-    _case(btf, cuda, 270, 2, 64, 24, [N], (F32, BF16, F32), seed=N)
+    _case(btf, cuda, 570, 2, 64, 24, [N], (F16, F16, F16), seed=N, base=False)
+    _case(btf, cuda, 1070, 2, 64, 24, [N], (F32, BF16, F32), seed=N)
 
 
 def test_many_adapters(cuda, btf):
     _case(btf, cuda, 700, 1024, 64, 8, [40], (F32, BF16, F32), seed=1)
     _case(btf, cuda, 130, 1024, 64, 8, [40], (BF16, BF16, BF16), seed=2)
+    _case(btf, cuda, 1300, 1024, 64, 8, [40], (F32, BF16, F32), seed=3)
+
+
+@pytest.mark.parametrize("T", [200, 700, 1500, 3000])
+def test_one_request_among_many(cuda, btf, T):
+    """How K is split follows the tiles that there are, not those that could be."""
+    index = torch.full((T,), 17, dtype=torch.int32, device=cuda)
+    for types in ((F32, BF16, F32), (F16, F16, F16)):
+        _case(btf, cuda, T, 24, 2056, 40, [70, 64, 9], types, seed=T, index=index, ranks=None)
+    _case(btf, cuda, T, 24, 2056, 40, [70], (BF16, BF16, BF16), seed=T, index=torch.arange(T, dtype=torch.int32, device=cuda) % 3)
 
 
 def test_no_row_has_an_adapter(cuda, btf):
-    for T in (3, 500):
+    for T in (3, 500, 1100):
         for base in (True, False):
             _case(btf, cuda, T, 4, 64, 16, [50, 64], (F32, BF16, F32), index=torch.full((T,), -1, dtype=torch.int32, device=cuda), base=base)
             _case(btf, cuda, T, 4, 64, 16, [50, 64], (BF16, BF16, BF16), index=torch.full((T,), 4, dtype=torch.int32, device=cuda), base=base)
@@ -163,7 +174,7 @@ def test_no_row_has_an_adapter(cuda, btf):
     assert out[0].shape == (0, 5)
 
 
-@pytest.mark.parametrize("T", [5, 301])
+@pytest.mark.parametrize("T", [5, 301, 1101])
 @pytest.mark.parametrize("w", [F16, BF16])
 def test_nothing_behind_a_rank_matters(cuda, btf, T, w):
     """What lies behind an adapter's rank, and other rows' NaN and infinities, touch nothing."""
@@ -189,9 +200,10 @@ def test_nothing_behind_a_rank_matters(cuda, btf, T, w):
                _reference(x.nan_to_num(0, 0, 0), a2, b2, base, index, r, None, F32))
 
 
-def test_range_of_magnitudes(cuda, btf):
+@pytest.mark.parametrize("T", [20, 1030])
+def test_range_of_magnitudes(cuda, btf, T):
     """fp32 rows far from 1, with fp16 and bf16 weights: h leaves fp16's range, and its rows differ by 2^80."""
-    n, K, R, N, T = 2, 64, 16, 40, 20
+    n, K, R, N = 2, 64, 16, 40
     for w in (F16, BF16):
         x, (a,), (b,), _ = _inputs(cuda, T, n, K, R, [N], F32, w, F32, 8)
         x *= 2.0 ** torch.linspace(-60, 60, T, device=cuda).round()[:, None]
@@ -201,7 +213,7 @@ def test_range_of_magnitudes(cuda, btf):
         _check(out, _reference(x, a, b, None, index, None, None, F32))
 
 
-@pytest.mark.parametrize("T", [11, 333])
+@pytest.mark.parametrize("T", [11, 333, 1111])
 @pytest.mark.parametrize("y_type", [F32, BF16])
 def test_strides_and_in_place(cuda, btf, T, y_type):
     n, K, R, N = 4, 128, 16, 61
@@ -229,9 +241,10 @@ def test_strides_and_in_place(cuda, btf, T, y_type):
     _check(got, _reference(x, a[:1], b[:1], one, same, None, None, y_type))
 
 
-def test_results_do_not_depend_on_the_run_and_rows_stand_alone(cuda, btf):
+@pytest.mark.parametrize("T", [200, 900])
+def test_results_do_not_depend_on_the_run_and_rows_stand_alone(cuda, btf, T):
     """The same call gives the same bits; a row's result does not depend on the rows beside it in a tile."""
-    T, n, K, R, N = 200, 6, 1024, 32, 300
+    n, K, R, N = 6, 1024, 32, 300
     x, (a,), (b,), (base,) = _inputs(cuda, T, n, K, R, [N], BF16, BF16, F32, 11)
     index = _index(cuda, T, n, 12)
     plan = btf.AdapterPlan(index, n)
@@ -245,9 +258,10 @@ def test_results_do_not_depend_on_the_run_and_rows_stand_alone(cuda, btf):
     assert torch.equal(again, first[p])
 
 
-def test_graph_and_streams(cuda, btf):
+@pytest.mark.parametrize("T", [40, 1200])
+def test_graph_and_streams(cuda, btf, T):
     """Plan and call captured in one graph and replayed with other rows; another stream."""
-    T, n, K, R, N = 40, 5, 256, 16, 128
+    n, K, R, N = 5, 256, 16, 128
     x, (a,), (b,), (base,) = _inputs(cuda, T, n, K, R, [N], F32, F16, F32, 2)
     index = _index(cuda, T, n, 3)
     plan = btf.AdapterPlan(index, n)
@@ -275,9 +289,10 @@ def test_graph_and_streams(cuda, btf):
     assert btf.device_error() == 0
 
 
-def test_plan_of_other_sizes_is_reported(cuda, btf):
+@pytest.mark.parametrize("T", [8, 1100])
+def test_plan_of_other_sizes_is_reported(cuda, btf, T):
     """The C call with a plan that was made for other sizes writes nothing and says so."""
-    T, n, K, R, N = 8, 2, 64, 8, 16
+    n, K, R, N = 2, 64, 8, 16
     x, (a,), (b,), (base,) = _inputs(cuda, T, n, K, R, [N], F32, F16, F32, 2)
     plan = btf.AdapterPlan(torch.zeros(T + 1, dtype=torch.int32, device=cuda), n)
     plan.T = T
