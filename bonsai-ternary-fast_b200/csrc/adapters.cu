@@ -543,13 +543,28 @@ __global__ void __launch_bounds__(kExpand, kBlocks == 4 ? 5 : 6) adapter_expand_
     load_b(q, q.wb, 0);
     const int n8 = q.n0 + 8 * t;  // the lane's outputs
     q.vec = s.vec && n8 + 8 <= s.N;
-    if (!s.base || !q.vec) return;
+    if (!s.base) return;
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int e = 0; e < 2; ++e) {
+      const TY* from = static_cast<const TY*>(s.base) + (row[e] >= 0 ? row[e] : 0) * s.base_row + n8;
+      if (q.vec) {
 #pragma unroll
-      for (int w = 0; w < kYWords; ++w)
-        q.bv[e][w] = row[e] >= 0 ? *(reinterpret_cast<const uint4*>(static_cast<const TY*>(s.base) + row[e] * s.base_row + n8) + w)
-                                 : make_uint4(0, 0, 0, 0);
+        for (int w = 0; w < kYWords; ++w)
+          q.bv[e][w] = row[e] >= 0 ? *(reinterpret_cast<const uint4*>(from) + w) : make_uint4(0, 0, 0, 0);
+      } else {  // rows that begin anywhere, and odd ends: an element at a time, all of them under way
+        constexpr int kPer = 4 / (int)sizeof(TY);
+        uint32_t v[8 / kPer];
+#pragma unroll
+        for (int i = 0; i < 8 / kPer; ++i) {
+          v[i] = 0;
+#pragma unroll
+          for (int k = 0; k < kPer; ++k)
+            if (row[e] >= 0 && n8 + i * kPer + k < s.N) v[i] |= (uint32_t)bits(from[i * kPer + k]) << (16 * k);
+        }
+#pragma unroll
+        for (int w = 0; w < kYWords; ++w) q.bv[e][w] = make_uint4(v[4 * w], v[4 * w + 1], v[4 * w + 2], v[4 * w + 3]);
+      }
+    }
   };
   int have = -1;  // the projection whose h lies in shared memory
   Piece now, next;
@@ -645,20 +660,20 @@ __global__ void __launch_bounds__(kExpand, kBlocks == 4 ? 5 : 6) adapter_expand_
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[2 * j] = c[j][2 * e] * f, v[2 * j + 1] = c[j][2 * e + 1] * f;
       TY* y = static_cast<TY*>(s.y) + row[e] * s.y_row + now.n0 + 8 * t;
-      if (now.vec) {
-        if (s.base) {
+      if (s.base) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if constexpr (kY32) {
-              const uint4 w = now.bv[e][i >> 1];
-              v[2 * i] += __uint_as_float(i & 1 ? w.z : w.x), v[2 * i + 1] += __uint_as_float(i & 1 ? w.w : w.y);
-            } else {
-              const uint4 w = now.bv[e][0];
-              const float2 q = unpack2<TY>(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w);
-              v[2 * i] += q.x, v[2 * i + 1] += q.y;
-            }
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (kY32) {
+            const uint4 w = now.bv[e][i >> 1];
+            v[2 * i] += __uint_as_float(i & 1 ? w.z : w.x), v[2 * i + 1] += __uint_as_float(i & 1 ? w.w : w.y);
+          } else {
+            const uint4 w = now.bv[e][0];
+            const float2 q = unpack2<TY>(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w);
+            v[2 * i] += q.x, v[2 * i + 1] += q.y;
           }
         }
+      }
+      if (now.vec) {
         if constexpr (kY32) {
           reinterpret_cast<float4*>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
           reinterpret_cast<float4*>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -667,10 +682,9 @@ __global__ void __launch_bounds__(kExpand, kBlocks == 4 ? 5 : 6) adapter_expand_
                                                     pack2<TY>(v[6], v[7]));
         }
       } else {
-        const TY* base = s.base ? static_cast<const TY*>(s.base) + row[e] * s.base_row + now.n0 + 8 * t : nullptr;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (now.n0 + 8 * t + i < s.N) y[i] = from_f32<TY>(base ? v[i] + to_f32(base[i]) : v[i]);
+          if (now.n0 + 8 * t + i < s.N) y[i] = from_f32<TY>(v[i]);
       }
     }
   }

@@ -108,6 +108,9 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
 }
+__device__ __forceinline__ uint32_t bits(float v) { return __float_as_uint(v); }
+__device__ __forceinline__ uint32_t bits(__half v) { return __half_as_ushort(v); }
+__device__ __forceinline__ uint32_t bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 // What is left of v behind its first term (0 behind an infinity, not inf - inf).
 __device__ __forceinline__ float rest(float v, float term) { return v == term ? 0.f : v - term; }
 

@@ -11,6 +11,10 @@
 // lanes a row. (Bulk copies of a row each are issued one after another by a warp: 178 us
 // for what takes 105 so: 6007 rows of 17408 in bf16 on a base, 418 MB, 4 TB/s.)
 //
+// Rows that begin anywhere (an odd width, rows of y that are not 16-byte aligned), which neither kind of copy takes, go
+// through registers, 32 outputs of a row by the lanes of a warp: 3655 rows of 2533 and 10797 among them 219 us, 610 with
+// base read row by row; these instructions, not bytes, are the time there.
+//
 // Work: the tiles of 128 rows times 128 outputs of all projections make a line, cut into
 // equal stretches of one CTA per SM. Warp 8 brings the terms of the rows' h (made by a
 // small kernel between) and the weights by TMA, warp 9 issues the MMAs.
@@ -376,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         cp_commit();  // (a group a unit, empty or not)
       };
       bulk_wait_read();
+      fence_proxy_async_smem();  // (what lay in the slots by ordinary stores; bulk copies come for a whole run or not at all)
       __syncwarp();
       for (int u = 0; u < p.slots - 1; ++u) fetch(u, q + u);
       if (!waited) {
@@ -393,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = ok && warp_wait(ms.acc_full[buf], (uint32_t)((now / kBufs) & 1));
           tc_fence_after();
         }
-#pragma unroll
+#pragma unroll 1  // (its code has to stay in its cache)
         for (int h = 0; h < kUnits; ++h, ++u, ++q) {
           const int n0 = output(u), bytes = bytes_of(n0), slot = q % p.slots;
           uint8_t* own = smem + own_at + slot * kSlot;
@@ -447,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 *mine = make_uint4(o[0], o[1], o[2], o[3]);
               }
-            } else {
+            } else if (n0 + c * 32 < s.N) {
               // rows that begin anywhere, and odd ends: a row at a time for the warp
               float* stage = reinterpret_cast<float*>(own);
 #pragma unroll
@@ -456,15 +461,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               TY* const to = static_cast<TY*>(s.y);
               const TY* const from = static_cast<const TY*>(s.base);
               const int n = n0 + c * 32 + lane;
-#pragma unroll 4
+              TY had[32];  // (all of base on its way before the first store, which it might lie behind otherwise)
+#pragma unroll
               for (int k = 0; k < 32; ++k) {
-                const int64_t at_row = __shfl_sync(0xffffffffu, row, k);
+                const int64_t at_row = __shfl_sync(0xffffffffu, (int)row, k);
+                if (from && k < rows && n < s.N) had[k] = from[at_row * s.base_row + n];
+              }
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const int64_t at_row = __shfl_sync(0xffffffffu, (int)row, k);
                 if (k < rows && n < s.N) {
                   const float o = stage[k * 32 + (lane ^ k)];
-                  to[at_row * s.y_row + n] = from_f32<TY>(from ? o + to_f32(from[at_row * s.base_row + n]) : o);
+                  to[at_row * s.y_row + n] = from_f32<TY>(from ? o + to_f32(had[k]) : o);
                 }
               }
-              fence_proxy_async_smem();  // (the slot's next content may come by a bulk copy)
               __syncwarp();
             }
           }
