@@ -14,8 +14,8 @@
 // For few rows the weights are what is read, once for the rows of an adapter, and there
 // the time is the latency of one pass through memory after another: 1 fp32 row, 6144 to
 // 5120, rank 16: 7.8 us (0.3 MB); 200 fp16 rows over 9 adapters, 1672 to 4091, rank 24:
-// 12 us; 48 fp32 rows over 24 adapters, 5120 to q, k and v, rank 64: 18.7 us (39 MB,
-// 2.1 TB/s). So the MMAs there are warp-level (m16n8k16), whose operands come from
+// 12 us; 48 fp32 rows over 24 adapters, 5120 to q, k and v, rank 64: 19.3 us (39 MB,
+// 2.0 TB/s). So the MMAs there are warp-level (m16n8k16), whose operands come from
 // global memory straight into registers, 16 bytes a lane: no shared memory, barrier or
 // transposition lies between a load and its product, N, strides and row order are free,
 // and the accumulators lie where y's rows are stored from. `expand` reads what does not

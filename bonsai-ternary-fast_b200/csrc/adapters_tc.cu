@@ -12,7 +12,7 @@
 // for what takes 105 so: 6007 rows of 17408 in bf16 on a base, 418 MB, 4 TB/s.)
 //
 // Rows that begin anywhere (an odd width, rows of y that are not 16-byte aligned), which neither kind of copy takes, go
-// through registers, 32 outputs of a row by the lanes of a warp: 3655 rows of 2533 and 10797 among them 219 us, 610 with
+// through registers, 32 outputs of a row by the lanes of a warp: 3655 rows of 2533 and 10797 among them 222 us, 610 with
 // base read row by row; these instructions, not bytes, are the time there.
 //
 // Work: the tiles of 128 rows times 128 outputs of all projections make a line, cut into
@@ -464,12 +464,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               TY had[32];  // (all of base on its way before the first store, which it might lie behind otherwise)
 #pragma unroll
               for (int k = 0; k < 32; ++k) {
-                const int64_t at_row = __shfl_sync(0xffffffffu, (int)row, k);
+                const int64_t at_row = __shfl_sync(0xffffffffu, row, k);
                 if (from && k < rows && n < s.N) had[k] = from[at_row * s.base_row + n];
               }
 #pragma unroll
               for (int k = 0; k < 32; ++k) {
-                const int64_t at_row = __shfl_sync(0xffffffffu, (int)row, k);
+                const int64_t at_row = __shfl_sync(0xffffffffu, row, k);
                 if (k < rows && n < s.N) {
                   const float o = stage[k * 32 + (lane ^ k)];
                   to[at_row * s.y_row + n] = from_f32<TY>(from ? o + to_f32(had[k]) : o);
