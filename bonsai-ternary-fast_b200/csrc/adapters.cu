@@ -14,8 +14,8 @@
 // For few rows the weights are what is read, once for the rows of an adapter, and there
 // the time is the latency of one pass through memory after another: 1 fp32 row, 6144 to
 // 5120, rank 16: 7.8 us (0.3 MB); 200 fp16 rows over 9 adapters, 1672 to 4091, rank 24:
-// 12 us; 48 fp32 rows over 24 adapters, 5120 to q, k and v, rank 64: 19.3 us (39 MB,
-// 2.0 TB/s). So the MMAs there are warp-level (m16n8k16), whose operands come from
+// 12 us; 48 fp32 rows over 24 adapters, 5120 to q, k and v, rank 64: 18.6 us (39 MB,
+// 2.1 TB/s). So the MMAs there are warp-level (m16n8k16), whose operands come from
 // global memory straight into registers, 16 bytes a lane: no shared memory, barrier or
 // transposition lies between a load and its product, N, strides and row order are free,
 // and the accumulators lie where y's rows are stored from. `expand` reads what does not
@@ -491,14 +491,21 @@ __global__ void __launch_bounds__(kExpand, kBlocks == 4 ? 5 : 6) adapter_expand_
   // The plan, the weights and base were complete before `shrink` let this grid start.
   // (A grid may only end after the one before it, or the one behind it starts too early: every way out waits.)
   pdl_launch_dependents();
-  const int range = blockIdx.x % p.ranges, ti = blockIdx.x / p.ranges;
+  const int range = blockIdx.x % p.ranges, place = blockIdx.x / p.ranges;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const SmallTile* st = p.small + ti;  // (read at once, as above)
-  const Tile tile = st->tile;
+  const SmallTile* st = p.small + place;  // (read at once, as above)
+  Tile tile = st->tile;
   int row[2] = {st->rows[g], st->rows[8 + g]};
-  if (!plan_ok(p) || ti >= p.head[p.which]) {
+  // places without a tile of their own share the others' ranges (72 rows of 18 requests among 64 adapters, rank 104, to
+  // 12514 outputs: 60 us without, 40 so)
+  const int tiles = max(1, min(p.head[p.which], p.most)), share = p.most / tiles, part = place / tiles;
+  if (!plan_ok(p) || part >= share) {
     pdl_wait();
     return;
+  }
+  if (part > 0) {
+    st = p.small + place % tiles;
+    tile = st->tile, row[0] = st->rows[g], row[1] = st->rows[8 + g];
   }
   const int rank = tile.adapter < 0 ? 0 : rank_of(p, tile.adapter);
   const int blocks = (rank + 31) / 32;
@@ -506,7 +513,11 @@ __global__ void __launch_bounds__(kExpand, kBlocks == 4 ? 5 : 6) adapter_expand_
   auto pieces = [&](int i) { return (p.seg[i].N + kExpand - 1) / kExpand; };
   int total = 0;
   for (int i = 0; i < p.nseg; ++i) total += pieces(i);
-  const int first = (int)((int64_t)range * total / p.ranges), last = (int)((int64_t)(range + 1) * total / p.ranges);
+  int first = (int)((int64_t)range * total / p.ranges), last = (int)((int64_t)(range + 1) * total / p.ranges);
+  if (share > 1) {
+    const int all = last - first;
+    last = first + (int)((int64_t)(part + 1) * all / share), first += (int)((int64_t)part * all / share);
+  }
 #pragma unroll
   for (int e = 0; e < 2; ++e)
     if (e * 8 + g >= tile.count) row[e] = -1;
