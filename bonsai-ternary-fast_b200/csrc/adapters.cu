@@ -708,10 +708,10 @@ bool sizes_ok(int T, int K, int R, int nseg, int n) {
 }
 
 // Tiles of 16 rows while the rows are few, of 128 for prompts: us as few and as prompts, with the rows of 1 request, of 8
-// and each with an adapter of its own. bf16 to 17408, rank 64: 384 rows 20, 26, 27 and 25, 33, 36; 512 rows 32, 29, 39 and
-// 25, 30, 37; 1024 rows 52, 67, 69 and 31, 40, 42. fp32 q, k and v, whose terms cost the more the fewer rows share their
-// weights: 512 rows 29, 41, 45 and 38, 48, 102; 1024 rows 58, 67, 74 and 46, 69, 109; 2048 rows 116, 138, 132 and 71,
-// 107, 136.
+// and each with an adapter of its own. bf16 to 17408, rank 64: 384 rows 21, 27, 28 and 25, 33, 36; 512 rows 33, 31, 41 and
+// 25, 30, 37; 1024 rows 52, 67, 69 and 31, 40, 42. fp16 to 4091, rank 24: 512 rows 19, 18, 19 and 28, 28, 38; 1024 rows 37,
+// 37, 34 and 30, 41, 40. fp32 q, k and v, whose terms cost the more the fewer rows share their weights: 512 rows 30, 40, 45
+// and 38, 48, 102; 1024 rows 58, 67, 74 and 46, 69, 109; 2048 rows 116, 138, 132 and 71, 107, 136.
 struct Shape {
   bool large;
   int tiles;   // at most
