@@ -322,6 +322,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     // ---------------------------------------------------------- the way out: 32 rows a warp, every other tile
+    // A group takes every other one of the tiles with an adapter, by their number t, so that an accumulator is always the same
+    // group's, which waits for each of its phases in turn: a wait tells a phase only from the one before it.
     const int group = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t own_at = off_slots + warp * p.slots * kSlot;  // the warp's slots
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int b = min(kUnit, (s.N - n0) * (int)sizeof(TY));
         return wide && b > 0 && b % 16 == 0 ? b : 0;
       };
-      const int start = at + ((at ^ group) & 1), units = start < end ? ((end - start + 1) >> 1) * kUnits : 0;
+      const int start = at + (((copy ? at : t) ^ group) & 1), units = start < end ? ((end - start + 1) >> 1) * kUnits : 0;
       const int first_n = (piece + start - at) * kCols;  // the run's first output of this group
       auto output = [&](int u) { return first_n + u / kUnits * 2 * kCols + u % kUnits * kWidth; };
       // base of the run's unit u to its slot, which its last store has been read from
@@ -392,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (; at < end; ++at) {
         const int now = t;
         t += !copy;
-        if ((at & 1) != group) continue;
+        if (((copy ? at : now) & 1) != group) continue;
         const int buf = now % kBufs;
         if (!copy) {
           ok = ok && warp_wait(ms.acc_full[buf], (uint32_t)((now / kBufs) & 1));
