@@ -923,26 +923,33 @@ ADAPTERS_MAX, ADAPTERS_MAX_RANK = 1024, 128  # BTF_ADAPTERS_MAX, BTF_ADAPTERS_MA
 
 class AdapterPlan:
     """Which rows of a batch belong to which adapter (btf_adapter_plan), sorted on the device for every adapters() call of
-    a step: index [T] (int32 on the device; -1: a row without adapter) of n_adapters."""
+    a step: index [T] (int32 on the device; -1: a row without adapter) of n_adapters. Its memory (`plan`) is allocated on
+    the stream that it is made on; calls on another one are ordered behind it by the caller, as with any tensor, who also
+    keeps the plan until they are done (or calls plan.record_stream)."""
 
     def __init__(self, index, n_adapters: int, stream=None):
-        torch = _torch()
         dev = _cuda_device("AdapterPlan", index)
-        self.T, self.n_adapters = index.numel(), n_adapters
+        self.T, self.n_adapters, self.plan = index.numel(), n_adapters, None
         size = lib().btf_adapter_plan_bytes(self.T, n_adapters)
         if size < 0:
             check(1, "btf_adapter_plan_bytes")
-        self.plan = torch.empty(size, dtype=torch.uint8, device=dev)
-        self.update(index, stream)
+        self._sort(dev, index, stream, size)
 
     def update(self, index, stream=None) -> None:
         """Sorts the rows of another step, as many as before, into the same plan (in stream order)."""
-        ptr = _vector("AdapterPlan", self.plan.device, "index", index, _torch().int32, (self.T,))
+        self._sort(self.plan.device, index, stream, None)
+
+    def _sort(self, dev, index, stream, size) -> None:
+        ptr = _vector("AdapterPlan", dev, "index", index, _torch().int32, (self.T,))
         if ptr is None:
             raise RuntimeError("AdapterPlan: index must be a tensor")
-        _launch(self.plan.device, stream, self._call, ptr)
+        _launch(dev, stream, self._call, (ptr, dev, size))
 
-    def _call(self, st, ptr) -> None:
+    def _call(self, st, args) -> None:
+        ptr, dev, size = args
+        if self.plan is None:  # (here: on the stream that fills it)
+            torch = _torch()
+            self.plan = torch.empty(size, dtype=torch.uint8, device=dev)
         check(lib().btf_adapter_plan(ptr, self.T, self.n_adapters, self.plan.data_ptr(), self.plan.nbytes, st),
               "btf_adapter_plan")
         _written(self.plan)
