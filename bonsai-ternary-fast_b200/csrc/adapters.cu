@@ -203,6 +203,33 @@ struct XTerms {
       }
     }
   }
+  // `products` of an fp32 x into sums of their own, which c takes by fp32 additions (see the top).
+  template <int RT>
+  __device__ __forceinline__ void add(float (&c)[RT][NT][4], const uint4 (&lo)[RT], const uint4 (&hi)[RT], int ms, int ns) const {
+    if constexpr (!kF32) {
+      products(c, lo, hi, ms, ns);
+    } else {
+      constexpr int MB = RT < 2 ? RT : 2;  // (registers)
+#pragma unroll
+      for (int m0 = 0; m0 < RT; m0 += MB) {
+        float d[MB][NT][4];
+        uint4 l[MB], h[MB];
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+          l[m] = lo[m0 + m], h[m] = hi[m0 + m];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) d[m][j][0] = d[m][j][1] = d[m][j][2] = d[m][j][3] = 0.f;
+        }
+        products(d, l, h, ms - m0, ns);
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[m0 + m][j][e] += d[m][j][e];
+      }
+    }
+  }
   // c += the products: lo and hi the weights' rows g and g + 8 of each 16; of the weights' 16s and the rows' 8s only the
   // first ms and ns have anything.
   template <int RT>
@@ -301,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XTerms<TX, TW
     }
 #pragma unroll
     for (int j = 0; j < NT / JT; ++j)
-      if (j * JT < nts) F(xw[j]).products(c[j], lo, hi, mts, nts - j * JT);
+      if (j * JT < nts) F(xw[j]).add(c[j], lo, hi, mts, nts - j * JT);
   }
   // c[m][j]: weight rows 16 m + g and + 8, rows 8 j + 2 t and + 1
   float* mine = red + warp * kRows * kPitch;
@@ -445,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, RT == 8 && std::is_same_v<TX, float>
           lo[m] = *reinterpret_cast<const uint4*>(as + r * L::kARow + ((kAWords == 8 ? w ^ spread(r) : w) << 4));
           hi[m] = *reinterpret_cast<const uint4*>(as + (r + 8) * L::kARow + ((kAWords == 8 ? w ^ spread(r) : w) << 4));
         }
-        terms.products(c[m0 / L::MB], lo, hi, mts - m0, NT);
+        terms.add(c[m0 / L::MB], lo, hi, mts - m0, NT);
         if (RT > L::MB) asm volatile("" ::: "memory");
       }
     }

@@ -301,14 +301,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         if (elect_one()) {
           const uint32_t d = tmem + buf * kCols;
-#pragma unroll 1
-          for (int k = 0; k < steps; ++k) {
-            const uint32_t off = (k >> 2) * kBlock + (k & 3) * 32;
-            const uint64_t bd = smem_desc_sw128(ws + off);
+          // (all steps of the lower terms before those of the first: the sum is cut off at its own size each time)
 #pragma unroll
-            for (int e = kTerms - 1; e >= 0; --e)
-              mma_f16_ss(d, smem_desc_sw128(sbase + hs * h_bytes + e * p.blocks * kBlock + off), bd, kDesc, k > 0 || e < kTerms - 1);
-          }
+          for (int e = kTerms - 1; e >= 0; --e)
+#pragma unroll 1
+            for (int k = 0; k < steps; ++k) {
+              const uint32_t off = (k >> 2) * kBlock + (k & 3) * 32;
+              mma_f16_ss(d, smem_desc_sw128(sbase + hs * h_bytes + e * p.blocks * kBlock + off), smem_desc_sw128(ws + off), kDesc,
+                         k > 0 || e < kTerms - 1);
+            }
           if (at + 1 == end) mma_commit(smem_u32(&ms.h_empty[hs]));
           mma_commit(smem_u32(&ms.empty[s]));
           mma_commit(smem_u32(&ms.acc_full[buf]));
