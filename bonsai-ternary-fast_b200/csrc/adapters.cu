@@ -888,7 +888,9 @@ int btf_adapters(const btf_adapters_args* a, void* stream) {
   if (a->T == 0) return BTF_OK;
   auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   const int xb = elem_bytes(a->x_type), yb = elem_bytes(a->y_type);
-  if (!a->x || !a->plan || !al(a->x) || !al(a->plan) || a->x_row < 0 || a->x_row * xb % 16)
+  // (of one row or adapter no stride matters)
+  const int64_t x_row = a->T > 1 ? a->x_row : 0;
+  if (!a->x || !a->plan || !al(a->x) || !al(a->plan) || x_row < 0 || x_row * xb % 16)
     return fail(BTF_ERR_ARG, "btf_adapters: x or the plan is null or not 16-byte aligned, or x's rows are not");
   if (a->plan_bytes < PlanLayout(a->T, a->n_adapters).bytes)
     return fail(BTF_ERR_ARG, "btf_adapters: the plan is of other sizes (%lld bytes, %lld are needed)", (long long)a->plan_bytes,
@@ -899,18 +901,20 @@ int btf_adapters(const btf_adapters_args* a, void* stream) {
     if (s.N < 1 || s.N > 1 << 24) return fail(BTF_ERR_ARG, "btf_adapters: need 1 <= N <= 2^24 (got %d)", s.N);
     if (!s.a || !s.b || !s.y || !al(s.a) || !al(s.b))
       return fail(BTF_ERR_ARG, "btf_adapters: a, b or y is null, or a or b is not 16-byte aligned");
-    for (int64_t v : {s.a_adapter, s.a_row, s.b_adapter, s.b_row})
+    const int64_t a_adapter = a->n_adapters > 1 ? s.a_adapter : 0, b_adapter = a->n_adapters > 1 ? s.b_adapter : 0;
+    const int64_t b_row = s.N > 1 ? s.b_row : 0;
+    for (int64_t v : {a_adapter, s.a_row, b_adapter, b_row})
       if (v < 0 || v % 8) return fail(BTF_ERR_ARG, "btf_adapters: the strides of a and b must be multiples of 8 elements, >= 0");
-    if (s.a_row == 0 || (s.N > 1 && s.b_row == 0)) return fail(BTF_ERR_ARG, "btf_adapters: the rows of a and b need a stride");
+    if (s.a_row == 0 || (s.N > 1 && b_row == 0)) return fail(BTF_ERR_ARG, "btf_adapters: the rows of a and b need a stride");
     if (reinterpret_cast<uintptr_t>(s.y) % yb || reinterpret_cast<uintptr_t>(s.base) % yb)
       return fail(BTF_ERR_ARG, "btf_adapters: y or base is not aligned to its type");
     if (a->T > 1 && s.y_row < s.N) return fail(BTF_ERR_ARG, "btf_adapters: the rows of y overlap");
-    if (s.base && s.base_row < 0) return fail(BTF_ERR_ARG, "btf_adapters: the stride of base is negative");
+    if (s.base && a->T > 1 && s.base_row < 0) return fail(BTF_ERR_ARG, "btf_adapters: the stride of base is negative");
     if (s.base == s.y && a->T > 1 && s.base_row != s.y_row)
       return fail(BTF_ERR_ARG, "btf_adapters: in place needs the same strides");
     const int64_t y_row = a->T > 1 ? s.y_row : 0, base_row = a->T > 1 ? s.base_row : 0;
     const bool vec = al(s.y) && y_row * yb % 16 == 0 && al(s.base) && base_row * yb % 16 == 0;
-    p.seg[i] = {s.a, s.b, s.base, s.y, s.a_adapter, s.a_row, s.b_adapter, s.b_row, base_row, y_row, s.N, vec};
+    p.seg[i] = {s.a, s.b, s.base, s.y, a_adapter, s.a_row, b_adapter, b_row, base_row, y_row, s.N, vec};
   }
   const DeviceInfo* dev = current_device();
   if (!dev) return BTF_ERR_STATE;
@@ -921,7 +925,7 @@ int btf_adapters(const btf_adapters_args* a, void* stream) {
                 (long long)a->work_bytes, (long long)w.bytes);
   const PlanLayout at(a->T, a->n_adapters);
   const uint8_t* plan = static_cast<const uint8_t*>(a->plan);
-  p.x = a->x, p.x_row = a->T > 1 ? a->x_row : 0;
+  p.x = a->x, p.x_row = x_row;
   p.T = a->T, p.K = a->K, p.R = a->R, p.n = a->n_adapters, p.nseg = a->nseg, p.splits = sh.splits, p.room = 2 * dev->sm_count, p.most = sh.tiles, p.ranges = 1;
   p.steps = (a->K * elem_bytes(a->x_type) + 127) / 128;
   p.ranks = a->ranks, p.scales = a->scales;

@@ -631,7 +631,7 @@ int btf_rope_axes(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, c
  * device into `plan` (btf_adapter_plan_bytes bytes, 16-byte aligned). Asynchronous; the calls that use it come behind it. */
 int64_t btf_adapter_plan_bytes(int T, int n_adapters);
 int btf_adapter_plan(const int32_t* index, int T, int n_adapters, void* plan, int64_t plan_bytes, void* stream);
-typedef struct btf_adapter_seg { /* one projection; strides in elements, rows contiguous */
+typedef struct btf_adapter_seg { /* one projection; strides in elements (of one row or adapter none matters), rows contiguous */
   const void* a;               /* [n_adapters][R][K], 16-byte aligned, strides multiples of 8 */
   int64_t a_adapter, a_row;
   const void* b;               /* [n_adapters][N][R], as a */
