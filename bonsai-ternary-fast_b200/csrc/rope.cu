@@ -296,6 +296,7 @@ int btf_rope_axes_table(const btf_rope_cfg* c, const int* sections, int n_axes, 
   }
   if (2 * pairs != c->n_rot)
     return fail(BTF_ERR_ARG, "btf_rope_axes_table: the axes have %lld pairs, n_rot is %d", (long long)pairs, c->n_rot);
+  if (pairs == 0) return fail(BTF_ERR_ARG, "btf_rope_axes_table: the axes have no pairs");
   btf_rope_cfg own = *c;
   if (layout != BTF_AXES_OWN) {
     if (int rc = btf_rope_table(c, turns, mscale)) return rc;

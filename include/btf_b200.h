@@ -602,7 +602,7 @@ int btf_rope(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, const 
  *                   over); f_i as btf_rope_table's
  *   BTF_AXES_OWN    as BTF_AXES_SPLIT, and every axis has frequencies of its own: those of btf_rope_table with n_rot = 2
  *                   sections[a]
- * An axis may have no pairs. Host only: fills turns_host[n_rot / 2] and axis_host[n_rot / 2], and *mscale. */
+ * An axis may have no pairs (not all of them). Host only: fills turns_host[n_rot / 2] and axis_host[n_rot / 2], and *mscale. */
 #define BTF_ROPE_MAX_AXES 4
 #define BTF_AXES_SPLIT 0
 #define BTF_AXES_TURNS 1
