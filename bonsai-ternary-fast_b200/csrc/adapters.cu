@@ -204,7 +204,9 @@ struct XTerms {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           v[j][0][i] = w[i] & 0xffffe000u;
-          const float r = rest(__uint_as_float(w[i]), __uint_as_float(v[j][0][i]));
+          // (at fp32's last exponent cut to 11 bits, not rounded up to 2^128 with the first)
+          float r = rest(__uint_as_float(w[i]), __uint_as_float(v[j][0][i]));
+          asm("min.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(r) : "f"(0x1.ffcp116f));
           asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(v[j][1][i]) : "f"(r));
         }
       }
@@ -669,7 +671,7 @@ __global__ void __launch_bounds__(kExpand, kBlocks == 4 ? 5 : 6) adapter_expand_
           float v0 = v[kb][2 * i] * f, v1 = v[kb][2 * i + 1] * f;
 #pragma unroll
           for (int e = 0; e < kTerms; ++e) {
-            const uint32_t w = pack2<TW>(v0, v1);
+            const uint32_t w = !kHalf && e == 0 ? pack2<TW>(in_bf16(v0), in_bf16(v1)) : pack2<TW>(v0, v1);
             to[(((i >> 1) * kTerms + e) * 32) * 4 + (i & 1) * 2] = w;
             const float2 u = unpack2<TW>(w);
             v0 = rest(v0, u.x), v1 = rest(v1, u.y);

@@ -111,6 +111,8 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
 __device__ __forceinline__ uint32_t bits(float v) { return __float_as_uint(v); }
 __device__ __forceinline__ uint32_t bits(__half v) { return __half_as_ushort(v); }
 __device__ __forceinline__ uint32_t bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+// v for its first bf16 term: a finite v rounds to a finite one (the next term has the rest, and all of an infinity or NaN)
+__device__ __forceinline__ float in_bf16(float v) { return fminf(fmaxf(v, -0x1.fep127f), 0x1.fep127f); }
 // What is left of v behind its first term (0 behind an infinity, not inf - inf).
 __device__ __forceinline__ float rest(float v, float term) { return v == term ? 0.f : v - term; }
 

@@ -150,9 +150,10 @@ __global__ void __launch_bounds__(256) adapter_terms_kernel(const __grid_constan
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        w[i] = pack2<TW>(v[b][2 * i], v[b][2 * i + 1]);
+        const float v0 = v[b][2 * i], v1 = v[b][2 * i + 1];
+        w[i] = !std::is_same_v<TW, __half> && e == 0 ? pack2<TW>(in_bf16(v0), in_bf16(v1)) : pack2<TW>(v0, v1);
         const float2 u = unpack2<TW>(w[i]);
-        v[b][2 * i] = rest(v[b][2 * i], u.x), v[b][2 * i + 1] = rest(v[b][2 * i + 1], u.y);
+        v[b][2 * i] = rest(v0, u.x), v[b][2 * i + 1] = rest(v1, u.y);
       }
       *reinterpret_cast<uint4*>(terms + (((int64_t)e * p.nseg + seg) * p.T + at) * wide + b * 64 + l * 8) =
           make_uint4(w[0], w[1], w[2], w[3]);

@@ -622,7 +622,8 @@ int btf_rope_axes(const btf_rope_seg* segs, int nseg, int T, int D, int n_rot, c
  * with A_a the first ranks[a] of R rows of K, and B_a the first ranks[a] of R columns of N rows (what lies behind an
  * adapter's rank is never part of a result). A row whose index is no adapter (-1, or any other number outside 0 ..
  * n_adapters - 1) is y_t = base_t. base is what the shared projection gave (btf_gemv's y) and may be y itself (same
- * stride), or NULL (0). Products are summed in fp32, and an fp32 x or y is served to fp32: see csrc/adapters.cu. The
+ * stride), or NULL (0). Products are summed in fp32, and an fp32 x or y is served to fp32 (to 22 bits of x and
+ * of A x with fp16 adapters): see csrc/adapters.cu. An infinity or NaN makes what it enters an infinity or NaN. The
  * reference has no adapters; the call stands beside launch_gemv (src/cuda/kernels.cuh:56). */
 #define BTF_ADAPTERS_MAX 1024         /* adapters of a call */
 #define BTF_ADAPTERS_MAX_RANK 128     /* R */
