@@ -9,14 +9,18 @@
 // on tcgen05 (adapters_tc.cu).
 //
 // What bounds it: bytes. A row's x is read once, y written and base read once: with
-// rank r that is 2 r (K + N) multiply-adds for (K + 2 N) elements, 64 a byte at r = 64
+// rank r that is 2 r (K + N) operations for (K + 2 N) elements, 32 to 64 a byte at r = 64
 // in 16 bits, where the card has 250 a byte on tcgen05 and 80 on the warp-level MMA.
+// (An fp32 x takes three times the MMAs, and its terms have to be made: prompts of it are
+// bound by the issue of these, 60 % of the slots and 37 % of the tensor pipe: 6007 rows of
+// 8 requests, 5120 to q, k and v, rank 64: 242 us, of which the bytes take 79.)
 // For few rows the weights are what is read, once for the rows of an adapter, and there
 // the time is the latency of one pass through memory after another: 1 fp32 row, 6144 to
-// 5120, rank 16: 7.8 us (0.3 MB); 200 fp16 rows over 9 adapters, 1672 to 4091, rank 24:
-// 12 us; 48 fp32 rows over 24 adapters, 5120 to q, k and v, rank 64: 18.6 us (39 MB,
-// 2.1 TB/s). So the MMAs there are warp-level (m16n8k16), whose operands come from
-// global memory straight into registers, 16 bytes a lane: no shared memory, barrier or
+// 5120, rank 16: 8.1 us (0.3 MB); 200 fp16 rows over 9 adapters, 1672 to 4091, rank 24:
+// 12 us; 48 fp32 rows over 24 adapters, 5120 to q, k and v, rank 64: 18.9 us (39 MB,
+// 2.1 TB/s). `expand` can start under `shrink`, but at rank 64 two CTAs of that take the
+// registers of an SM, so most of it comes behind. The MMAs there are warp-level
+// (m16n8k16), whose operands come from global memory straight into registers, 16 bytes a lane: no shared memory, barrier or
 // transposition lies between a load and its product, N, strides and row order are free,
 // and the accumulators lie where y's rows are stored from. `expand` reads what does not
 // depend on h before it waits for it, and a piece's weights and base under the piece
@@ -32,8 +36,8 @@
 // element, a 500th of y's own rounding), or two fp16 terms (22 bits) of h over a power
 // of two of its row, which keeps fp16's range.
 //
-// The tensor cores cut a sum off at its own size (an MMA adds up to 2^-23 of it, towards 0)
-// where fp32 additions round. So the products of an fp32 x are summed there over 32 of K only,
+// The tensor cores cut a sum off, by up to 2^-23 of its size towards 0 in every MMA, where
+// fp32 additions round. So the products of an fp32 x are summed there over 32 of K only,
 // the lower terms first, and those sums by fp32 additions: 6007 rows of 17408, rank 64, against
 // 64 bits: 2.2e-7 of y's root mean square (1.0e-5 with one tensor-core sum over a stretch of K,
 // for up to 4 % less time; rows of 5120: 1.7e-7 and 3.0e-6). A 16-bit x keeps to one: 1.6e-6
@@ -52,6 +56,10 @@ constexpr int kThreads = 256, kExpand = 64;
 // ------------------------------------------------------------------ plan
 // One CTA. Warp w counts and later places its own stretch of the rows, so that the
 // order within an adapter is that of the rows whatever runs first.
+//
+// What bounds it: chains of reads, and the tiles of an adapter, T / 16 and T / 128 of them, that one lane
+// lists: 48 rows of 24 adapters 2.8 us, 6007 rows 7.2 (all of one adapter 17.7), 100000 rows 91 (263); of 1024
+// adapters, whose counters 32 warps have each, 15 to 19 for up to 1024 rows, 22 for 6007. Once a step.
 __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t* index, int T, int n, uint8_t* plan, PlanLayout at) {
   extern __shared__ int hist[];  // [32 warps][n + 1]
   __shared__ int total[BTF_ADAPTERS_MAX + 1], first[BTF_ADAPTERS_MAX + 1];
@@ -746,8 +754,8 @@ bool sizes_ok(int T, int K, int R, int nseg, int n) {
 // Tiles of 16 rows while the rows are few, of 128 for prompts: us as few and as prompts, with the rows of 1 request, of 8
 // and each with an adapter of its own. bf16 to 17408, rank 64: 384 rows 21, 27, 28 and 25, 33, 36; 512 rows 33, 31, 41 and
 // 25, 30, 37; 1024 rows 52, 67, 69 and 31, 40, 42. fp16 to 4091, rank 24: 512 rows 19, 18, 19 and 28, 28, 38; 1024 rows 37,
-// 37, 34 and 30, 41, 40. fp32 q, k and v, whose terms cost the more the fewer rows share their weights: 512 rows 30, 40, 45
-// and 38, 48, 102; 1024 rows 58, 67, 74 and 46, 69, 109; 2048 rows 116, 138, 132 and 71, 107, 136.
+// 37, 34 and 30, 41, 40. fp32 q, k and v, whose terms cost the more the fewer rows share their weights: 512 rows 31, 42, 46
+// and 38, 47, 95; 1024 rows 60, 70, 75 and 44, 68, 99; 2048 rows 121, 143, 134 and 68, 104, 127.
 struct Shape {
   bool large;
   int tiles;   // at most

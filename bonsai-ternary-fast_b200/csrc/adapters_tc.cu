@@ -1,9 +1,9 @@
 // Low-rank adapters of prompts (btf_adapters with many rows), on the tcgen05 tensor
 // cores: y = base + s B h for tiles of 128 rows of one adapter.
 //
-// What bounds it: y's and base's bytes. An element of y takes 2 r multiply-adds for each
-// term of h (see adapters.cu), 256 at r = 64 in bf16: 0.06 ns of a card that moves 4 bytes
-// in 0.6. So the MMAs (128 x 128 outputs at a time, four accumulators in tensor memory)
+// What bounds it: y's and base's bytes. An element of y takes 2 r operations for each
+// term of h (see adapters.cu), 256 at r = 64 in bf16: 0.15 ps of a card that moves the
+// element's 4 bytes, base and y, in 0.61. So the MMAs (128 x 128 outputs at a time, four accumulators in tensor memory)
 // run far ahead and the kernel is its way out: 8 warps, each with 32 rows of every other
 // tile. A lane has a row: copies bring 256 bytes of its base into shared memory ahead of
 // their turn and take the sum from the same place to y: one TMA copy of 32 rows x 128

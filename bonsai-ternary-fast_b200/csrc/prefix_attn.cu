@@ -14,11 +14,20 @@
 // rows takes one or several of equal stretches of (kv-head, M tile); neighbours have the
 // same rows of K and V and different M tiles, so that those come from L2.
 //
-// What bounds it: for few rows latency, as in attn.cuh; for many M tiles what the tensor cores read of shared memory, 96
-// KB a 64-row tile at D = 128 with the tile's arrival: 768 cycles, where its MMAs take 512. Measured (device time): 4
-// sequences over 1000 shared rows, 24/4 fp16 heads of 256: 16.9 us; 48 over 4099, 20/5 bf16 heads of 96: 23.5; 16 of 8
-// nodes over 16384 and up to 1100 own, 24/4 fp16 heads of 256: 59 to 63 (29 GFLOP, 490 TFLOP/s); 128 over 65536 and up to
-// 2000 own, 32/8 bf16 heads of 128: 171 to 189 (138 GFLOP, 770 TFLOP/s; own rows read by each sequence would be 34 GB).
+// What bounds it. Few rows: latency, as in attn.cuh. Many M tiles: a tile of 64 rows is bound by what the tensor cores read
+// of shared memory, 96 KB at D = 128 with the tile's arrival (768 cycles, 512 of them the MMAs) and as in attn.cuh at D =
+// 256 (1560); each segment's ways in and out come on top, one after another, since nothing of the next segment begins before
+// the last one's O is out. Measured (device time; cycles of a CTA's softmax warps, on average, from the wait on):
+//   4 sequences over 1000 shared rows, 24/4 fp16 heads of 256: 16.9 us.
+//   48 over 4099, 20/5 bf16 heads of 96: 23.5 us. A CTA of the shared rows has 5 tiles, 7.4 of 21 thousand cycles (the
+//     split 4, q's way in 5.4, the first S 1.1, the way out 2.6); one of own rows 1.5 segments of a tile, 4 of 20 (6.2, 3.6,
+//     1.6, 2.6); the rest of the time is the launches and the join.
+//   16 of 8 nodes over 16384 and up to 1100 own, 24/4 fp16 heads of 256: 59 to 64 us (29 GFLOP, 480 TFLOP/s). The shared rows'
+//     26 tiles take 45 of 73 thousand cycles, 1750 each; q's way in 16, the split 4, the way out 5; the join comes behind.
+//   128 over 65536 and up to 2000 own, 32/8 bf16 heads of 128: 171 to 203 us (138 GFLOP, 680 to 810 TFLOP/s; own rows read by
+//     each sequence would be 34 GB). The shared rows' 146 tiles take 239 of 259 thousand cycles, 1630 each with two CTAs an
+//     SM, at 1.4 to 1.6 GHz under the power cap; a quarter of the CTAs has own rows, 15 segments each, whose ways in and out
+//     are 85 of 228 thousand cycles.
 #include "attn.cuh"
 
 namespace btf {
