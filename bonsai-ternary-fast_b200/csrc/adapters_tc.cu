@@ -354,9 +354,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < 8; ++i) rows_at[i] = (int)__shfl_sync(0xffffffffu, row, i * 4 + (lane >> 3));
       // bytes of a row of the unit from output n0 that copies move; 0: rows that begin anywhere, and odd ends
       auto bytes_of = [&](int n0) {
-        if (tiled) return n0 < s.N ? kUnit : 0;  // (a TMA copy stops at N)
+        // (a TMA copy stops at N, but a store only between 16-byte words: it would write zeros to the end of N's)
         const int b = min(kUnit, (s.N - n0) * (int)sizeof(TY));
-        return wide && b > 0 && b % 16 == 0 ? b : 0;
+        return !wide || b <= 0 || b % 16 ? 0 : tiled ? kUnit : b;
       };
       const int start = at + (((copy ? at : t) ^ group) & 1), units = start < end ? ((end - start + 1) >> 1) * kUnits : 0;
       const int first_n = (piece + start - at) * kCols;  // the run's first output of this group
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         cp_commit();  // (a group a unit, empty or not)
       };
       bulk_wait_read();
-      fence_proxy_async_smem();  // (what lay in the slots by ordinary stores; bulk copies come for a whole run or not at all)
+      fence_proxy_async_smem();  // (what lay in the slots by ordinary stores; in a run those come behind its last bulk copy)
       __syncwarp();
       for (int u = 0; u < p.slots - 1; ++u) fetch(u, q + u);
       if (!waited) {
