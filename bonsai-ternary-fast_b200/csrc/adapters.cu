@@ -175,8 +175,14 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 ld16(const void* p, bool on) {
+__device__ __forceinline__ uint4 ld16(const void* p, bool on) {  // of weights
   return on ? __ldg(static_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+}
+// of x, which the kernel before may still have been writing when this one started: not a read-only load
+__device__ __forceinline__ uint4 ld16_x(const void* p, bool on) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (on) asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
 // 8 consecutive elements of NT rows of x as the B operands of a 32-wide step: `kTerms` terms of 4 words of 16-bit pairs,
 // or (fp32 x, fp16 weights) 2 terms of 8 tf32 values.
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, RT == 8 || (RT == 4 && XTerms<TX, TW
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int l = 0; l < F::kLoads; ++l) xw[j / JT][j % JT][l] = ld16(x[j] + k + 4 * l, kin && on[j]);
+      for (int l = 0; l < F::kLoads; ++l) xw[j / JT][j % JT][l] = ld16_x(x[j] + k + 4 * l, kin && on[j]);
 #pragma unroll
     for (int m = 0; m < RT; ++m) {
       lo[m] = ld16(a + (int64_t)(m * 16 + g) * s.a_row + k, kin && m < mts && m * 16 + g < p.R);
